@@ -58,13 +58,15 @@ int64_t tesm_hip_launch_log_read(char* buf, int64_t cap, int clear);
 int tesm_hip_stream_copy(void* dst, const void* src, int64_t bytes, void* stream);
 
 /* Device status word of the library's bounded waits on the current device, no reference
- * counterpart (the reference's kernels never wait on one another).  Bit 0 (TESM_STATUS_SCAN_GAVE_UP):
+ * counterpart (the reference's kernels never wait on one another), and of the indices that only the
+ * device sees (bit 1, TESM_STATUS_BAD_PARENT).  Bit 0 (TESM_STATUS_SCAN_GAVE_UP):
  * a single-pass scan's look-back poll gave up; the states of that span are NaN.  The kernels still
  * return, so a caller that wants certainty checks this word after its work.  Synchronises with the
  * device (a diagnostic, not for the hot path); clear != 0 zeroes the word after reading it.
  * tesm_hip_debug_scan_spin_limit sets the poll limit of later scans (default 1 << 20 rounds; a
  * negative limit gives up at once, which tests use to exercise the report). */
 #define TESM_STATUS_SCAN_GAVE_UP 1u
+#define TESM_STATUS_BAD_PARENT 2u /* tesm_hip_reorder_rows met a parent outside [0, K); that row stayed as it was */
 int tesm_hip_device_status(uint32_t* status, int clear);
 int tesm_hip_debug_scan_spin_limit(int limit);
 
@@ -497,6 +499,130 @@ typedef struct tesm_hip_ffn {
 
 int64_t tesm_hip_ffn_ws_bytes(const tesm_hip_ffn* p);
 int tesm_hip_ffn_forward(const tesm_hip_ffn* p, void* ws, int64_t ws_bytes, void* stream);
+
+/* Short causal convolution over time, one filter per channel, no reference counterpart:
+ * y[t, c] = act(bias[c] + sum_j weight[c, j] x[t - W + 1 + j, c]), act = silu or (silu == 0) the identity,
+ * sums in float32.  The rows are B sequences of L (S = B), or with seq_starts S sequences packed one
+ * behind the other in one row axis (B = 1, L rows): sequence s is rows seq_starts[s] .. seq_starts[s+1]-1
+ * (not decreasing; empty sequences allowed; rows in front of the first and behind the last are neither
+ * read nor written).  state: the W - 1 rows before each sequence, oldest first (NULL: zeros); state_out
+ * (another buffer): its last W - 1 rows, of state and sequence together.  2 <= W <= 8. */
+typedef struct tesm_hip_conv {
+  int dt;                     /* x, y and states */
+  int w_dt;                   /* weight and bias */
+  int64_t B, L, C, W, S;
+  int silu;
+  const void* x;              /* (B * L, ld_x) */
+  int64_t ld_x;
+  const void* weight;         /* (C, W) */
+  const void* bias;           /* optional (C) */
+  const int32_t* seq_starts;  /* optional (S + 1) */
+  const void* state;          /* optional (S, W - 1, C) */
+  void* y;                    /* (B * L, ld_y) */
+  int64_t ld_y;
+  void* state_out;            /* optional (S, W - 1, C) */
+} tesm_hip_conv;
+
+int tesm_hip_causal_conv(const tesm_hip_conv* p, void* stream);
+
+/* Selective state space scan, no reference counterpart (tesm_hip_scan is the scan with one state per
+ * channel and given decays).  Head h of H, its group g = h / (H / G), row t:
+ *   d = softplus(dt[t,h] + dt_bias[h]) (softplus == 0: dt + dt_bias),  a = exp(d * A[h]),
+ *   state[p,n] = a * state[p,n] + d * x[t,h,p] * B[t,g,n],
+ *   y[t,h,p] = sum_n state[p,n] C[t,g,n] + D[h] x[t,h,p],  times silu(z[t,h,p]) with z.
+ * Rows and seq_starts as in tesm_hip_causal_conv.  h0 / h_out: (S, H, P, N) float32, the states before and
+ * after each sequence (NULL h0: zeros; h_out is another buffer).  N <= 256; ws: selective_scan_ws_bytes. */
+typedef struct tesm_hip_ssm {
+  int dt;                     /* x, dts, Bm, Cm, z, y */
+  int64_t B, L, H, P, G, N, S;
+  int softplus;
+  const void* x;              /* row r, head h, p at x[r * ld_x + h * P + p] */
+  int64_t ld_x;
+  const void* dts;            /* (rows, ld_dt), H values per row */
+  int64_t ld_dt;
+  const float* A;             /* (H) */
+  const void* Bm;             /* row r, group g, n at Bm[r * ld_b + g * N + n] */
+  int64_t ld_b;
+  const void* Cm;
+  int64_t ld_c;
+  const float* D;             /* optional (H) */
+  const void* z;              /* optional, as x */
+  int64_t ld_z;
+  const float* dt_bias;       /* optional (H) */
+  const int32_t* seq_starts;  /* optional (S + 1) */
+  const float* h0;            /* optional (S, H, P, N) */
+  void* y;                    /* as x */
+  int64_t ld_y;
+  float* h_out;               /* optional (S, H, P, N) */
+} tesm_hip_ssm;
+
+int64_t tesm_hip_selective_scan_ws_bytes(const tesm_hip_ssm* p);
+int tesm_hip_selective_scan(const tesm_hip_ssm* p, void* ws, int64_t ws_bytes, void* stream);
+
+/* One token of the convolution and the scan for B sequences, no reference counterpart.  row holds the token's
+ * x (H * P), B (G * N) and C (G * N) before the convolution; the convolved values stay in float32.
+ * conv_state: the W - 1 rows before the token, conv_state_out (another buffer) those before the next;
+ * conv_weight NULL: no convolution, row is used as it is.  state is updated in place. */
+typedef struct tesm_hip_ssm_step {
+  int dt;                     /* row, conv states, dts, z, y */
+  int w_dt;                   /* conv_weight, conv_bias */
+  int64_t B, H, P, G, N, W;
+  int softplus;
+  int silu;
+  const void* row;            /* (B, ld_row) */
+  int64_t ld_row;
+  const void* conv_weight;    /* optional (H * P + 2 * G * N, W) */
+  const void* conv_bias;      /* optional */
+  const void* conv_state;     /* (B, W - 1, H * P + 2 * G * N) */
+  void* conv_state_out;       /* the same shape, another buffer */
+  const void* dts;            /* (B, ld_dt) */
+  int64_t ld_dt;
+  const float* A;             /* (H) */
+  const float* D;             /* optional (H) */
+  const void* z;              /* optional (B, ld_z) */
+  int64_t ld_z;
+  const float* dt_bias;       /* optional (H) */
+  float* state;               /* (B, H, P, N) */
+  void* y;                    /* (B, ld_y) */
+  int64_t ld_y;
+} tesm_hip_ssm_step;
+
+int tesm_hip_selective_scan_step(const tesm_hip_ssm_step* p, void* stream);
+
+/* Beam search's choice, no reference counterpart.  Beam k of request b offers every token v at
+ * scores[b,k] + logits[b,k,v] - logsumexp(logits[b,k,:]); the n best offers of a request's K beams are
+ * written in falling order, equal ones by k * V + v.  Offers that are no number (a NaN logit; a row with
+ * a +infinite logit or none above -infinity) and all offers of a beam whose score is not finite count as
+ * -infinity.  A beam with finished != 0 offers token pad alone, at its own score.  finished_out: the
+ * parent was finished, or the token is eos (eos < 0: no such token).  K, n <= 64, n <= K * V. */
+typedef struct tesm_hip_beam {
+  int dt;                     /* logits */
+  int64_t B, K, V, n;
+  const void* logits;         /* beam b * K + k at logits[(b * K + k) * ld] */
+  int64_t ld;
+  const float* scores;        /* (B, K) */
+  const uint8_t* finished;    /* optional (B, K) */
+  int64_t pad, eos;
+  float* out_scores;          /* (B, n) */
+  int64_t* parents;           /* (B, n) beams */
+  int64_t* tokens;            /* (B, n) */
+  uint8_t* finished_out;      /* optional (B, n) */
+} tesm_hip_beam;
+
+int64_t tesm_hip_beam_select_ws_bytes(const tesm_hip_beam* p);
+int tesm_hip_beam_select(const tesm_hip_beam* p, void* ws, int64_t ws_bytes, void* stream);
+
+/* Rows of `count` tensors moved to their new beams, in place, no reference counterpart: row b * K + k of
+ * each becomes the old row b * K + parents[b,k].  The tensors must not overlap.  A parent outside [0, K)
+ * leaves its row as it is and sets TESM_STATUS_BAD_PARENT.  K <= 64. */
+typedef struct tesm_hip_rows {
+  void* p;
+  int64_t pitch;              /* bytes from row to row */
+  int64_t bytes;              /* bytes of a row */
+} tesm_hip_rows;
+
+int tesm_hip_reorder_rows(const tesm_hip_rows* t, int64_t count, const int64_t* parents, int64_t B, int64_t K,
+                          void* stream);
 
 #ifdef __cplusplus
 }

@@ -155,6 +155,56 @@ class Ffn(ctypes.Structure):
     ]
 
 
+class Conv(ctypes.Structure):
+    """``tesm_hip_conv``."""
+    _fields_ = [
+        ("dt", I32), ("w_dt", I32),
+        ("B", I64), ("L", I64), ("C", I64), ("W", I64), ("S", I64),
+        ("silu", I32),
+        ("x", P), ("ld_x", I64), ("weight", P), ("bias", P), ("seq_starts", P), ("state", P),
+        ("y", P), ("ld_y", I64), ("state_out", P),
+    ]
+
+
+class Ssm(ctypes.Structure):
+    """``tesm_hip_ssm``."""
+    _fields_ = [
+        ("dt", I32),
+        ("B", I64), ("L", I64), ("H", I64), ("P", I64), ("G", I64), ("N", I64), ("S", I64),
+        ("softplus", I32),
+        ("x", P), ("ld_x", I64), ("dts", P), ("ld_dt", I64), ("A", P), ("Bm", P), ("ld_b", I64),
+        ("Cm", P), ("ld_c", I64), ("D", P), ("z", P), ("ld_z", I64), ("dt_bias", P), ("seq_starts", P),
+        ("h0", P), ("y", P), ("ld_y", I64), ("h_out", P),
+    ]
+
+
+class SsmStep(ctypes.Structure):
+    """``tesm_hip_ssm_step``."""
+    _fields_ = [
+        ("dt", I32), ("w_dt", I32),
+        ("B", I64), ("H", I64), ("P", I64), ("G", I64), ("N", I64), ("W", I64),
+        ("softplus", I32), ("silu", I32),
+        ("row", P), ("ld_row", I64), ("conv_weight", P), ("conv_bias", P), ("conv_state", P), ("conv_state_out", P),
+        ("dts", P), ("ld_dt", I64), ("A", P), ("D", P), ("z", P), ("ld_z", I64), ("dt_bias", P),
+        ("state", P), ("y", P), ("ld_y", I64),
+    ]
+
+
+class Beam(ctypes.Structure):
+    """``tesm_hip_beam``."""
+    _fields_ = [
+        ("dt", I32),
+        ("B", I64), ("K", I64), ("V", I64), ("n", I64),
+        ("logits", P), ("ld", I64), ("scores", P), ("finished", P), ("pad", I64), ("eos", I64),
+        ("out_scores", P), ("parents", P), ("tokens", P), ("finished_out", P),
+    ]
+
+
+class Rows(ctypes.Structure):
+    """``tesm_hip_rows``."""
+    _fields_ = [("p", P), ("pitch", I64), ("bytes", I64)]
+
+
 class Taps(ctypes.Structure):
     """``tesm_hip_taps``."""
     _fields_ = [("q_u", P), ("s_u", P), ("q_cs", P), ("s_cs", P), ("q_te", P), ("s_te", P), ("q_c", P), ("s_c", P),
@@ -198,6 +248,13 @@ _SIGNATURES = {
     "tesm_hip_add_rmsnorm": ([ctypes.POINTER(RmsNorm), P], I32),
     "tesm_hip_ffn_ws_bytes": ([ctypes.POINTER(Ffn)], I64),
     "tesm_hip_ffn_forward": ([ctypes.POINTER(Ffn), P, I64, P], I32),
+    "tesm_hip_causal_conv": ([ctypes.POINTER(Conv), P], I32),
+    "tesm_hip_selective_scan_ws_bytes": ([ctypes.POINTER(Ssm)], I64),
+    "tesm_hip_selective_scan": ([ctypes.POINTER(Ssm), P, I64, P], I32),
+    "tesm_hip_selective_scan_step": ([ctypes.POINTER(SsmStep), P], I32),
+    "tesm_hip_beam_select_ws_bytes": ([ctypes.POINTER(Beam)], I64),
+    "tesm_hip_beam_select": ([ctypes.POINTER(Beam), P, I64, P], I32),
+    "tesm_hip_reorder_rows": ([P, I64, P, I64, I64, P], I32),
     "tesm_hip_mimo_coef": ([P, P, I32, I64, I64, I64, P, P, P], I32),
     "tesm_hip_mimo_prefill_ws_bytes": ([ctypes.POINTER(MimoLayer)], I64),
     "tesm_hip_mimo_prefill": ([ctypes.POINTER(MimoLayer), P, I64, P], I32),

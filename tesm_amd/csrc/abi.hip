@@ -10,12 +10,14 @@
 #include <mutex>
 #include <string>
 
+#include "beam.h"
 #include "decode.h"
 #include "entangle.h"
 #include "global.h"
 #include "mimo.h"
 #include "norm.h"
 #include "scan.h"
+#include "ssm.h"
 #include "tesm_hip_internal.h"
 #include "../../include/tesm_hip.h"
 
@@ -675,7 +677,9 @@ int tesm_hip_stream_copy(void* dst, const void* src, int64_t bytes, void* stream
 int tesm_hip_device_status(uint32_t* status, int clear) {
   unsigned v = 0;
   if (int rc = scan_status(&v, clear)) return rc;
-  if (status) *status = v;
+  unsigned r = 0;
+  if (int rc = reorder_status(&r, clear)) return rc;
+  if (status) *status = v | r;
   return kOk;
 }
 
@@ -1900,6 +1904,129 @@ int tesm_hip_ffn_forward(const tesm_hip_ffn* pp, void* ws, int64_t ws_bytes, voi
     return rc;
   if (tapping && (rc = tap_codes(tp.q_h, tp.s_h, s.hq, p.M, st))) return rc;
   return run_linear(s.hq, p.down_proj, p.M, p.d_model, p.d_inter, p.y, p.dt, p.ld_y, st);
+}
+
+int tesm_hip_causal_conv(const tesm_hip_conv* p, void* stream) {
+  TESM_REQUIRE(p != nullptr, kErrInvalidArg, "causal conv: null descriptor");
+  if (int rc = check_ptrs("causal conv", {{p->x, "x"}, {p->weight, "weight"}, {p->bias, "bias"},
+                                          {p->seq_starts, "seq_starts"}, {p->state, "state"}, {p->y, "y"},
+                                          {p->state_out, "state_out"}}))
+    return rc;
+  ConvArgs a;
+  a.dt = p->dt;
+  a.w_dt = p->w_dt;
+  a.B = p->B, a.L = p->L, a.C = p->C, a.W = p->W, a.S = p->S;
+  a.silu = p->silu;
+  a.x = p->x, a.ld_x = p->ld_x;
+  a.weight = p->weight, a.bias = p->bias;
+  a.seq_starts = p->seq_starts;
+  a.state = p->state;
+  a.y = p->y, a.ld_y = p->ld_y;
+  a.state_out = p->state_out;
+  return launch_causal_conv(a, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"
+
+namespace tesm {
+namespace {
+SsmArgs ssm_args(const tesm_hip_ssm& p) {
+  SsmArgs a;
+  a.dt = p.dt;
+  a.B = p.B, a.L = p.L, a.H = p.H, a.P = p.P, a.G = p.G, a.N = p.N, a.S = p.S;
+  a.softplus = p.softplus;
+  a.x = p.x, a.ld_x = p.ld_x;
+  a.dts = p.dts, a.ld_dt = p.ld_dt;
+  a.A = p.A;
+  a.Bm = p.Bm, a.ld_b = p.ld_b;
+  a.Cm = p.Cm, a.ld_c = p.ld_c;
+  a.D = p.D;
+  a.z = p.z, a.ld_z = p.ld_z;
+  a.dt_bias = p.dt_bias;
+  a.seq_starts = p.seq_starts;
+  a.h0 = p.h0;
+  a.y = p.y, a.ld_y = p.ld_y;
+  a.h_out = p.h_out;
+  return a;
+}
+
+BeamArgs beam_args(const tesm_hip_beam& p) {
+  BeamArgs a;
+  a.dt = p.dt;
+  a.B = p.B, a.K = p.K, a.V = p.V, a.n = p.n;
+  a.logits = p.logits, a.ld = p.ld;
+  a.scores = p.scores;
+  a.finished = p.finished;
+  a.pad = p.pad, a.eos = p.eos;
+  a.out_scores = p.out_scores;
+  a.parents = p.parents;
+  a.tokens = p.tokens;
+  a.finished_out = p.finished_out;
+  return a;
+}
+}  // namespace
+}  // namespace tesm
+
+extern "C" {
+
+int64_t tesm_hip_selective_scan_ws_bytes(const tesm_hip_ssm* p) {
+  return p ? selective_scan_ws_bytes(ssm_args(*p)) : -1;
+}
+
+int tesm_hip_selective_scan(const tesm_hip_ssm* p, void* ws, int64_t ws_bytes, void* stream) {
+  TESM_REQUIRE(p != nullptr, kErrInvalidArg, "selective scan: null descriptor");
+  if (int rc = check_ptrs("selective scan",
+                          {{p->x, "x"}, {p->dts, "dt"}, {p->A, "A"}, {p->Bm, "B"}, {p->Cm, "C"}, {p->D, "D"},
+                           {p->z, "z"}, {p->dt_bias, "dt_bias"}, {p->seq_starts, "seq_starts"}, {p->h0, "h0"},
+                           {p->y, "y"}, {p->h_out, "h_out"}, {ws, "workspace"}}))
+    return rc;
+  return launch_selective_scan(ssm_args(*p), ws, ws_bytes, static_cast<hipStream_t>(stream));
+}
+
+int tesm_hip_selective_scan_step(const tesm_hip_ssm_step* p, void* stream) {
+  TESM_REQUIRE(p != nullptr, kErrInvalidArg, "selective scan step: null descriptor");
+  if (int rc = check_ptrs("selective scan step",
+                          {{p->row, "row"}, {p->conv_weight, "conv_weight"}, {p->conv_bias, "conv_bias"},
+                           {p->conv_state, "conv_state"}, {p->conv_state_out, "conv_state_out"}, {p->dts, "dt"},
+                           {p->A, "A"}, {p->D, "D"}, {p->z, "z"}, {p->dt_bias, "dt_bias"}, {p->state, "state"},
+                           {p->y, "y"}}))
+    return rc;
+  SsmStepArgs a;
+  a.dt = p->dt, a.w_dt = p->w_dt;
+  a.B = p->B, a.H = p->H, a.P = p->P, a.G = p->G, a.N = p->N, a.W = p->W;
+  a.softplus = p->softplus, a.silu = p->silu;
+  a.row = p->row, a.ld_row = p->ld_row;
+  a.conv_weight = p->conv_weight, a.conv_bias = p->conv_bias;
+  a.conv_state = p->conv_state, a.conv_state_out = p->conv_state_out;
+  a.dts = p->dts, a.ld_dt = p->ld_dt;
+  a.A = p->A, a.D = p->D;
+  a.z = p->z, a.ld_z = p->ld_z;
+  a.dt_bias = p->dt_bias;
+  a.state = p->state;
+  a.y = p->y, a.ld_y = p->ld_y;
+  return launch_selective_scan_step(a, static_cast<hipStream_t>(stream));
+}
+
+int64_t tesm_hip_beam_select_ws_bytes(const tesm_hip_beam* p) { return p ? beam_select_ws_bytes(beam_args(*p)) : -1; }
+
+int tesm_hip_beam_select(const tesm_hip_beam* p, void* ws, int64_t ws_bytes, void* stream) {
+  TESM_REQUIRE(p != nullptr, kErrInvalidArg, "beam select: null descriptor");
+  if (int rc = check_ptrs("beam select", {{p->logits, "logits"}, {p->scores, "scores"}, {p->finished, "finished"},
+                                          {p->out_scores, "out_scores"}, {p->parents, "parents"},
+                                          {p->tokens, "tokens"}, {p->finished_out, "finished_out"},
+                                          {ws, "workspace"}}))
+    return rc;
+  return launch_beam_select(beam_args(*p), ws, ws_bytes, static_cast<hipStream_t>(stream));
+}
+
+int tesm_hip_reorder_rows(const tesm_hip_rows* t, int64_t count, const int64_t* parents, int64_t B, int64_t K,
+                          void* stream) {
+  static_assert(sizeof(tesm_hip_rows) == sizeof(ReorderRows), "one layout");
+  if (int rc = check_ptrs("reorder rows", {{parents, "parents"}})) return rc;
+  for (int64_t i = 0; t && i < count; ++i)
+    if (int rc = check_ptr(t[i].p, "a tensor", "reorder rows")) return rc;
+  return launch_reorder_rows(reinterpret_cast<const ReorderRows*>(t), count, parents, B, K,
+                             static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -10,6 +10,7 @@ projection output are passed without copies.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 from typing import Optional
@@ -431,3 +432,337 @@ def output_gate(te, cc, sp_packed, sp_cw, ep_packed, ep_cw, local, gate, d_state
     with torch.cuda.device(dev):
         _lib.check(lib.tesm_hip_output_gate_i2(ctypes.byref(d), _stream(local)))
     return y, qy
+
+
+# ---------------------------------------------------------------------------
+# selective state space pieces: short causal convolution, selective scan, their one-token step
+# ---------------------------------------------------------------------------
+def _no_grad(what: str, *ts) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"{what}: the hip kernels are forward-only: run under torch.no_grad()")
+
+
+def _row_pitch(x: torch.Tensor, lead: int):
+    """The pitch in elements of ``x``'s rows (the first ``lead`` dimensions flattened into one row axis, the others
+    one contiguous row), or None where ``x`` is not laid out in such rows."""
+    width = 1
+    for n, st in zip(reversed(x.shape[lead:]), reversed(x.stride()[lead:])):
+        if n != 1 and st != width:
+            return None
+        width *= n
+    if x.numel() == 0:
+        return max(width, 1)
+    pitch = None  # from the last row dimension that has more than one entry
+    for d in range(lead - 1, -1, -1):
+        n, st = x.shape[d], x.stride(d)
+        if n == 1:
+            continue
+        if pitch is None:
+            pitch, span = st, n * st
+        elif st != span:
+            return None
+        else:
+            span *= n
+    pitch = width if pitch is None else pitch
+    return pitch if pitch >= width else None
+
+
+def _as_rows(x: Optional[torch.Tensor], lead: int):
+    """``x`` and its row pitch, copied only where it is not laid out in rows."""
+    if x is None:
+        return None, 0
+    pitch = _row_pitch(x, lead)
+    if pitch is None:
+        x = x.contiguous()
+        pitch = _row_pitch(x, lead)
+    return x, pitch
+
+
+def _out_rows(out: torch.Tensor, shape, dtype, lead: int, what: str) -> int:
+    pitch = _row_pitch(out, lead) if out.dtype == dtype and out.shape == torch.Size(shape) else None
+    if pitch is None:
+        raise ValueError(f"{what}: out must be a {dtype} tensor of shape {tuple(shape)} in contiguous rows, each at the "
+                         "same distance from the last")
+    return pitch
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _f32(t: Optional[torch.Tensor], n: int, name: str, what: str):
+    if t is None:
+        return None
+    if t.numel() != n:
+        raise ValueError(f"{what}: {name} must hold {n} values, got {tuple(t.shape)}")
+    return t.to(torch.float32).contiguous()
+
+
+def _sequences(seq_starts: Optional[torch.Tensor], B: int, what: str):
+    """``seq_starts`` as the kernels take it (int32, contiguous), and the number of sequences."""
+    if seq_starts is None:
+        return None, B
+    if B != 1:
+        raise ValueError(f"{what}: packed sequences lie in one row axis: with seq_starts the first dimension must be 1")
+    if seq_starts.dim() != 1 or seq_starts.numel() < 1 or seq_starts.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: seq_starts must be a 1-D int32 or int64 tensor of one entry more than sequences")
+    return seq_starts.to(torch.int32).contiguous(), seq_starts.numel() - 1
+
+
+def _same_dtype(what: str, dtype: torch.dtype, **ts) -> None:
+    for name, t in ts.items():
+        if t is not None and t.dtype != dtype:
+            raise TypeError(f"{what}: {name} is {t.dtype}, expected {dtype} as the first argument")
+
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, silu: bool = True,
+                state: Optional[torch.Tensor] = None, seq_starts: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None):
+    """Short causal convolution over time, one filter per channel; returns ``(y (B, L, C), state (S, W - 1, C))``.
+
+    ``y[b, t, c] = silu(bias[c] + sum_j weight[c, j] x[b, t - W + 1 + j, c])`` (``silu=False``: no activation) for x
+    (B, L, C) and ``weight`` (C, W), 2 <= W <= 8, summed in float32.  With ``seq_starts`` (S + 1, on the device, not
+    decreasing) x is (1, rows, C) and holds S sequences one behind the other, sequence s in rows
+    ``seq_starts[s] .. seq_starts[s + 1] - 1``; rows in front of the first and behind the last one stay as they are in
+    ``out`` (zero without ``out``).  ``state`` (S, W - 1, C): the rows before each sequence, oldest first, zeros by
+    default.  The state returned holds each sequence's last W - 1 rows.  ``out`` must not overlap x.  x, state and y
+    share a dtype; weight and bias share one (float32 or bfloat16) of their own.
+    """
+    if x.dim() != 3 or weight.dim() != 2 or weight.shape[0] != x.shape[2]:
+        raise ValueError("causal_conv: x must be (B, L, C) and weight (C, W)")
+    _no_grad("causal_conv", x, weight, bias, state)
+    B, L, C = x.shape
+    W = weight.shape[1]
+    if not 2 <= W <= 8:
+        raise ValueError(f"causal_conv: the filter must have 2 to 8 taps, got {W}")
+    seq_starts, S = _sequences(seq_starts, B, "causal_conv")
+    _same_dtype("causal_conv", x.dtype, state=state)
+    _same_dtype("causal_conv", weight.dtype, bias=bias)
+    if bias is not None and bias.numel() != C:
+        raise ValueError(f"causal_conv: bias must hold {C} values, got {tuple(bias.shape)}")
+    if state is not None and state.shape != (S, W - 1, C):
+        raise ValueError(f"causal_conv: state must be {(S, W - 1, C)}, got {tuple(state.shape)}")
+    d = _lib.Conv()
+    d.dt, d.w_dt = dt_code(x.dtype), dt_code(weight.dtype)
+    weight = weight.contiguous()
+    bias = bias.contiguous() if bias is not None else None
+    state = state.contiguous() if state is not None else None
+    x, ld = _as_rows(x, 2)
+    require_device(x, weight, bias, state, seq_starts, out)
+    if out is None:
+        out = (torch.zeros if seq_starts is not None else torch.empty)((B, L, C), dtype=x.dtype, device=x.device)
+    if out.data_ptr() == x.data_ptr() and x.numel():
+        raise ValueError("causal_conv: out must not be x")
+    d.B, d.L, d.C, d.W, d.S, d.silu = B, L, C, W, S, int(silu)
+    new = torch.empty((S, W - 1, C), dtype=x.dtype, device=x.device)
+    d.x, d.ld_x, d.weight, d.bias = x.data_ptr(), ld, weight.data_ptr(), _ptr(bias)
+    d.seq_starts, d.state = _ptr(seq_starts), _ptr(state)
+    d.y, d.ld_y = out.data_ptr(), _out_rows(out, (B, L, C), x.dtype, 2, "causal_conv")
+    d.state_out = new.data_ptr()
+    on_device(x.device.index, _lib.load().tesm_hip_causal_conv, ctypes.byref(d), raw_stream(x.device.index))
+    return out, new
+
+
+def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
+                   D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
+                   dt_bias: Optional[torch.Tensor] = None, softplus: bool = True,
+                   state: Optional[torch.Tensor] = None, seq_starts: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None):
+    """Selective state space scan; returns ``(y (B, L, H, P), state (S, H, P, N) float32)``.
+
+    Per head h with its group's B and C (H heads share G groups), over rows t:
+    ``d = softplus(dt + dt_bias)`` (``softplus=False``: ``dt + dt_bias``), ``state = exp(d A) state + d x B^T``,
+    ``y = state C + D x``, times ``silu(z)`` with ``z``.  x, z: (B, L, H, P); dt: (B, L, H); B, C: (B, L, G, N),
+    N <= 256; A, D, dt_bias: (H); ``state`` (S, H, P, N) float32: the states before each sequence (zeros by default).
+    ``seq_starts`` and ``out`` as in ``causal_conv``.  x, dt, B, C, z and y share a dtype and may be column slices of
+    wider rows.  States and sums are float32; with bfloat16 operands the decayed scores and the state read by a chunk's
+    rows are rounded to bfloat16 for the products.
+    """
+    if x.dim() != 4 or dt.dim() != 3 or B.dim() != 4 or dt.shape != x.shape[:3] or B.shape[:2] != x.shape[:2] or \
+            C.shape != B.shape or (z is not None and z.shape != x.shape):
+        raise ValueError("selective_scan: x and z must be (B, L, H, P), dt (B, L, H), B and C (B, L, G, N)")
+    _no_grad("selective_scan", x, dt, A, B, C, D, z, dt_bias, state)
+    nb, L, H, P = x.shape
+    G, N = B.shape[2:]
+    if H < 1 or P < 1 or G < 1 or N < 1 or H % G:
+        raise ValueError(f"selective_scan: {H} heads of {P} channels do not share {G} groups of {N} states evenly")
+    if N > 256:
+        raise ValueError(f"selective_scan: at most 256 states, got {N}")
+    _same_dtype("selective_scan", x.dtype, dt=dt, B=B, C=C, z=z)
+    seq_starts, S = _sequences(seq_starts, nb, "selective_scan")
+    if state is not None and (state.shape != (S, H, P, N) or state.dtype != torch.float32):
+        raise ValueError(f"selective_scan: state must be float32 {(S, H, P, N)}, got {state.dtype} {tuple(state.shape)}")
+    A, D, dt_bias = (_f32(t, H, n, "selective_scan") for t, n in ((A, "A"), (D, "D"), (dt_bias, "dt_bias")))
+    state = state.contiguous() if state is not None else None
+    d = _lib.Ssm()
+    d.dt = dt_code(x.dtype)
+    (x, d.ld_x), (dt, d.ld_dt), (B, d.ld_b), (C, d.ld_c), (z, d.ld_z) = (_as_rows(t, 2) for t in (x, dt, B, C, z))
+    dev = x.device
+    require_device(x, dt, A, B, C, D, z, dt_bias, state, seq_starts, out)
+    if out is None:
+        out = (torch.zeros if seq_starts is not None else torch.empty)((nb, L, H, P), dtype=x.dtype, device=dev)
+    if x.numel() and out.data_ptr() in (x.data_ptr(), B.data_ptr(), C.data_ptr(), _ptr(z)):
+        raise ValueError("selective_scan: out must not be one of the operands")
+    new = torch.empty((S, H, P, N), dtype=torch.float32, device=dev)
+    d.B, d.L, d.H, d.P, d.G, d.N, d.S, d.softplus = nb, L, H, P, G, N, S, int(softplus)
+    d.x, d.dts, d.A, d.Bm, d.Cm = x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr()
+    d.D, d.z, d.dt_bias, d.seq_starts, d.h0 = _ptr(D), _ptr(z), _ptr(dt_bias), _ptr(seq_starts), _ptr(state)
+    d.y, d.ld_y = out.data_ptr(), _out_rows(out, (nb, L, H, P), x.dtype, 2, "selective_scan")
+    d.h_out = new.data_ptr()
+    lib = _lib.load()
+    nbytes = int(lib.tesm_hip_selective_scan_ws_bytes(ctypes.byref(d)))
+    ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=dev)
+    on_device(dev.index, lib.tesm_hip_selective_scan, ctypes.byref(d), ws.data_ptr(), nbytes, raw_stream(dev.index))
+    return out, new
+
+
+def selective_scan_step(row: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, state: torch.Tensor,
+                        conv_weight: Optional[torch.Tensor] = None, conv_bias: Optional[torch.Tensor] = None,
+                        conv_state: Optional[torch.Tensor] = None, *, n_groups: int = 1,
+                        D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
+                        dt_bias: Optional[torch.Tensor] = None, softplus: bool = True, silu: bool = True,
+                        out: Optional[torch.Tensor] = None, conv_state_out: Optional[torch.Tensor] = None):
+    """One token of ``causal_conv`` and ``selective_scan``: returns ``(y (B, H, P), conv_state)``.
+
+    ``row`` (B, H * P + 2 * G * N) holds the token's x, B and C before the convolution, whose result stays in float32;
+    without ``conv_weight`` the row is used as it is.  ``state`` (B, H, P, N) float32 is updated in place;
+    ``conv_state`` (B, W - 1, H * P + 2 * G * N) is read, and the state after the token is returned in a tensor of its
+    own (``conv_state_out``, which must not be ``conv_state``; captured graphs alternate between two).  dt (B, H),
+    z (B, H, P); the rest as in ``selective_scan``.
+    """
+    if state.dim() != 4 or row.dim() != 2 or row.shape[0] != state.shape[0] or dt.shape != state.shape[:2] or \
+            (z is not None and z.shape != state.shape[:3]):
+        raise ValueError("selective_scan_step: row must be (B, channels), dt (B, H), z (B, H, P) and state (B, H, P, N)")
+    _no_grad("selective_scan_step", row, dt, A, state, conv_weight, conv_bias, conv_state, D, z, dt_bias)
+    nb, H, P, N = state.shape
+    G, width = int(n_groups), row.shape[1]
+    if G < 1 or H < 1 or P < 1 or N < 1 or H % G or width != H * P + 2 * G * N:
+        raise ValueError(f"selective_scan_step: a row of {H} heads x {P} channels and {G} groups x 2 x {N} states has "
+                         f"{H * P + 2 * G * N} values, got {width}")
+    if N > 256:
+        raise ValueError(f"selective_scan_step: at most 256 states, got {N}")
+    if state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError("selective_scan_step: state must be a contiguous float32 tensor (it is updated in place)")
+    _same_dtype("selective_scan_step", row.dtype, dt=dt, z=z, conv_state=conv_state)
+    A, D, dt_bias = (_f32(t, H, n, "selective_scan_step") for t, n in ((A, "A"), (D, "D"), (dt_bias, "dt_bias")))
+    d = _lib.SsmStep()
+    d.dt = d.w_dt = dt_code(row.dtype)
+    dev = row.device
+    if conv_weight is not None:
+        W = conv_weight.shape[-1]
+        if conv_weight.shape != (width, W) or not 2 <= W <= 8:
+            raise ValueError(f"selective_scan_step: conv_weight must be ({width}, 2 to 8), got {tuple(conv_weight.shape)}")
+        if conv_bias is not None and (conv_bias.numel() != width or conv_bias.dtype != conv_weight.dtype):
+            raise ValueError(f"selective_scan_step: conv_bias must hold {width} values of conv_weight's dtype")
+        if conv_state is None or conv_state.shape != (nb, W - 1, width):
+            raise ValueError(f"selective_scan_step: conv_state must be {(nb, W - 1, width)}")
+        conv_weight, conv_state = conv_weight.contiguous(), conv_state.contiguous()
+        conv_bias = conv_bias.contiguous() if conv_bias is not None else None
+        if conv_state_out is None:
+            conv_state_out = torch.empty_like(conv_state)
+        elif conv_state_out.shape != conv_state.shape or conv_state_out.dtype != row.dtype or \
+                not conv_state_out.is_contiguous() or (nb and conv_state_out.data_ptr() == conv_state.data_ptr()):
+            raise ValueError("selective_scan_step: conv_state_out must be another contiguous tensor like conv_state")
+        d.W, d.w_dt = W, dt_code(conv_weight.dtype)
+        d.conv_weight, d.conv_bias = conv_weight.data_ptr(), _ptr(conv_bias)
+        d.conv_state, d.conv_state_out = conv_state.data_ptr(), conv_state_out.data_ptr()
+    elif conv_bias is not None or conv_state is not None or conv_state_out is not None:
+        raise ValueError("selective_scan_step: conv_bias and conv_state need conv_weight")
+    (row, d.ld_row), (dt, d.ld_dt), (z, d.ld_z) = (_as_rows(t, 1) for t in (row, dt, z))
+    require_device(row, dt, A, state, conv_weight, conv_bias, conv_state, conv_state_out, D, z, dt_bias, out)
+    if out is None:
+        out = torch.empty((nb, H, P), dtype=row.dtype, device=dev)
+    d.B, d.H, d.P, d.G, d.N, d.softplus, d.silu = nb, H, P, G, N, int(softplus), int(silu)
+    d.row, d.dts, d.A, d.D, d.z, d.dt_bias = row.data_ptr(), dt.data_ptr(), A.data_ptr(), _ptr(D), _ptr(z), _ptr(dt_bias)
+    d.state = state.data_ptr()
+    d.y, d.ld_y = out.data_ptr(), _out_rows(out, (nb, H, P), row.dtype, 1, "selective_scan_step")
+    on_device(dev.index, _lib.load().tesm_hip_selective_scan_step, ctypes.byref(d), raw_stream(dev.index))
+    return out, conv_state_out
+
+
+# ---------------------------------------------------------------------------
+# beam search: the choice of the next tokens, and the states that follow the beams
+# ---------------------------------------------------------------------------
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = None, *,
+                finished: Optional[torch.Tensor] = None, pad_token: int = 0, eos_token: Optional[int] = None):
+    """The n best continuations of every request's K beams: ``(scores, parents, tokens, finished)``, each (B, n).
+
+    ``logits`` (B, K, V) and ``scores`` (B, K) float32: beam k offers token v at
+    ``scores[b, k] + log_softmax(logits[b, k])[v]``.  The n (default K) best offers come in falling order, equal ones in
+    the order of ``k * V + v``.  NaN logits, rows with a +infinite logit and beams whose score is not finite offer
+    -infinity.  A beam with ``finished`` (B, K) bool offers ``pad_token`` alone, at its own score; the last result says
+    whether the parent was finished or the token is ``eos_token`` (None where neither argument is given).  parents and
+    tokens are int64.  K and n are at most 64.
+    """
+    if logits.dim() != 3 or scores.shape != logits.shape[:2]:
+        raise ValueError("beam_select: logits must be (B, K, V) and scores (B, K)")
+    _no_grad("beam_select", logits, scores)
+    B, K, V = logits.shape
+    n = K if n is None else int(n)
+    if not (1 <= K <= 64 and 1 <= n <= 64 and n <= K * V):
+        raise ValueError(f"beam_select: 1 to 64 beams and candidates, at most K * V of them; got K={K}, V={V}, n={n}")
+    if scores.dtype != torch.float32:
+        raise TypeError(f"beam_select: scores must be float32, got {scores.dtype}")
+    if finished is not None and (finished.shape != scores.shape or finished.dtype not in (torch.bool, torch.uint8)):
+        raise ValueError("beam_select: finished must be a (B, K) bool tensor")
+    for name, t in (("pad_token", pad_token if finished is not None else None), ("eos_token", eos_token)):
+        if t is not None and not 0 <= t < V:
+            raise ValueError(f"beam_select: {name} {t} is outside the vocabulary of {V}")
+    d = _lib.Beam()
+    d.dt = dt_code(logits.dtype)
+    logits, d.ld = _as_rows(logits, 2)
+    scores = scores.contiguous()
+    finished = finished.contiguous() if finished is not None else None
+    require_device(logits, scores, finished)
+    dev = logits.device
+    out = torch.empty((B, n), dtype=torch.float32, device=dev)
+    parents, tokens = (torch.empty((B, n), dtype=torch.int64, device=dev) for _ in range(2))
+    done = torch.empty((B, n), dtype=torch.bool, device=dev) if finished is not None or eos_token is not None else None
+    d.B, d.K, d.V, d.n = B, K, V, n
+    d.logits, d.scores, d.finished = logits.data_ptr(), scores.data_ptr(), _ptr(finished)
+    d.pad, d.eos = int(pad_token), -1 if eos_token is None else int(eos_token)
+    d.out_scores, d.parents, d.tokens, d.finished_out = out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _ptr(done)
+    lib = _lib.load()
+    nbytes = int(lib.tesm_hip_beam_select_ws_bytes(ctypes.byref(d)))
+    ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=dev)
+    on_device(dev.index, lib.tesm_hip_beam_select, ctypes.byref(d), ws.data_ptr(), nbytes, raw_stream(dev.index))
+    return out, parents, tokens, done
+
+
+def reorder_rows(tensors, parents: torch.Tensor) -> None:
+    """Row ``b * K + k`` of every tensor becomes its old row ``b * K + parents[b, k]``, in place and in one launch.
+
+    ``parents`` (B, K) int64, K <= 64; each tensor has B * K rows (its first dimension), each row contiguous; any
+    dtype.  The tensors must not overlap.  A parent outside 0 .. K - 1 leaves its row as it is and sets bit 1 of
+    ``device_status``.
+    """
+    if parents.dim() != 2 or parents.dtype != torch.int64:
+        raise ValueError("reorder_rows: parents must be a (B, K) int64 tensor")
+    B, K = parents.shape
+    if not 1 <= K <= 64:
+        raise ValueError(f"reorder_rows: 1 to 64 beams, got {K}")
+    tensors = list(tensors)
+    grad = torch.is_grad_enabled()
+    rows, dev = B * K, parents.device
+    table = []  # (address, pitch, row bytes) of each: a decode step hands over every layer's caches, so the loop is lean
+    for t in tensors:
+        if t.dim() < 1 or t.size(0) != rows:
+            raise ValueError(f"reorder_rows: a tensor of shape {tuple(t.shape)} does not have {rows} rows")
+        if grad:
+            _no_grad("reorder_rows", t)
+        nbytes = t.nbytes // rows if rows else 0
+        if t.is_contiguous():
+            pitch = nbytes
+        else:
+            pitch = _row_pitch(t, 1)
+            if pitch is None:
+                raise ValueError("reorder_rows: the rows of a tensor must be contiguous and must not overlap")
+            pitch *= t.element_size()
+        table += (t.data_ptr(), pitch, nbytes)
+    if len(set(table[::3])) != len(tensors) and rows and all(table[2::3]):
+        raise ValueError("reorder_rows: a tensor is given twice")
+    parents = parents.contiguous()
+    require_device(parents, *tensors)
+    table = array.array("q", table)
+    on_device(dev.index, _lib.load().tesm_hip_reorder_rows, table.buffer_info()[0], len(tensors), parents.data_ptr(), B, K,
+              raw_stream(dev.index))

@@ -211,6 +211,12 @@ class MixerModel(nn.Module):
         return {i: layer.allocate_inference_cache(batch_size, max_seqlen, dtype=dtype, **kwargs)
                 for i, layer in enumerate(self.layers)}
 
+    def reorder_inference_cache(self, caches, parents):
+        """Moves every layer's cache to its new beams, in place and in one launch: row ``b * K + k`` of the state and
+        the rings becomes the old row ``b * K + parents[b, k]`` (``hip_ops.reorder_rows``; parents (B, K) int64)."""
+        hip_ops.reorder_rows([cache[k] for cache in caches.values() for k in ("state", "ent_k_cache", "ent_v_cache")],
+                             parents)
+
     def forward(self, input_ids, inference_params=None, prev_states=None, **mixer_kwargs):
         """mixer_seq_simple.py:171-239: embeddings + positions (offset by layer 0's cache position in
         a one-token decode step), the blocks with each layer's cache and the previous layer's
@@ -285,6 +291,51 @@ class TESMLMHeadModel(nn.Module):
 
     def allocate_inference_cache(self, batch_size, max_seqlen, dtype=None, **kwargs):
         return self.backbone.allocate_inference_cache(batch_size, max_seqlen, dtype=dtype, **kwargs)
+
+    def reorder_inference_cache(self, caches, parents):
+        return self.backbone.reorder_inference_cache(caches, parents)
+
+    @torch.no_grad()
+    def beam_search(self, input_ids: torch.Tensor, num_beams: int, max_new_tokens: int,
+                    eos_token: Optional[int] = None, pad_token: Optional[int] = None):
+        """The ``num_beams`` best continuations of each prompt found by beam search: ``(tokens (B, num_beams, n),
+        scores (B, num_beams))``, best first; a score is the sum of the tokens' log probabilities.
+
+        ``input_ids`` (B, L), prompts of one length.  ``eos_token`` (default: the configuration's) ends a continuation,
+        which then holds ``pad_token`` (default: the configuration's); the search ends after ``max_new_tokens``, or when
+        every beam has ended.  Each step is the one-token decode step, ``hip_ops.beam_select`` and one
+        ``reorder_inference_cache``.
+        """
+        cfg = self.tesm_config
+        eos_token = cfg.eos_token_id if eos_token is None else eos_token
+        pad_token = cfg.pad_token_id if pad_token is None else pad_token
+        B, L = input_ids.shape
+        if not 1 <= num_beams <= min(64, cfg.vocab_size):
+            raise ValueError(f"beam_search: 1 to {min(64, cfg.vocab_size)} beams, got {num_beams}")
+        if max_new_tokens < 1:
+            raise ValueError(f"beam_search: max_new_tokens must be positive, got {max_new_tokens}")
+        if L + max_new_tokens - 1 > cfg.max_seq_len:  # the last token chosen is not read
+            raise ValueError(f"beam_search: {L} + {max_new_tokens} tokens exceed max_seq_len {cfg.max_seq_len}")
+        caches = self.allocate_inference_cache(B, L + max_new_tokens)
+        params = {"state_cache": caches}
+        logits = self(input_ids, inference_params=params, logits_to_keep=1)[0].logits
+        scores = torch.zeros((B, 1), dtype=torch.float32, device=logits.device)
+        scores, _, tokens, done = hip_ops.beam_select(logits, scores, num_beams, pad_token=pad_token, eos_token=eos_token)
+        for cache in caches.values():
+            for k in ("state", "ent_k_cache", "ent_v_cache"):
+                cache[k] = cache[k].repeat_interleave(num_beams, 0)
+        chosen = torch.full((B * num_beams, max_new_tokens), pad_token, dtype=torch.int64, device=logits.device)
+        chosen[:, 0] = tokens.view(-1)
+        n = 1
+        while n < max_new_tokens and not (done is not None and bool(done.all())):
+            logits = self(tokens.view(-1, 1), inference_params=params)[0].logits
+            scores, parents, tokens, done = hip_ops.beam_select(logits.view(B, num_beams, -1), scores, finished=done,
+                                                                pad_token=pad_token, eos_token=eos_token)
+            self.reorder_inference_cache(caches, parents)
+            hip_ops.reorder_rows([chosen], parents)
+            chosen[:, n] = tokens.view(-1)
+            n += 1
+        return chosen[:, :n].view(B, num_beams, n), scores
 
     def forward(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
                 inference_params: Optional[dict] = None, prev_states=None, logits_to_keep: int = 0,
