@@ -8,50 +8,689 @@ namespace tesm {
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
-
 __device__ __forceinline__ float softplusf_(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
 __device__ __forceinline__ float siluf_(float v) { return v * sigmoidf_(v); }
 
-// One wave per (sequence, head, p): lanes over the N states, row after row.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// ---------------------------------------------------------------------------
+// The scan in chunks of Q rows.  With c_i the sum of d A over the chunk's rows up to i, and h the state on entry:
+//   Y = W X + exp(c) C h,   W_ij = (C_i . B_j) exp(c_i - c_j) d_j for j <= i, else 0
+//   h' = exp(c_Q) h + sum_j exp(c_Q - c_j) d_j x_j B_j^T
+// so that all of it is matrix products.  A workgroup of 4 waves walks a segment of one sequence for 128 columns of one
+// group (4 slices of 32 columns, each inside one head, one per wave); a wave keeps its slice's state in its
+// accumulators.  The products are formed transposed, with the state's layout in mind:
+//   scores  S^T = B C^T   (shared by the heads of the workgroup), scaled to W and kept in LDS, a matrix per head
+//   Y^T     = h C^T, scaled by exp(c_i) per column, + X^T W^T
+//   h       = exp(c_Q) h + B^T (w x)
+// where a result's lane holds 4 consecutive rows of one column.  Rows of a 32-wide block are taken in the order
+// row m of tile T  <->  8 (m / 4) + 4 T + m % 4: two tiles of the state are then the 8 consecutive states per lane that
+// the next product's operand needs, with no exchange, and two tiles of Y are 8 consecutive columns of one row, one
+// 16-byte store.
+// ---------------------------------------------------------------------------
+constexpr int kCols = 128;  // columns per workgroup
+constexpr int64_t kMinSegment = 256;
+
 template <int DT>
-__global__ __launch_bounds__(256) void ssm_rows_kernel(SsmArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (u >= a.S * a.H * a.P) return;
-  const int64_t s = u / (a.H * a.P), h = u / a.P % a.H, p = u % a.P, g = h / (a.H / a.G);
-  int64_t first, end;
-  if (a.seq_starts) {
-    seq_rows(a.seq_starts, s, a.B * a.L, first, end);
-  } else {
-    first = s * a.L;
-    end = first + a.L;
+struct Tile;
+template <>
+struct Tile<kBF16> {
+  using E = uint16_t;
+  static constexpr int Q = 64, EV = 8, PAD = 8;
+  using Frag = uint4;  // 8 consecutive k of one row: lane l holds row l & 15, k = 8 (l >> 4) ..
+  static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
   }
-  float st4[4];
-  for (int i = 0; i < 4; ++i) {
-    const int64_t n = lane + 64 * i;
-    st4[i] = a.h0 && n < a.N ? a.h0[u * a.N + n] : 0.0f;
+  static __device__ __forceinline__ Frag row(const E* p) { return *reinterpret_cast<const uint4*>(p); }
+  // 8 k from 8 rows of pitch `pitch`; p: the lane's place in the first rows (see tr_at)
+  static __device__ __forceinline__ Frag column(const E* p, int pitch) {
+    const uint2 a = tr(p), b = tr(p + 4 * pitch);
+    return make_uint4(a.x, a.y, b.x, b.y);
   }
-  for (int64_t r = first; r < end; ++r) {
-    const float raw = ld<DT>(a.dts, r * a.ld_dt + h) + (a.dt_bias ? a.dt_bias[h] : 0.0f);
-    const float d = a.softplus ? softplusf_(raw) : raw;
-    const float decay = fast_exp(d * a.A[h]);
-    const float x = ld<DT>(a.x, r * a.ld_x + h * a.P + p);
-    float acc = 0.0f;
+  static __device__ __forceinline__ uint2 tr(const E* p) {
+    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+    return __builtin_bit_cast(uint2, v);
+  }
+  // Lane's place for column(): rows 8 g .., 4 columns 8 (m % 4) + 4 T of row m / 4
+  static __device__ __forceinline__ int tr_at(int g, int m, int T, int pitch) {
+    return (8 * g + (m >> 2)) * pitch + 8 * (m & 3) + 4 * T;
+  }
+  static __device__ __forceinline__ Frag pack(const f32x4& lo, const f32x4& hi) {
+    return make_uint4(pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
+                      pack_bf16x2(hi[2], hi[3]));
+  }
+  static __device__ __forceinline__ void unpack(const Frag& f, float (&v)[8]) {
+    const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t n = lane + 64 * i;
-      if (n >= a.N) continue;
-      st4[i] = decay * st4[i] + d * x * ld<DT>(a.Bm, r * a.ld_b + g * a.N + n);
-      acc += st4[i] * ld<DT>(a.Cm, r * a.ld_c + g * a.N + n);
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
-    float y = wave_sum_f<64>(acc);
-    if (a.D) y += a.D[h] * x;
-    if (a.z) y *= siluf_(ld<DT>(a.z, r * a.ld_z + h * a.P + p));
-    if (lane == 0) st<DT>(a.y, r * a.ld_y + h * a.P + p, y);
   }
-  if (a.h_out)
-    for (int i = 0; i < 4; ++i)
-      if (lane + 64 * i < a.N) a.h_out[u * a.N + lane + 64 * i] = st4[i];
+  static __device__ __forceinline__ void store4(E* p, const f32x4& v) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+  }
+};
+template <>
+struct Tile<kF32> {
+  using E = float;
+  static constexpr int Q = 32, EV = 4, PAD = 4;
+  struct Frag {
+    float v[8];
+  };
+  static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ Frag row(const E* p) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    return Frag{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+  }
+  static __device__ __forceinline__ Frag column(const E* p, int pitch) {
+    Frag f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = p[e * pitch];
+    return f;
+  }
+  static __device__ __forceinline__ int tr_at(int g, int m, int T, int pitch) {
+    return 8 * g * pitch + 8 * (m >> 2) + 4 * T + (m & 3);
+  }
+  static __device__ __forceinline__ Frag pack(const f32x4& lo, const f32x4& hi) {
+    return Frag{{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
+  }
+  static __device__ __forceinline__ void unpack(const Frag& f, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = f.v[i];
+  }
+  static __device__ __forceinline__ void store4(E* p, const f32x4& v) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+};
+
+// The compiler is to form what depends on h, and what is read from memory, anew from here on (kept values would have
+// to be spilled).
+template <int NS>
+__device__ __forceinline__ void anew(f32x4 (&h)[NS][2][2]) {
+#pragma unroll
+  for (int s = 0; s < NS; ++s) asm volatile("" : "+v"(h[s][0][0]), "+v"(h[s][0][1]), "+v"(h[s][1][0]), "+v"(h[s][1][1])::"memory");
+}
+
+// How the launch divides the work.
+struct SsmGrid {
+  int64_t seg = 0;      // rows per segment, a multiple of 64
+  int64_t slots = 0;    // segments of all sequences (packed: at most)
+  int ps = 0, sg = 0;   // slices per head, per group
+  int wpg = 0;          // workgroups per group
+  int nh = 0;           // heads per workgroup, at most
+  float* carry = nullptr;  // (slots, G * wpg, kCols * 32 NS): a segment's end state, in accumulator order
+  float* decay = nullptr;  // (slots, H): the product of its decays
+};
+
+struct Segment {  // uniform over the workgroup, in scalar registers
+  int seq, k, r0, r1;  // sequence, its k-th segment, rows
+  bool last, valid;
+};
+
+__device__ __forceinline__ int64_t segments_of(int64_t len, int64_t seg) { return len <= seg ? 1 : (len + seg - 1) / seg; }
+
+// Segment `slot`, counted through the sequences; every sequence has one at least.
+__device__ __forceinline__ Segment find_segment(const SsmArgs& a, const SsmGrid& gr, int slot) {
+  Segment s;
+  int64_t first, end;
+  int seq = 0, k = 0;
+  bool valid = true;
+  if (!a.seq_starts) {
+    const int n = static_cast<int>(segments_of(a.L, gr.seg));
+    seq = slot / n;
+    k = slot - seq * n;
+    first = seq * a.L;
+    end = first + a.L;
+  } else {
+    const int lane = threadIdx.x & 63;
+    const int64_t M = a.B * a.L;
+    int before = 0;
+    valid = false;
+    for (int base = 0; base < static_cast<int>(a.S) && !valid; base += 64) {
+      int n = 0;
+      if (base + lane < a.S) {
+        seq_rows(a.seq_starts, base + lane, M, first, end);
+        n = static_cast<int>(segments_of(end - first, gr.seg));
+      }
+      int upto = n;
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+      }
+      const uint64_t past = __ballot(before + upto > slot);
+      if (past) {
+        const int l = __ffsll(static_cast<long long>(past)) - 1;
+        seq = base + l;
+        k = slot - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
+        valid = true;
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    if (valid)
+      seq_rows(a.seq_starts, seq, M, first, end);
+    else
+      first = end = 0;
+  }
+  s.valid = valid;
+  s.seq = __builtin_amdgcn_readfirstlane(seq);
+  s.k = __builtin_amdgcn_readfirstlane(k);
+  const int64_t r0 = first + k * gr.seg, r1 = r0 + gr.seg < end ? r0 + gr.seg : end;
+  s.r0 = __builtin_amdgcn_readfirstlane(static_cast<int>(r0));
+  s.r1 = __builtin_amdgcn_readfirstlane(static_cast<int>(r1));
+  s.last = s.r1 >= __builtin_amdgcn_readfirstlane(static_cast<int>(end));
+  return s;
+}
+
+// EV elements of a row from column `col` of `count`, zeros past its end.
+template <int DT>
+__device__ __forceinline__ uint4 load_unit(const void* p, int64_t at, int col, int count) {
+  using TT = Tile<DT>;
+  using E = typename TT::E;
+  const E* q = static_cast<const E*>(p) + at + col;
+  E v[TT::EV];
+#pragma unroll
+  for (int i = 0; i < TT::EV; ++i) v[i] = col + i < count ? q[i] : E(0);
+  uint4 o;
+  __builtin_memcpy(&o, v, 16);
+  return o;
+}
+
+__device__ __forceinline__ double readlane_d(double v, int l) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), l);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), l);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Inclusive sums over the wave's lanes: shifts inside rows of 16 lanes, then the totals of the rows before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROWS, 0xF, false);
+  return v + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_scan_d(double v) {
+  v = dpp_add<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);  // lane 15 of the row before, to rows 1 and 3
+  return dpp_add<0x143, 0xC>(v);  // lane 31, to rows 2 and 3
+}
+
+template <int DT, int NS>
+struct SsmLds {
+  using TT = Tile<DT>;
+  static constexpr int XP = kCols + TT::PAD, NP = 32 * NS + TT::PAD, WP = TT::Q + TT::PAD;
+  static constexpr int kSmall = 6 * TT::Q;  // per head: c high, c low, d, exp(c_Q - c) d, exp(c), spare
+  static constexpr int64_t bytes(int nh, bool full) {
+    const int64_t e = sizeof(typename TT::E);
+    return TT::Q * (XP + (full ? 2 : 1) * NP) * e + (full ? nh * TT::Q * WP * e : 0) + (nh * kSmall + 4) * 4;
+  }
+};
+
+// FULL: y and the final state of a segment from its carried-in state; otherwise the segment's end state from zero.
+// VEC: whole 32-column slices and 32-state steps in 16-byte vectors, and 32-bit offsets inside a chunk.
+template <int DT, int NS, bool FULL, bool VEC>
+__global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs a, SsmGrid gr) {
+  using TT = Tile<DT>;
+  using E = typename TT::E;
+  using Frag = typename TT::Frag;
+  using Lds = SsmLds<DT, NS>;
+  constexpr int Q = TT::Q, EV = TT::EV, XP = Lds::XP, NP = Lds::NP, WP = Lds::WP;
+  constexpr int UX = kCols / EV, UB = 32 * NS / EV;  // 16-byte units per row
+  constexpr int KS = Q / 32, IT = Q / 16;
+  extern __shared__ __attribute__((aligned(16))) char lds_s[];
+  E* X = reinterpret_cast<E*>(lds_s);
+  E* Bs = X + Q * XP;
+  E* Cs = Bs + Q * NP;
+  E* Ws = FULL ? Cs + Q * NP : Cs;
+  float* small = reinterpret_cast<float*>(Ws + (FULL ? gr.nh * Q * WP : 0));
+  float* tots = small + gr.nh * Lds::kSmall;  // exp(c_Q) per head
+
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Segment sg = find_segment(a, gr, blockIdx.y);
+  if (!sg.valid || (!FULL && sg.last)) return;
+  const int grp = blockIdx.x / gr.wpg, wgi = blockIdx.x % gr.wpg;
+  const int hg = static_cast<int>(a.H / a.G);
+  const int N = static_cast<int>(a.N), P = static_cast<int>(a.P);
+  // this wave's slice, and the heads of the workgroup
+  const int sl = wgi * 4 + wave, head0 = wgi * 4 / gr.ps;  // within the group
+  const bool active = sl < gr.sg;
+  const int last_sl = min(wgi * 4 + 3, gr.sg - 1), nh = last_sl / gr.ps - head0 + 1;
+  const int hh = active ? sl / gr.ps - head0 : 0, head = grp * hg + head0 + hh, p0 = (sl % gr.ps) * 32;
+  // this thread's column of x and of B and C
+  const int xc = (tid % UX) * EV, xsl = wgi * 4 + xc / 32, xhead = xsl / gr.ps, xp = (xsl % gr.ps) * 32 + xc % 32;
+  const int64_t xat = static_cast<int64_t>(grp * hg + xhead) * P;
+  const bool xok = xsl < gr.sg;
+  const int bc = (tid % UB) * EV;
+
+  // state: tile (s, T2) of rows n = 32 s + 8 (m / 4) + 4 T2 + m % 4, tile T of columns p0 + 8 (m / 4) + 4 T + m % 4;
+  // this lane: states 32 s + 8 g + 4 T2 .. + 3 of column p0 + 8 (m / 4) + 4 T + m % 4
+  f32x4 h[NS][2][2];
+  const int64_t frags = static_cast<int64_t>(NS) * 4 * 64;  // vectors of 4 per wave
+  const int64_t wg_all = static_cast<int64_t>(gr.wpg) * a.G;
+  const f32x4* carry_in = nullptr;
+  if (FULL && sg.k > 0)
+    carry_in = reinterpret_cast<const f32x4*>(gr.carry) + (((blockIdx.y - 1) * wg_all + blockIdx.x) * 4 + wave) * frags;
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+      for (int T = 0; T < 2; ++T) {
+        h[s][t2][T] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (!FULL || !active) continue;
+        if (carry_in) {
+          h[s][t2][T] = carry_in[((s * 2 + t2) * 2 + T) * 64 + lane];
+        } else if (a.h0) {
+          const int p = p0 + 8 * (m >> 2) + 4 * T + (m & 3), n = 32 * s + 8 * g + 4 * t2;
+          const float* src = a.h0 + (static_cast<int64_t>(sg.seq) * a.H + head) * P * N + p * N + n;
+          if constexpr (VEC) {
+            h[s][t2][T] = *reinterpret_cast<const f32x4*>(src);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (p < P && n + r < N) h[s][t2][T][r] = src[r];
+          }
+        }
+      }
+
+  if constexpr (FULL) {  // the blocks of W above the diagonal that a 32-wide step reads: zero throughout
+    for (int e = tid; e < nh * IT / 2 * 16 * 16; e += 256) {
+      const int j = e & 15, i = (e >> 4) & 15, b = (e >> 8) % (IT / 2), w = (e >> 8) / (IT / 2);
+      Ws[(w * Q + 32 * b + i) * WP + 32 * b + 16 + j] = E(0);
+    }
+  }
+
+  uint4 xr[4], br[NS], cr[FULL ? NS : 1];
+  uint32_t dtr = 0;  // bits of dt, converted where it is used
+  const int64_t es = sizeof(E), gn = static_cast<int64_t>(grp) * N;
+  // One chunk's units ahead of their use.  VEC: uniform bases and 32-bit offsets; rows past the end read the last one
+  // and are cleared when staged.
+  auto load_bc = [&](const void* p, int64_t ld, int row0, auto& u) {
+    const int left = sg.r1 - row0;  // rows of the chunk that exist
+    const char* base = static_cast<const char*>(p) + (row0 * ld + gn) * es;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int r = tid / UB + i * (256 / UB);
+      if constexpr (VEC) {
+        u[i] = *reinterpret_cast<const uint4*>(base + (static_cast<uint32_t>(min(r, left - 1)) * static_cast<uint32_t>(ld * es) +
+                                                       static_cast<uint32_t>(bc * es)));
+      } else {
+        u[i] = make_uint4(0, 0, 0, 0);
+        if (r < left && bc < N) u[i] = load_unit<DT>(p, (row0 + r) * ld + gn, bc, N);
+      }
+    }
+  };
+  auto load_chunk = [&](int row0) {  // x, B and dt
+    const int left = sg.r1 - row0;
+    const char* base = static_cast<const char*>(a.x) + row0 * a.ld_x * es;
+    const uint32_t xo = static_cast<uint32_t>((xok ? xat + xp : 0) * es);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = tid / UX + i * (256 / UX);
+      if constexpr (VEC) {
+        xr[i] = *reinterpret_cast<const uint4*>(base + (static_cast<uint32_t>(min(r, left - 1)) * static_cast<uint32_t>(a.ld_x * es) + xo));
+      } else {
+        xr[i] = make_uint4(0, 0, 0, 0);
+        if (xok && r < left && xp < P) xr[i] = load_unit<DT>(a.x, (row0 + r) * a.ld_x + xat, xp, P);
+      }
+    }
+    load_bc(a.Bm, a.ld_b, row0, br);
+    if (wave < nh) {
+      const int r = min(lane, left - 1);
+      dtr = ld_bits<DT>(a.dts, (row0 + r) * a.ld_dt + grp * hg + head0 + wave);
+    }
+  };
+
+  float decay = 1.0f;  // of the segment so far (this wave's head)
+  const float Aw = wave < nh ? a.A[grp * hg + head0 + wave] : 0.0f;
+  const float bias = wave < nh && a.dt_bias ? a.dt_bias[grp * hg + head0 + wave] : 0.0f;
+  const float skip = FULL && a.D && active ? a.D[head] : 0.0f;
+  if (sg.r0 < sg.r1) {
+    load_chunk(sg.r0);
+    if constexpr (FULL) load_bc(a.Cm, a.ld_c, sg.r0, cr);
+  }
+  for (int row0 = sg.r0; row0 < sg.r1; row0 += Q) {
+    const int left = sg.r1 - row0;
+    if (VEC && left < Q) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (tid / UX + i * (256 / UX) >= left) xr[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        if (tid / UB + i * (256 / UB) >= left) {
+          br[i] = make_uint4(0, 0, 0, 0);
+          if constexpr (FULL) cr[i] = make_uint4(0, 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(X + (tid / UX + i * (256 / UX)) * XP + xc) = xr[i];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      *reinterpret_cast<uint4*>(Bs + (tid / UB + i * (256 / UB)) * NP + bc) = br[i];
+      if constexpr (FULL) *reinterpret_cast<uint4*>(Cs + (tid / UB + i * (256 / UB)) * NP + bc) = cr[i];
+    }
+    if (wave < nh) {  // this wave's head: d and the sums c, in units of log 2, 64 bits split into two floats
+      const float raw = from_bits<DT>(dtr) + bias;
+      const float d = lane < left && lane < Q ? (a.softplus ? softplusf_(raw) : raw) : 0.0f;
+      const double c = wave_scan_d(static_cast<double>(d) * static_cast<double>(Aw) * 1.4426950408889634074);
+      const double all = readlane_d(c, Q - 1);
+      float* sm = small + wave * Lds::kSmall;
+      if (lane < Q) {
+        const float hi = static_cast<float>(c), lo = static_cast<float>(c - static_cast<double>(hi));
+        sm[lane] = hi;
+        sm[Q + lane] = lo;
+        sm[2 * Q + lane] = d;
+        sm[3 * Q + lane] = __builtin_amdgcn_exp2f(static_cast<float>(all - c)) * d;
+        sm[4 * Q + lane] = __builtin_amdgcn_exp2f(hi);
+      }
+      if (lane == 0) tots[wave] = __builtin_amdgcn_exp2f(static_cast<float>(all));
+    }
+    __syncthreads();
+    if (row0 + Q < sg.r1) load_chunk(row0 + Q);
+
+    const float* sm = small + hh * Lds::kSmall;
+    Frag xf[2][KS];  // x of this wave's columns, 8 rows of a column per lane
+    auto read_x = [&]() {
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          xf[T][ks] = TT::column(X + 32 * ks * XP + 32 * wave + TT::tr_at(g, m, T, XP), XP);
+    };
+    if constexpr (FULL) {
+      // scores, tile (it, jt) of the lower triangle, dealt over the waves; W of every head of the workgroup
+      for (int e = wave; e < IT * (IT + 1) / 2; e += 4) {
+        int it = 0;
+        while ((it + 1) * (it + 2) / 2 <= e) ++it;
+        const int jt = e - it * (it + 1) / 2;
+        f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < NS; ++k)
+          s = TT::mma(TT::row(Bs + (16 * jt + m) * NP + 32 * k + 8 * g), TT::row(Cs + (16 * it + m) * NP + 32 * k + 8 * g), s);
+        const int i = 16 * it + m, j0 = 16 * jt + 4 * g;
+        for (int w = 0; w < nh; ++w) {
+          const float* sw = small + w * Lds::kSmall;
+          const float hi = sw[i], lo = sw[Q + i];
+          const f32x4 hj = *reinterpret_cast<const f32x4*>(sw + j0), lj = *reinterpret_cast<const f32x4*>(sw + Q + j0);
+          const f32x4 dj = *reinterpret_cast<const f32x4*>(sw + 2 * Q + j0);
+          f32x4 v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float x = (hi - hj[r]) + (lo - lj[r]);
+            v[r] = j0 + r <= i ? s[r] * __builtin_amdgcn_exp2f(x) * dj[r] : 0.0f;
+          }
+          TT::store4(Ws + (w * Q + i) * WP + j0, v);
+        }
+      }
+    }
+    if (active) read_x();
+    if constexpr (FULL) {
+      __syncthreads();
+      if (active) {
+        const int64_t hp = static_cast<int64_t>(head) * P;
+        const int pc = p0 + 8 * g;  // this lane's outputs: columns pc .. + 7 of rows 16 it + m
+        const char* zb = static_cast<const char*>(a.z) + (row0 * a.ld_z + hp + p0) * es;
+        char* yb = static_cast<char*>(a.y) + (row0 * a.ld_y + hp + p0) * es;
+#pragma unroll
+        for (int hf = 0; hf < IT / 2; ++hf) {  // 32 rows at a time, for the registers
+          f32x4 y[2][2];
+          uint4 zr[2][8 / EV];
+          if (VEC && a.z) {  // the gate, ahead of its use
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const uint32_t r = min(32 * hf + 16 * q + m, left - 1);
+              const uint4* src = reinterpret_cast<const uint4*>(
+                  zb + (r * static_cast<uint32_t>(a.ld_z * es) + 8 * g * static_cast<uint32_t>(es)));
+#pragma unroll
+              for (int k = 0; k < 8 / EV; ++k) zr[q][k] = src[k];
+            }
+          }
+          // exp(c_i) C_i . h (bfloat16 operands: h is rounded here, once, for the product)
+          auto across = [&]() {
+            anew(h);
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+              for (int T = 0; T < 2; ++T) y[q][T] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+              const Frag h0 = TT::pack(h[s][0][0], h[s][1][0]), h1 = TT::pack(h[s][0][1], h[s][1][1]);
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const Frag c = TT::row(Cs + (32 * hf + 16 * q + m) * NP + 32 * s + 8 * g);
+                y[q][0] = TT::mma(h0, c, y[q][0]);
+                y[q][1] = TT::mma(h1, c, y[q][1]);
+              }
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const float e = sm[4 * Q + 32 * hf + 16 * q + m];
+              y[q][0] *= e;
+              y[q][1] *= e;
+            }
+          };
+          across();
+          // + W x over the rows up to each
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int ks = 0; ks <= hf; ++ks) {
+              const Frag w = TT::row(Ws + (hh * Q + 32 * hf + 16 * q + m) * WP + 32 * ks + 8 * g);
+              y[q][0] = TT::mma(xf[0][ks], w, y[q][0]);
+              y[q][1] = TT::mma(xf[1][ks], w, y[q][1]);
+            }
+          // An infinite or NaN x must not reach the rows before it through a weight 0.  Rows with one near have sums
+          // that are not finite: they are formed again without such values, which are then added from their row on.
+          bool odd = false;
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int T = 0; T < 2; ++T)
+              odd |= !(fabsf(y[q][T][0]) + fabsf(y[q][T][1]) + fabsf(y[q][T][2]) + fabsf(y[q][T][3]) < __builtin_inff());
+          if (__any(odd)) {
+            across();
+#pragma unroll
+            for (int ks = 0; ks <= hf; ++ks)
+#pragma unroll
+              for (int T = 0; T < 2; ++T) {
+                float v[8];
+                TT::unpack(TT::column(X + 32 * ks * XP + 32 * wave + TT::tr_at(g, m, T, XP), XP), v);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) v[r] = fabsf(v[r]) < __builtin_inff() ? v[r] : 0.0f;
+                const Frag f = TT::pack(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                  y[q][T] = TT::mma(f, TT::row(Ws + (hh * Q + 32 * hf + 16 * q + m) * WP + 32 * ks + 8 * g), y[q][T]);
+              }
+#pragma unroll 1
+            for (int j = 0; j < 32 * hf + 32; ++j)
+#pragma unroll 1
+              for (int c = 0; c < 8; ++c) {
+                const float x = ld<DT>(X, j * XP + 32 * wave + 8 * g + c);
+                if (fabsf(x) < __builtin_inff()) continue;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  const int i = 32 * hf + 16 * q + m;
+                  const float add = j <= i ? ld<DT>(Ws, (hh * Q + i) * WP + j) * x : 0.0f;
+#pragma unroll
+                  for (int r = 0; r < 8; ++r)
+                    if (r == c) y[q][r >> 2][r & 3] += add;
+                }
+              }
+          }
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int i = 32 * hf + 16 * q + m;
+            if (i >= left || pc >= P) continue;
+            float v[8], x[8];
+            TT::unpack(TT::row(X + i * XP + 32 * wave + 8 * g), x);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] = y[q][r >> 2][r & 3] + (a.D ? skip * x[r] : 0.0f);
+            if (a.z) {
+              float z[8];
+              uint4 u[8 / EV];
+#pragma unroll
+              for (int k = 0; k < 8 / EV; ++k) {
+                if constexpr (VEC) {
+                  u[k] = zr[q][k];
+                } else {
+                  u[k] = make_uint4(0, 0, 0, 0);
+                  if (pc + k * EV < P) u[k] = load_unit<DT>(a.z, (row0 + i) * a.ld_z + hp, pc + k * EV, P);
+                }
+              }
+              TT::unpack(__builtin_bit_cast(Frag, u), z);
+#pragma unroll
+              for (int r = 0; r < 8; ++r) v[r] *= siluf_(z[r]);
+            }
+            if constexpr (VEC) {
+              *reinterpret_cast<Frag*>(yb + (static_cast<uint32_t>(i) * static_cast<uint32_t>(a.ld_y * es) +
+                                             8 * g * static_cast<uint32_t>(es))) =
+                  TT::pack(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
+            } else {
+              E* dst = static_cast<E*>(a.y) + (row0 + i) * a.ld_y + hp + pc;
+#pragma unroll
+              for (int r = 0; r < 8; ++r)
+                if (pc + r < P) st<DT>(dst, r, v[r]);
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    if constexpr (FULL)
+      if (row0 + Q < sg.r1) load_bc(a.Cm, a.ld_c, row0 + Q, cr);  // (earlier, the sums of y are in the way)
+    if (active) {  // the state
+      const float tot = tots[hh];
+      decay *= tot;
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+          for (int T = 0; T < 2; ++T) h[s][t2][T] *= tot;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const f32x4 w0 = *reinterpret_cast<const f32x4*>(sm + 3 * Q + 32 * ks + 8 * g);
+        const f32x4 w1 = *reinterpret_cast<const f32x4*>(sm + 3 * Q + 32 * ks + 8 * g + 4);
+        // w x: float32, or as two bfloat16 halves (2^-17 relative), each a product of its own
+        Frag hi[2], lo[2];
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          float v[8];
+          TT::unpack(xf[T][ks], v);
+          f32x4 v0, v1;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v0[r] = v[r] * w0[r], v1[r] = v[4 + r] * w1[r];
+          hi[T] = TT::pack(v0, v1);
+          if constexpr (DT == kBF16) {
+            TT::unpack(hi[T], v);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {  // (nothing is left of an infinity)
+              v0[r] = fabsf(v[r]) < __builtin_inff() ? v0[r] - v[r] : 0.0f;
+              v1[r] = fabsf(v[4 + r]) < __builtin_inff() ? v1[r] - v[4 + r] : 0.0f;
+            }
+            lo[T] = TT::pack(v0, v1);
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int t2 = 0; t2 < 2; ++t2) {
+            const Frag b = TT::column(Bs + 32 * ks * NP + 32 * s + TT::tr_at(g, m, t2, NP), NP);
+#pragma unroll
+            for (int T = 0; T < 2; ++T) {
+              h[s][t2][T] = TT::mma(b, hi[T], h[s][t2][T]);
+              if constexpr (DT == kBF16) h[s][t2][T] = TT::mma(b, lo[T], h[s][t2][T]);
+            }
+            if (t2) __builtin_amdgcn_sched_barrier(0);
+          }
+      }
+    }
+    __syncthreads();
+  }
+
+  if (!active) return;
+  if constexpr (!FULL) {
+    f32x4* out = reinterpret_cast<f32x4*>(gr.carry) + ((blockIdx.y * wg_all + blockIdx.x) * 4 + wave) * frags;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+        for (int T = 0; T < 2; ++T) out[((s * 2 + t2) * 2 + T) * 64 + lane] = h[s][t2][T];
+    if (lane == 0) gr.decay[blockIdx.y * a.H + head] = decay;  // (slices of one head write the same value)
+  } else if (sg.last && a.h_out) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          const int p = p0 + 8 * (m >> 2) + 4 * T + (m & 3), n = 32 * s + 8 * g + 4 * t2;
+          float* dst = a.h_out + (static_cast<int64_t>(sg.seq) * a.H + head) * P * N + p * N + n;
+          if constexpr (VEC) {
+            *reinterpret_cast<f32x4*>(dst) = h[s][t2][T];
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (p < P && n + r < N) dst[r] = h[s][t2][T][r];
+          }
+        }
+  }
+}
+
+// The segments' end states from zero become the states at their ends: a sequence's are folded in order, one vector of
+// 4 states per thread.
+template <int NS>
+__global__ __launch_bounds__(256) void ssm_carry_kernel(SsmArgs a, SsmGrid gr) {
+  constexpr int VW = NS * 4 * 64;  // vectors per wave
+  const int64_t wg_all = static_cast<int64_t>(gr.wpg) * a.G;
+  const int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;  // vector of a slot
+  const int64_t wg = u / (4 * VW);
+  const int wave = static_cast<int>(u / VW % 4), v = static_cast<int>(u % VW);
+  const int grp = static_cast<int>(wg / gr.wpg), sl = static_cast<int>(wg % gr.wpg) * 4 + wave;
+  int64_t slot = 0, nseg;
+  if (!a.seq_starts) {
+    nseg = segments_of(a.L, gr.seg);
+    slot = blockIdx.y * nseg;
+  } else {
+    int64_t first, end;
+    for (int64_t s = threadIdx.x & 63; s < static_cast<int64_t>(blockIdx.y); s += 64) {
+      seq_rows(a.seq_starts, s, a.B * a.L, first, end);
+      slot += segments_of(end - first, gr.seg);
+    }
+    for (int d = 32; d > 0; d >>= 1) slot += __shfl_xor(static_cast<long long>(slot), d);
+    seq_rows(a.seq_starts, blockIdx.y, a.B * a.L, first, end);
+    nseg = segments_of(end - first, gr.seg);
+  }
+  if (sl >= gr.sg || nseg < 2) return;
+  const int hg = static_cast<int>(a.H / a.G), head = grp * hg + sl / gr.ps;
+  const int lane = v & 63, m = lane & 15, g = lane >> 4, T = (v >> 6) & 1, t2 = (v >> 7) & 1, s = v >> 8;
+  f32x4 h = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int64_t p = (sl % gr.ps) * 32 + 8 * (m >> 2) + 4 * T + (m & 3), n = 32 * s + 8 * g + 4 * t2;
+  if (a.h0 && p < a.P) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < a.N) h[r] = a.h0[((blockIdx.y * a.H + head) * a.P + p) * a.N + n + r];
+  }
+  f32x4* c = reinterpret_cast<f32x4*>(gr.carry) + (slot * wg_all + wg) * 4 * VW + wave * VW + v;
+  const float* dec = gr.decay + slot * a.H + head;
+  for (int64_t k = 0; k + 1 < nseg; ++k) {
+    h = h * dec[k * a.H] + c[k * wg_all * 4 * VW];
+    c[k * wg_all * 4 * VW] = h;
+  }
 }
 
 // Convolved value of channel c of the token; the state moves on where `keep`.
@@ -103,9 +742,60 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepArgs a) {
 
 }  // namespace
 
-int64_t selective_scan_ws_bytes(const SsmArgs&) { return 0; }
+namespace {
 
-int launch_selective_scan(const SsmArgs& a, void*, int64_t, hipStream_t st) {
+int states32(const SsmArgs& a) {  // 32-state steps, rounded up to an instantiation
+  const int n = static_cast<int>((a.N + 31) / 32);
+  return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8;
+}
+
+// Segments so that about one workgroup per CU runs; a segment's end state costs as much traffic as about 85 of its
+// rows, so it has several times that.
+SsmGrid ssm_grid(const SsmArgs& a) {
+  SsmGrid g;
+  const int64_t hg = a.H / a.G;
+  g.ps = static_cast<int>((a.P + 31) / 32);
+  g.sg = static_cast<int>(hg * g.ps);
+  g.wpg = (g.sg + 3) / 4;
+  g.nh = 4 % g.ps == 0 ? 4 / g.ps : g.ps % 4 == 0 ? 1 : 2;
+  const int64_t wgs = a.G * g.wpg, rows = a.seq_starts ? a.B * a.L : a.L;
+  const int64_t each = a.seq_starts ? 1 : std::max<int64_t>(a.S, 1);
+  const int64_t want = std::max<int64_t>(1, 256 / std::max<int64_t>(1, wgs * each));
+  g.seg = std::max<int64_t>(kMinSegment, round_up((rows + want - 1) / want, 64));
+  if (a.seq_starts)
+    g.slots = rows / g.seg + a.S;
+  else
+    g.slots = a.S * std::max<int64_t>(1, (a.L + g.seg - 1) / g.seg);
+  return g;
+}
+
+bool ssm_split(const SsmArgs& a, const SsmGrid& g) { return (a.seq_starts ? a.B * a.L : a.L) > g.seg; }
+
+template <int DT, int NS, bool VEC>
+int run_ssm(const SsmArgs& a, const SsmGrid& g, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(a.G * g.wpg), static_cast<unsigned>(g.slots));
+  if (ssm_split(a, g)) {
+    const unsigned part = static_cast<unsigned>(SsmLds<DT, NS>::bytes(g.nh, false));
+    ssm_chunk_kernel<DT, NS, false, VEC><<<grid, 256, part, TESM_LOGGED(st, ssm_chunk_kernel<DT, NS, false, VEC>)>>>(a, g);
+    const dim3 cg(static_cast<unsigned>(a.G * g.wpg * NS * 4), static_cast<unsigned>(a.S));
+    ssm_carry_kernel<NS><<<cg, 256, 0, TESM_LOGGED(st, ssm_carry_kernel<NS>)>>>(a, g);
+  }
+  const unsigned full = static_cast<unsigned>(SsmLds<DT, NS>::bytes(g.nh, true));
+  ssm_chunk_kernel<DT, NS, true, VEC><<<grid, 256, full, TESM_LOGGED(st, ssm_chunk_kernel<DT, NS, true, VEC>)>>>(a, g);
+  return check_launch("selective scan");
+}
+
+template <int DT, bool VEC>
+int run_ssm_dt(const SsmArgs& a, const SsmGrid& g, hipStream_t st) {
+  switch (states32(a)) {
+    case 1: return run_ssm<DT, 1, VEC>(a, g, st);
+    case 2: return run_ssm<DT, 2, VEC>(a, g, st);
+    case 4: return run_ssm<DT, 4, VEC>(a, g, st);
+    default: return run_ssm<DT, 8, VEC>(a, g, st);
+  }
+}
+
+int ssm_check(const SsmArgs& a) {
   TESM_REQUIRE(a.dt == kF32 || a.dt == kBF16, kErrInvalidArg, "selective scan: dtype must be 0 or 1");
   TESM_REQUIRE(a.B >= 0 && a.L >= 0 && a.S >= 0 && a.H >= 1 && a.P >= 1 && a.G >= 1 && a.N >= 1 && a.H % a.G == 0 &&
                    a.B < (1LL << 31) && a.L < (1LL << 31) && a.B * a.L < (1LL << 31) && a.S < (1LL << 24) &&
@@ -114,20 +804,41 @@ int launch_selective_scan(const SsmArgs& a, void*, int64_t, hipStream_t st) {
   TESM_REQUIRE(a.N <= kSsmMaxN, kErrUnsupported, "selective scan: need at most 256 states");
   TESM_REQUIRE(a.seq_starts ? a.B == 1 : a.S == a.B, kErrInvalidArg,
                "selective scan: packed sequences lie in one row axis (B = 1), others have S = B");
+  return kOk;
+}
+
+}  // namespace
+
+int64_t selective_scan_ws_bytes(const SsmArgs& a) {
+  if (ssm_check(a) != kOk) return -1;
+  const SsmGrid g = ssm_grid(a);
+  if (!ssm_split(a, g)) return 0;
+  return round_up(g.slots * a.G * g.wpg * kCols * 32 * states32(a) * 4, 256) + round_up(g.slots * a.H * 4, 256);
+}
+
+int launch_selective_scan(const SsmArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+  if (int rc = ssm_check(a)) return rc;
   TESM_REQUIRE(a.A && (a.B * a.L == 0 || (a.x && a.dts && a.Bm && a.Cm && a.y)), kErrInvalidArg,
                "selective scan: need x, dt, A, B, C and y");
   TESM_REQUIRE(a.ld_x >= a.H * a.P && a.ld_y >= a.H * a.P && a.ld_dt >= a.H && a.ld_b >= a.G * a.N &&
                    a.ld_c >= a.G * a.N && (!a.z || a.ld_z >= a.H * a.P),
                kErrInvalidArg, "selective scan: a row pitch is shorter than its row");
   TESM_REQUIRE(!a.h_out || a.h_out != a.h0, kErrInvalidArg, "selective scan: the states out need a buffer of their own");
-  TESM_REQUIRE(a.S * a.H * a.P < (1LL << 32), kErrUnsupported, "selective scan: too many states");
   if (a.S == 0) return kOk;
-  const unsigned grid = static_cast<unsigned>((a.S * a.H * a.P + 3) / 4);
-  if (a.dt == kBF16)
-    ssm_rows_kernel<kBF16><<<grid, 256, 0, TESM_LOGGED(st, ssm_rows_kernel<kBF16>)>>>(a);
-  else
-    ssm_rows_kernel<kF32><<<grid, 256, 0, TESM_LOGGED(st, ssm_rows_kernel<kF32>)>>>(a);
-  return check_launch("selective scan");
+  SsmGrid g = ssm_grid(a);
+  TESM_REQUIRE(g.slots < 65536, kErrUnsupported, "selective scan: too many sequences");
+  if (ssm_split(a, g)) {
+    TESM_REQUIRE(ws && ws_bytes >= selective_scan_ws_bytes(a) && aligned(ws, 16), kErrWorkspace,
+                 "selective scan: workspace too small or not 16-byte aligned");
+    g.carry = static_cast<float*>(ws);
+    g.decay = g.carry + round_up(g.slots * a.G * g.wpg * kCols * 32 * states32(a) * 4, 256) / 4;
+  }
+  const int64_t es = a.dt == kBF16 ? 2 : 4;
+  const auto vec = [&](const void* p, int64_t ld) { return aligned(p, 16) && ld * es % 16 == 0 && ld < (1LL << 23); };
+  const bool v = aligned(a.h0, 16) && aligned(a.h_out, 16) && a.P % 32 == 0 && a.N == 32 * states32(a) && vec(a.x, a.ld_x) && vec(a.Bm, a.ld_b) && vec(a.Cm, a.ld_c) &&
+                 (!a.z || vec(a.z, a.ld_z)) && vec(a.y, a.ld_y);
+  if (a.dt == kBF16) return v ? run_ssm_dt<kBF16, true>(a, g, st) : run_ssm_dt<kBF16, false>(a, g, st);
+  return v ? run_ssm_dt<kF32, true>(a, g, st) : run_ssm_dt<kF32, false>(a, g, st);
 }
 
 int launch_selective_scan_step(const SsmStepArgs& a, hipStream_t st) {
