@@ -2,6 +2,7 @@
 //   d_t = softplus(dt_t + dt_bias)        a_t = exp(d_t A)
 //   h_t = a_t h_{t-1} + d_t x_t B_t^T     (P x N, float32)
 //   y_t = h_t C_t + D x_t                 times silu(z_t) where there is a gate
+#include <cstdlib>
 #include "ssm.h"
 
 namespace tesm {
@@ -10,6 +11,13 @@ namespace {
 
 __device__ __forceinline__ float softplusf_(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
 __device__ __forceinline__ float siluf_(float v) { return v * sigmoidf_(v); }
+
+// silu for a bfloat16 result: the exponent's rounding (2^-24 |v| log2 e) is far below the result's, so it is taken as it is.
+template <int DT>
+__device__ __forceinline__ float gatef_(float v) {
+  if constexpr (DT == kF32) return siluf_(v);
+  return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
+}
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
@@ -39,23 +47,39 @@ template <>
 struct Tile<kBF16> {
   using E = uint16_t;
   static constexpr int Q = 64, EV = 8, PAD = 8;
+  // Rows of U 16-byte units (4, 8, 16 or 32) lie one behind the other without padding; unit u of row r is kept at
+  // u ^ swz(r).  Then the 8 rows of one unit that a row operand reads at once, and the 4 rows x 4 units of a column
+  // operand, fall on different banks (64 of 4 bytes).
+  template <int U>
+  static __device__ __forceinline__ int swz(int r) {
+    const int block = U >= 16 ? r & 3 : U == 8 ? (r >> 1) & 1 : 0;
+    return block << 2 | ((r >> 2) & 3);
+  }
+  template <int U>
+  static constexpr int pitch() { return U * EV; }
+  template <int U>
+  static __device__ __forceinline__ int unit(int r, int u) { return r * U * EV + (u ^ swz<U>(r)) * EV; }
   using Frag = uint4;  // 8 consecutive k of one row: lane l holds row l & 15, k = 8 (l >> 4) ..
   static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ Frag row(const E* p) { return *reinterpret_cast<const uint4*>(p); }
-  // 8 k from 8 rows of pitch `pitch`; p: the lane's place in the first rows (see tr_at)
-  static __device__ __forceinline__ Frag column(const E* p, int pitch) {
-    const uint2 a = tr(p), b = tr(p + 4 * pitch);
+  // Rows r0 + m (r0 a multiple of 16), columns 32 s + 8 g .. + 7
+  template <int U>
+  static __device__ __forceinline__ Frag rows(const E* p, int r0, int m, int g, int s) {
+    return row(p + r0 * U * EV + unit<U>(m, 4 * s + g));
+  }
+  // Rows r0 + 8 g .. + 7 (r0 a multiple of 16), one column per lane: 32 s + 8 (m / 4) + 4 T + m % 4
+  template <int U>
+  static __device__ __forceinline__ Frag column(const E* p, int r0, int m, int g, int s, int T) {
+    const int r = 8 * g + (m >> 2);  // the lane's place: 4 columns of row m / 4, then of the row 4 below
+    const uint2 a = tr(p + r0 * U * EV + unit<U>(r, 4 * s + (m & 3)) + 4 * T);
+    const uint2 b = tr(p + r0 * U * EV + unit<U>(r + 4, 4 * s + (m & 3)) + 4 * T);
     return make_uint4(a.x, a.y, b.x, b.y);
   }
   static __device__ __forceinline__ uint2 tr(const E* p) {
     const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
     return __builtin_bit_cast(uint2, v);
-  }
-  // Lane's place for column(): rows 8 g .., 4 columns 8 (m % 4) + 4 T of row m / 4
-  static __device__ __forceinline__ int tr_at(int g, int m, int T, int pitch) {
-    return (8 * g + (m >> 2)) * pitch + 8 * (m & 3) + 4 * T;
   }
   static __device__ __forceinline__ Frag pack(const f32x4& lo, const f32x4& hi) {
     return make_uint4(pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
@@ -77,6 +101,10 @@ template <>
 struct Tile<kF32> {
   using E = float;
   static constexpr int Q = 32, EV = 4, PAD = 4;
+  template <int U>
+  static constexpr int pitch() { return U * EV + PAD; }
+  template <int U>
+  static __device__ __forceinline__ int unit(int r, int u) { return r * pitch<U>() + u * EV; }
   struct Frag {
     float v[8];
   };
@@ -89,14 +117,17 @@ struct Tile<kF32> {
     const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
     return Frag{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
   }
-  static __device__ __forceinline__ Frag column(const E* p, int pitch) {
+  template <int U>
+  static __device__ __forceinline__ Frag rows(const E* p, int r0, int m, int g, int s) {
+    return row(p + (r0 + m) * pitch<U>() + 32 * s + 8 * g);
+  }
+  template <int U>
+  static __device__ __forceinline__ Frag column(const E* p, int r0, int m, int g, int s, int T) {
+    const E* q = p + (r0 + 8 * g) * pitch<U>() + 32 * s + 8 * (m >> 2) + 4 * T + (m & 3);
     Frag f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.v[e] = p[e * pitch];
+    for (int e = 0; e < 8; ++e) f.v[e] = q[e * pitch<U>()];
     return f;
-  }
-  static __device__ __forceinline__ int tr_at(int g, int m, int T, int pitch) {
-    return 8 * g * pitch + 8 * (m >> 2) + 4 * T + (m & 3);
   }
   static __device__ __forceinline__ Frag pack(const f32x4& lo, const f32x4& hi) {
     return Frag{{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
@@ -109,6 +140,10 @@ struct Tile<kF32> {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
   }
 };
+
+// Tile e of a lower triangle counted row by row.
+__device__ __forceinline__ int tile_row(int e) { return (0x3333222110ull >> (4 * e)) & 15; }
+__device__ __forceinline__ int tile_col(int e) { return (0x3210210100ull >> (4 * e)) & 15; }
 
 // The compiler is to form what depends on h, and what is read from memory, anew from here on (kept values would have
 // to be spilled).
@@ -229,7 +264,8 @@ __device__ __forceinline__ double wave_scan_d(double v) {
 template <int DT, int NS>
 struct SsmLds {
   using TT = Tile<DT>;
-  static constexpr int XP = kCols + TT::PAD, NP = 32 * NS + TT::PAD, WP = TT::Q + TT::PAD;
+  static constexpr int UX = kCols / TT::EV, UB = 32 * NS / TT::EV;  // 16-byte units per row
+  static constexpr int XP = TT::template pitch<UX>(), NP = TT::template pitch<UB>(), WP = TT::Q + TT::PAD;
   static constexpr int kSmall = 6 * TT::Q;  // per head: c high, c low, d, exp(c_Q - c) d, exp(c), spare
   static constexpr int64_t bytes(int nh, bool full) {
     const int64_t e = sizeof(typename TT::E);
@@ -246,7 +282,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
   using Frag = typename TT::Frag;
   using Lds = SsmLds<DT, NS>;
   constexpr int Q = TT::Q, EV = TT::EV, XP = Lds::XP, NP = Lds::NP, WP = Lds::WP;
-  constexpr int UX = kCols / EV, UB = 32 * NS / EV;  // 16-byte units per row
+  constexpr int UX = Lds::UX, UB = Lds::UB;
   constexpr int KS = Q / 32, IT = Q / 16;
   extern __shared__ __attribute__((aligned(16))) char lds_s[];
   E* X = reinterpret_cast<E*>(lds_s);
@@ -375,11 +411,12 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(X + (tid / UX + i * (256 / UX)) * XP + xc) = xr[i];
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(X + TT::template unit<UX>(tid / UX + i * (256 / UX), tid % UX)) = xr[i];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-      *reinterpret_cast<uint4*>(Bs + (tid / UB + i * (256 / UB)) * NP + bc) = br[i];
-      if constexpr (FULL) *reinterpret_cast<uint4*>(Cs + (tid / UB + i * (256 / UB)) * NP + bc) = cr[i];
+      const int at = TT::template unit<UB>(tid / UB + i * (256 / UB), tid % UB);
+      *reinterpret_cast<uint4*>(Bs + at) = br[i];
+      if constexpr (FULL) *reinterpret_cast<uint4*>(Cs + at) = cr[i];
     }
     if (wave < nh) {  // this wave's head: d and the sums c, in units of log 2, 64 bits split into two floats
       const float raw = from_bits<DT>(dtr) + bias;
@@ -400,6 +437,18 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
     __syncthreads();
     if (row0 + Q < sg.r1) load_chunk(row0 + Q);
 
+    uint4 zr[IT][8 / EV];
+    if (FULL && VEC && a.z && active) {  // the gate of this lane's outputs, ahead of its use
+      const char* zb = static_cast<const char*>(a.z) + (row0 * a.ld_z + static_cast<int64_t>(head) * P + p0) * es;
+#pragma unroll
+      for (int it = 0; it < IT; ++it) {
+        const uint32_t r = min(16 * it + m, left - 1);
+        const uint4* src = reinterpret_cast<const uint4*>(
+            zb + (r * static_cast<uint32_t>(a.ld_z * es) + 8 * g * static_cast<uint32_t>(es)));
+#pragma unroll
+        for (int k = 0; k < 8 / EV; ++k) zr[it][k] = src[k];
+      }
+    }
     const float* sm = small + hh * Lds::kSmall;
     Frag xf[2][KS];  // x of this wave's columns, 8 rows of a column per lane
     auto read_x = [&]() {
@@ -407,29 +456,48 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
       for (int T = 0; T < 2; ++T)
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-          xf[T][ks] = TT::column(X + 32 * ks * XP + 32 * wave + TT::tr_at(g, m, T, XP), XP);
+          xf[T][ks] = TT::template column<UX>(X, 32 * ks, m, g, wave, T);
     };
     if constexpr (FULL) {
       // scores, tile (it, jt) of the lower triangle, dealt over the waves; W of every head of the workgroup
-      for (int e = wave; e < IT * (IT + 1) / 2; e += 4) {
-        int it = 0;
-        while ((it + 1) * (it + 2) / 2 <= e) ++it;
-        const int jt = e - it * (it + 1) / 2;
-        f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+      constexpr int TILES = IT * (IT + 1) / 2, TW = (TILES + 3) / 4;
+      f32x4 sc[TW];
+      int mo = m;
+      asm volatile("" : "+v"(mo));  // addresses formed here, not kept over the loop
+#pragma unroll
+      for (int e = 0; e < TW; ++e) {
+        sc[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (wave + 4 * e >= TILES) continue;
+        const int it = tile_row(wave + 4 * e), jt = tile_col(wave + 4 * e);
 #pragma unroll
         for (int k = 0; k < NS; ++k)
-          s = TT::mma(TT::row(Bs + (16 * jt + m) * NP + 32 * k + 8 * g), TT::row(Cs + (16 * it + m) * NP + 32 * k + 8 * g), s);
-        const int i = 16 * it + m, j0 = 16 * jt + 4 * g;
-        for (int w = 0; w < nh; ++w) {
-          const float* sw = small + w * Lds::kSmall;
-          const float hi = sw[i], lo = sw[Q + i];
-          const f32x4 hj = *reinterpret_cast<const f32x4*>(sw + j0), lj = *reinterpret_cast<const f32x4*>(sw + Q + j0);
-          const f32x4 dj = *reinterpret_cast<const f32x4*>(sw + 2 * Q + j0);
+          sc[e] = TT::mma(TT::template rows<UB>(Bs, 16 * jt, mo, g, k), TT::template rows<UB>(Cs, 16 * it, mo, g, k), sc[e]);
+      }
+      for (int w = 0; w < nh; ++w) {
+        const float* sw = small + w * Lds::kSmall;
+        // the low halves of the sums matter where the sums are large against the result's own rounding
+        const bool low = DT == kF32 || !(__builtin_amdgcn_readfirstlane(__float_as_int(fabsf(sw[Q - 1]))) < __float_as_int(512.0f));
+#pragma unroll
+        for (int e = 0; e < TW; ++e) {
+          if (wave + 4 * e >= TILES) continue;
+          const int i = 16 * tile_row(wave + 4 * e) + m, j0 = 16 * tile_col(wave + 4 * e) + 4 * g;
+          const float hi = sw[i];
+          const f32x4 hj = *reinterpret_cast<const f32x4*>(sw + j0), dj = *reinterpret_cast<const f32x4*>(sw + 2 * Q + j0);
           f32x4 v;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float x = (hi - hj[r]) + (lo - lj[r]);
-            v[r] = j0 + r <= i ? s[r] * __builtin_amdgcn_exp2f(x) * dj[r] : 0.0f;
+          for (int r = 0; r < 4; ++r) v[r] = hi - hj[r];
+          if (low) {
+            const float lo = sw[Q + i];
+            const f32x4 lj = *reinterpret_cast<const f32x4*>(sw + Q + j0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] += lo - lj[r];
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = sc[e][r] * __builtin_amdgcn_exp2f(v[r]) * dj[r];
+          if (tile_row(wave + 4 * e) == tile_col(wave + 4 * e)) {  // on the diagonal
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (j0 + r > i) v[r] = 0.0f;
           }
           TT::store4(Ws + (w * Q + i) * WP + j0, v);
         }
@@ -441,22 +509,10 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
       if (active) {
         const int64_t hp = static_cast<int64_t>(head) * P;
         const int pc = p0 + 8 * g;  // this lane's outputs: columns pc .. + 7 of rows 16 it + m
-        const char* zb = static_cast<const char*>(a.z) + (row0 * a.ld_z + hp + p0) * es;
         char* yb = static_cast<char*>(a.y) + (row0 * a.ld_y + hp + p0) * es;
 #pragma unroll
         for (int hf = 0; hf < IT / 2; ++hf) {  // 32 rows at a time, for the registers
           f32x4 y[2][2];
-          uint4 zr[2][8 / EV];
-          if (VEC && a.z) {  // the gate, ahead of its use
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const uint32_t r = min(32 * hf + 16 * q + m, left - 1);
-              const uint4* src = reinterpret_cast<const uint4*>(
-                  zb + (r * static_cast<uint32_t>(a.ld_z * es) + 8 * g * static_cast<uint32_t>(es)));
-#pragma unroll
-              for (int k = 0; k < 8 / EV; ++k) zr[q][k] = src[k];
-            }
-          }
           // exp(c_i) C_i . h (bfloat16 operands: h is rounded here, once, for the product)
           auto across = [&]() {
             anew(h);
@@ -469,7 +525,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
               const Frag h0 = TT::pack(h[s][0][0], h[s][1][0]), h1 = TT::pack(h[s][0][1], h[s][1][1]);
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
-                const Frag c = TT::row(Cs + (32 * hf + 16 * q + m) * NP + 32 * s + 8 * g);
+                const Frag c = TT::template rows<UB>(Cs, 32 * hf + 16 * q, m, g, s);
                 y[q][0] = TT::mma(h0, c, y[q][0]);
                 y[q][1] = TT::mma(h1, c, y[q][1]);
               }
@@ -506,7 +562,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
 #pragma unroll
               for (int T = 0; T < 2; ++T) {
                 float v[8];
-                TT::unpack(TT::column(X + 32 * ks * XP + 32 * wave + TT::tr_at(g, m, T, XP), XP), v);
+                TT::unpack(TT::template column<UX>(X, 32 * ks, m, g, wave, T), v);
 #pragma unroll
                 for (int r = 0; r < 8; ++r) v[r] = fabsf(v[r]) < __builtin_inff() ? v[r] : 0.0f;
                 const Frag f = TT::pack(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
@@ -518,7 +574,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
             for (int j = 0; j < 32 * hf + 32; ++j)
 #pragma unroll 1
               for (int c = 0; c < 8; ++c) {
-                const float x = ld<DT>(X, j * XP + 32 * wave + 8 * g + c);
+                const float x = ld<DT>(X, TT::template unit<UX>(j, (32 * wave + 8 * g + c) / EV) + c % EV);
                 if (fabsf(x) < __builtin_inff()) continue;
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
@@ -535,7 +591,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
             const int i = 32 * hf + 16 * q + m;
             if (i >= left || pc >= P) continue;
             float v[8], x[8];
-            TT::unpack(TT::row(X + i * XP + 32 * wave + 8 * g), x);
+            TT::unpack(TT::template rows<UX>(X, 32 * hf + 16 * q, m, g, wave), x);
 #pragma unroll
             for (int r = 0; r < 8; ++r) v[r] = y[q][r >> 2][r & 3] + (a.D ? skip * x[r] : 0.0f);
             if (a.z) {
@@ -544,7 +600,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
 #pragma unroll
               for (int k = 0; k < 8 / EV; ++k) {
                 if constexpr (VEC) {
-                  u[k] = zr[q][k];
+                  u[k] = zr[2 * hf + q][k];
                 } else {
                   u[k] = make_uint4(0, 0, 0, 0);
                   if (pc + k * EV < P) u[k] = load_unit<DT>(a.z, (row0 + i) * a.ld_z + hp, pc + k * EV, P);
@@ -552,11 +608,12 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
               }
               TT::unpack(__builtin_bit_cast(Frag, u), z);
 #pragma unroll
-              for (int r = 0; r < 8; ++r) v[r] *= siluf_(z[r]);
+              for (int r = 0; r < 8; ++r) v[r] *= gatef_<DT>(z[r]);
             }
             if constexpr (VEC) {
-              *reinterpret_cast<Frag*>(yb + (static_cast<uint32_t>(i) * static_cast<uint32_t>(a.ld_y * es) +
-                                             8 * g * static_cast<uint32_t>(es))) =
+              uint32_t at = static_cast<uint32_t>(i) * static_cast<uint32_t>(a.ld_y * es) + 8 * g * static_cast<uint32_t>(es);
+              asm volatile("" : "+v"(at));  // formed here, not kept over the loop
+              *reinterpret_cast<Frag*>(yb + at) =
                   TT::pack(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
             } else {
               E* dst = static_cast<E*>(a.y) + (row0 + i) * a.ld_y + hp + pc;
@@ -597,25 +654,23 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
           if constexpr (DT == kBF16) {
             TT::unpack(hi[T], v);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {  // (nothing is left of an infinity)
-              v0[r] = fabsf(v[r]) < __builtin_inff() ? v0[r] - v[r] : 0.0f;
-              v1[r] = fabsf(v[4 + r]) < __builtin_inff() ? v1[r] - v[4 + r] : 0.0f;
-            }
+            for (int r = 0; r < 4; ++r) v0[r] -= v[r], v1[r] -= v[4 + r];  // (an infinity's states become NaN)
             lo[T] = TT::pack(v0, v1);
           }
         }
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+        for (int s = 0; s < NS; ++s) {
+          Frag b[2];
 #pragma unroll
-          for (int t2 = 0; t2 < 2; ++t2) {
-            const Frag b = TT::column(Bs + 32 * ks * NP + 32 * s + TT::tr_at(g, m, t2, NP), NP);
+          for (int t2 = 0; t2 < 2; ++t2)
+            b[t2] = TT::template column<UB>(Bs, 32 * ks, m, g, s, t2);
 #pragma unroll
-            for (int T = 0; T < 2; ++T) {
-              h[s][t2][T] = TT::mma(b, hi[T], h[s][t2][T]);
-              if constexpr (DT == kBF16) h[s][t2][T] = TT::mma(b, lo[T], h[s][t2][T]);
-            }
-            if (t2) __builtin_amdgcn_sched_barrier(0);
-          }
+          for (int half = 0; half < (DT == kBF16 ? 2 : 1); ++half)
+#pragma unroll
+            for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+              for (int T = 0; T < 2; ++T) h[s][t2][T] = TT::mma(b[t2], half ? lo[T] : hi[T], h[s][t2][T]);
+        }
       }
     }
     __syncthreads();
@@ -751,6 +806,8 @@ int states32(const SsmArgs& a) {  // 32-state steps, rounded up to an instantiat
 
 // Segments so that about one workgroup per CU runs; a segment's end state costs as much traffic as about 85 of its
 // rows, so it has several times that.
+int64_t ssm_target() { const char* e = getenv("SSM_TARGET"); return e ? atoi(e) : 512; }
+int64_t ssm_min() { const char* e = getenv("SSM_MIN"); return e ? atoi(e) : kMinSegment; }
 SsmGrid ssm_grid(const SsmArgs& a) {
   SsmGrid g;
   const int64_t hg = a.H / a.G;
@@ -760,8 +817,8 @@ SsmGrid ssm_grid(const SsmArgs& a) {
   g.nh = 4 % g.ps == 0 ? 4 / g.ps : g.ps % 4 == 0 ? 1 : 2;
   const int64_t wgs = a.G * g.wpg, rows = a.seq_starts ? a.B * a.L : a.L;
   const int64_t each = a.seq_starts ? 1 : std::max<int64_t>(a.S, 1);
-  const int64_t want = std::max<int64_t>(1, 256 / std::max<int64_t>(1, wgs * each));
-  g.seg = std::max<int64_t>(kMinSegment, round_up((rows + want - 1) / want, 64));
+  const int64_t want = std::max<int64_t>(1, ssm_target() / std::max<int64_t>(1, wgs * each));
+  g.seg = std::max<int64_t>(ssm_min(), round_up((rows + want - 1) / want, 64));
   if (a.seq_starts)
     g.slots = rows / g.seg + a.S;
   else
