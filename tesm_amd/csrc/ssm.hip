@@ -24,7 +24,7 @@ typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------------------
-// The scan in chunks of Q rows.  With c_i the sum of d A over the chunk's rows up to i, and h the state on entry:
+// The scan in chunks of 32 rows.  With c_i the sum of d A over the chunk's rows up to i, and h the state on entry:
 //   Y = W X + exp(c) C h,   W_ij = (C_i . B_j) exp(c_i - c_j) d_j for j <= i, else 0
 //   h' = exp(c_Q) h + sum_j exp(c_Q - c_j) d_j x_j B_j^T
 // so that all of it is matrix products.  A workgroup of 4 waves walks a segment of one sequence for 128 columns of one
@@ -39,6 +39,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // 16-byte store.
 // ---------------------------------------------------------------------------
 constexpr int kCols = 128;  // columns per workgroup
+constexpr int kQ = 32;      // rows per chunk
 constexpr int64_t kMinSegment = 256;
 
 template <int DT>
@@ -46,7 +47,7 @@ struct Tile;
 template <>
 struct Tile<kBF16> {
   using E = uint16_t;
-  static constexpr int Q = 64, EV = 8, PAD = 8;
+  static constexpr int EV = 8, PAD = 8, NB = 2;  // elements per 16 bytes, padding, chunks staged at once
   // Rows of U 16-byte units (4, 8, 16 or 32) lie one behind the other without padding; unit u of row r is kept at
   // u ^ swz(r).  Then the 8 rows of one unit that a row operand reads at once, and the 4 rows x 4 units of a column
   // operand, fall on different banks (64 of 4 bytes).
@@ -100,7 +101,7 @@ struct Tile<kBF16> {
 template <>
 struct Tile<kF32> {
   using E = float;
-  static constexpr int Q = 32, EV = 4, PAD = 4;
+  static constexpr int EV = 4, PAD = 4, NB = 1;
   template <int U>
   static constexpr int pitch() { return U * EV + PAD; }
   template <int U>
@@ -140,10 +141,6 @@ struct Tile<kF32> {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
   }
 };
-
-// Tile e of a lower triangle counted row by row.
-__device__ __forceinline__ int tile_row(int e) { return (0x3333222110ull >> (4 * e)) & 15; }
-__device__ __forceinline__ int tile_col(int e) { return (0x3210210100ull >> (4 * e)) & 15; }
 
 // The compiler is to form what depends on h, and what is read from memory, anew from here on (kept values would have
 // to be spilled).
@@ -244,7 +241,7 @@ __device__ __forceinline__ double readlane_d(double v, int l) {
   return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-// Inclusive sums over the wave's lanes: shifts inside rows of 16 lanes, then the totals of the rows before.
+// Inclusive sums over each half of the wave: shifts inside rows of 16 lanes, then the total of the row before.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp_add(double v) {
   const uint64_t b = __builtin_bit_cast(uint64_t, v);
@@ -252,45 +249,41 @@ __device__ __forceinline__ double dpp_add(double v) {
   const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROWS, 0xF, false);
   return v + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
-__device__ __forceinline__ double wave_scan_d(double v) {
+__device__ __forceinline__ double half_scan_d(double v) {
   v = dpp_add<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
   v = dpp_add<0x112, 0xF>(v);
   v = dpp_add<0x114, 0xF>(v);
   v = dpp_add<0x118, 0xF>(v);
-  v = dpp_add<0x142, 0xA>(v);  // lane 15 of the row before, to rows 1 and 3
-  return dpp_add<0x143, 0xC>(v);  // lane 31, to rows 2 and 3
+  return dpp_add<0x142, 0xA>(v);  // lane 15 of the row before, to rows 1 and 3
 }
 
-template <int DT, int NS>
+template <int DT, int NS, bool FULL>
 struct SsmLds {
   using TT = Tile<DT>;
   static constexpr int UX = kCols / TT::EV, UB = 32 * NS / TT::EV;  // 16-byte units per row
-  static constexpr int XP = TT::template pitch<UX>(), NP = TT::template pitch<UB>(), WP = TT::Q + TT::PAD;
-  static constexpr int kSmall = 6 * TT::Q;  // per head: c high, c low, d, exp(c_Q - c) d, exp(c), spare
-  static constexpr int64_t bytes(int nh, bool full) {
+  static constexpr int XP = TT::template pitch<UX>(), NP = TT::template pitch<UB>(), WP = kQ + TT::PAD;
+  static constexpr int kStage = kQ * (XP + (FULL ? 2 : 1) * NP);  // x, B and C of a chunk
+  static constexpr int kSmall = 6 * kQ;  // per head: c high, c low, d, exp(c_Q - c) d, exp(c), and exp(c_Q) at 5 kQ
+  static constexpr int64_t bytes(int nh) {
     const int64_t e = sizeof(typename TT::E);
-    return TT::Q * (XP + (full ? 2 : 1) * NP) * e + (full ? nh * TT::Q * WP * e : 0) + (nh * kSmall + 4) * 4;
+    return TT::NB * kStage * e + (FULL ? nh * kQ * WP * e : 0) + 2 * nh * kSmall * 4;
   }
 };
 
 // FULL: y and the final state of a segment from its carried-in state; otherwise the segment's end state from zero.
 // VEC: whole 32-column slices and 32-state steps in 16-byte vectors, and 32-bit offsets inside a chunk.
 template <int DT, int NS, bool FULL, bool VEC>
-__global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs a, SsmGrid gr) {
+__global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_kernel(SsmArgs a, SsmGrid gr) {
   using TT = Tile<DT>;
   using E = typename TT::E;
   using Frag = typename TT::Frag;
-  using Lds = SsmLds<DT, NS>;
-  constexpr int Q = TT::Q, EV = TT::EV, XP = Lds::XP, NP = Lds::NP, WP = Lds::WP;
-  constexpr int UX = Lds::UX, UB = Lds::UB;
-  constexpr int KS = Q / 32, IT = Q / 16;
+  using Lds = SsmLds<DT, NS, FULL>;
+  constexpr int EV = TT::EV, NB = TT::NB, WP = Lds::WP, UX = Lds::UX, UB = Lds::UB;
+  constexpr int XR = kQ * UX / 256, BR = kQ * UB >= 256 ? kQ * UB / 256 : 1;  // units per thread
   extern __shared__ __attribute__((aligned(16))) char lds_s[];
-  E* X = reinterpret_cast<E*>(lds_s);
-  E* Bs = X + Q * XP;
-  E* Cs = Bs + Q * NP;
-  E* Ws = FULL ? Cs + Q * NP : Cs;
-  float* small = reinterpret_cast<float*>(Ws + (FULL ? gr.nh * Q * WP : 0));
-  float* tots = small + gr.nh * Lds::kSmall;  // exp(c_Q) per head
+  E* const stages = reinterpret_cast<E*>(lds_s);
+  E* const Ws = stages + NB * Lds::kStage;
+  float* const smalls = reinterpret_cast<float*>(Ws + (FULL ? gr.nh * kQ * WP : 0));
 
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -341,23 +334,15 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
         }
       }
 
-  if constexpr (FULL) {  // the blocks of W above the diagonal that a 32-wide step reads: zero throughout
-    for (int e = tid; e < nh * IT / 2 * 16 * 16; e += 256) {
-      const int j = e & 15, i = (e >> 4) & 15, b = (e >> 8) % (IT / 2), w = (e >> 8) / (IT / 2);
-      Ws[(w * Q + 32 * b + i) * WP + 32 * b + 16 + j] = E(0);
-    }
-  }
-
-  uint4 xr[4], br[NS], cr[FULL ? NS : 1];
-  uint32_t dtr = 0;  // bits of dt, converted where it is used
-  const int64_t es = sizeof(E), gn = static_cast<int64_t>(grp) * N;
-  // One chunk's units ahead of their use.  VEC: uniform bases and 32-bit offsets; rows past the end read the last one
-  // and are cleared when staged.
+  // A chunk's units, one chunk ahead of their use.  VEC: uniform bases and 32-bit offsets; rows past the end read the
+  // last one and are cleared when staged.
+  uint4 xr[XR], br[BR], cr[FULL ? BR : 1], zr[2][8 / EV];
+  const int64_t es = sizeof(E), gn = static_cast<int64_t>(grp) * N, hp = static_cast<int64_t>(head) * P;
   auto load_bc = [&](const void* p, int64_t ld, int row0, auto& u) {
     const int left = sg.r1 - row0;  // rows of the chunk that exist
     const char* base = static_cast<const char*>(p) + (row0 * ld + gn) * es;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
+    for (int i = 0; i < BR; ++i) {
       const int r = tid / UB + i * (256 / UB);
       if constexpr (VEC) {
         u[i] = *reinterpret_cast<const uint4*>(base + (static_cast<uint32_t>(min(r, left - 1)) * static_cast<uint32_t>(ld * es) +
@@ -368,12 +353,12 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
       }
     }
   };
-  auto load_chunk = [&](int row0) {  // x, B and dt
+  auto load_chunk = [&](int row0) {
     const int left = sg.r1 - row0;
     const char* base = static_cast<const char*>(a.x) + row0 * a.ld_x * es;
     const uint32_t xo = static_cast<uint32_t>((xok ? xat + xp : 0) * es);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < XR; ++i) {
       const int r = tid / UX + i * (256 / UX);
       if constexpr (VEC) {
         xr[i] = *reinterpret_cast<const uint4*>(base + (static_cast<uint32_t>(min(r, left - 1)) * static_cast<uint32_t>(a.ld_x * es) + xo));
@@ -383,253 +368,270 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
       }
     }
     load_bc(a.Bm, a.ld_b, row0, br);
-    if (wave < nh) {
-      const int r = min(lane, left - 1);
-      dtr = ld_bits<DT>(a.dts, (row0 + r) * a.ld_dt + grp * hg + head0 + wave);
+    if constexpr (FULL) load_bc(a.Cm, a.ld_c, row0, cr);
+    if (FULL && VEC && a.z && active) {  // the gate of this lane's outputs
+      const char* zb = static_cast<const char*>(a.z) + (row0 * a.ld_z + hp + p0) * es;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const uint32_t r = min(16 * q + m, left - 1);
+        const uint4* src = reinterpret_cast<const uint4*>(
+            zb + (r * static_cast<uint32_t>(a.ld_z * es) + 8 * g * static_cast<uint32_t>(es)));
+#pragma unroll
+        for (int k = 0; k < 8 / EV; ++k) zr[q][k] = src[k];
+      }
+    }
+  };
+
+  // d and the sums c of a chunk, formed by the last wave for two heads at a time, 32 lanes each, while the others form
+  // the chunk before's scores; dt is read two chunks ahead.
+  uint32_t dtr[2] = {0, 0};
+  float Ar[2] = {0.0f, 0.0f}, biasr[2] = {0.0f, 0.0f};
+  const int dh = lane >> 5;
+  auto load_dt = [&](int row0) {
+    const int r = min(row0 + (lane & 31), sg.r1 - 1);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (2 * k + dh < nh) dtr[k] = ld_bits<DT>(a.dts, r * a.ld_dt + grp * hg + head0 + 2 * k + dh);
+  };
+  auto sums = [&](int row0, float* to) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (2 * k >= nh) break;
+      const float raw = from_bits<DT>(dtr[k]) + biasr[k];
+      const float d = row0 + (lane & 31) < sg.r1 ? (a.softplus ? softplusf_(raw) : raw) : 0.0f;
+      // in units of log 2, 64 bits split into two floats
+      const double c = half_scan_d(static_cast<double>(d) * static_cast<double>(Ar[k]) * 1.4426950408889634074);
+      const double all = dh ? readlane_d(c, 63) : readlane_d(c, 31);
+      if (2 * k + dh < nh) {
+        float* sm = to + (2 * k + dh) * Lds::kSmall + (lane & 31);
+        const float hi = static_cast<float>(c), lo = static_cast<float>(c - static_cast<double>(hi));
+        sm[0] = hi;
+        sm[kQ] = lo;
+        sm[2 * kQ] = d;
+        sm[3 * kQ] = __builtin_amdgcn_exp2f(static_cast<float>(all - c)) * d;
+        sm[4 * kQ] = __builtin_amdgcn_exp2f(hi);
+        if ((lane & 31) == 0) sm[5 * kQ] = __builtin_amdgcn_exp2f(static_cast<float>(all));
+      }
     }
   };
 
   float decay = 1.0f;  // of the segment so far (this wave's head)
-  const float Aw = wave < nh ? a.A[grp * hg + head0 + wave] : 0.0f;
-  const float bias = wave < nh && a.dt_bias ? a.dt_bias[grp * hg + head0 + wave] : 0.0f;
   const float skip = FULL && a.D && active ? a.D[head] : 0.0f;
   if (sg.r0 < sg.r1) {
     load_chunk(sg.r0);
-    if constexpr (FULL) load_bc(a.Cm, a.ld_c, sg.r0, cr);
-  }
-  for (int row0 = sg.r0; row0 < sg.r1; row0 += Q) {
-    const int left = sg.r1 - row0;
-    if (VEC && left < Q) {
+    if (wave == 3) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int k = 0; k < 2; ++k)
+        if (2 * k + dh < nh) {
+          Ar[k] = a.A[grp * hg + head0 + 2 * k + dh];
+          if (a.dt_bias) biasr[k] = a.dt_bias[grp * hg + head0 + 2 * k + dh];
+        }
+      load_dt(sg.r0);
+      sums(sg.r0, smalls);
+      load_dt(sg.r0 + kQ);
+    }
+    if constexpr (FULL) {  // the block of W above the diagonal that a 32-wide step reads: zero throughout
+      for (int e = tid; e < nh * 256; e += 256) Ws[((e >> 8) * kQ + ((e >> 4) & 15)) * WP + 16 + (e & 15)] = E(0);
+    }
+  }
+  int buf = 0;
+  for (int row0 = sg.r0; row0 < sg.r1; row0 += kQ, buf ^= 1) {
+    const int left = sg.r1 - row0;
+    E* const X = stages + (NB == 2 ? buf * Lds::kStage : 0);
+    E* const Bs = X + kQ * Lds::XP;
+    E* const Cs = Bs + kQ * Lds::NP;
+    const float* const sw = smalls + buf * gr.nh * Lds::kSmall;
+    float* const next = smalls + (buf ^ 1) * gr.nh * Lds::kSmall;
+    if (VEC && left < kQ) {
+#pragma unroll
+      for (int i = 0; i < XR; ++i)
         if (tid / UX + i * (256 / UX) >= left) xr[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
+      for (int i = 0; i < BR; ++i)
         if (tid / UB + i * (256 / UB) >= left) {
           br[i] = make_uint4(0, 0, 0, 0);
           if constexpr (FULL) cr[i] = make_uint4(0, 0, 0, 0);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(X + TT::template unit<UX>(tid / UX + i * (256 / UX), tid % UX)) = xr[i];
+    for (int i = 0; i < XR; ++i) *reinterpret_cast<uint4*>(X + TT::template unit<UX>(tid / UX + i * (256 / UX), tid % UX)) = xr[i];
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
+    for (int i = 0; i < BR; ++i) {
+      if (kQ * UB < 256 && tid >= kQ * UB) break;
       const int at = TT::template unit<UB>(tid / UB + i * (256 / UB), tid % UB);
       *reinterpret_cast<uint4*>(Bs + at) = br[i];
       if constexpr (FULL) *reinterpret_cast<uint4*>(Cs + at) = cr[i];
     }
-    if (wave < nh) {  // this wave's head: d and the sums c, in units of log 2, 64 bits split into two floats
-      const float raw = from_bits<DT>(dtr) + bias;
-      const float d = lane < left && lane < Q ? (a.softplus ? softplusf_(raw) : raw) : 0.0f;
-      const double c = wave_scan_d(static_cast<double>(d) * static_cast<double>(Aw) * 1.4426950408889634074);
-      const double all = readlane_d(c, Q - 1);
-      float* sm = small + wave * Lds::kSmall;
-      if (lane < Q) {
-        const float hi = static_cast<float>(c), lo = static_cast<float>(c - static_cast<double>(hi));
-        sm[lane] = hi;
-        sm[Q + lane] = lo;
-        sm[2 * Q + lane] = d;
-        sm[3 * Q + lane] = __builtin_amdgcn_exp2f(static_cast<float>(all - c)) * d;
-        sm[4 * Q + lane] = __builtin_amdgcn_exp2f(hi);
-      }
-      if (lane == 0) tots[wave] = __builtin_amdgcn_exp2f(static_cast<float>(all));
+    uint4 zc[2][8 / EV];
+    if constexpr (FULL && VEC) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int k = 0; k < 8 / EV; ++k) zc[q][k] = zr[q][k];
     }
-    __syncthreads();
-    if (row0 + Q < sg.r1) load_chunk(row0 + Q);
-
-    uint4 zr[IT][8 / EV];
-    if (FULL && VEC && a.z && active) {  // the gate of this lane's outputs, ahead of its use
-      const char* zb = static_cast<const char*>(a.z) + (row0 * a.ld_z + static_cast<int64_t>(head) * P + p0) * es;
-#pragma unroll
-      for (int it = 0; it < IT; ++it) {
-        const uint32_t r = min(16 * it + m, left - 1);
-        const uint4* src = reinterpret_cast<const uint4*>(
-            zb + (r * static_cast<uint32_t>(a.ld_z * es) + 8 * g * static_cast<uint32_t>(es)));
-#pragma unroll
-        for (int k = 0; k < 8 / EV; ++k) zr[it][k] = src[k];
+    lds_barrier();
+    if (left > kQ) load_chunk(row0 + kQ);
+    const float* const sm = sw + hh * Lds::kSmall;
+    if (wave == 3) {
+      if (left > kQ) {
+        sums(row0 + kQ, next);
+        if (left > 2 * kQ) load_dt(row0 + 2 * kQ);
       }
-    }
-    const float* sm = small + hh * Lds::kSmall;
-    Frag xf[2][KS];  // x of this wave's columns, 8 rows of a column per lane
-    auto read_x = [&]() {
+    } else if (FULL) {
+      // scores: one 16 x 16 tile (it, jt) of the lower triangle per wave, then W of every head of the workgroup
+      const int it = wave ? 1 : 0, jt = wave == 2 ? 1 : 0;
+      f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int T = 0; T < 2; ++T)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          xf[T][ks] = TT::template column<UX>(X, 32 * ks, m, g, wave, T);
-    };
-    if constexpr (FULL) {
-      // scores, tile (it, jt) of the lower triangle, dealt over the waves; W of every head of the workgroup
-      constexpr int TILES = IT * (IT + 1) / 2, TW = (TILES + 3) / 4;
-      f32x4 sc[TW];
-      int mo = m;
-      asm volatile("" : "+v"(mo));  // addresses formed here, not kept over the loop
-#pragma unroll
-      for (int e = 0; e < TW; ++e) {
-        sc[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (wave + 4 * e >= TILES) continue;
-        const int it = tile_row(wave + 4 * e), jt = tile_col(wave + 4 * e);
-#pragma unroll
-        for (int k = 0; k < NS; ++k)
-          sc[e] = TT::mma(TT::template rows<UB>(Bs, 16 * jt, mo, g, k), TT::template rows<UB>(Cs, 16 * it, mo, g, k), sc[e]);
-      }
+      for (int k = 0; k < NS; ++k)
+        sc = TT::mma(TT::template rows<UB>(Bs, 16 * jt, m, g, k), TT::template rows<UB>(Cs, 16 * it, m, g, k), sc);
+      const int i = 16 * it + m, j0 = 16 * jt + 4 * g;
       for (int w = 0; w < nh; ++w) {
-        const float* sw = small + w * Lds::kSmall;
+        const float* const s = sw + w * Lds::kSmall;
         // the low halves of the sums matter where the sums are large against the result's own rounding
-        const bool low = DT == kF32 || !(__builtin_amdgcn_readfirstlane(__float_as_int(fabsf(sw[Q - 1]))) < __float_as_int(512.0f));
+        const bool low = DT == kF32 || !(__builtin_amdgcn_readfirstlane(__float_as_int(fabsf(s[kQ - 1]))) < __float_as_int(512.0f));
+        const float hi = s[i];
+        const f32x4 hj = *reinterpret_cast<const f32x4*>(s + j0), dj = *reinterpret_cast<const f32x4*>(s + 2 * kQ + j0);
+        f32x4 v;
 #pragma unroll
-        for (int e = 0; e < TW; ++e) {
-          if (wave + 4 * e >= TILES) continue;
-          const int i = 16 * tile_row(wave + 4 * e) + m, j0 = 16 * tile_col(wave + 4 * e) + 4 * g;
-          const float hi = sw[i];
-          const f32x4 hj = *reinterpret_cast<const f32x4*>(sw + j0), dj = *reinterpret_cast<const f32x4*>(sw + 2 * Q + j0);
-          f32x4 v;
+        for (int r = 0; r < 4; ++r) v[r] = hi - hj[r];
+        if (low) {
+          const float lo = s[kQ + i];
+          const f32x4 lj = *reinterpret_cast<const f32x4*>(s + kQ + j0);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = hi - hj[r];
-          if (low) {
-            const float lo = sw[Q + i];
-            const f32x4 lj = *reinterpret_cast<const f32x4*>(sw + Q + j0);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] += lo - lj[r];
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = sc[e][r] * __builtin_amdgcn_exp2f(v[r]) * dj[r];
-          if (tile_row(wave + 4 * e) == tile_col(wave + 4 * e)) {  // on the diagonal
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (j0 + r > i) v[r] = 0.0f;
-          }
-          TT::store4(Ws + (w * Q + i) * WP + j0, v);
+          for (int r = 0; r < 4; ++r) v[r] += lo - lj[r];
         }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = sc[r] * __builtin_amdgcn_exp2f(v[r]) * dj[r];
+        if (it == jt) {  // on the diagonal
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (j0 + r > i) v[r] = 0.0f;
+        }
+        TT::store4(Ws + (w * kQ + i) * WP + j0, v);
       }
     }
-    if (active) read_x();
+    Frag xf[2];  // x of this wave's columns, 8 rows of a column per lane
+    if (active) {
+#pragma unroll
+      for (int T = 0; T < 2; ++T) xf[T] = TT::template column<UX>(X, 0, m, g, wave, T);
+    }
     if constexpr (FULL) {
-      __syncthreads();
-      if (active) {
-        const int64_t hp = static_cast<int64_t>(head) * P;
-        const int pc = p0 + 8 * g;  // this lane's outputs: columns pc .. + 7 of rows 16 it + m
-        char* yb = static_cast<char*>(a.y) + (row0 * a.ld_y + hp + p0) * es;
+      f32x4 y[2][2];
+      // exp(c_i) C_i . h (bfloat16 operands: h is rounded here, once, for the product)
+      auto across = [&]() {
+        anew(h);
 #pragma unroll
-        for (int hf = 0; hf < IT / 2; ++hf) {  // 32 rows at a time, for the registers
-          f32x4 y[2][2];
-          // exp(c_i) C_i . h (bfloat16 operands: h is rounded here, once, for the product)
-          auto across = [&]() {
-            anew(h);
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
+          for (int T = 0; T < 2; ++T) y[q][T] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-              for (int T = 0; T < 2; ++T) y[q][T] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {
-              const Frag h0 = TT::pack(h[s][0][0], h[s][1][0]), h1 = TT::pack(h[s][0][1], h[s][1][1]);
-#pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                const Frag c = TT::template rows<UB>(Cs, 32 * hf + 16 * q, m, g, s);
-                y[q][0] = TT::mma(h0, c, y[q][0]);
-                y[q][1] = TT::mma(h1, c, y[q][1]);
-              }
-            }
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const float e = sm[4 * Q + 32 * hf + 16 * q + m];
-              y[q][0] *= e;
-              y[q][1] *= e;
-            }
-          };
-          across();
-          // + W x over the rows up to each
-#pragma unroll
-          for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int ks = 0; ks <= hf; ++ks) {
-              const Frag w = TT::row(Ws + (hh * Q + 32 * hf + 16 * q + m) * WP + 32 * ks + 8 * g);
-              y[q][0] = TT::mma(xf[0][ks], w, y[q][0]);
-              y[q][1] = TT::mma(xf[1][ks], w, y[q][1]);
-            }
-          // An infinite or NaN x must not reach the rows before it through a weight 0.  Rows with one near have sums
-          // that are not finite: they are formed again without such values, which are then added from their row on.
-          bool odd = false;
-#pragma unroll
-          for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int T = 0; T < 2; ++T)
-              odd |= !(fabsf(y[q][T][0]) + fabsf(y[q][T][1]) + fabsf(y[q][T][2]) + fabsf(y[q][T][3]) < __builtin_inff());
-          if (__any(odd)) {
-            across();
-#pragma unroll
-            for (int ks = 0; ks <= hf; ++ks)
-#pragma unroll
-              for (int T = 0; T < 2; ++T) {
-                float v[8];
-                TT::unpack(TT::template column<UX>(X, 32 * ks, m, g, wave, T), v);
-#pragma unroll
-                for (int r = 0; r < 8; ++r) v[r] = fabsf(v[r]) < __builtin_inff() ? v[r] : 0.0f;
-                const Frag f = TT::pack(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-                  y[q][T] = TT::mma(f, TT::row(Ws + (hh * Q + 32 * hf + 16 * q + m) * WP + 32 * ks + 8 * g), y[q][T]);
-              }
-#pragma unroll 1
-            for (int j = 0; j < 32 * hf + 32; ++j)
-#pragma unroll 1
-              for (int c = 0; c < 8; ++c) {
-                const float x = ld<DT>(X, TT::template unit<UX>(j, (32 * wave + 8 * g + c) / EV) + c % EV);
-                if (fabsf(x) < __builtin_inff()) continue;
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                  const int i = 32 * hf + 16 * q + m;
-                  const float add = j <= i ? ld<DT>(Ws, (hh * Q + i) * WP + j) * x : 0.0f;
-#pragma unroll
-                  for (int r = 0; r < 8; ++r)
-                    if (r == c) y[q][r >> 2][r & 3] += add;
-                }
-              }
-          }
+        for (int s = 0; s < NS; ++s) {
+          const Frag h0 = TT::pack(h[s][0][0], h[s][1][0]), h1 = TT::pack(h[s][0][1], h[s][1][1]);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const int i = 32 * hf + 16 * q + m;
-            if (i >= left || pc >= P) continue;
-            float v[8], x[8];
-            TT::unpack(TT::template rows<UX>(X, 32 * hf + 16 * q, m, g, wave), x);
-#pragma unroll
-            for (int r = 0; r < 8; ++r) v[r] = y[q][r >> 2][r & 3] + (a.D ? skip * x[r] : 0.0f);
-            if (a.z) {
-              float z[8];
-              uint4 u[8 / EV];
-#pragma unroll
-              for (int k = 0; k < 8 / EV; ++k) {
-                if constexpr (VEC) {
-                  u[k] = zr[2 * hf + q][k];
-                } else {
-                  u[k] = make_uint4(0, 0, 0, 0);
-                  if (pc + k * EV < P) u[k] = load_unit<DT>(a.z, (row0 + i) * a.ld_z + hp, pc + k * EV, P);
-                }
-              }
-              TT::unpack(__builtin_bit_cast(Frag, u), z);
-#pragma unroll
-              for (int r = 0; r < 8; ++r) v[r] *= gatef_<DT>(z[r]);
-            }
-            if constexpr (VEC) {
-              uint32_t at = static_cast<uint32_t>(i) * static_cast<uint32_t>(a.ld_y * es) + 8 * g * static_cast<uint32_t>(es);
-              asm volatile("" : "+v"(at));  // formed here, not kept over the loop
-              *reinterpret_cast<Frag*>(yb + at) =
-                  TT::pack(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
-            } else {
-              E* dst = static_cast<E*>(a.y) + (row0 + i) * a.ld_y + hp + pc;
-#pragma unroll
-              for (int r = 0; r < 8; ++r)
-                if (pc + r < P) st<DT>(dst, r, v[r]);
-            }
+            const Frag c = TT::template rows<UB>(Cs, 16 * q, m, g, s);
+            y[q][0] = TT::mma(h0, c, y[q][0]);
+            y[q][1] = TT::mma(h1, c, y[q][1]);
           }
-          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const float e = sm[4 * kQ + 16 * q + m];
+          y[q][0] *= e;
+          y[q][1] *= e;
+        }
+      };
+      if (active) across();
+      lds_barrier();
+      if (active) {
+        // + W x over the rows up to each
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const Frag w = TT::row(Ws + (hh * kQ + 16 * q + m) * WP + 8 * g);
+          y[q][0] = TT::mma(xf[0], w, y[q][0]);
+          y[q][1] = TT::mma(xf[1], w, y[q][1]);
+        }
+        // An infinite or NaN x must not reach the rows before it through a weight 0.  Rows with one near have sums
+        // that are not finite: they are formed again without such values, which are then added from their row on.
+        bool odd = false;
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int T = 0; T < 2; ++T)
+            odd |= !(fabsf(y[q][T][0]) + fabsf(y[q][T][1]) + fabsf(y[q][T][2]) + fabsf(y[q][T][3]) < __builtin_inff());
+        if (__any(odd)) {
+          across();
+#pragma unroll
+          for (int T = 0; T < 2; ++T) {
+            float v[8];
+            TT::unpack(TT::template column<UX>(X, 0, m, g, wave, T), v);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] = fabsf(v[r]) < __builtin_inff() ? v[r] : 0.0f;
+            const Frag f = TT::pack(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
+#pragma unroll
+            for (int q = 0; q < 2; ++q) y[q][T] = TT::mma(f, TT::row(Ws + (hh * kQ + 16 * q + m) * WP + 8 * g), y[q][T]);
+          }
+#pragma unroll 1
+          for (int j = 0; j < kQ; ++j)
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              const float x = ld<DT>(X, TT::template unit<UX>(j, (32 * wave + 8 * g + c) / EV) + c % EV);
+              if (fabsf(x) < __builtin_inff()) continue;
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const int i = 16 * q + m;
+                const float add = j <= i ? ld<DT>(Ws, (hh * kQ + i) * WP + j) * x : 0.0f;
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                  if (r == c) y[q][r >> 2][r & 3] += add;
+              }
+            }
+        }
+        const int pc = p0 + 8 * g;  // this lane's outputs: columns pc .. + 7 of rows 16 q + m
+        char* yb = static_cast<char*>(a.y) + (row0 * a.ld_y + hp + p0) * es;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int i = 16 * q + m;
+          if (i >= left || pc >= P) continue;
+          float v[8], x[8];
+          TT::unpack(TT::template rows<UX>(X, 16 * q, m, g, wave), x);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) v[r] = y[q][r >> 2][r & 3];
+          if (a.D) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] = __builtin_fmaf(skip, x[r], v[r]);
+          }
+          if (a.z) {
+            float z[8];
+            uint4 u[8 / EV];
+#pragma unroll
+            for (int k = 0; k < 8 / EV; ++k) {
+              if constexpr (VEC) {
+                u[k] = zc[q][k];
+              } else {
+                u[k] = make_uint4(0, 0, 0, 0);
+                if (pc + k * EV < P) u[k] = load_unit<DT>(a.z, (row0 + i) * a.ld_z + hp, pc + k * EV, P);
+              }
+            }
+            TT::unpack(__builtin_bit_cast(Frag, u), z);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] *= gatef_<DT>(z[r]);
+          }
+          if constexpr (VEC) {
+            uint32_t at = static_cast<uint32_t>(i) * static_cast<uint32_t>(a.ld_y * es) + 8 * g * static_cast<uint32_t>(es);
+            asm volatile("" : "+v"(at));  // formed here, not kept over the loop
+            *reinterpret_cast<Frag*>(yb + at) = TT::pack(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
+          } else {
+            E* dst = static_cast<E*>(a.y) + (row0 + i) * a.ld_y + hp + pc;
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+              if (pc + r < P) st<DT>(dst, r, v[r]);
+          }
         }
       }
     }
-    if constexpr (FULL)
-      if (row0 + Q < sg.r1) load_bc(a.Cm, a.ld_c, row0 + Q, cr);  // (earlier, the sums of y are in the way)
     if (active) {  // the state
-      const float tot = tots[hh];
+      const float tot = sm[5 * kQ];
       decay *= tot;
 #pragma unroll
       for (int s = 0; s < NS; ++s)
@@ -637,43 +639,39 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : 2) void ssm_chunk_kernel(SsmArgs
         for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
           for (int T = 0; T < 2; ++T) h[s][t2][T] *= tot;
+      const f32x4 w0 = *reinterpret_cast<const f32x4*>(sm + 3 * kQ + 8 * g);
+      const f32x4 w1 = *reinterpret_cast<const f32x4*>(sm + 3 * kQ + 8 * g + 4);
+      // w x: float32, or as two bfloat16 halves (2^-17 relative), each a product of its own
+      Frag hi[2], lo[2];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const f32x4 w0 = *reinterpret_cast<const f32x4*>(sm + 3 * Q + 32 * ks + 8 * g);
-        const f32x4 w1 = *reinterpret_cast<const f32x4*>(sm + 3 * Q + 32 * ks + 8 * g + 4);
-        // w x: float32, or as two bfloat16 halves (2^-17 relative), each a product of its own
-        Frag hi[2], lo[2];
+      for (int T = 0; T < 2; ++T) {
+        float v[8];
+        TT::unpack(xf[T], v);
+        f32x4 v0, v1;
 #pragma unroll
-        for (int T = 0; T < 2; ++T) {
-          float v[8];
-          TT::unpack(xf[T][ks], v);
-          f32x4 v0, v1;
+        for (int r = 0; r < 4; ++r) v0[r] = v[r] * w0[r], v1[r] = v[4 + r] * w1[r];
+        hi[T] = TT::pack(v0, v1);
+        if constexpr (DT == kBF16) {
+          TT::unpack(hi[T], v);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v0[r] = v[r] * w0[r], v1[r] = v[4 + r] * w1[r];
-          hi[T] = TT::pack(v0, v1);
-          if constexpr (DT == kBF16) {
-            TT::unpack(hi[T], v);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v0[r] -= v[r], v1[r] -= v[4 + r];  // (an infinity's states become NaN)
-            lo[T] = TT::pack(v0, v1);
-          }
-        }
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          Frag b[2];
-#pragma unroll
-          for (int t2 = 0; t2 < 2; ++t2)
-            b[t2] = TT::template column<UB>(Bs, 32 * ks, m, g, s, t2);
-#pragma unroll
-          for (int half = 0; half < (DT == kBF16 ? 2 : 1); ++half)
-#pragma unroll
-            for (int t2 = 0; t2 < 2; ++t2)
-#pragma unroll
-              for (int T = 0; T < 2; ++T) h[s][t2][T] = TT::mma(b[t2], half ? lo[T] : hi[T], h[s][t2][T]);
+          for (int r = 0; r < 4; ++r) v0[r] -= v[r], v1[r] -= v[4 + r];  // (an infinity's states become NaN)
+          lo[T] = TT::pack(v0, v1);
         }
       }
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        Frag b[2];
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) b[t2] = TT::template column<UB>(Bs, 0, m, g, s, t2);
+#pragma unroll
+        for (int half = 0; half < (DT == kBF16 ? 2 : 1); ++half)
+#pragma unroll
+          for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+            for (int T = 0; T < 2; ++T) h[s][t2][T] = TT::mma(b[t2], half ? lo[T] : hi[T], h[s][t2][T]);
+      }
     }
-    __syncthreads();
+    if (NB == 1) lds_barrier();
   }
 
   if (!active) return;
@@ -832,12 +830,12 @@ template <int DT, int NS, bool VEC>
 int run_ssm(const SsmArgs& a, const SsmGrid& g, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(a.G * g.wpg), static_cast<unsigned>(g.slots));
   if (ssm_split(a, g)) {
-    const unsigned part = static_cast<unsigned>(SsmLds<DT, NS>::bytes(g.nh, false));
+    const unsigned part = static_cast<unsigned>(SsmLds<DT, NS, false>::bytes(g.nh));
     ssm_chunk_kernel<DT, NS, false, VEC><<<grid, 256, part, TESM_LOGGED(st, ssm_chunk_kernel<DT, NS, false, VEC>)>>>(a, g);
     const dim3 cg(static_cast<unsigned>(a.G * g.wpg * NS * 4), static_cast<unsigned>(a.S));
     ssm_carry_kernel<NS><<<cg, 256, 0, TESM_LOGGED(st, ssm_carry_kernel<NS>)>>>(a, g);
   }
-  const unsigned full = static_cast<unsigned>(SsmLds<DT, NS>::bytes(g.nh, true));
+  const unsigned full = static_cast<unsigned>(SsmLds<DT, NS, true>::bytes(g.nh));
   ssm_chunk_kernel<DT, NS, true, VEC><<<grid, 256, full, TESM_LOGGED(st, ssm_chunk_kernel<DT, NS, true, VEC>)>>>(a, g);
   return check_launch("selective scan");
 }
