@@ -32,7 +32,11 @@ __device__ __forceinline__ int conv_seq_of(const int32_t* starts, int64_t S, int
 // 16 bytes at any address of an element.
 typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ uint4 load16(const void* p) { return __builtin_bit_cast(uint4, *static_cast<const any16*>(p)); }
-__device__ __forceinline__ void store16(void* p, const uint4& v) { *static_cast<any16*>(p) = __builtin_bit_cast(any16, v); }
+// (non-temporal: y is written once and read by another kernel, and the cache is left to the rows that two threads read;
+// 29 MB of bfloat16 rows 15.3 us against 16.6, 51 MB of float32 ones 27 against 33)
+__device__ __forceinline__ void store16(void* p, const uint4& v) {
+  __builtin_nontemporal_store(__builtin_bit_cast(any16, v), static_cast<any16*>(p));
+}
 
 // V elements of a row.
 template <int DT, int V>

@@ -746,50 +746,141 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmArgs a, SsmGrid gr) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// One token.  A workgroup owns one head of one sequence: its state, read and written once, is what the call costs.  Rows of
+// N states are held 4 per lane by LPR lanes, 256 / LPR rows at a time; the state's loads are issued first, and the
+// convolution of the head's x and its group's B and C (in float32, to LDS) runs while they are on their way.  Every head
+// forms its group's B and C again; the first head of a group writes their convolution state.
+// ---------------------------------------------------------------------------
+typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(4)));
+
 // Convolved value of channel c of the token; the state moves on where `keep`.
 template <int DT>
-__device__ __forceinline__ float step_channel(const SsmStepArgs& a, int64_t b, int64_t c, int64_t C, bool keep) {
-  const float now = ld<DT>(a.row, b * a.ld_row + c);
-  if (!a.conv_weight) return now;
+__device__ __forceinline__ float step_channel(const SsmStepArgs& a, int64_t b, int c, int64_t C, bool keep) {
+  const uint32_t now = ld_bits<DT>(a.row, b * a.ld_row + c);
+  if (!a.conv_weight) return from_bits<DT>(now);
   const int W = static_cast<int>(a.W);
+  uint32_t past[kConvMaxW];
+  float w[kConvMaxW];
+#pragma unroll
+  for (int j = 0; j < kConvMaxW; ++j)
+    if (j < W) {
+      past[j] = j < W - 1 ? ld_bits<DT>(a.conv_state, (b * (W - 1) + j) * C + c) : now;
+      w[j] = a.w_dt == kBF16 ? ld<kBF16>(a.conv_weight, static_cast<int64_t>(c) * W + j)
+                             : ld<kF32>(a.conv_weight, static_cast<int64_t>(c) * W + j);
+    }
   float acc = a.conv_bias ? (a.w_dt == kBF16 ? ld<kBF16>(a.conv_bias, c) : ld<kF32>(a.conv_bias, c)) : 0.0f;
-  for (int j = 0; j < W; ++j) {
-    const float v = j < W - 1 ? ld<DT>(a.conv_state, (b * (W - 1) + j) * C + c) : now;
-    const float w = a.w_dt == kBF16 ? ld<kBF16>(a.conv_weight, c * W + j) : ld<kF32>(a.conv_weight, c * W + j);
-    acc = __builtin_fmaf(v, w, acc);
-    if (keep && j > 0) st<DT>(a.conv_state_out, (b * (W - 1) + j - 1) * C + c, v);
-  }
+#pragma unroll
+  for (int j = 0; j < kConvMaxW; ++j)
+    if (j < W) {
+      acc = __builtin_fmaf(from_bits<DT>(past[j]), w[j], acc);
+      if (keep && j > 0) {
+        if constexpr (DT == kBF16)
+          static_cast<uint16_t*>(a.conv_state_out)[(b * (W - 1) + j - 1) * C + c] = static_cast<uint16_t>(past[j]);
+        else
+          static_cast<uint32_t*>(a.conv_state_out)[(b * (W - 1) + j - 1) * C + c] = past[j];
+      }
+    }
   return a.silu ? siluf_(acc) : acc;
 }
 
-// One workgroup per (sequence, head).
-template <int DT>
+// Sum over groups of LPR lanes, in every lane.
+template <int LPR>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (LPR >= 2) v += __int_as_float(dpp_mov<kDppXor1>(__float_as_int(v)));
+  if constexpr (LPR >= 4) v += __int_as_float(dpp_mov<kDppXor2>(__float_as_int(v)));
+  if constexpr (LPR >= 8) v += __int_as_float(dpp_mov<kDppHalfMirror>(__float_as_int(v)));
+  if constexpr (LPR >= 16) v += __int_as_float(dpp_mov<kDppMirror>(__float_as_int(v)));
+  if constexpr (LPR >= 32) v += __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v), kSwzXor16));
+  if constexpr (LPR >= 64) v += __shfl_xor(v, 32);
+  return v;
+}
+
+// N4: rows are whole vectors of 4 states.
+template <int DT, int LPR, bool N4>
 __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepArgs a) {
-  __shared__ float bs[kSsmMaxN], cs[kSsmMaxN];
-  const int64_t b = blockIdx.y, h = blockIdx.x, hg = a.H / a.G, g = h / hg;
-  const int64_t HP = a.H * a.P, C = HP + 2 * a.G * a.N;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int64_t n = threadIdx.x; n < a.N; n += 256) {
-    bs[n] = step_channel<DT>(a, b, HP + g * a.N + n, C, h % hg == 0);
-    cs[n] = step_channel<DT>(a, b, HP + (a.G + g) * a.N + n, C, h % hg == 0);
+  constexpr int RP = 256 / LPR, K = 8;  // rows at a time, and how many times ahead
+  extern __shared__ __attribute__((aligned(16))) float lds_step[];
+  const int N = static_cast<int>(a.N), P = static_cast<int>(a.P), n4 = (N + 3) & ~3;
+  float* const bs = lds_step;  // B, C: n4 each; x: P; y: P
+  float* const cs = bs + n4;
+  float* const xs = cs + n4;
+  float* const ys = xs + P;
+  const int64_t b = blockIdx.y;
+  const int h = blockIdx.x, hg = static_cast<int>(a.H / a.G), grp = h / hg;
+  const int HP = static_cast<int>(a.H) * P;
+  const int64_t C = HP + 2 * a.G * a.N;
+  const int tid = threadIdx.x, n = (tid % LPR) * 4, p0 = tid / LPR;
+  float* const state = a.state + (b * a.H + h) * P * static_cast<int64_t>(N);
+  any16 raw[K];
+  auto load = [&](int p, any16& v) {
+    v = any16{0, 0, 0, 0};
+    if (p >= P || n >= N) return;
+    const float* q = state + static_cast<int64_t>(p) * N + n;
+    if (N4 || n + 4 <= N) {
+      v = *reinterpret_cast<const any16*>(q);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 3; ++r)
+        if (n + r < N) v[r] = __float_as_uint(q[r]);
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < K; ++k) load(p0 + k * RP, raw[k]);
+  for (int e = tid; e < 2 * n4 + P; e += 256) {
+    float v = 0.0f;
+    if (e >= 2 * n4) {
+      v = step_channel<DT>(a, b, h * P + e - 2 * n4, C, true);
+    } else {
+      const int c = e >= n4, i = e - c * n4;
+      if (i < N) v = step_channel<DT>(a, b, HP + (c * static_cast<int>(a.G) + grp) * N + i, C, h % hg == 0);
+    }
+    lds_step[e] = v;
   }
-  const float raw = ld<DT>(a.dts, b * a.ld_dt + h) + (a.dt_bias ? a.dt_bias[h] : 0.0f);
-  const float d = a.softplus ? softplusf_(raw) : raw;
+  const float in = ld<DT>(a.dts, b * a.ld_dt + h) + (a.dt_bias ? a.dt_bias[h] : 0.0f);
+  const float d = a.softplus ? softplusf_(in) : in;
   const float decay = fast_exp(d * a.A[h]);
   __syncthreads();
-  for (int64_t p = wave; p < a.P; p += 4) {
-    const float x = step_channel<DT>(a, b, h * a.P + p, C, lane == 0);
-    float* row = a.state + ((b * a.H + h) * a.P + p) * a.N;
-    float acc = 0.0f;
-    for (int64_t n = lane; n < a.N; n += 64) {
-      const float v = decay * row[n] + d * x * bs[n];
-      row[n] = v;
-      acc += v * cs[n];
+  f32x4 bv = {0.0f, 0.0f, 0.0f, 0.0f}, cv = bv;
+  if (n < N) {
+    bv = *reinterpret_cast<const f32x4*>(bs + n) * d;
+    cv = *reinterpret_cast<const f32x4*>(cs + n);
+  }
+  for (int pb = p0; pb < P; pb += K * RP) {
+    float sum[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int p = pb + k * RP;
+      const float x = p < P ? xs[p] : 0.0f;
+      const f32x4 v = __builtin_bit_cast(f32x4, raw[k]) * decay + bv * x;
+      sum[k] = (v[0] * cv[0] + v[1] * cv[1]) + (v[2] * cv[2] + v[3] * cv[3]);
+      if (p < P && n < N) {
+        float* q = state + static_cast<int64_t>(p) * N + n;
+        if (N4 || n + 4 <= N) {
+          *reinterpret_cast<any16*>(q) = __builtin_bit_cast(any16, v);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 3; ++r)
+            if (n + r < N) q[r] = v[r];
+        }
+      }
     }
-    float y = wave_sum_f<64>(acc);
-    if (a.D) y += a.D[h] * x;
-    if (a.z) y *= siluf_(ld<DT>(a.z, b * a.ld_z + h * a.P + p));
-    if (lane == 0) st<DT>(a.y, b * a.ld_y + h * a.P + p, y);
+    if (pb + K * RP - p0 < P) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) load(pb + (K + k) * RP, raw[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      sum[k] = lanes_sum<LPR>(sum[k]);
+      if (tid % LPR == 0 && pb + k * RP < P) ys[pb + k * RP] = sum[k];
+    }
+  }
+  __syncthreads();
+  for (int p = tid; p < P; p += 256) {
+    float y = ys[p];
+    if (a.D) y += a.D[h] * xs[p];
+    if (a.z) y *= siluf_(ld<DT>(a.z, b * a.ld_z + static_cast<int64_t>(h) * P + p));
+    st<DT>(a.y, b * a.ld_y + static_cast<int64_t>(h) * P + p, y);
   }
 }
 
@@ -896,11 +987,34 @@ int launch_selective_scan(const SsmArgs& a, void* ws, int64_t ws_bytes, hipStrea
   return v ? run_ssm_dt<kF32, true>(a, g, st) : run_ssm_dt<kF32, false>(a, g, st);
 }
 
+namespace {
+
+template <int DT, int LPR>
+int run_step(const SsmStepArgs& a, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(a.H), static_cast<unsigned>(a.B));
+  const unsigned lds = static_cast<unsigned>((2 * round_up(a.N, 4) + 2 * a.P) * 4);
+  if (a.N % 4 == 0)
+    ssm_step_kernel<DT, LPR, true><<<grid, 256, lds, TESM_LOGGED(st, ssm_step_kernel<DT, LPR, true>)>>>(a);
+  else
+    ssm_step_kernel<DT, LPR, false><<<grid, 256, lds, TESM_LOGGED(st, ssm_step_kernel<DT, LPR, false>)>>>(a);
+  return check_launch("selective scan step");
+}
+
+template <int DT>
+int run_step_dt(const SsmStepArgs& a, hipStream_t st) {
+  if (a.N <= 16) return run_step<DT, 4>(a, st);
+  if (a.N <= 32) return run_step<DT, 8>(a, st);
+  if (a.N <= 64) return run_step<DT, 16>(a, st);
+  return a.N <= 128 ? run_step<DT, 32>(a, st) : run_step<DT, 64>(a, st);
+}
+
+}  // namespace
+
 int launch_selective_scan_step(const SsmStepArgs& a, hipStream_t st) {
   TESM_REQUIRE((a.dt == kF32 || a.dt == kBF16) && (a.w_dt == kF32 || a.w_dt == kBF16), kErrInvalidArg,
                "selective scan step: dtypes must be 0 or 1");
   TESM_REQUIRE(a.B >= 0 && a.H >= 1 && a.P >= 1 && a.G >= 1 && a.N >= 1 && a.H % a.G == 0 && a.B < 65536 &&
-                   a.H < (1LL << 20) && a.P < (1LL << 20) && a.H * a.P < (1LL << 24),
+                   a.H < (1LL << 20) && a.P <= 4096 && a.H * a.P < (1LL << 24),
                kErrInvalidArg, "selective scan step: bad sizes (n_groups must divide the heads)");
   TESM_REQUIRE(a.N <= kSsmMaxN, kErrUnsupported, "selective scan step: need at most 256 states");
   const int64_t C = a.H * a.P + 2 * a.G * a.N;
@@ -914,12 +1028,7 @@ int launch_selective_scan_step(const SsmStepArgs& a, hipStream_t st) {
                  "selective scan step: the convolution needs its state, and another buffer for the state after");
   }
   if (a.B == 0) return kOk;
-  const dim3 grid(static_cast<unsigned>(a.H), static_cast<unsigned>(a.B));
-  if (a.dt == kBF16)
-    ssm_step_kernel<kBF16><<<grid, 256, 0, TESM_LOGGED(st, ssm_step_kernel<kBF16>)>>>(a);
-  else
-    ssm_step_kernel<kF32><<<grid, 256, 0, TESM_LOGGED(st, ssm_step_kernel<kF32>)>>>(a);
-  return check_launch("selective scan step");
+  return a.dt == kBF16 ? run_step_dt<kBF16>(a, st) : run_step_dt<kF32>(a, st);
 }
 
 }  // namespace tesm
