@@ -754,33 +754,44 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmArgs a, SsmGrid gr) {
 // ---------------------------------------------------------------------------
 typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(4)));
 
-// Convolved value of channel c of the token; the state moves on where `keep`.
-template <int DT>
-__device__ __forceinline__ float step_channel(const SsmStepArgs& a, int64_t b, int c, int64_t C, bool keep) {
-  const uint32_t now = ld_bits<DT>(a.row, b * a.ld_row + c);
-  if (!a.conv_weight) return from_bits<DT>(now);
+// A channel's inputs, as raw bits: the rows before the token and the token's, its filter and bias.
+struct StepChannel {
+  uint32_t past[kConvMaxW], w[kConvMaxW], bias;
+};
+template <int DT, int WDT>
+__device__ __forceinline__ void step_load(const SsmStepArgs& a, int64_t b, int c, int64_t C, StepChannel& s) {
+  const int W = a.conv_weight ? static_cast<int>(a.W) : 1;
+#pragma unroll
+  for (int j = 0; j < kConvMaxW; ++j)
+    if (j < W - 1) {
+      s.past[j] = ld_bits<DT>(a.conv_state, (b * (W - 1) + j) * C + c);
+      s.w[j] = ld_bits<WDT>(a.conv_weight, static_cast<int64_t>(c) * W + j);
+    }
+  s.past[kConvMaxW - 1] = ld_bits<DT>(a.row, b * a.ld_row + c);
+  if (a.conv_weight) s.w[kConvMaxW - 1] = ld_bits<WDT>(a.conv_weight, static_cast<int64_t>(c) * W + W - 1);
+  s.bias = 0;
+  if (a.conv_bias) s.bias = ld_bits<WDT>(a.conv_bias, c);
+}
+// Its convolved value; the state moves on where `keep`.
+template <int DT, int WDT>
+__device__ __forceinline__ float step_value(const SsmStepArgs& a, int64_t b, int c, int64_t C, const StepChannel& s, bool keep) {
+  if (!a.conv_weight) return from_bits<DT>(s.past[kConvMaxW - 1]);
   const int W = static_cast<int>(a.W);
-  uint32_t past[kConvMaxW];
-  float w[kConvMaxW];
+  auto put = [&](int j, uint32_t v) {
+    if constexpr (DT == kBF16)
+      static_cast<uint16_t*>(a.conv_state_out)[(b * (W - 1) + j) * C + c] = static_cast<uint16_t>(v);
+    else
+      static_cast<uint32_t*>(a.conv_state_out)[(b * (W - 1) + j) * C + c] = v;
+  };
+  float acc = from_bits<WDT>(s.bias);
 #pragma unroll
   for (int j = 0; j < kConvMaxW; ++j)
-    if (j < W) {
-      past[j] = j < W - 1 ? ld_bits<DT>(a.conv_state, (b * (W - 1) + j) * C + c) : now;
-      w[j] = a.w_dt == kBF16 ? ld<kBF16>(a.conv_weight, static_cast<int64_t>(c) * W + j)
-                             : ld<kF32>(a.conv_weight, static_cast<int64_t>(c) * W + j);
+    if (j < W - 1) {
+      acc = __builtin_fmaf(from_bits<DT>(s.past[j]), from_bits<WDT>(s.w[j]), acc);
+      if (keep && j > 0) put(j - 1, s.past[j]);
     }
-  float acc = a.conv_bias ? (a.w_dt == kBF16 ? ld<kBF16>(a.conv_bias, c) : ld<kF32>(a.conv_bias, c)) : 0.0f;
-#pragma unroll
-  for (int j = 0; j < kConvMaxW; ++j)
-    if (j < W) {
-      acc = __builtin_fmaf(from_bits<DT>(past[j]), w[j], acc);
-      if (keep && j > 0) {
-        if constexpr (DT == kBF16)
-          static_cast<uint16_t*>(a.conv_state_out)[(b * (W - 1) + j - 1) * C + c] = static_cast<uint16_t>(past[j]);
-        else
-          static_cast<uint32_t*>(a.conv_state_out)[(b * (W - 1) + j - 1) * C + c] = past[j];
-      }
-    }
+  acc = __builtin_fmaf(from_bits<DT>(s.past[kConvMaxW - 1]), from_bits<WDT>(s.w[kConvMaxW - 1]), acc);
+  if (keep) put(W - 2, s.past[kConvMaxW - 1]);
   return a.silu ? siluf_(acc) : acc;
 }
 
@@ -797,7 +808,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 
 // N4: rows are whole vectors of 4 states.
-template <int DT, int LPR, bool N4>
+template <int DT, int WDT, int LPR, bool N4>
 __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepArgs a) {
   constexpr int RP = 256 / LPR, K = 8;  // rows at a time, and how many times ahead
   extern __shared__ __attribute__((aligned(16))) float lds_step[];
@@ -827,19 +838,31 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepArgs a) {
   };
 #pragma unroll
   for (int k = 0; k < K; ++k) load(p0 + k * RP, raw[k]);
-  for (int e = tid; e < 2 * n4 + P; e += 256) {
-    float v = 0.0f;
-    if (e >= 2 * n4) {
-      v = step_channel<DT>(a, b, h * P + e - 2 * n4, C, true);
-    } else {
-      const int c = e >= n4, i = e - c * n4;
-      if (i < N) v = step_channel<DT>(a, b, HP + (c * static_cast<int>(a.G) + grp) * N + i, C, h % hg == 0);
+  const uint32_t in = ld_bits<DT>(a.dts, b * a.ld_dt + h);
+  const float bias = a.dt_bias ? a.dt_bias[h] : 0.0f, rate = a.A[h];
+  // two channels of B, C and x at a time: both are on their way before either is used
+  const int count = 2 * n4 + P;
+  auto channel = [&](int e) {  // -1: padding
+    if (e >= 2 * n4) return h * P + e - 2 * n4;
+    const int c = e >= n4, i = e - c * n4;
+    return i < N ? HP + (c * static_cast<int>(a.G) + grp) * N + i : -1;
+  };
+  for (int e = tid; e < count; e += 512) {
+    StepChannel s[2];
+    int c[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      c[k] = e + 256 * k < count ? channel(e + 256 * k) : -1;
+      if (c[k] >= 0) step_load<DT, WDT>(a, b, c[k], C, s[k]);
     }
-    lds_step[e] = v;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (e + 256 * k < count)
+        lds_step[e + 256 * k] = c[k] < 0 ? 0.0f : step_value<DT, WDT>(a, b, c[k], C, s[k], c[k] < HP || h % hg == 0);
   }
-  const float in = ld<DT>(a.dts, b * a.ld_dt + h) + (a.dt_bias ? a.dt_bias[h] : 0.0f);
-  const float d = a.softplus ? softplusf_(in) : in;
-  const float decay = fast_exp(d * a.A[h]);
+  const float sum_in = from_bits<DT>(in) + bias;
+  const float d = a.softplus ? softplusf_(sum_in) : sum_in;
+  const float decay = fast_exp(d * rate);
   __syncthreads();
   f32x4 bv = {0.0f, 0.0f, 0.0f, 0.0f}, cv = bv;
   if (n < N) {
@@ -989,23 +1012,23 @@ int launch_selective_scan(const SsmArgs& a, void* ws, int64_t ws_bytes, hipStrea
 
 namespace {
 
-template <int DT, int LPR>
+template <int DT, int WDT, int LPR>
 int run_step(const SsmStepArgs& a, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(a.H), static_cast<unsigned>(a.B));
   const unsigned lds = static_cast<unsigned>((2 * round_up(a.N, 4) + 2 * a.P) * 4);
   if (a.N % 4 == 0)
-    ssm_step_kernel<DT, LPR, true><<<grid, 256, lds, TESM_LOGGED(st, ssm_step_kernel<DT, LPR, true>)>>>(a);
+    ssm_step_kernel<DT, WDT, LPR, true><<<grid, 256, lds, TESM_LOGGED(st, ssm_step_kernel<DT, WDT, LPR, true>)>>>(a);
   else
-    ssm_step_kernel<DT, LPR, false><<<grid, 256, lds, TESM_LOGGED(st, ssm_step_kernel<DT, LPR, false>)>>>(a);
+    ssm_step_kernel<DT, WDT, LPR, false><<<grid, 256, lds, TESM_LOGGED(st, ssm_step_kernel<DT, WDT, LPR, false>)>>>(a);
   return check_launch("selective scan step");
 }
 
-template <int DT>
+template <int DT, int WDT>
 int run_step_dt(const SsmStepArgs& a, hipStream_t st) {
-  if (a.N <= 16) return run_step<DT, 4>(a, st);
-  if (a.N <= 32) return run_step<DT, 8>(a, st);
-  if (a.N <= 64) return run_step<DT, 16>(a, st);
-  return a.N <= 128 ? run_step<DT, 32>(a, st) : run_step<DT, 64>(a, st);
+  if (a.N <= 16) return run_step<DT, WDT, 4>(a, st);
+  if (a.N <= 32) return run_step<DT, WDT, 8>(a, st);
+  if (a.N <= 64) return run_step<DT, WDT, 16>(a, st);
+  return a.N <= 128 ? run_step<DT, WDT, 32>(a, st) : run_step<DT, WDT, 64>(a, st);
 }
 
 }  // namespace
@@ -1028,7 +1051,8 @@ int launch_selective_scan_step(const SsmStepArgs& a, hipStream_t st) {
                  "selective scan step: the convolution needs its state, and another buffer for the state after");
   }
   if (a.B == 0) return kOk;
-  return a.dt == kBF16 ? run_step_dt<kBF16>(a, st) : run_step_dt<kF32>(a, st);
+  if (a.dt == kBF16) return a.w_dt == kBF16 ? run_step_dt<kBF16, kBF16>(a, st) : run_step_dt<kBF16, kF32>(a, st);
+  return a.w_dt == kBF16 ? run_step_dt<kF32, kBF16>(a, st) : run_step_dt<kF32, kF32>(a, st);
 }
 
 }  // namespace tesm
