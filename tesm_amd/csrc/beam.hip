@@ -4,8 +4,13 @@
 // (a NaN logit, a row with an infinite one) and all offers of a beam without a finite score count as -infinity; a
 // finished beam offers its padding token alone, at its own score.
 //
-// Inside a beam the order of the offers is the order of the logits, so each row is reduced to its n largest logits
-// and its logsumexp; requests then merge K lists of n, with the offers compared in 64 bits.
+// Inside a beam the order of the offers is the order of the logits, so each row is reduced to its n largest logits and
+// its logsumexp in one pass (beam_row_kernel), and requests then merge their beams' lists, the offers compared in 64
+// bits (beam_merge_kernel).  Bound by reading the logits once, and next to that by arithmetic: 7 operations per logit, of
+// which the exponential takes four.
+#include <float.h>
+
+#include <cstdlib>
 #include "beam.h"
 
 namespace tesm {
@@ -14,115 +19,306 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// A logit and its index as one number: the larger is the better, equal logits by the lower index.  0 is below all.
+__device__ __forceinline__ uint64_t top_key(float v, int i) {
+  const uint32_t b = __float_as_uint(v + 0.0f);  // (-0 is 0)
+  return static_cast<uint64_t>(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | static_cast<uint32_t>(~i);
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t b = static_cast<uint32_t>(k >> 32);
+  return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ int key_index(uint64_t k) { return static_cast<int>(~static_cast<uint32_t>(k)); }
+
+__device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int d) {
+  const uint32_t lo = __shfl_xor(static_cast<int>(v), d), hi = __shfl_xor(static_cast<int>(v >> 32), d);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+// One step of a bitonic network over the lanes: the larger of a lane and the one d away goes to the lower lane where `down`.
+__device__ __forceinline__ uint64_t bitonic(uint64_t v, int d, bool down) {
+  const uint64_t o = shfl_xor_u64(v, d);
+  const bool low = (threadIdx.x & d) == 0;
+  return (v > o) == (low == down) ? v : o;
+}
+// The 64 best of a falling list (one per lane) and 64 more keys in any order, as a falling list.
+__device__ __forceinline__ uint64_t merge64(uint64_t list, uint64_t more) {
+  const int lane = threadIdx.x & 63;
+  for (int k = 2; k <= 64; k <<= 1)  // `more` rising
+    for (int d = k >> 1; d > 0; d >>= 1) more = bitonic(more, d, (lane & k) != 0);
+  list = list > more ? list : more;
+  for (int d = 32; d > 0; d >>= 1) list = bitonic(list, d, true);
+  return list;
+}
+// The same for two falling lists.
+__device__ __forceinline__ uint64_t merge_lists(uint64_t a, uint64_t b) {
+  const int r = 63 - (threadIdx.x & 63);
+  const uint32_t lo = __shfl(static_cast<int>(b), r), hi = __shfl(static_cast<int>(b >> 32), r);
+  const uint64_t o = static_cast<uint64_t>(hi) << 32 | lo;
+  a = a > o ? a : o;
+  for (int d = 32; d > 0; d >>= 1) a = bitonic(a, d, true);
+  return a;
+}
+__device__ __forceinline__ uint64_t readlane_u64(uint64_t v, int l) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), l);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), l);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(2)));
+
+template <int DT>
+__device__ __forceinline__ void unpack_logits(const any16& u, float (&v)[DT == kBF16 ? 8 : 4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == kBF16) {
+      v[2 * i] = __uint_as_float(u[i] << 16);
+      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    } else {
+      v[i] = __uint_as_float(u[i]);
+    }
+  }
+}
+
+// What a wave knows of its part of a row.
+struct RowPart {
+  uint64_t list;   // falling, one key per lane
+  float max, sum;  // per lane: the largest logit, and the sum of exp(logit - max)
+};
+struct PartSum {
+  double ref, sum;  // the sum of exp(logit) is sum * exp(ref)
+};
+__device__ __forceinline__ PartSum add(const PartSum& a, const PartSum& b) {
+  const double ref = fmax(a.ref, b.ref);  // (equal references may be infinite)
+  return {ref, (a.ref == ref ? a.sum : a.sum * exp(a.ref - ref)) + (b.ref == ref ? b.sum : b.sum * exp(b.ref - ref))};
+}
+
+constexpr int kBeamWaves = 4, kBeamVecs = 4;  // waves per workgroup, 16-byte vectors per lane and step
+
+// One pass over logits [lo, hi) of a row by one wave.  A lane keeps its running maximum and sum.  A logit that may belong
+// to the n best (not below the last of the list) is put into a buffer in LDS; a full buffer is sorted and merged into the
+// list.  The first step's bound is the n-th largest of the lanes' own maxima, so few pass it.
+// The sum's terms are 2^(logit L - ref) with L = log2 e and ref = L times the maximum, rounded: one fused operation and the
+// exponential.  Where a logit is NaN, +infinite or beyond 2e38 this form's sum is NaN or too
+// small, and the pass is made again with CLEAN: terms 2^((logit - max) L), a NaN counts as -infinity.
+template <int DT, bool CLEAN>
+__device__ __forceinline__ RowPart row_pass(const void* row, int lo, int hi, int n, uint64_t* buffer) {
+  constexpr int EV = DT == kBF16 ? 8 : 4, ES = 16 / EV, STEP = 64 * EV * kBeamVecs;
+  const int lane = threadIdx.x & 63;
+  const float inf = __builtin_inff();
+  RowPart p{0, -inf, 0.0f};
+  float bound = -inf;          // a logit below is not among the n best
+  int bound_index = INT32_MAX;  // one equal to it is, up to this index
+  int held = 0;
+  auto flush = [&]() {
+    __builtin_amdgcn_wave_barrier();
+    uint64_t k = lane < held ? buffer[lane] : 0;
+    p.list = merge64(p.list, k);
+    if (held > 64) {
+      k = lane + 64 < held ? buffer[lane + 64] : 0;
+      p.list = merge64(p.list, k);
+    }
+    __builtin_amdgcn_wave_barrier();
+    held = 0;
+    const uint64_t last = readlane_u64(p.list, n - 1);
+    if (last) {
+      bound = key_value(last);
+      bound_index = key_index(last);
+    }
+  };
+  for (int at = lo; at < hi; at += STEP) {
+    any16 raw[kBeamVecs];
+    const bool whole = at + STEP <= hi;
+#pragma unroll
+    for (int u = 0; u < kBeamVecs; ++u) {
+      const int i = at + (u * 64 + lane) * EV;
+      const char* q = static_cast<const char*>(row) + static_cast<int64_t>(i) * ES;
+      if (whole || i + EV <= hi) {
+        raw[u] = *reinterpret_cast<const any16*>(q);
+      } else {  // the last ones: -infinity behind the end, which no test below takes for a logit
+        raw[u] = DT == kBF16 ? any16{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}
+                             : any16{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u};
+#pragma unroll
+        for (int e = 0; e < EV; ++e)
+          if (i + e < hi) {
+            if constexpr (DT == kBF16) {
+              const uint32_t b = reinterpret_cast<const uint16_t*>(q)[e];
+              raw[u][e / 2] = e % 2 ? (raw[u][e / 2] & 0xffffu) | b << 16 : (raw[u][e / 2] & 0xffff0000u) | b;
+            } else {
+              raw[u][e] = reinterpret_cast<const uint32_t*>(q)[e];
+            }
+          }
+      }
+    }
+    float vmax[kBeamVecs], top = -inf;
+#pragma unroll
+    for (int u = 0; u < kBeamVecs; ++u) {
+      float v[EV];
+      unpack_logits<DT>(raw[u], v);
+      vmax[u] = -inf;
+#pragma unroll
+      for (int e = 0; e < EV; ++e) vmax[u] = fmaxf(vmax[u], v[e]);
+      top = fmaxf(top, vmax[u]);
+    }
+    const float mx = fmaxf(p.max, top);
+    float ref, scale;
+    if constexpr (CLEAN) {
+      ref = fmaxf(mx, -FLT_MAX);
+      scale = p.max == mx ? 1.0f : __builtin_amdgcn_exp2f((fmaxf(p.max, -FLT_MAX) - ref) * kLog2e);
+    } else {
+      ref = fmaxf(mx, -2.0e38f) * kLog2e;
+      scale = __builtin_amdgcn_exp2f(fmaxf(p.max, -2.0e38f) * kLog2e - ref);
+    }
+    float sum = p.sum * scale;
+#pragma unroll
+    for (int u = 0; u < kBeamVecs; ++u) {
+      float v[EV];
+      unpack_logits<DT>(raw[u], v);
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        if constexpr (CLEAN) {
+          const float x = __builtin_amdgcn_exp2f((v[e] - ref) * kLog2e);
+          sum += x == x ? x : v[e] == v[e] ? 1.0f : 0.0f;  // (infinity - infinity; a NaN logit)
+        } else {
+          sum += __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], kLog2e, -ref));
+        }
+      }
+    }
+    p.max = mx;
+    p.sum = sum;
+    if (at == lo) {  // n lanes' maxima are not below their n-th largest
+      float s = top == top ? top : -inf;
+      for (int k = 2; k <= 64; k <<= 1)
+        for (int d = k >> 1; d > 0; d >>= 1) {
+          const float o = __shfl_xor(s, d);
+          s = ((lane & d) == 0) == ((lane & k) == 0) ? fmaxf(s, o) : fminf(s, o);
+        }
+      bound = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s), n - 1));
+    }
+#pragma unroll
+    for (int u = 0; u < kBeamVecs; ++u) {
+      if (!__any(vmax[u] >= bound)) continue;
+      float v[EV];
+      unpack_logits<DT>(raw[u], v);
+      const int i = at + (u * 64 + lane) * EV;
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        float x = v[e];
+        if (CLEAN && !(x == x)) x = -inf;
+        const bool take = x >= bound && (x > bound || i + e <= bound_index) && i + e < hi;
+        const uint64_t who = __ballot(take);
+        if (who == 0) continue;
+        if (held + __popcll(who) > 128) {
+          flush();
+          const bool still = take && x >= bound && (x > bound || i + e <= bound_index);
+          const uint64_t left = __ballot(still);
+          const int place = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(left >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(left), 0));
+          if (still) buffer[place] = top_key(x, i + e);
+          held = __popcll(left);
+        } else {
+          const int place = held + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
+          if (take) buffer[place] = top_key(x, i + e);
+          held += __popcll(who);
+        }
+      }
+      if (held >= 64) flush();
+    }
+  }
+  if (held) flush();
+  return p;
+}
+
+// Part blockIdx.x of row blockIdx.y, a quarter of it per wave: its m best keys and its sum.
+template <int DT>
+__global__ __launch_bounds__(64 * kBeamWaves) void beam_row_kernel(BeamArgs a, int m, int part, uint64_t* keys, PartSum* sums) {
+  __shared__ uint64_t buffer[kBeamWaves][128];
+  __shared__ PartSum ps[kBeamWaves];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t r = blockIdx.y;
+  // (offers that do not depend on the logits)
+  if ((a.finished && a.finished[r]) || !(fabsf(a.scores[r]) < __builtin_inff())) return;
+  const char* row = static_cast<const char*>(a.logits) + r * a.ld * (DT == kBF16 ? 2 : 4);
+  const int each = part / kBeamWaves, V = static_cast<int>(a.V);
+  const int lo = min(static_cast<int>(blockIdx.x) * part + wave * each, V), hi = min(lo + each, V);
+  RowPart p = row_pass<DT, false>(row, lo, hi, m, buffer[wave]);
+  // a lane that saw a finite logit has a sum of 1 or more: the largest one's own term
+  const bool again = __any(!(p.sum > 0.5f) && p.max > -__builtin_inff()) || __any(!(p.sum == p.sum));
+  if (again) p = row_pass<DT, true>(row, lo, hi, m, buffer[wave]);
+  // over the lanes, then the waves
+  const float mx = wave_max<64>(p.max), top = fmaxf(mx, again ? -FLT_MAX : -2.0e38f), own = fmaxf(p.max, again ? -FLT_MAX : -2.0e38f);
+  const float scale = p.max == mx ? 1.0f : __builtin_amdgcn_exp2f(again ? (own - top) * kLog2e : own * kLog2e - top * kLog2e);
+  const float s = wave_sum_f<64>(p.sum * scale);
+  const double ref = again ? static_cast<double>(mx) : static_cast<double>(mx * kLog2e) * 0.69314718055994530942;
+  if (lane == 0) ps[wave] = {ref, s};
+  buffer[wave][lane] = p.list;
+  __syncthreads();
+  if (wave) return;
+  for (int w = 1; w < kBeamWaves; ++w) p.list = merge_lists(p.list, buffer[w][lane]);
+  const int64_t at = r * gridDim.x + blockIdx.x;
+  if (lane < m) keys[at * m + lane] = p.list;
+  if (lane == 0) {
+    PartSum o = ps[0];
+    for (int w = 1; w < kBeamWaves; ++w) o = add(o, ps[w]);
+    sums[at] = o;
+  }
+}
+
 // Larger first, equal ones by index.
 __device__ __forceinline__ bool before(double v, int64_t i, double w, int64_t j) { return v > w || (v == w && i < j); }
 
-template <int DT>
-__device__ __forceinline__ float logit(const void* row, int64_t v) {
-  const float x = ld<DT>(row, v);
-  return x == x ? x : -__builtin_inff();
-}
-
-struct RowTop {
-  float value;
-  int32_t index;
+struct Offer {
+  double value;
+  int64_t flat;  // k * V + v
 };
 
-template <int DT>
-__global__ __launch_bounds__(256) void beam_row_kernel(BeamArgs a, int m, RowTop* top, double* lse) {
-  __shared__ double red[4];
-  __shared__ RowTop best[4];
-  const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const char* row = static_cast<const char*>(a.logits) + r * a.ld * (DT == kBF16 ? 2 : 4);
-  float mx = -__builtin_inff();
-  for (int64_t v = tid; v < a.V; v += 256) mx = fmaxf(mx, logit<DT>(row, v));
-  mx = wave_max<64>(mx);
-  if (lane == 0) red[wave] = mx;
-  __syncthreads();
-  mx = static_cast<float>(fmax(fmax(red[0], red[1]), fmax(red[2], red[3])));
-  __syncthreads();
-  double sum = 0.0;
-  for (int64_t v = tid; v < a.V; v += 256) sum += __builtin_amdgcn_exp2f((logit<DT>(row, v) - mx) * kLog2e);
-  sum = wave_sum_d<64>(sum);
-  if (lane == 0) red[wave] = sum;
-  __syncthreads();
-  if (tid == 0) lse[r] = static_cast<double>(mx) + log((red[0] + red[1]) + (red[2] + red[3]));
-  float pv = __builtin_inff();
-  int64_t pi = -1;
-  for (int i = 0; i < m; ++i) {  // the next one in order
-    float bv = -__builtin_inff();
-    int64_t bi = INT32_MAX;
-    for (int64_t v = tid; v < a.V; v += 256) {
-      const float x = logit<DT>(row, v);
-      if (before(pv, pi, x, v) && before(x, v, bv, bi)) bv = x, bi = v;
-    }
-    for (int d = 32; d > 0; d >>= 1) {
-      const float ov = __shfl_xor(bv, d);
-      const int64_t oi = __shfl_xor(static_cast<int>(bi), d);
-      if (before(ov, oi, bv, bi)) bv = ov, bi = oi;
-    }
-    __syncthreads();
-    if (lane == 0) best[wave] = {bv, static_cast<int32_t>(bi)};
-    __syncthreads();
-    for (int w = 0; w < 4; ++w)
-      if (before(best[w].value, best[w].index, bv, bi)) bv = best[w].value, bi = best[w].index;
-    if (tid == 0) top[r * m + i] = {bv, static_cast<int32_t>(bi)};
-    pv = bv;
-    pi = bi;
-  }
-}
-
-// Offer i of beam k in the beam's own order: its value, and its token.
-__device__ __forceinline__ double offer(const BeamArgs& a, int64_t r, int m, int i, const RowTop* top, const double* lse,
-                                        int64_t& token) {
-  const float s = a.scores[r];
-  const double inf = __builtin_inf();
-  const bool live = fabsf(s) < __builtin_inff();
-  if (live && a.finished && a.finished[r]) {
-    token = i == 0 ? a.pad : (i <= a.pad ? i - 1 : i);
-    return i == 0 ? static_cast<double>(s) : -inf;
-  }
-  if (live && fabs(lse[r]) < inf) {
-    token = top[r * m + i].index;
-    return static_cast<double>(s) + (static_cast<double>(top[r * m + i].value) - lse[r]);
-  }
-  token = i;
-  return -inf;
-}
-
-// One wave per request.
-__global__ __launch_bounds__(64) void beam_merge_kernel(BeamArgs a, int m, const RowTop* top, const double* lse) {
+// One workgroup per request: a wave per beam merges its parts' lists into the beam's m best offers; the offers' ranks
+// among all beams' are then counted.
+__global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a, int m, int parts, const uint64_t* keys, const PartSum* sums) {
+  extern __shared__ __attribute__((aligned(16))) char lds_beam[];
+  Offer* const offers = reinterpret_cast<Offer*>(lds_beam);
   const int64_t b = blockIdx.x;
-  const int lane = threadIdx.x;
-  const int count = static_cast<int>(a.K) * m;
-  double pv = __builtin_inf();
-  int64_t pi = -1;
-  for (int o = 0; o < static_cast<int>(a.n); ++o) {
-    double bv = -__builtin_inf();
-    int64_t bi = INT64_MAX;
-    for (int c = lane; c < count; c += 64) {
-      const int64_t k = c / m;
-      int64_t token;
-      const double v = offer(a, b * a.K + k, m, c % m, top, lse, token);
-      const int64_t flat = k * a.V + token;
-      if (before(pv, pi, v, flat) && before(v, flat, bv, bi)) bv = v, bi = flat;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int K = static_cast<int>(a.K), n = static_cast<int>(a.n), count = K * m;
+  const double inf = __builtin_inf();
+  for (int k = wave; k < K; k += 4) {
+    const int64_t r = b * K + k;
+    const float score = a.scores[r];
+    const bool live = fabsf(score) < __builtin_inff(), done = a.finished && a.finished[r];
+    double value = -inf;
+    int64_t token = lane;
+    if (live && done) {
+      token = lane == 0 ? a.pad : (lane <= a.pad ? lane - 1 : lane);
+      if (lane == 0) value = score;
+    } else if (live) {
+      const uint64_t* kr = keys + r * parts * m;
+      uint64_t list = 0;
+      for (int c = 0; c < parts * m; c += 64) list = merge64(list, c + lane < parts * m ? kr[c + lane] : 0);
+      PartSum q{-inf, 0.0};
+      for (int c = lane; c < parts; c += 64) q = add(q, sums[r * parts + c]);
+      for (int d = 32; d > 0; d >>= 1) q = add(q, {__shfl_xor(q.ref, d), __shfl_xor(q.sum, d)});
+      const double lse = q.ref + log(q.sum);
+      if (fabs(lse) < inf) {
+        value = static_cast<double>(score) + (static_cast<double>(key_value(list)) - lse);
+        token = key_index(list);
+      }
     }
-    for (int d = 32; d > 0; d >>= 1) {
-      const double ov = __shfl_xor(bv, d);
-      const int64_t oi = __shfl_xor(static_cast<long long>(bi), d);
-      if (before(ov, oi, bv, bi)) bv = ov, bi = oi;
+    if (lane < m) offers[k * m + lane] = {value, k * a.V + token};
+  }
+  __syncthreads();
+  for (int c = tid; c < count; c += 256) {
+    const Offer o = offers[c];
+    int rank = 0;
+    if (c % m >= n) continue;
+    for (int j = 0; j < count; ++j) {
+      const Offer q = offers[j];
+      rank += before(q.value, q.flat, o.value, o.flat);
     }
-    if (lane == 0) {
-      const int64_t k = bi / a.V, token = bi % a.V;
-      a.out_scores[b * a.n + o] = static_cast<float>(bv);
-      a.parents[b * a.n + o] = k;
-      a.tokens[b * a.n + o] = token;
-      if (a.finished_out)
-        a.finished_out[b * a.n + o] = (a.finished && a.finished[b * a.K + k]) || (a.eos >= 0 && token == a.eos);
-    }
-    pv = bv;
-    pi = bi;
+    if (rank >= n) continue;
+    const int64_t k = c / m, token = o.flat - k * a.V;
+    a.out_scores[b * n + rank] = static_cast<float>(o.value);
+    a.parents[b * n + rank] = k;
+    a.tokens[b * n + rank] = token;
+    if (a.finished_out)
+      a.finished_out[b * n + rank] = (a.finished && a.finished[b * K + k]) || (a.eos >= 0 && token == a.eos);
   }
 }
 
@@ -141,29 +337,24 @@ struct ReorderTable {
   } t[kReorderTensors];
 };
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 // A thread moves one unit of all K rows of a request: every load before the first store, so a row may be the parent
-// of several others and be overwritten itself.  Rows that stay are neither read nor written.
+// of several others and be overwritten itself.  Rows that stay are neither read nor written: in their place one that is
+// read anyway is read again (a branch per row around the loads would keep them from being under way together).
 template <typename U, int KM>
-__device__ __forceinline__ void reorder_unit(char* at, int64_t pitch, const int64_t* parents, int K) {
+__device__ __forceinline__ void reorder_unit(char* at, int64_t pitch, const int (&from)[KM], uint64_t moves) {
   U v[KM];
-#pragma unroll
-  for (int k = 0; k < KM; ++k) {
-    if (k >= K) break;
-    const int64_t p = parents[k];
-    if (p != k && p >= 0 && p < K) v[k] = *reinterpret_cast<const U*>(at + p * pitch);
-  }
-#pragma unroll
-  for (int k = 0; k < KM; ++k) {
-    if (k >= K) break;
-    const int64_t p = parents[k];
-    if (p != k && p >= 0 && p < K) *reinterpret_cast<U*>(at + k * pitch) = v[k];
-  }
+#pragma clang loop unroll(full)
+  for (int k = 0; k < KM; ++k) v[k] = *reinterpret_cast<const U*>(at + from[k] * pitch);
+#pragma clang loop unroll(full)
+  for (int k = 0; k < KM; ++k)
+    if (moves >> k & 1) *reinterpret_cast<U*>(at + k * pitch) = v[k];
 }
 
 template <int KM>
-__global__ __launch_bounds__(256) void reorder_rows_kernel(ReorderTable tab, const int64_t* parents, int K) {
+__global__ __launch_bounds__(256) void reorder_rows_kernel(ReorderTable tab, const int64_t* __restrict__ parents, int K) {
   const int64_t b = blockIdx.y;
-  const int64_t* par = parents + b * K;
   int lo = 0, hi = tab.count;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -173,53 +364,94 @@ __global__ __launch_bounds__(256) void reorder_rows_kernel(ReorderTable tab, con
       hi = mid;
   }
   const ReorderTable::Entry& e = tab.t[lo];
-  const int64_t off = (static_cast<int64_t>(blockIdx.x - e.block0) * 256 + threadIdx.x) * e.unit;
-  if (blockIdx.x == 0 && threadIdx.x < K && (par[threadIdx.x] < 0 || par[threadIdx.x] >= K))
+  // the rows' sources, uniform over the workgroup
+  int from[KM], any = 0;
+  uint64_t moves = 0;
+  bool bad = false;
+#pragma clang loop unroll(full)
+  for (int k = 0; k < KM; ++k) {
+    from[k] = k;
+    if (k < K) {
+      const int64_t p = parents[b * K + k];
+      if (p < 0 || p >= K)
+        bad = true;
+      else
+        from[k] = __builtin_amdgcn_readfirstlane(static_cast<int>(p));
+    }
+    if (from[k] != k) moves |= 1ull << k, any = from[k];
+  }
+  if (bad && blockIdx.x == 0 && threadIdx.x == 0)
     __hip_atomic_fetch_or(&g_reorder_status, 2u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (off >= e.bytes) return;
+  const int64_t off = (static_cast<int64_t>(blockIdx.x - e.block0) * 256 + threadIdx.x) * e.unit;
+  if (moves == 0 || off >= e.bytes) return;
+#pragma clang loop unroll(full)
+  for (int k = 0; k < KM; ++k)
+    if (!(moves >> k & 1)) from[k] = any;
   char* at = e.p + b * K * e.pitch + off;
   if (e.unit == 16)
-    reorder_unit<uint4, KM>(at, e.pitch, par, K);
+    reorder_unit<u32x4, KM>(at, e.pitch, from, moves);
   else if (e.unit == 4)
-    reorder_unit<uint32_t, KM>(at, e.pitch, par, K);
+    reorder_unit<uint32_t, KM>(at, e.pitch, from, moves);
   else
-    reorder_unit<uint8_t, KM>(at, e.pitch, par, K);
+    reorder_unit<uint8_t, KM>(at, e.pitch, from, moves);
 }
 
 int64_t round256(int64_t v) { return round_up(std::max<int64_t>(v, 1), 256); }
 
-}  // namespace
-
-int64_t beam_select_ws_bytes(const BeamArgs& a) {
-  const int64_t m = std::min(a.n, a.V), rows = a.B * a.K;
-  return round256(rows * m * static_cast<int64_t>(sizeof(RowTop))) + round256(rows * 8);
+int64_t beam_target() { const char* e = getenv("BEAM_TARGET"); return e ? atoi(e) : 2048; }
+// Logits per workgroup: parts of a row until about 8 waves per SIMD run, of at least one step per wave.
+int64_t beam_part(const BeamArgs& a) {
+  const int64_t step = 64 * kBeamVecs * (a.dt == kBF16 ? 8 : 4) * kBeamWaves;
+  const int64_t want = std::max<int64_t>(1, beam_target() / std::max<int64_t>(1, a.B * a.K));
+  return std::max<int64_t>(1, ((a.V + want - 1) / want + step - 1) / step) * step;
+}
+int64_t beam_parts(const BeamArgs& a) {
+  const int64_t part = beam_part(a);
+  return (a.V + part - 1) / part;
 }
 
-int launch_beam_select(const BeamArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+int beam_check(const BeamArgs& a) {
   TESM_REQUIRE(a.dt == kF32 || a.dt == kBF16, kErrInvalidArg, "beam select: dtype must be 0 or 1");
-  TESM_REQUIRE(a.B >= 0 && a.K >= 1 && a.V >= 1 && a.n >= 1 && a.B < (1LL << 24) && a.V < (1LL << 31) - 65536, kErrInvalidArg,
-               "beam select: bad sizes");
+  TESM_REQUIRE(a.B >= 0 && a.K >= 1 && a.V >= 1 && a.n >= 1 && a.B < (1LL << 24) && a.V < (1LL << 31) - 65536,
+               kErrInvalidArg, "beam select: bad sizes");
   TESM_REQUIRE(a.K <= kBeamMaxN && a.n <= kBeamMaxN, kErrUnsupported,
                "beam select: at most 64 beams and 64 chosen candidates");
   TESM_REQUIRE(a.n <= a.K * a.V, kErrInvalidArg, "beam select: more candidates asked for than there are");
+  return kOk;
+}
+
+}  // namespace
+
+int64_t beam_select_ws_bytes(const BeamArgs& a) {
+  if (beam_check(a) != kOk) return -1;
+  const int64_t all = a.B * a.K * beam_parts(a), m = std::min(a.n, a.V);
+  return round256(all * m * 8) + round256(all * static_cast<int64_t>(sizeof(PartSum)));
+}
+
+int launch_beam_select(const BeamArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+  if (int rc = beam_check(a)) return rc;
   TESM_REQUIRE(a.ld >= a.V, kErrInvalidArg, "beam select: ld < V");
   TESM_REQUIRE(!a.finished || (a.pad >= 0 && a.pad < a.V), kErrInvalidArg, "beam select: pad outside the vocabulary");
   TESM_REQUIRE(a.eos < a.V, kErrInvalidArg, "beam select: eos outside the vocabulary");
   if (a.B == 0) return kOk;
   TESM_REQUIRE(a.logits && a.scores && a.out_scores && a.parents && a.tokens, kErrInvalidArg,
                "beam select: need logits, scores and the three outputs");
+  TESM_REQUIRE(a.B * a.K < 65536, kErrUnsupported, "beam select: too many beams for one call");
   TESM_REQUIRE(ws && ws_bytes >= beam_select_ws_bytes(a) && aligned(ws, 8), kErrWorkspace,
                "beam select: workspace too small or not 8-byte aligned");
-  const int m = static_cast<int>(std::min(a.n, a.V));
+  const int m = static_cast<int>(std::min(a.n, a.V)), parts = static_cast<int>(beam_parts(a));
+  const int part = static_cast<int>(beam_part(a));
   const int64_t rows = a.B * a.K;
-  RowTop* top = static_cast<RowTop*>(ws);
-  double* lse = reinterpret_cast<double*>(static_cast<char*>(ws) + round256(rows * m * static_cast<int64_t>(sizeof(RowTop))));
-  const unsigned grid = static_cast<unsigned>(rows);
+  uint64_t* keys = static_cast<uint64_t*>(ws);
+  PartSum* sums = reinterpret_cast<PartSum*>(static_cast<char*>(ws) + round256(rows * parts * m * 8));
+  const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(rows));
+  constexpr int T = 64 * kBeamWaves;
   if (a.dt == kBF16)
-    beam_row_kernel<kBF16><<<grid, 256, 0, TESM_LOGGED(st, beam_row_kernel<kBF16>)>>>(a, m, top, lse);
+    beam_row_kernel<kBF16><<<grid, T, 0, TESM_LOGGED(st, beam_row_kernel<kBF16>)>>>(a, m, part, keys, sums);
   else
-    beam_row_kernel<kF32><<<grid, 256, 0, TESM_LOGGED(st, beam_row_kernel<kF32>)>>>(a, m, top, lse);
-  beam_merge_kernel<<<static_cast<unsigned>(a.B), 64, 0, TESM_LOGGED(st, beam_merge_kernel)>>>(a, m, top, lse);
+    beam_row_kernel<kF32><<<grid, T, 0, TESM_LOGGED(st, beam_row_kernel<kF32>)>>>(a, m, part, keys, sums);
+  const unsigned lds = static_cast<unsigned>(a.K * m * static_cast<int64_t>(sizeof(Offer)));
+  beam_merge_kernel<<<static_cast<unsigned>(a.B), 256, lds, TESM_LOGGED(st, beam_merge_kernel)>>>(a, m, parts, keys, sums);
   return check_launch("beam select");
 }
 
