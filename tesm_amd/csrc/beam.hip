@@ -10,7 +10,6 @@
 // which the exponential takes four.
 #include <float.h>
 
-#include <cstdlib>
 #include "beam.h"
 
 namespace tesm {
@@ -79,6 +78,12 @@ __device__ __forceinline__ void unpack_logits(const any16& u, float (&v)[DT == k
   }
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // What a wave knows of its part of a row.
 struct RowPart {
   uint64_t list;   // falling, one key per lane
@@ -96,7 +101,8 @@ constexpr int kBeamWaves = 4, kBeamVecs = 4;  // waves per workgroup, 16-byte ve
 
 // One pass over logits [lo, hi) of a row by one wave.  A lane keeps its running maximum and sum.  A logit that may belong
 // to the n best (not below the last of the list) is put into a buffer in LDS; a full buffer is sorted and merged into the
-// list.  The first step's bound is the n-th largest of the lanes' own maxima, so few pass it.
+// list.  The n-th largest of the lanes' own maxima is not above the n-th largest logit so far: taken as the bound after
+// the first step and whenever the steps have doubled, it lets few logits through.
 // The sum's terms are 2^(logit L - ref) with L = log2 e and ref = L times the maximum, rounded: one fused operation and the
 // exponential.  Where a logit is NaN, +infinite or beyond 2e38 this form's sum is NaN or too
 // small, and the pass is made again with CLEAN: terms 2^((logit - max) L), a NaN counts as -infinity.
@@ -108,7 +114,7 @@ __device__ __forceinline__ RowPart row_pass(const void* row, int lo, int hi, int
   RowPart p{0, -inf, 0.0f};
   float bound = -inf;          // a logit below is not among the n best
   int bound_index = INT32_MAX;  // one equal to it is, up to this index
-  int held = 0;
+  int held = 0, step = 0;
   auto flush = [&]() {
     __builtin_amdgcn_wave_barrier();
     uint64_t k = lane < held ? buffer[lane] : 0;
@@ -125,39 +131,51 @@ __device__ __forceinline__ RowPart row_pass(const void* row, int lo, int hi, int
       bound_index = key_index(last);
     }
   };
-  for (int at = lo; at < hi; at += STEP) {
-    any16 raw[kBeamVecs];
+  any16 raw[kBeamVecs], ahead[kBeamVecs];
+  auto load = [&](int at, any16 (&to)[kBeamVecs]) {
     const bool whole = at + STEP <= hi;
 #pragma unroll
     for (int u = 0; u < kBeamVecs; ++u) {
       const int i = at + (u * 64 + lane) * EV;
       const char* q = static_cast<const char*>(row) + static_cast<int64_t>(i) * ES;
       if (whole || i + EV <= hi) {
-        raw[u] = *reinterpret_cast<const any16*>(q);
+        to[u] = *reinterpret_cast<const any16*>(q);
       } else {  // the last ones: -infinity behind the end, which no test below takes for a logit
-        raw[u] = DT == kBF16 ? any16{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}
-                             : any16{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u};
+        to[u] = DT == kBF16 ? any16{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}
+                            : any16{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u};
 #pragma unroll
         for (int e = 0; e < EV; ++e)
           if (i + e < hi) {
             if constexpr (DT == kBF16) {
               const uint32_t b = reinterpret_cast<const uint16_t*>(q)[e];
-              raw[u][e / 2] = e % 2 ? (raw[u][e / 2] & 0xffffu) | b << 16 : (raw[u][e / 2] & 0xffff0000u) | b;
+              to[u][e / 2] = e % 2 ? (to[u][e / 2] & 0xffffu) | b << 16 : (to[u][e / 2] & 0xffff0000u) | b;
             } else {
-              raw[u][e] = reinterpret_cast<const uint32_t*>(q)[e];
+              to[u][e] = reinterpret_cast<const uint32_t*>(q)[e];
             }
           }
       }
     }
+  };
+  if (lo < hi) load(lo, ahead);
+  for (int at = lo; at < hi; at += STEP) {
+#pragma unroll
+    for (int u = 0; u < kBeamVecs; ++u) raw[u] = ahead[u];
+    if (at + STEP < hi) load(at + STEP, ahead);  // under this step's arithmetic
     float vmax[kBeamVecs], top = -inf;
 #pragma unroll
     for (int u = 0; u < kBeamVecs; ++u) {
       float v[EV];
       unpack_logits<DT>(raw[u], v);
-      vmax[u] = -inf;
+      if constexpr (CLEAN) {
+        vmax[u] = -inf;
 #pragma unroll
-      for (int e = 0; e < EV; ++e) vmax[u] = fmaxf(vmax[u], v[e]);
-      top = fmaxf(top, vmax[u]);
+        for (int e = 0; e < EV; ++e) vmax[u] = fmaxf(vmax[u], v[e]);
+        top = fmaxf(top, vmax[u]);
+      } else {  // (the library's fmaxf first quiets each operand; a NaN voids this pass anyway)
+        vmax[u] = max3(v[0], v[1], max3(v[2], v[3], v[3]));
+        if constexpr (EV == 8) vmax[u] = max3(vmax[u], v[4], max3(v[5], v[6], v[7]));
+        top = max3(top, vmax[u], vmax[u]);
+      }
     }
     const float mx = fmaxf(p.max, top);
     float ref, scale;
@@ -185,15 +203,20 @@ __device__ __forceinline__ RowPart row_pass(const void* row, int lo, int hi, int
     }
     p.max = mx;
     p.sum = sum;
-    if (at == lo) {  // n lanes' maxima are not below their n-th largest
-      float s = top == top ? top : -inf;
+    if ((step & (step + 1)) == 0) {  // after 1, 2, 4, 8 .. steps
+      float s = mx == mx ? mx : -inf;
       for (int k = 2; k <= 64; k <<= 1)
         for (int d = k >> 1; d > 0; d >>= 1) {
           const float o = __shfl_xor(s, d);
           s = ((lane & d) == 0) == ((lane & k) == 0) ? fmaxf(s, o) : fminf(s, o);
         }
-      bound = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s), n - 1));
+      s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s), n - 1));
+      if (s > bound) {
+        bound = s;
+        bound_index = INT32_MAX;
+      }
     }
+    ++step;
 #pragma unroll
     for (int u = 0; u < kBeamVecs; ++u) {
       if (!__any(vmax[u] >= bound)) continue;
@@ -272,14 +295,14 @@ struct Offer {
 
 // One workgroup per request: a wave per beam merges its parts' lists into the beam's m best offers; the offers' ranks
 // among all beams' are then counted.
-__global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a, int m, int parts, const uint64_t* keys, const PartSum* sums) {
+__global__ __launch_bounds__(512) void beam_merge_kernel(BeamArgs a, int m, int parts, const uint64_t* keys, const PartSum* sums) {
   extern __shared__ __attribute__((aligned(16))) char lds_beam[];
   Offer* const offers = reinterpret_cast<Offer*>(lds_beam);
   const int64_t b = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int K = static_cast<int>(a.K), n = static_cast<int>(a.n), count = K * m;
   const double inf = __builtin_inf();
-  for (int k = wave; k < K; k += 4) {
+  for (int k = wave; k < K; k += 8) {
     const int64_t r = b * K + k;
     const float score = a.scores[r];
     const bool live = fabsf(score) < __builtin_inff(), done = a.finished && a.finished[r];
@@ -292,10 +315,15 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a, int m, int 
       const uint64_t* kr = keys + r * parts * m;
       uint64_t list = 0;
       for (int c = 0; c < parts * m; c += 64) list = merge64(list, c + lane < parts * m ? kr[c + lane] : 0);
-      PartSum q{-inf, 0.0};
-      for (int c = lane; c < parts; c += 64) q = add(q, sums[r * parts + c]);
-      for (int d = 32; d > 0; d >>= 1) q = add(q, {__shfl_xor(q.ref, d), __shfl_xor(q.sum, d)});
-      const double lse = q.ref + log(q.sum);
+      double ref = -inf, s = 0.0;
+      for (int c = lane; c < parts; c += 64) ref = fmax(ref, sums[r * parts + c].ref);
+      for (int d = 32; d > 0; d >>= 1) ref = fmax(ref, __shfl_xor(ref, d));
+      for (int c = lane; c < parts; c += 64) {
+        const PartSum q = sums[r * parts + c];
+        s += q.ref == ref ? q.sum : q.sum * exp(q.ref - ref);
+      }
+      s = wave_sum_d<64>(s);
+      const double lse = ref + log(s);
       if (fabs(lse) < inf) {
         value = static_cast<double>(score) + (static_cast<double>(key_value(list)) - lse);
         token = key_index(list);
@@ -304,7 +332,7 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(BeamArgs a, int m, int 
     if (lane < m) offers[k * m + lane] = {value, k * a.V + token};
   }
   __syncthreads();
-  for (int c = tid; c < count; c += 256) {
+  for (int c = tid; c < count; c += 512) {
     const Offer o = offers[c];
     int rank = 0;
     if (c % m >= n) continue;
@@ -398,11 +426,12 @@ __global__ __launch_bounds__(256) void reorder_rows_kernel(ReorderTable tab, con
 
 int64_t round256(int64_t v) { return round_up(std::max<int64_t>(v, 1), 256); }
 
-int64_t beam_target() { const char* e = getenv("BEAM_TARGET"); return e ? atoi(e) : 2048; }
-// Logits per workgroup: parts of a row until about 8 waves per SIMD run, of at least one step per wave.
+// Logits per workgroup: rows are divided until about 4 workgroups per CU run, into at least one step per wave.  More of
+// them sort and merge more often, fewer leave loads uncovered: 512 rows of 151936 logits in 512, 1024, 2048 and 4096
+// workgroups 51, 46, 50 and 54 us.
 int64_t beam_part(const BeamArgs& a) {
   const int64_t step = 64 * kBeamVecs * (a.dt == kBF16 ? 8 : 4) * kBeamWaves;
-  const int64_t want = std::max<int64_t>(1, beam_target() / std::max<int64_t>(1, a.B * a.K));
+  const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(1, a.B * a.K));
   return std::max<int64_t>(1, ((a.V + want - 1) / want + step - 1) / step) * step;
 }
 int64_t beam_parts(const BeamArgs& a) {
@@ -451,7 +480,7 @@ int launch_beam_select(const BeamArgs& a, void* ws, int64_t ws_bytes, hipStream_
   else
     beam_row_kernel<kF32><<<grid, T, 0, TESM_LOGGED(st, beam_row_kernel<kF32>)>>>(a, m, part, keys, sums);
   const unsigned lds = static_cast<unsigned>(a.K * m * static_cast<int64_t>(sizeof(Offer)));
-  beam_merge_kernel<<<static_cast<unsigned>(a.B), 256, lds, TESM_LOGGED(st, beam_merge_kernel)>>>(a, m, parts, keys, sums);
+  beam_merge_kernel<<<static_cast<unsigned>(a.B), 512, lds, TESM_LOGGED(st, beam_merge_kernel)>>>(a, m, parts, keys, sums);
   return check_launch("beam select");
 }
 

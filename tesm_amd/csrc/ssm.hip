@@ -2,7 +2,6 @@
 //   d_t = softplus(dt_t + dt_bias)        a_t = exp(d_t A)
 //   h_t = a_t h_{t-1} + d_t x_t B_t^T     (P x N, float32)
 //   y_t = h_t C_t + D x_t                 times silu(z_t) where there is a gate
-#include <cstdlib>
 #include "ssm.h"
 
 namespace tesm {
@@ -916,10 +915,8 @@ int states32(const SsmArgs& a) {  // 32-state steps, rounded up to an instantiat
   return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8;
 }
 
-// Segments so that about one workgroup per CU runs; a segment's end state costs as much traffic as about 85 of its
+// Segments so that about two workgroups per CU run; a segment's end state costs as much traffic as about 85 of its
 // rows, so it has several times that.
-int64_t ssm_target() { const char* e = getenv("SSM_TARGET"); return e ? atoi(e) : 512; }
-int64_t ssm_min() { const char* e = getenv("SSM_MIN"); return e ? atoi(e) : kMinSegment; }
 SsmGrid ssm_grid(const SsmArgs& a) {
   SsmGrid g;
   const int64_t hg = a.H / a.G;
@@ -929,8 +926,8 @@ SsmGrid ssm_grid(const SsmArgs& a) {
   g.nh = 4 % g.ps == 0 ? 4 / g.ps : g.ps % 4 == 0 ? 1 : 2;
   const int64_t wgs = a.G * g.wpg, rows = a.seq_starts ? a.B * a.L : a.L;
   const int64_t each = a.seq_starts ? 1 : std::max<int64_t>(a.S, 1);
-  const int64_t want = std::max<int64_t>(1, ssm_target() / std::max<int64_t>(1, wgs * each));
-  g.seg = std::max<int64_t>(ssm_min(), round_up((rows + want - 1) / want, 64));
+  const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(1, wgs * each));
+  g.seg = std::max<int64_t>(kMinSegment, round_up((rows + want - 1) / want, 64));
   if (a.seq_starts)
     g.slots = rows / g.seg + a.S;
   else
