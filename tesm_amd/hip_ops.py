@@ -13,6 +13,7 @@ from __future__ import annotations
 import array
 import ctypes
 import functools
+import math
 from typing import Optional
 
 import torch
@@ -438,32 +439,36 @@ def output_gate(te, cc, sp_packed, sp_cw, ep_packed, ep_cw, local, gate, d_state
 # selective state space pieces: short causal convolution, selective scan, their one-token step
 # ---------------------------------------------------------------------------
 def _no_grad(what: str, *ts) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError(f"{what}: the hip kernels are forward-only: run under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what}: the hip kernels are forward-only: run under torch.no_grad()")
 
 
 def _row_pitch(x: torch.Tensor, lead: int):
     """The pitch in elements of ``x``'s rows (the first ``lead`` dimensions flattened into one row axis, the others
     one contiguous row), or None where ``x`` is not laid out in such rows."""
+    shape, strides = x.shape, x.stride()
     width = 1
-    for n, st in zip(reversed(x.shape[lead:]), reversed(x.stride()[lead:])):
-        if n != 1 and st != width:
-            return None
+    for d in range(len(shape) - 1, lead - 1, -1):
+        n = shape[d]
+        if n != 1 and strides[d] != width:
+            return None if x.numel() else max(math.prod(shape[lead:]), 1)
         width *= n
-    if x.numel() == 0:
-        return max(width, 1)
-    pitch = None  # from the last row dimension that has more than one entry
+    pitch, span = -1, 0  # from the last row dimension that has more than one entry
     for d in range(lead - 1, -1, -1):
-        n, st = x.shape[d], x.stride(d)
+        n = shape[d]
         if n == 1:
             continue
-        if pitch is None:
-            pitch, span = st, n * st
-        elif st != span:
+        if n == 0 or width == 0:
+            return max(width, 1)
+        if pitch < 0:
+            pitch = span = strides[d]
+        elif strides[d] != span:
             return None
-        else:
-            span *= n
-    pitch = width if pitch is None else pitch
+        span *= n
+    if pitch < 0:
+        return width
     return pitch if pitch >= width else None
 
 
@@ -495,7 +500,7 @@ def _f32(t: Optional[torch.Tensor], n: int, name: str, what: str):
         return None
     if t.numel() != n:
         raise ValueError(f"{what}: {name} must hold {n} values, got {tuple(t.shape)}")
-    return t.to(torch.float32).contiguous()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
 def _sequences(seq_starts: Optional[torch.Tensor], B: int, what: str):
@@ -542,8 +547,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         raise ValueError(f"causal_conv: bias must hold {C} values, got {tuple(bias.shape)}")
     if state is not None and state.shape != (S, W - 1, C):
         raise ValueError(f"causal_conv: state must be {(S, W - 1, C)}, got {tuple(state.shape)}")
-    d = _lib.Conv()
-    d.dt, d.w_dt = dt_code(x.dtype), dt_code(weight.dtype)
+    codes = dt_code(x.dtype), dt_code(weight.dtype)
     weight = weight.contiguous()
     bias = bias.contiguous() if bias is not None else None
     state = state.contiguous() if state is not None else None
@@ -553,12 +557,10 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         out = (torch.zeros if seq_starts is not None else torch.empty)((B, L, C), dtype=x.dtype, device=x.device)
     if out.data_ptr() == x.data_ptr() and x.numel():
         raise ValueError("causal_conv: out must not be x")
-    d.B, d.L, d.C, d.W, d.S, d.silu = B, L, C, W, S, int(silu)
     new = torch.empty((S, W - 1, C), dtype=x.dtype, device=x.device)
-    d.x, d.ld_x, d.weight, d.bias = x.data_ptr(), ld, weight.data_ptr(), _ptr(bias)
-    d.seq_starts, d.state = _ptr(seq_starts), _ptr(state)
-    d.y, d.ld_y = out.data_ptr(), _out_rows(out, (B, L, C), x.dtype, 2, "causal_conv")
-    d.state_out = new.data_ptr()
+    # (fields in the descriptor's order)
+    d = _lib.Conv(*codes, B, L, C, W, S, int(silu), x.data_ptr(), ld, weight.data_ptr(), _ptr(bias), _ptr(seq_starts),
+                  _ptr(state), out.data_ptr(), _out_rows(out, (B, L, C), x.dtype, 2, "causal_conv"), new.data_ptr())
     on_device(x.device.index, _lib.load().tesm_hip_causal_conv, ctypes.byref(d), raw_stream(x.device.index))
     return out, new
 
@@ -594,25 +596,26 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         raise ValueError(f"selective_scan: state must be float32 {(S, H, P, N)}, got {state.dtype} {tuple(state.shape)}")
     A, D, dt_bias = (_f32(t, H, n, "selective_scan") for t, n in ((A, "A"), (D, "D"), (dt_bias, "dt_bias")))
     state = state.contiguous() if state is not None else None
-    d = _lib.Ssm()
-    d.dt = dt_code(x.dtype)
-    (x, d.ld_x), (dt, d.ld_dt), (B, d.ld_b), (C, d.ld_c), (z, d.ld_z) = (_as_rows(t, 2) for t in (x, dt, B, C, z))
+    code = dt_code(x.dtype)
+    (x, ld_x), (dt, ld_dt), (B, ld_b), (C, ld_c), (z, ld_z) = (_as_rows(x, 2), _as_rows(dt, 2), _as_rows(B, 2),
+                                                              _as_rows(C, 2), _as_rows(z, 2))
     dev = x.device
     require_device(x, dt, A, B, C, D, z, dt_bias, state, seq_starts, out)
     if out is None:
         out = (torch.zeros if seq_starts is not None else torch.empty)((nb, L, H, P), dtype=x.dtype, device=dev)
-    if x.numel() and out.data_ptr() in (x.data_ptr(), B.data_ptr(), C.data_ptr(), _ptr(z)):
+    px, pb, pc, pz, py = x.data_ptr(), B.data_ptr(), C.data_ptr(), _ptr(z), out.data_ptr()
+    if py in (px, pb, pc, pz) and x.numel():
         raise ValueError("selective_scan: out must not be one of the operands")
     new = torch.empty((S, H, P, N), dtype=torch.float32, device=dev)
-    d.B, d.L, d.H, d.P, d.G, d.N, d.S, d.softplus = nb, L, H, P, G, N, S, int(softplus)
-    d.x, d.dts, d.A, d.Bm, d.Cm = x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr()
-    d.D, d.z, d.dt_bias, d.seq_starts, d.h0 = _ptr(D), _ptr(z), _ptr(dt_bias), _ptr(seq_starts), _ptr(state)
-    d.y, d.ld_y = out.data_ptr(), _out_rows(out, (nb, L, H, P), x.dtype, 2, "selective_scan")
-    d.h_out = new.data_ptr()
+    # (fields in the descriptor's order)
+    d = _lib.Ssm(code, nb, L, H, P, G, N, S, int(softplus), px, ld_x, dt.data_ptr(), ld_dt, A.data_ptr(), pb, ld_b, pc, ld_c,
+                 _ptr(D), pz, ld_z, _ptr(dt_bias), _ptr(seq_starts), _ptr(state), py,
+                 _out_rows(out, (nb, L, H, P), x.dtype, 2, "selective_scan"), new.data_ptr())
     lib = _lib.load()
-    nbytes = int(lib.tesm_hip_selective_scan_ws_bytes(ctypes.byref(d)))
-    ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=dev)
-    on_device(dev.index, lib.tesm_hip_selective_scan, ctypes.byref(d), ws.data_ptr(), nbytes, raw_stream(dev.index))
+    ref = ctypes.byref(d)
+    nbytes = lib.tesm_hip_selective_scan_ws_bytes(ref)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes > 0 else None
+    on_device(dev.index, lib.tesm_hip_selective_scan, ref, _ptr(ws), nbytes, raw_stream(dev.index))
     return out, new
 
 
@@ -645,9 +648,8 @@ def selective_scan_step(row: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, st
         raise ValueError("selective_scan_step: state must be a contiguous float32 tensor (it is updated in place)")
     _same_dtype("selective_scan_step", row.dtype, dt=dt, z=z, conv_state=conv_state)
     A, D, dt_bias = (_f32(t, H, n, "selective_scan_step") for t, n in ((A, "A"), (D, "D"), (dt_bias, "dt_bias")))
-    d = _lib.SsmStep()
-    d.dt = d.w_dt = dt_code(row.dtype)
-    dev = row.device
+    code = w_code = dt_code(row.dtype)
+    W, dev = 0, row.device
     if conv_weight is not None:
         W = conv_weight.shape[-1]
         if conv_weight.shape != (width, W) or not 2 <= W <= 8:
@@ -663,19 +665,20 @@ def selective_scan_step(row: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, st
         elif conv_state_out.shape != conv_state.shape or conv_state_out.dtype != row.dtype or \
                 not conv_state_out.is_contiguous() or (nb and conv_state_out.data_ptr() == conv_state.data_ptr()):
             raise ValueError("selective_scan_step: conv_state_out must be another contiguous tensor like conv_state")
-        d.W, d.w_dt = W, dt_code(conv_weight.dtype)
-        d.conv_weight, d.conv_bias = conv_weight.data_ptr(), _ptr(conv_bias)
-        d.conv_state, d.conv_state_out = conv_state.data_ptr(), conv_state_out.data_ptr()
+        w_code = dt_code(conv_weight.dtype)
     elif conv_bias is not None or conv_state is not None or conv_state_out is not None:
         raise ValueError("selective_scan_step: conv_bias and conv_state need conv_weight")
-    (row, d.ld_row), (dt, d.ld_dt), (z, d.ld_z) = (_as_rows(t, 1) for t in (row, dt, z))
+    (row, ld_row), (dt, ld_dt), (z, ld_z) = _as_rows(row, 1), _as_rows(dt, 1), _as_rows(z, 1)
     require_device(row, dt, A, state, conv_weight, conv_bias, conv_state, conv_state_out, D, z, dt_bias, out)
     if out is None:
         out = torch.empty((nb, H, P), dtype=row.dtype, device=dev)
-    d.B, d.H, d.P, d.G, d.N, d.softplus, d.silu = nb, H, P, G, N, int(softplus), int(silu)
-    d.row, d.dts, d.A, d.D, d.z, d.dt_bias = row.data_ptr(), dt.data_ptr(), A.data_ptr(), _ptr(D), _ptr(z), _ptr(dt_bias)
-    d.state = state.data_ptr()
-    d.y, d.ld_y = out.data_ptr(), _out_rows(out, (nb, H, P), row.dtype, 1, "selective_scan_step")
+        ld_y = H * P
+    else:
+        ld_y = _out_rows(out, (nb, H, P), row.dtype, 1, "selective_scan_step")
+    # (fields in the descriptor's order)
+    d = _lib.SsmStep(code, w_code, nb, H, P, G, N, W, int(softplus), int(silu), row.data_ptr(), ld_row, _ptr(conv_weight),
+                     _ptr(conv_bias), _ptr(conv_state), _ptr(conv_state_out), dt.data_ptr(), ld_dt, A.data_ptr(), _ptr(D),
+                     _ptr(z), ld_z, _ptr(dt_bias), state.data_ptr(), out.data_ptr(), ld_y)
     on_device(dev.index, _lib.load().tesm_hip_selective_scan_step, ctypes.byref(d), raw_stream(dev.index))
     return out, conv_state_out
 
@@ -708,24 +711,23 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
     for name, t in (("pad_token", pad_token if finished is not None else None), ("eos_token", eos_token)):
         if t is not None and not 0 <= t < V:
             raise ValueError(f"beam_select: {name} {t} is outside the vocabulary of {V}")
-    d = _lib.Beam()
-    d.dt = dt_code(logits.dtype)
-    logits, d.ld = _as_rows(logits, 2)
+    code = dt_code(logits.dtype)
+    logits, ld = _as_rows(logits, 2)
     scores = scores.contiguous()
     finished = finished.contiguous() if finished is not None else None
     require_device(logits, scores, finished)
     dev = logits.device
     out = torch.empty((B, n), dtype=torch.float32, device=dev)
-    parents, tokens = (torch.empty((B, n), dtype=torch.int64, device=dev) for _ in range(2))
+    parents, tokens = torch.empty((2, B, n), dtype=torch.int64, device=dev).unbind()
     done = torch.empty((B, n), dtype=torch.bool, device=dev) if finished is not None or eos_token is not None else None
-    d.B, d.K, d.V, d.n = B, K, V, n
-    d.logits, d.scores, d.finished = logits.data_ptr(), scores.data_ptr(), _ptr(finished)
-    d.pad, d.eos = int(pad_token), -1 if eos_token is None else int(eos_token)
-    d.out_scores, d.parents, d.tokens, d.finished_out = out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _ptr(done)
+    # (fields in the descriptor's order)
+    d = _lib.Beam(code, B, K, V, n, logits.data_ptr(), ld, scores.data_ptr(), _ptr(finished), int(pad_token),
+                  -1 if eos_token is None else int(eos_token), out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _ptr(done))
     lib = _lib.load()
-    nbytes = int(lib.tesm_hip_beam_select_ws_bytes(ctypes.byref(d)))
+    ref = ctypes.byref(d)
+    nbytes = lib.tesm_hip_beam_select_ws_bytes(ref)
     ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=dev)
-    on_device(dev.index, lib.tesm_hip_beam_select, ctypes.byref(d), ws.data_ptr(), nbytes, raw_stream(dev.index))
+    on_device(dev.index, lib.tesm_hip_beam_select, ref, ws.data_ptr(), nbytes, raw_stream(dev.index))
     return out, parents, tokens, done
 
 
@@ -745,24 +747,26 @@ def reorder_rows(tensors, parents: torch.Tensor) -> None:
     grad = torch.is_grad_enabled()
     rows, dev = B * K, parents.device
     table = []  # (address, pitch, row bytes) of each: a decode step hands over every layer's caches, so the loop is lean
+    index = parents.get_device()
     for t in tensors:
-        if t.dim() < 1 or t.size(0) != rows:
-            raise ValueError(f"reorder_rows: a tensor of shape {tuple(t.shape)} does not have {rows} rows")
-        if grad:
+        shape = t.shape
+        if not shape or shape[0] != rows:
+            raise ValueError(f"reorder_rows: a tensor of shape {tuple(shape)} does not have {rows} rows")
+        if grad and t.requires_grad:
             _no_grad("reorder_rows", t)
-        nbytes = t.nbytes // rows if rows else 0
-        if t.is_contiguous():
-            pitch = nbytes
-        else:
+        pitch = nbytes = t.nbytes // rows if rows else 0
+        if not t.is_contiguous():
             pitch = _row_pitch(t, 1)
             if pitch is None:
                 raise ValueError("reorder_rows: the rows of a tensor must be contiguous and must not overlap")
             pitch *= t.element_size()
+        if t.get_device() != index:
+            require_device(parents, t)
         table += (t.data_ptr(), pitch, nbytes)
     if len(set(table[::3])) != len(tensors) and rows and all(table[2::3]):
         raise ValueError("reorder_rows: a tensor is given twice")
     parents = parents.contiguous()
-    require_device(parents, *tensors)
+    require_device(parents)
     table = array.array("q", table)
     on_device(dev.index, _lib.load().tesm_hip_reorder_rows, table.buffer_info()[0], len(tensors), parents.data_ptr(), B, K,
               raw_stream(dev.index))
