@@ -2,6 +2,8 @@
 //   d_t = softplus(dt_t + dt_bias)        a_t = exp(d_t A)
 //   h_t = a_t h_{t-1} + d_t x_t B_t^T     (P x N, float32)
 //   y_t = h_t C_t + D x_t                 times silu(z_t) where there is a gate
+#include <type_traits>
+
 #include "ssm.h"
 
 namespace tesm {
@@ -149,6 +151,10 @@ __device__ __forceinline__ void anew(f32x4 (&h)[NS][2][2]) {
   for (int s = 0; s < NS; ++s) asm volatile("" : "+v"(h[s][0][0]), "+v"(h[s][0][1]), "+v"(h[s][1][0]), "+v"(h[s][1][1])::"memory");
 }
 
+typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(2)));  // 16 bytes at any address of an element
+__device__ __forceinline__ uint4 load16(const void* p) { return __builtin_bit_cast(uint4, *static_cast<const any16*>(p)); }
+__device__ __forceinline__ void store16(void* p, const uint4& v) { *static_cast<any16*>(p) = __builtin_bit_cast(any16, v); }
+
 // How the launch divides the work.
 struct SsmGrid {
   int64_t seg = 0;      // rows per segment, a multiple of 64
@@ -225,6 +231,7 @@ __device__ __forceinline__ uint4 load_unit(const void* p, int64_t at, int col, i
   using TT = Tile<DT>;
   using E = typename TT::E;
   const E* q = static_cast<const E*>(p) + at + col;
+  if (col + TT::EV <= count) return load16(q);
   E v[TT::EV];
 #pragma unroll
   for (int i = 0; i < TT::EV; ++i) v[i] = col + i < count ? q[i] : E(0);
@@ -270,7 +277,7 @@ struct SsmLds {
 };
 
 // FULL: y and the final state of a segment from its carried-in state; otherwise the segment's end state from zero.
-// VEC: whole 32-column slices and 32-state steps in 16-byte vectors, and 32-bit offsets inside a chunk.
+// VEC: whole 32-column slices and 32-state steps, and 32-bit offsets inside a chunk.
 template <int DT, int NS, bool FULL, bool VEC>
 __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_kernel(SsmArgs a, SsmGrid gr) {
   using TT = Tile<DT>;
@@ -298,7 +305,6 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
   const int hh = active ? sl / gr.ps - head0 : 0, head = grp * hg + head0 + hh, p0 = (sl % gr.ps) * 32;
   // this thread's column of x and of B and C
   const int xc = (tid % UX) * EV, xsl = wgi * 4 + xc / 32, xhead = xsl / gr.ps, xp = (xsl % gr.ps) * 32 + xc % 32;
-  const int64_t xat = static_cast<int64_t>(grp * hg + xhead) * P;
   const bool xok = xsl < gr.sg;
   const int bc = (tid % UB) * EV;
 
@@ -323,62 +329,56 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
         } else if (a.h0) {
           const int p = p0 + 8 * (m >> 2) + 4 * T + (m & 3), n = 32 * s + 8 * g + 4 * t2;
           const float* src = a.h0 + (static_cast<int64_t>(sg.seq) * a.H + head) * P * N + p * N + n;
-          if constexpr (VEC) {
-            h[s][t2][T] = *reinterpret_cast<const f32x4*>(src);
+          if (VEC || (p < P && n + 4 <= N)) {
+            h[s][t2][T] = __builtin_bit_cast(f32x4, load16(src));
           } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 3; ++r)
               if (p < P && n + r < N) h[s][t2][T][r] = src[r];
           }
         }
       }
 
-  // A chunk's units, one chunk ahead of their use.  VEC: uniform bases and 32-bit offsets; rows past the end read the
-  // last one and are cleared when staged.
+  // A chunk's units, one chunk ahead of their use: uniform bases and 32-bit offsets.  Rows past the end read the last one
+  // and are cleared when staged.
   uint4 xr[XR], br[BR], cr[FULL ? BR : 1], zr[2][8 / EV];
   const int64_t es = sizeof(E), gn = static_cast<int64_t>(grp) * N, hp = static_cast<int64_t>(head) * P;
-  auto load_bc = [&](const void* p, int64_t ld, int row0, auto& u) {
-    const int left = sg.r1 - row0;  // rows of the chunk that exist
-    const char* base = static_cast<const char*>(p) + (row0 * ld + gn) * es;
-#pragma unroll
-    for (int i = 0; i < BR; ++i) {
-      const int r = tid / UB + i * (256 / UB);
-      if constexpr (VEC) {
-        u[i] = *reinterpret_cast<const uint4*>(base + (static_cast<uint32_t>(min(r, left - 1)) * static_cast<uint32_t>(ld * es) +
-                                                       static_cast<uint32_t>(bc * es)));
-      } else {
-        u[i] = make_uint4(0, 0, 0, 0);
-        if (r < left && bc < N) u[i] = load_unit<DT>(p, (row0 + r) * ld + gn, bc, N);
-      }
+  const bool xin = VEC ? xok : xok && xp < P, bin = VEC || bc < N;
+  auto load_rows = [&](const void* p, int64_t ld, int64_t col, int row0, int last, auto whole, int r, int lane_col, int count, bool in) __attribute__((always_inline)) {
+    const int row = whole.value ? r : min(r, last);
+    if constexpr (VEC) {
+      const char* base = static_cast<const char*>(p) + (row0 * ld + col) * es;
+      return load16(base + (static_cast<uint32_t>(row) * static_cast<uint32_t>(ld * es) + static_cast<uint32_t>(lane_col * es)));
+    } else {
+      if (!in) return make_uint4(0, 0, 0, 0);
+      return load_unit<DT>(p, (row0 + row) * ld + col, lane_col, count);
     }
   };
-  auto load_chunk = [&](int row0) {
-    const int left = sg.r1 - row0;
-    const char* base = static_cast<const char*>(a.x) + row0 * a.ld_x * es;
-    const uint32_t xo = static_cast<uint32_t>((xok ? xat + xp : 0) * es);
+  auto load_as = [&](int row0, auto whole) __attribute__((always_inline)) {
+    const int last = sg.r1 - 1 - row0;
+    const int64_t xbase = static_cast<int64_t>(grp * hg + head0) * P;  // uniform; a thread's own head by its offset
+    const int xcol = xok ? (xhead - head0) * P + xp : 0;
 #pragma unroll
-    for (int i = 0; i < XR; ++i) {
-      const int r = tid / UX + i * (256 / UX);
-      if constexpr (VEC) {
-        xr[i] = *reinterpret_cast<const uint4*>(base + (static_cast<uint32_t>(min(r, left - 1)) * static_cast<uint32_t>(a.ld_x * es) + xo));
-      } else {
-        xr[i] = make_uint4(0, 0, 0, 0);
-        if (xok && r < left && xp < P) xr[i] = load_unit<DT>(a.x, (row0 + r) * a.ld_x + xat, xp, P);
-      }
+    for (int i = 0; i < XR; ++i)
+      xr[i] = load_rows(a.x, a.ld_x, xbase, row0, last, whole, tid / UX + i * (256 / UX), xcol, xcol - xp + P, xin);
+#pragma unroll
+    for (int i = 0; i < BR; ++i) {
+      br[i] = load_rows(a.Bm, a.ld_b, gn, row0, last, whole, tid / UB + i * (256 / UB), bc, N, bin);
+      if constexpr (FULL) cr[i] = load_rows(a.Cm, a.ld_c, gn, row0, last, whole, tid / UB + i * (256 / UB), bc, N, bin);
     }
-    load_bc(a.Bm, a.ld_b, row0, br);
-    if constexpr (FULL) load_bc(a.Cm, a.ld_c, row0, cr);
-    if (FULL && VEC && a.z && active) {  // the gate of this lane's outputs
-      const char* zb = static_cast<const char*>(a.z) + (row0 * a.ld_z + hp + p0) * es;
+    if (FULL && a.z && active) {  // the gate of this lane's outputs
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const uint32_t r = min(16 * q + m, left - 1);
-        const uint4* src = reinterpret_cast<const uint4*>(
-            zb + (r * static_cast<uint32_t>(a.ld_z * es) + 8 * g * static_cast<uint32_t>(es)));
+      for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int k = 0; k < 8 / EV; ++k) zr[q][k] = src[k];
-      }
+        for (int k = 0; k < 8 / EV; ++k)
+          zr[q][k] = load_rows(a.z, a.ld_z, hp + p0, row0, last, whole, 16 * q + m, 8 * g + k * EV, P - p0, p0 + 8 * g + k * EV < P);
     }
+  };
+  auto load_chunk = [&](int row0) __attribute__((always_inline)) {
+    if (row0 + kQ <= sg.r1)
+      load_as(row0, std::true_type{});
+    else
+      load_as(row0, std::false_type{});
   };
 
   // d and the sums c of a chunk, formed by the last wave for two heads at a time, 32 lanes each, while the others form
@@ -386,13 +386,13 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
   uint32_t dtr[2] = {0, 0};
   float Ar[2] = {0.0f, 0.0f}, biasr[2] = {0.0f, 0.0f};
   const int dh = lane >> 5;
-  auto load_dt = [&](int row0) {
+  auto load_dt = [&](int row0) __attribute__((always_inline)) {
     const int r = min(row0 + (lane & 31), sg.r1 - 1);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       if (2 * k + dh < nh) dtr[k] = ld_bits<DT>(a.dts, r * a.ld_dt + grp * hg + head0 + 2 * k + dh);
   };
-  auto sums = [&](int row0, float* to) {
+  auto sums = [&](int row0, float* to) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       if (2 * k >= nh) break;
@@ -415,6 +415,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
   };
 
   float decay = 1.0f;  // of the segment so far (this wave's head)
+  float scale = 1.0f;  // of h
   const float skip = FULL && a.D && active ? a.D[head] : 0.0f;
   if (sg.r0 < sg.r1) {
     load_chunk(sg.r0);
@@ -441,7 +442,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
     E* const Cs = Bs + kQ * Lds::NP;
     const float* const sw = smalls + buf * gr.nh * Lds::kSmall;
     float* const next = smalls + (buf ^ 1) * gr.nh * Lds::kSmall;
-    if (VEC && left < kQ) {
+    if (left < kQ) {
 #pragma unroll
       for (int i = 0; i < XR; ++i)
         if (tid / UX + i * (256 / UX) >= left) xr[i] = make_uint4(0, 0, 0, 0);
@@ -462,7 +463,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
       if constexpr (FULL) *reinterpret_cast<uint4*>(Cs + at) = cr[i];
     }
     uint4 zc[2][8 / EV];
-    if constexpr (FULL && VEC) {
+    if constexpr (FULL) {
 #pragma unroll
       for (int q = 0; q < 2; ++q)
 #pragma unroll
@@ -517,7 +518,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
     if constexpr (FULL) {
       f32x4 y[2][2];
       // exp(c_i) C_i . h (bfloat16 operands: h is rounded here, once, for the product)
-      auto across = [&]() {
+      auto across = [&]() __attribute__((always_inline)) {
         anew(h);
 #pragma unroll
         for (int q = 0; q < 2; ++q)
@@ -535,7 +536,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
         }
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const float e = sm[4 * kQ + 16 * q + m];
+          const float e = sm[4 * kQ + 16 * q + m] * scale;
           y[q][0] *= e;
           y[q][1] *= e;
         }
@@ -602,44 +603,43 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
           }
           if (a.z) {
             float z[8];
-            uint4 u[8 / EV];
-#pragma unroll
-            for (int k = 0; k < 8 / EV; ++k) {
-              if constexpr (VEC) {
-                u[k] = zc[q][k];
-              } else {
-                u[k] = make_uint4(0, 0, 0, 0);
-                if (pc + k * EV < P) u[k] = load_unit<DT>(a.z, (row0 + i) * a.ld_z + hp, pc + k * EV, P);
-              }
-            }
-            TT::unpack(__builtin_bit_cast(Frag, u), z);
+            TT::unpack(__builtin_bit_cast(Frag, zc[q]), z);
 #pragma unroll
             for (int r = 0; r < 8; ++r) v[r] *= gatef_<DT>(z[r]);
           }
-          if constexpr (VEC) {
-            uint32_t at = static_cast<uint32_t>(i) * static_cast<uint32_t>(a.ld_y * es) + 8 * g * static_cast<uint32_t>(es);
-            asm volatile("" : "+v"(at));  // formed here, not kept over the loop
-            *reinterpret_cast<Frag*>(yb + at) = TT::pack(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
-          } else {
-            E* dst = static_cast<E*>(a.y) + (row0 + i) * a.ld_y + hp + pc;
+          uint32_t at = static_cast<uint32_t>(i) * static_cast<uint32_t>(a.ld_y * es) + 8 * g * static_cast<uint32_t>(es);
+          asm volatile("" : "+v"(at));  // formed here, not kept over the loop
+          const Frag o = TT::pack(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
+          if (VEC || pc + 8 <= P) {
+            const __attribute__((ext_vector_type(4))) uint32_t* u = reinterpret_cast<const __attribute__((ext_vector_type(4))) uint32_t*>(&o);
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
-              if (pc + r < P) st<DT>(dst, r, v[r]);
+            for (int k = 0; k < 8 / EV; ++k) *reinterpret_cast<any16*>(yb + at + 16 * k) = u[k];
+          } else {
+#pragma unroll
+            for (int r = 0; r < 7; ++r)
+              if (pc + r < P) st<DT>(yb + at, r, v[r]);
           }
         }
       }
     }
     if (active) {  // the state
-      const float tot = sm[5 * kQ];
+      const float tot = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sm[5 * kQ])));
       decay *= tot;
+      // The state is kept as h * scale: the chunk's decay goes to the scale, and what is added is divided by it; only
+      // where the scale has become small is h itself multiplied.
+      scale *= tot;
+      if (scale < 0x1p-40f) {
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
+        for (int s = 0; s < NS; ++s)
 #pragma unroll
-        for (int t2 = 0; t2 < 2; ++t2)
+          for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
-          for (int T = 0; T < 2; ++T) h[s][t2][T] *= tot;
-      const f32x4 w0 = *reinterpret_cast<const f32x4*>(sm + 3 * kQ + 8 * g);
-      const f32x4 w1 = *reinterpret_cast<const f32x4*>(sm + 3 * kQ + 8 * g + 4);
+            for (int T = 0; T < 2; ++T) h[s][t2][T] *= scale;
+        scale = 1.0f;
+      }
+      const float per = 1.0f / scale;
+      const f32x4 w0 = *reinterpret_cast<const f32x4*>(sm + 3 * kQ + 8 * g) * per;
+      const f32x4 w1 = *reinterpret_cast<const f32x4*>(sm + 3 * kQ + 8 * g + 4) * per;
       // w x: float32, or as two bfloat16 halves (2^-17 relative), each a product of its own
       Frag hi[2], lo[2];
 #pragma unroll
@@ -681,7 +681,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
 #pragma unroll
       for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
-        for (int T = 0; T < 2; ++T) out[((s * 2 + t2) * 2 + T) * 64 + lane] = h[s][t2][T];
+        for (int T = 0; T < 2; ++T) out[((s * 2 + t2) * 2 + T) * 64 + lane] = h[s][t2][T] * scale;
     if (lane == 0) gr.decay[blockIdx.y * a.H + head] = decay;  // (slices of one head write the same value)
   } else if (sg.last && a.h_out) {
 #pragma unroll
@@ -692,12 +692,13 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
         for (int T = 0; T < 2; ++T) {
           const int p = p0 + 8 * (m >> 2) + 4 * T + (m & 3), n = 32 * s + 8 * g + 4 * t2;
           float* dst = a.h_out + (static_cast<int64_t>(sg.seq) * a.H + head) * P * N + p * N + n;
-          if constexpr (VEC) {
-            *reinterpret_cast<f32x4*>(dst) = h[s][t2][T];
+          const f32x4 v = h[s][t2][T] * scale;
+          if (VEC || (p < P && n + 4 <= N)) {
+            store16(dst, __builtin_bit_cast(uint4, v));
           } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (p < P && n + r < N) dst[r] = h[s][t2][T][r];
+            for (int r = 0; r < 3; ++r)
+              if (p < P && n + r < N) dst[r] = v[r];
           }
         }
   }
@@ -751,8 +752,6 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmArgs a, SsmGrid gr) {
 // convolution of the head's x and its group's B and C (in float32, to LDS) runs while they are on their way.  Every head
 // forms its group's B and C again; the first head of a group writes their convolution state.
 // ---------------------------------------------------------------------------
-typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(4)));
-
 // A channel's inputs, as raw bits: the rows before the token and the token's, its filter and bias.
 struct StepChannel {
   uint32_t past[kConvMaxW], w[kConvMaxW], bias;
@@ -999,10 +998,10 @@ int launch_selective_scan(const SsmArgs& a, void* ws, int64_t ws_bytes, hipStrea
     g.carry = static_cast<float*>(ws);
     g.decay = g.carry + round_up(g.slots * a.G * g.wpg * kCols * 32 * states32(a) * 4, 256) / 4;
   }
-  const int64_t es = a.dt == kBF16 ? 2 : 4;
-  const auto vec = [&](const void* p, int64_t ld) { return aligned(p, 16) && ld * es % 16 == 0 && ld < (1LL << 23); };
-  const bool v = aligned(a.h0, 16) && aligned(a.h_out, 16) && a.P % 32 == 0 && a.N == 32 * states32(a) && vec(a.x, a.ld_x) && vec(a.Bm, a.ld_b) && vec(a.Cm, a.ld_c) &&
-                 (!a.z || vec(a.z, a.ld_z)) && vec(a.y, a.ld_y);
+  // 32-bit offsets inside a chunk: 32 rows of pitch ld, 4 bytes at most
+  const int64_t ld = std::max({a.ld_x, a.ld_b, a.ld_c, a.z ? a.ld_z : 0, a.ld_y});
+  TESM_REQUIRE(ld < (1LL << 24), kErrUnsupported, "selective scan: row pitches must be below 2^24 elements");
+  const bool v = a.P % 32 == 0 && a.N == 32 * states32(a);
   if (a.dt == kBF16) return v ? run_ssm_dt<kBF16, true>(a, g, st) : run_ssm_dt<kBF16, false>(a, g, st);
   return v ? run_ssm_dt<kF32, true>(a, g, st) : run_ssm_dt<kF32, false>(a, g, st);
 }
