@@ -10,7 +10,20 @@ namespace tesm {
 
 namespace {
 
-__device__ __forceinline__ float softplusf_(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
+// log(1 + e^v) = max(v, 0) + log(1 + u), u = e^-|v|, and with s = u / (2 + u) <= 1/3 the logarithm is 2 artanh(s) =
+// 2 s (1 + s^2 / 3 + s^4 / 5 + ..), cut after s^12 (what is left is below 2e-8 of it).  NaN stays NaN.
+__device__ __forceinline__ float softplusf_(float v) {
+  const float u = fast_exp(-fabsf(v));
+  const float s = u * __builtin_amdgcn_rcpf(2.0f + u), s2 = s * s;
+  float p = 1.0f / 13.0f;
+  p = __builtin_fmaf(p, s2, 1.0f / 11.0f);
+  p = __builtin_fmaf(p, s2, 1.0f / 9.0f);
+  p = __builtin_fmaf(p, s2, 1.0f / 7.0f);
+  p = __builtin_fmaf(p, s2, 1.0f / 5.0f);
+  p = __builtin_fmaf(p, s2, 1.0f / 3.0f);
+  p = __builtin_fmaf(p, s2, 1.0f);
+  return (v < 0.0f ? 0.0f : v) + (v == -__builtin_inff() || v == __builtin_inff() ? 0.0f : 2.0f * s * p);
+}
 __device__ __forceinline__ float siluf_(float v) { return v * sigmoidf_(v); }
 
 // silu for a bfloat16 result: the exponent's rounding (2^-24 |v| log2 e) is far below the result's, so it is taken as it is.
@@ -344,34 +357,42 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
   uint4 xr[XR], br[BR], cr[FULL ? BR : 1], zr[2][8 / EV];
   const int64_t es = sizeof(E), gn = static_cast<int64_t>(grp) * N, hp = static_cast<int64_t>(head) * P;
   const bool xin = VEC ? xok : xok && xp < P, bin = VEC || bc < N;
-  auto load_rows = [&](const void* p, int64_t ld, int64_t col, int row0, int last, auto whole, int r, int lane_col, int count, bool in) __attribute__((always_inline)) {
-    const int row = whole.value ? r : min(r, last);
-    if constexpr (VEC) {
-      const char* base = static_cast<const char*>(p) + (row0 * ld + col) * es;
-      return load16(base + (static_cast<uint32_t>(row) * static_cast<uint32_t>(ld * es) + static_cast<uint32_t>(lane_col * es)));
-    } else {
-      if (!in) return make_uint4(0, 0, 0, 0);
-      return load_unit<DT>(p, (row0 + row) * ld + col, lane_col, count);
-    }
+  // at: the uniform address of the chunk's first row and the operand's first column here, moved on chunk by chunk
+  const char* xat = static_cast<const char*>(a.x) + (sg.r0 * a.ld_x + static_cast<int64_t>(grp * hg + head0) * P) * es;
+  const char* bat = static_cast<const char*>(a.Bm) + (sg.r0 * a.ld_b + gn) * es;
+  const char* cat = static_cast<const char*>(a.Cm) + (sg.r0 * a.ld_c + gn) * es;
+  const char* zat = static_cast<const char*>(a.z) + (sg.r0 * a.ld_z + hp + p0) * es;
+  char* yat = static_cast<char*>(a.y) + (sg.r0 * a.ld_y + hp + p0) * es;
+  const uint32_t px = static_cast<uint32_t>(a.ld_x * es), pb = static_cast<uint32_t>(a.ld_b * es), pc = static_cast<uint32_t>(a.ld_c * es);
+  const uint32_t pz = static_cast<uint32_t>(a.ld_z * es), py = static_cast<uint32_t>(a.ld_y * es);
+  auto load_rows = [&](const char* at, uint32_t pitch, int last, auto whole, int r, int col, int count, bool in) __attribute__((always_inline)) {
+    const uint32_t off = static_cast<uint32_t>(whole.value ? r : min(r, last)) * pitch;
+    if constexpr (VEC) return load16(at + (off + static_cast<uint32_t>(col * sizeof(E))));
+    return in ? load_unit<DT>(at + off, 0, col, count) : make_uint4(0, 0, 0, 0);
   };
+  const int xcol = xok ? (xhead - head0) * P + xp : 0;
   auto load_as = [&](int row0, auto whole) __attribute__((always_inline)) {
     const int last = sg.r1 - 1 - row0;
-    const int64_t xbase = static_cast<int64_t>(grp * hg + head0) * P;  // uniform; a thread's own head by its offset
-    const int xcol = xok ? (xhead - head0) * P + xp : 0;
 #pragma unroll
     for (int i = 0; i < XR; ++i)
-      xr[i] = load_rows(a.x, a.ld_x, xbase, row0, last, whole, tid / UX + i * (256 / UX), xcol, xcol - xp + P, xin);
+      xr[i] = load_rows(xat, px, last, whole, tid / UX + i * (256 / UX), xcol, xcol - xp + P, xin);
 #pragma unroll
     for (int i = 0; i < BR; ++i) {
-      br[i] = load_rows(a.Bm, a.ld_b, gn, row0, last, whole, tid / UB + i * (256 / UB), bc, N, bin);
-      if constexpr (FULL) cr[i] = load_rows(a.Cm, a.ld_c, gn, row0, last, whole, tid / UB + i * (256 / UB), bc, N, bin);
+      br[i] = load_rows(bat, pb, last, whole, tid / UB + i * (256 / UB), bc, N, bin);
+      if constexpr (FULL) cr[i] = load_rows(cat, pc, last, whole, tid / UB + i * (256 / UB), bc, N, bin);
     }
     if (FULL && a.z && active) {  // the gate of this lane's outputs
 #pragma unroll
       for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int k = 0; k < 8 / EV; ++k)
-          zr[q][k] = load_rows(a.z, a.ld_z, hp + p0, row0, last, whole, 16 * q + m, 8 * g + k * EV, P - p0, p0 + 8 * g + k * EV < P);
+          zr[q][k] = load_rows(zat, pz, last, whole, 16 * q + m, 8 * g + k * EV, P - p0, p0 + 8 * g + k * EV < P);
+    }
+    xat += kQ * static_cast<int64_t>(px);
+    bat += kQ * static_cast<int64_t>(pb);
+    if constexpr (FULL) {
+      cat += kQ * static_cast<int64_t>(pc);
+      zat += kQ * static_cast<int64_t>(pz);
     }
   };
   auto load_chunk = [&](int row0) __attribute__((always_inline)) {
@@ -381,8 +402,8 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
       load_as(row0, std::false_type{});
   };
 
-  // d and the sums c of a chunk, formed by the last wave for two heads at a time, 32 lanes each, while the others form
-  // the chunk before's scores; dt is read two chunks ahead.
+  // d and the sums c of a chunk, formed by one wave for two heads at a time, 32 lanes each, while the others work on the
+  // chunk before; dt is read two chunks ahead.
   uint32_t dtr[2] = {0, 0};
   float Ar[2] = {0.0f, 0.0f}, biasr[2] = {0.0f, 0.0f};
   const int dh = lane >> 5;
@@ -587,12 +608,11 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
               }
             }
         }
-        const int pc = p0 + 8 * g;  // this lane's outputs: columns pc .. + 7 of rows 16 q + m
-        char* yb = static_cast<char*>(a.y) + (row0 * a.ld_y + hp + p0) * es;
+        const int pcol = p0 + 8 * g;  // this lane's outputs: columns pcol .. + 7 of rows 16 q + m
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const int i = 16 * q + m;
-          if (i >= left || pc >= P) continue;
+          if (i >= left || pcol >= P) continue;
           float v[8], x[8];
           TT::unpack(TT::template rows<UX>(X, 16 * q, m, g, wave), x);
 #pragma unroll
@@ -607,21 +627,22 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
 #pragma unroll
             for (int r = 0; r < 8; ++r) v[r] *= gatef_<DT>(z[r]);
           }
-          uint32_t at = static_cast<uint32_t>(i) * static_cast<uint32_t>(a.ld_y * es) + 8 * g * static_cast<uint32_t>(es);
+          uint32_t at = static_cast<uint32_t>(i) * py + 8 * g * static_cast<uint32_t>(es);
           asm volatile("" : "+v"(at));  // formed here, not kept over the loop
           const Frag o = TT::pack(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
-          if (VEC || pc + 8 <= P) {
+          if (VEC || pcol + 8 <= P) {
             const __attribute__((ext_vector_type(4))) uint32_t* u = reinterpret_cast<const __attribute__((ext_vector_type(4))) uint32_t*>(&o);
 #pragma unroll
-            for (int k = 0; k < 8 / EV; ++k) *reinterpret_cast<any16*>(yb + at + 16 * k) = u[k];
+            for (int k = 0; k < 8 / EV; ++k) *reinterpret_cast<any16*>(yat + at + 16 * k) = u[k];
           } else {
 #pragma unroll
             for (int r = 0; r < 7; ++r)
-              if (pc + r < P) st<DT>(yb + at, r, v[r]);
+              if (pcol + r < P) st<DT>(yat + at, r, v[r]);
           }
         }
       }
     }
+    if constexpr (FULL) yat += kQ * static_cast<int64_t>(py);
     if (active) {  // the state
       const float tot = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sm[5 * kQ])));
       decay *= tot;
