@@ -647,9 +647,9 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
       const float tot = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sm[5 * kQ])));
       decay *= tot;
       // The state is kept as h * scale: the chunk's decay goes to the scale, and what is added is divided by it; only
-      // where the scale has become small is h itself multiplied.
+      // where the scale has left 2^-8 .. 2^8 is h itself multiplied (so that neither runs out of its range early).
       scale *= tot;
-      if (scale < 0x1p-40f) {
+      if (scale < 0x1p-8f || scale > 0x1p8f) {
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -658,11 +658,12 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
             for (int T = 0; T < 2; ++T) h[s][t2][T] *= scale;
         scale = 1.0f;
       }
-      const float per = 1.0f / scale;
+      const float per = __builtin_amdgcn_rcpf(scale);
       const f32x4 w0 = *reinterpret_cast<const f32x4*>(sm + 3 * kQ + 8 * g) * per;
       const f32x4 w1 = *reinterpret_cast<const f32x4*>(sm + 3 * kQ + 8 * g + 4) * per;
-      // w x: float32, or as two bfloat16 halves (2^-17 relative), each a product of its own
-      Frag hi[2], lo[2];
+      // w x: float32, or as three bfloat16 parts that hold all its 24 bits, each a product of its own
+      constexpr int PARTS = DT == kBF16 ? 3 : 1;
+      Frag wx[PARTS][2];
 #pragma unroll
       for (int T = 0; T < 2; ++T) {
         float v[8];
@@ -670,12 +671,13 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
         f32x4 v0, v1;
 #pragma unroll
         for (int r = 0; r < 4; ++r) v0[r] = v[r] * w0[r], v1[r] = v[4 + r] * w1[r];
-        hi[T] = TT::pack(v0, v1);
-        if constexpr (DT == kBF16) {
-          TT::unpack(hi[T], v);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          wx[part][T] = TT::pack(v0, v1);
+          if (part + 1 == PARTS) break;
+          TT::unpack(wx[part][T], v);
 #pragma unroll
           for (int r = 0; r < 4; ++r) v0[r] -= v[r], v1[r] -= v[4 + r];  // (an infinity's states become NaN)
-          lo[T] = TT::pack(v0, v1);
         }
       }
 #pragma unroll
@@ -684,11 +686,11 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) b[t2] = TT::template column<UB>(Bs, 0, m, g, s, t2);
 #pragma unroll
-        for (int half = 0; half < (DT == kBF16 ? 2 : 1); ++half)
+        for (int part = 0; part < PARTS; ++part)
 #pragma unroll
           for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
-            for (int T = 0; T < 2; ++T) h[s][t2][T] = TT::mma(b[t2], half ? lo[T] : hi[T], h[s][t2][T]);
+            for (int T = 0; T < 2; ++T) h[s][t2][T] = TT::mma(b[t2], wx[part][T], h[s][t2][T]);
       }
     }
     if (NB == 1) lds_barrier();
@@ -848,7 +850,7 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepArgs a) {
     if (p >= P || n >= N) return;
     const float* q = state + static_cast<int64_t>(p) * N + n;
     if (N4 || n + 4 <= N) {
-      v = *reinterpret_cast<const any16*>(q);
+      v = __builtin_nontemporal_load(reinterpret_cast<const any16*>(q));
     } else {
 #pragma unroll
       for (int r = 0; r < 3; ++r)
@@ -858,7 +860,9 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepArgs a) {
 #pragma unroll
   for (int k = 0; k < K; ++k) load(p0 + k * RP, raw[k]);
   const uint32_t in = ld_bits<DT>(a.dts, b * a.ld_dt + h);
-  const float bias = a.dt_bias ? a.dt_bias[h] : 0.0f, rate = a.A[h];
+  const float bias = a.dt_bias ? a.dt_bias[h] : 0.0f, rate = a.A[h], skip = a.D ? a.D[h] : 0.0f;
+  const int64_t zat = b * a.ld_z + static_cast<int64_t>(h) * P;
+  const uint32_t z0 = a.z && tid < P ? ld_bits<DT>(a.z, zat + tid) : 0;
   // two channels of B, C and x at a time: both are on their way before either is used
   const int count = 2 * n4 + P;
   auto channel = [&](int e) {  // -1: padding
@@ -899,7 +903,7 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepArgs a) {
       if (p < P && n < N) {
         float* q = state + static_cast<int64_t>(p) * N + n;
         if (N4 || n + 4 <= N) {
-          *reinterpret_cast<any16*>(q) = __builtin_bit_cast(any16, v);
+          __builtin_nontemporal_store(__builtin_bit_cast(any16, v), reinterpret_cast<any16*>(q));
         } else {
 #pragma unroll
           for (int r = 0; r < 3; ++r)
@@ -920,8 +924,8 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepArgs a) {
   __syncthreads();
   for (int p = tid; p < P; p += 256) {
     float y = ys[p];
-    if (a.D) y += a.D[h] * xs[p];
-    if (a.z) y *= siluf_(ld<DT>(a.z, b * a.ld_z + static_cast<int64_t>(h) * P + p));
+    if (a.D) y += skip * xs[p];
+    if (a.z) y *= siluf_(from_bits<DT>(p < 256 ? z0 : ld_bits<DT>(a.z, zat + p)));
     st<DT>(a.y, b * a.ld_y + static_cast<int64_t>(h) * P + p, y);
   }
 }
