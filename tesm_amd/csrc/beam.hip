@@ -441,7 +441,7 @@ int64_t beam_parts(const BeamArgs& a) {
 
 int beam_check(const BeamArgs& a) {
   TESM_REQUIRE(a.dt == kF32 || a.dt == kBF16, kErrInvalidArg, "beam select: dtype must be 0 or 1");
-  TESM_REQUIRE(a.B >= 0 && a.K >= 1 && a.V >= 1 && a.n >= 1 && a.B < (1LL << 24) && a.V < (1LL << 31) - 65536,
+  TESM_REQUIRE(a.B >= 0 && a.K >= 1 && a.V >= 1 && a.n >= 1 && a.B < (1LL << 24) && a.V < (1LL << 30),
                kErrInvalidArg, "beam select: bad sizes");
   TESM_REQUIRE(a.K <= kBeamMaxN && a.n <= kBeamMaxN, kErrUnsupported,
                "beam select: at most 64 beams and 64 chosen candidates");
@@ -493,7 +493,7 @@ int launch_reorder_rows(const ReorderRows* t, int64_t count, const int64_t* pare
     TESM_REQUIRE(t[i].bytes >= 0 && t[i].bytes < (1LL << 36) && (B * K <= 1 || t[i].pitch >= t[i].bytes) &&
                      (t[i].p || t[i].bytes == 0),
                  kErrInvalidArg, "reorder rows: a tensor has no memory or a pitch shorter than its row");
-  if (B == 0 || K == 1) return kOk;
+  if (B == 0) return kOk;
   for (int64_t i0 = 0; i0 < count; i0 += kReorderTensors) {
     ReorderTable tab;
     tab.count = 0;

@@ -751,7 +751,7 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmArgs a, SsmGrid gr) {
     seq_rows(a.seq_starts, blockIdx.y, a.B * a.L, first, end);
     nseg = segments_of(end - first, gr.seg);
   }
-  if (sl >= gr.sg || nseg < 2) return;
+  if (sl >= gr.sg || nseg < 2 || slot + nseg > gr.slots) return;  // (more segments than rows allow: starts that decrease)
   const int hg = static_cast<int>(a.H / a.G), head = grp * hg + sl / gr.ps;
   const int lane = v & 63, m = lane & 15, g = lane >> 4, T = (v >> 6) & 1, t2 = (v >> 7) & 1, s = v >> 8;
   f32x4 h = {0.0f, 0.0f, 0.0f, 0.0f};

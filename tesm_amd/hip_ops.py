@@ -236,7 +236,8 @@ def stream_copy(dst: torch.Tensor, src: torch.Tensor) -> None:
 
 
 def device_status(clear: bool = True) -> int:
-    """The device status word of the current device (bit 0: a scan look-back gave up); synchronises."""
+    """The device status word of the current device (bit 0: a scan look-back gave up; bit 1: a parent of
+    ``reorder_rows`` was none of the beams); synchronises."""
     v = ctypes.c_uint32(0)
     lib = _lib.load()
     _lib.check(lib.tesm_hip_device_status(ctypes.byref(v), int(clear)))
@@ -528,14 +529,14 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     ``y[b, t, c] = silu(bias[c] + sum_j weight[c, j] x[b, t - W + 1 + j, c])`` (``silu=False``: no activation) for x
     (B, L, C) and ``weight`` (C, W), 2 <= W <= 8, summed in float32.  With ``seq_starts`` (S + 1, on the device, not
     decreasing) x is (1, rows, C) and holds S sequences one behind the other, sequence s in rows
-    ``seq_starts[s] .. seq_starts[s + 1] - 1``; rows in front of the first and behind the last one stay as they are in
+    ``seq_starts[s] .. seq_starts[s + 1] - 1`` (starts past the rows count as their end); rows in front of the first and behind the last one stay as they are in
     ``out`` (zero without ``out``).  ``state`` (S, W - 1, C): the rows before each sequence, oldest first, zeros by
     default.  The state returned holds each sequence's last W - 1 rows.  ``out`` must not overlap x.  x, state and y
     share a dtype; weight and bias share one (float32 or bfloat16) of their own.
     """
     if x.dim() != 3 or weight.dim() != 2 or weight.shape[0] != x.shape[2]:
         raise ValueError("causal_conv: x must be (B, L, C) and weight (C, W)")
-    _no_grad("causal_conv", x, weight, bias, state)
+    _no_grad("causal_conv", x, weight, bias, state, out)
     B, L, C = x.shape
     W = weight.shape[1]
     if not 2 <= W <= 8:
@@ -578,12 +579,13 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     N <= 256; A, D, dt_bias: (H); ``state`` (S, H, P, N) float32: the states before each sequence (zeros by default).
     ``seq_starts`` and ``out`` as in ``causal_conv``.  x, dt, B, C, z and y share a dtype and may be column slices of
     wider rows.  States and sums are float32; with bfloat16 operands the decayed scores and the state read by a chunk's
-    rows are rounded to bfloat16 for the products.
+    rows are rounded to bfloat16 for the products.  A NaN or an infinity in row t reaches no row before it; an infinite
+    x may leave NaN where the formula's state is infinite.  Fewer than 65536 sequences, H * P and row pitches below 2^24.
     """
     if x.dim() != 4 or dt.dim() != 3 or B.dim() != 4 or dt.shape != x.shape[:3] or B.shape[:2] != x.shape[:2] or \
             C.shape != B.shape or (z is not None and z.shape != x.shape):
         raise ValueError("selective_scan: x and z must be (B, L, H, P), dt (B, L, H), B and C (B, L, G, N)")
-    _no_grad("selective_scan", x, dt, A, B, C, D, z, dt_bias, state)
+    _no_grad("selective_scan", x, dt, A, B, C, D, z, dt_bias, state, out)
     nb, L, H, P = x.shape
     G, N = B.shape[2:]
     if H < 1 or P < 1 or G < 1 or N < 1 or H % G:
@@ -631,12 +633,13 @@ def selective_scan_step(row: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, st
     without ``conv_weight`` the row is used as it is.  ``state`` (B, H, P, N) float32 is updated in place;
     ``conv_state`` (B, W - 1, H * P + 2 * G * N) is read, and the state after the token is returned in a tensor of its
     own (``conv_state_out``, which must not be ``conv_state``; captured graphs alternate between two).  dt (B, H),
-    z (B, H, P); the rest as in ``selective_scan``.
+    z (B, H, P); the rest as in ``selective_scan``.  ``out`` must not overlap the other arguments.  B < 65536, P <= 4096.
     """
     if state.dim() != 4 or row.dim() != 2 or row.shape[0] != state.shape[0] or dt.shape != state.shape[:2] or \
             (z is not None and z.shape != state.shape[:3]):
         raise ValueError("selective_scan_step: row must be (B, channels), dt (B, H), z (B, H, P) and state (B, H, P, N)")
-    _no_grad("selective_scan_step", row, dt, A, state, conv_weight, conv_bias, conv_state, D, z, dt_bias)
+    _no_grad("selective_scan_step", row, dt, A, state, conv_weight, conv_bias, conv_state, D, z, dt_bias, out,
+             conv_state_out)
     nb, H, P, N = state.shape
     G, width = int(n_groups), row.shape[1]
     if G < 1 or H < 1 or P < 1 or N < 1 or H % G or width != H * P + 2 * G * N:
@@ -695,7 +698,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
     the order of ``k * V + v``.  NaN logits, rows with a +infinite logit and beams whose score is not finite offer
     -infinity.  A beam with ``finished`` (B, K) bool offers ``pad_token`` alone, at its own score; the last result says
     whether the parent was finished or the token is ``eos_token`` (None where neither argument is given).  parents and
-    tokens are int64.  K and n are at most 64.
+    tokens are int64.  K and n are at most 64, B * K < 65536, V < 2^30.
     """
     if logits.dim() != 3 or scores.shape != logits.shape[:2]:
         raise ValueError("beam_select: logits must be (B, K, V) and scores (B, K)")
@@ -734,7 +737,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: Optional[int] = N
 def reorder_rows(tensors, parents: torch.Tensor) -> None:
     """Row ``b * K + k`` of every tensor becomes its old row ``b * K + parents[b, k]``, in place and in one launch.
 
-    ``parents`` (B, K) int64, K <= 64; each tensor has B * K rows (its first dimension), each row contiguous; any
+    ``parents`` (B, K) int64, B < 65536, K <= 64; each tensor has B * K rows (its first dimension), each row contiguous; any
     dtype.  The tensors must not overlap.  A parent outside 0 .. K - 1 leaves its row as it is and sets bit 1 of
     ``device_status``.
     """

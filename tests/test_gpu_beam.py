@@ -201,6 +201,34 @@ def test_reorder_reports_bad_parents():
     assert t[:, 0].div(3).tolist() == [0, 1, 1, 3, 7, 7, 6, 4]
     assert hip_ops.device_status() == 2
     assert hip_ops.device_status() == 0
+    hip_ops.reorder_rows([t], torch.tensor([[0]] * 7 + [[1]], device=DEV))
+    assert t[:, 0].div(3).tolist() == [0, 1, 1, 3, 7, 7, 6, 4] and hip_ops.device_status() == 2
+
+
+def test_reorder_captured_and_replayed_on_another_stream():
+    """Parents are read when the graph runs; an eager call on another stream moves other tensors at the same time."""
+    g = torch.Generator().manual_seed(11)
+    host = _tensors(g, 12)
+    first, dev, other = [t.to(DEV) for t in host], [t.to(DEV) for t in host], [t.to(DEV) for t in host]
+    parents = torch.zeros(3, 4, dtype=torch.int64, device=DEV)
+    side = torch.cuda.Stream()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, capture_error_mode="relaxed"):
+        hip_ops.reorder_rows(dev, parents)
+    for step in range(3):
+        p = torch.randint(0, 4, (3, 4), generator=g)
+        rows = (p + 4 * torch.arange(3)[:, None]).flatten()
+        for d, f in zip(dev, first):
+            d.copy_(f)
+        parents.copy_(p)
+        side.wait_stream(torch.cuda.current_stream())
+        gr.replay()
+        with torch.cuda.stream(side):
+            hip_ops.reorder_rows(other, parents)
+        torch.cuda.synchronize()
+        assert all(torch.equal(d.cpu(), t[rows]) for d, t in zip(dev, host)), step
+        host2 = [t[rows] for t in host] if step == 0 else [t[rows] for t in host2]
+        assert all(torch.equal(d.cpu(), t) for d, t in zip(other, host2)), step
 
 
 # ---------------------------------------------------------------------------

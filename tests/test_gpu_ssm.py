@@ -319,6 +319,45 @@ def test_scan_strong_decays(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scan_growing_states_and_large_values(dtype):
+    """Rates above zero (the state grows by e^4 over a chunk), and channels near 2^100: no scale on the way overflows."""
+    c = _scan_case(42, 1, 200, 4, 32, 1, 32, dtype, softplus=False, bias=False, gate=False)
+    c["A"] = torch.tensor([0.8, 0.4, 1e-3, -0.8])
+    c["x"][0, :, 2:] *= 2.0 ** 100
+    _check_scan(c, *_run_scan(c))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scan_state_holds_float32(dtype):
+    """One row's addend, decayed over two chunks.  In units of 2^-24: the decay inside the chunk and the second chunk's, 2 for
+    the exponential's value and 1 for its rounded argument each; d's and x's products 2; the scale's reciprocal and its two
+    uses 4; the three parts of the addend's product 6 (the matrix unit may cut instead of rounding); the scale's product 1:
+    19, and with as much again for what the library's exponential adds, 32."""
+    c = _scan_case(43, 1, 50, 4, 64, 1, 128, dtype, init=False, softplus=False, bias=False, gate=False, skip=False)
+    x = torch.zeros_like(c["x"])
+    x[0, 5] = c["x"][0, 5]
+    c["x"], c["A"] = x, -0.05 * torch.arange(1.0, 5.0)
+    c["dt"] = torch.full_like(c["dt"], 0.25)
+    c["A"] = c["A"].bfloat16().float()
+    h = _run_scan(c)[1].cpu().double()
+    decay = (c["A"].double() * 0.25 * 44).exp()
+    want = 0.25 * decay[:, None, None] * c["x"][0, 5].double()[..., None] * c["B"][0, 5, 0].double()
+    assert bool(((h[0] - want).abs() <= 32 * U * want.abs()).all())
+
+
+def test_scan_of_decreasing_starts_stays_in_its_memory():
+    """Starts that decrease are no valid input: what they give is not looked at, but nothing else is touched."""
+    c = _scan_case(72, 1, 1000, 2, 16, 1, 16, torch.float32, starts=[0, 1000])
+    y, h = _run_scan(c)
+    bad = dict(c, starts=[0, 1000] * 8, h0=torch.zeros(15, 2, 16, 16))
+    keep = [t.clone() for t in (y, h)]
+    _run_scan(bad)
+    assert torch.equal(y, keep[0]) and torch.equal(h, keep[1])
+    again = _run_scan(c)
+    assert torch.equal(again[0], y) and torch.equal(again[1], h)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_scan_same_bits_twice_and_for_equal_sequences(dtype):
     c = _scan_case(51, 1, 333, 4, 64, 1, 128, dtype)
     for k in ("x", "dt", "B", "C", "z", "h0"):
@@ -337,6 +376,45 @@ def test_scan_empty(dtype):
     c = _scan_case(61, 0, 5, 2, 8, 1, 16, dtype)
     y, h = _run_scan(c)
     assert y.shape == (0, 5, 2, 8) and h.shape == (0, 2, 8, 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_conv_and_scan_on_two_streams_at_once(dtype):
+    """Calls under way together keep to workspaces of their own; a captured convolution repeats."""
+    cs = [_scan_case(91 + i, 1, 900, 4, 64, 1, 128, dtype) for i in range(2)]
+    args = [{k: (_dev(v) if torch.is_tensor(v) else v) for k, v in c.items()} for c in cs]
+    w = _randn(torch.Generator().manual_seed(3), 4 * 64, 4, dtype=dtype).to(DEV)
+
+    def call(a):
+        x, _ = hip_ops.causal_conv(a["x"].view(1, 900, 256), w)
+        return hip_ops.selective_scan(x.view(1, 900, 4, 64), a["dt"], a["A"], a["B"], a["C"], dt_bias=a["dt_bias"])
+    want = [call(a) for a in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, capture_error_mode="relaxed"):
+        held = call(args[0])
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for a, st in zip(args, streams):
+            with torch.cuda.stream(st):
+                got.append(call(a))
+        gr.replay()
+        torch.cuda.synchronize()
+        for o, v in zip(got + [held], want + want[:1]):
+            assert torch.equal(o[0], v[0]) and torch.equal(o[1], v[1])
+
+
+def test_scan_launches():
+    """Whole slices and states take the kernels without edges; long sequences are divided, short ones are not."""
+    def names(*a):
+        c = _scan_case(5, *a, torch.bfloat16)
+        with hip_ops.launch_log() as log:
+            _run_scan(c)
+        return [k for k in log.kernels if "ssm_" in k]
+    short, long, ragged = names(1, 64, 2, 64, 1, 128), names(1, 700, 2, 64, 1, 128), names(1, 700, 2, 40, 1, 100)
+    assert len(short) == 1 and len(long) == 3 and len(ragged) == 3
+    assert "ssm_carry_kernel" in long[1] and "ssm_carry_kernel" in ragged[1] and long[2] == short[0] != ragged[2]
 
 
 def test_scan_reads_starts_that_run_past_the_rows_as_the_last_row():

@@ -190,6 +190,8 @@ def test_c_entries_refuse_bad_descriptors():
     assert lib.tesm_hip_beam_select(ctypes.byref(b), None, 0, None) == 3
     b.K, b.ld = 4, 8
     assert lib.tesm_hip_beam_select(ctypes.byref(b), None, 0, None) == 1 and b"ld" in err()
+    b.V = b.ld = 1 << 30
+    assert lib.tesm_hip_beam_select(ctypes.byref(b), None, 0, None) == 1 and b"sizes" in err()
     assert lib.tesm_hip_reorder_rows(None, 1, None, 2, 4, None) == 1
     assert lib.tesm_hip_reorder_rows(None, 0, None, 2, 65, None) == 3
 
