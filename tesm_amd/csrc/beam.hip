@@ -7,7 +7,8 @@
 // Inside a beam the order of the offers is the order of the logits, so each row is reduced to its n largest logits and
 // its logsumexp in one pass (beam_row_kernel), and requests then merge their beams' lists, the offers compared in 64
 // bits (beam_merge_kernel).  Bound by reading the logits once, and next to that by arithmetic: 7 operations per logit, of
-// which the exponential takes four.
+// which the exponential takes four.  Measured, bfloat16, a quarter of the beams finished: 512 rows of 151936 logits (117 MB
+// read) 47 us + 12 for the merge, 2.5 TB/s; 4 rows 10 + 7 us.
 #include <float.h>
 
 #include "beam.h"
@@ -294,7 +295,8 @@ struct Offer {
 };
 
 // One workgroup per request: a wave per beam merges its parts' lists into the beam's m best offers; the offers' ranks
-// among all beams' are then counted.
+// among all beams' are then counted.  Bound by latency: the chains of sorting steps and of the 64-bit exponentials and
+// logarithm, 7 to 12 us.
 __global__ __launch_bounds__(512) void beam_merge_kernel(BeamArgs a, int m, int parts, const uint64_t* keys, const PartSum* sums) {
   extern __shared__ __attribute__((aligned(16))) char lds_beam[];
   Offer* const offers = reinterpret_cast<Offer*>(lds_beam);
@@ -369,7 +371,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // A thread moves one unit of all K rows of a request: every load before the first store, so a row may be the parent
 // of several others and be overwritten itself.  Rows that stay are neither read nor written: in their place one that is
-// read anyway is read again (a branch per row around the loads would keep them from being under way together).
+// read anyway is read again (a branch per row around the loads would keep them from being under way together).  Bound by
+// HBM where the rows are long: 16 requests of 8 beams, 655 MB if all rows moved, 104 us; a layer stack's small caches 4.3 us.
 template <typename U, int KM>
 __device__ __forceinline__ void reorder_unit(char* at, int64_t pitch, const int (&from)[KM], uint64_t moves) {
   U v[KM];

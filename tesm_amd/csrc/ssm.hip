@@ -51,10 +51,22 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // row m of tile T  <->  8 (m / 4) + 4 T + m % 4: two tiles of the state are then the 8 consecutive states per lane that
 // the next product's operand needs, with no exchange, and two tiles of Y are 8 consecutive columns of one row, one
 // 16-byte store.
+//
+// A chunk's x, B and C come through registers, read one chunk ahead, into LDS (two chunks' worth for bfloat16, so that
+// one barrier separates a chunk's writes from its reads; float32 rows fill it with one).  Three of the waves form the
+// scores; the fourth meanwhile forms d and the sums c of the next chunk (in 64 bits: c is a difference's operand, and is
+// kept as a high and a low float).  Roundings with bfloat16 operands: W and the h that C reads go to bfloat16 once, like
+// the operands they meet (y is rounded to it as well); the state itself takes its addends in three parts, unrounded.
+//
+// Bound by the vector unit: per wave and chunk about 650 instructions, the exponentials and reciprocals among them at a
+// quarter of the rate, next to 72 matrix instructions (about a quarter of the time), at the two waves per SIMD that the
+// state's and the next operands' registers leave; with every operand in the cache it gained a seventh.  Chunks of 64 rows
+// (one staged, with the work inside a chunk doubled) took 628 us where these took 520.  Measured, bfloat16 with 128
+// states: 4 x 2048 rows of 1536 columns 42 us + 30 for the states of the segments, 32768 rows of 8192 columns (1.76 GB)
+// 585 + 270 us, 2.1 TB/s.
 // ---------------------------------------------------------------------------
 constexpr int kCols = 128;  // columns per workgroup
 constexpr int kQ = 32;      // rows per chunk
-constexpr int64_t kMinSegment = 256;
 
 template <int DT>
 struct Tile;
@@ -728,7 +740,8 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
 }
 
 // The segments' end states from zero become the states at their ends: a sequence's are folded in order, one vector of
-// 4 states per thread.
+// 4 states per thread, the reads of eight segments under way together.  Bound by the bytes: 8 segments of 4 MB, 63 MB
+// read and written, in 12 us.
 template <int NS>
 __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmArgs a, SsmGrid gr) {
   constexpr int VW = NS * 4 * 64;  // vectors per wave
@@ -763,9 +776,21 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmArgs a, SsmGrid gr) {
   }
   f32x4* c = reinterpret_cast<f32x4*>(gr.carry) + (slot * wg_all + wg) * 4 * VW + wave * VW + v;
   const float* dec = gr.decay + slot * a.H + head;
-  for (int64_t k = 0; k + 1 < nseg; ++k) {
-    h = h * dec[k * a.H] + c[k * wg_all * 4 * VW];
-    c[k * wg_all * 4 * VW] = h;
+  for (int64_t k0 = 0; k0 + 1 < nseg; k0 += 8) {  // eight segments' loads at once
+    f32x4 own[8];
+    float d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k0 + i + 1 < nseg) {
+        own[i] = c[(k0 + i) * wg_all * 4 * VW];
+        d[i] = dec[(k0 + i) * a.H];
+      }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k0 + i + 1 < nseg) {
+        h = h * d[i] + own[i];
+        c[(k0 + i) * wg_all * 4 * VW] = h;
+      }
   }
 }
 
@@ -773,7 +798,9 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmArgs a, SsmGrid gr) {
 // One token.  A workgroup owns one head of one sequence: its state, read and written once, is what the call costs.  Rows of
 // N states are held 4 per lane by LPR lanes, 256 / LPR rows at a time; the state's loads are issued first, and the
 // convolution of the head's x and its group's B and C (in float32, to LDS) runs while they are on their way.  Every head
-// forms its group's B and C again; the first head of a group writes their convolution state.
+// forms its group's B and C again; the first head of a group writes their convolution state.  The states go past the
+// caches both ways: 16 to 512 MB of them are never slower for it, used again at once or not (256 MB 96 us against 96 and
+// 108, 512 MB 189 against 206).  Measured: 64 sequences of 128 heads of 64 x 128 states, 537 MB read and written, 98 us, 5.5 TB/s.
 // ---------------------------------------------------------------------------
 // A channel's inputs, as raw bits: the rows before the token and the token's, its filter and bias.
 struct StepChannel {
@@ -939,8 +966,11 @@ int states32(const SsmArgs& a) {  // 32-state steps, rounded up to an instantiat
   return n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8;
 }
 
-// Segments so that about two workgroups per CU run; a segment's end state costs as much traffic as about 85 of its
-// rows, so it has several times that.
+// Segments: a divided sequence costs a second pass over its x, B and dt, a state per segment written, read, written and
+// read again, and two launches, so that three of them at least are made, of 64 rows at least: as many as give each CU a
+// workgroup, and where they keep 128 rows then, two (as many as fit).  Bfloat16 with 24 heads of 64 channels and 128
+// states, divided against in one pass: 2048 rows 4 x 72 us against 172, 8 x 101 against 172, 16 x (two segments) 204
+// against 175; 512 rows 25 us against 44 in segments of 256; 160 rows 19.3 against 19.5; 128 rows (two) 20 against 17.
 SsmGrid ssm_grid(const SsmArgs& a) {
   SsmGrid g;
   const int64_t hg = a.H / a.G;
@@ -950,8 +980,12 @@ SsmGrid ssm_grid(const SsmArgs& a) {
   g.nh = 4 % g.ps == 0 ? 4 / g.ps : g.ps % 4 == 0 ? 1 : 2;
   const int64_t wgs = a.G * g.wpg, rows = a.seq_starts ? a.B * a.L : a.L;
   const int64_t each = a.seq_starts ? 1 : std::max<int64_t>(a.S, 1);
-  const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(1, wgs * each));
-  g.seg = std::max<int64_t>(kMinSegment, round_up((rows + want - 1) / want, 64));
+  auto rows_for = [&](int64_t all) {
+    const int64_t n = std::max<int64_t>(1, all / std::max<int64_t>(1, wgs * each));
+    return round_up((rows + n - 1) / n, 64);
+  };
+  g.seg = std::max<int64_t>(64, std::min(rows_for(256), std::max<int64_t>(128, rows_for(512))));
+  if (!a.seq_starts && a.L <= 2 * g.seg) g.seg = round_up(std::max<int64_t>(a.L, 1), 64);
   if (a.seq_starts)
     g.slots = rows / g.seg + a.S;
   else
