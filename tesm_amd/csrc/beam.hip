@@ -8,8 +8,10 @@
 // its logsumexp in one pass (beam_row_kernel), and requests then merge their beams' lists, the offers compared in 64
 // bits (beam_merge_kernel).  Bound by reading the logits once, and next to that by arithmetic: 7 operations per logit, of
 // which the exponential takes four.  Measured, bfloat16, a quarter of the beams finished: 512 rows of 151936 logits (117 MB
-// read) 47 us + 12 for the merge, 2.5 TB/s; 4 rows 10 + 7 us.
+// read) 47 us + 12 for the merge, 2.5 TB/s; 4 rows 8.5 + 6.2 us.
 #include <float.h>
+
+#include <type_traits>
 
 #include "beam.h"
 
@@ -30,33 +32,77 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 }
 __device__ __forceinline__ int key_index(uint64_t k) { return static_cast<int>(~static_cast<uint32_t>(k)); }
 
-__device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int d) {
-  const uint32_t lo = __shfl_xor(static_cast<int>(v), d), hi = __shfl_xor(static_cast<int>(v >> 32), d);
-  return static_cast<uint64_t>(hi) << 32 | lo;
+// The value of the lane D away (D a power of 2), by the vector unit alone: a step of a sorting network waits for it, and by
+// way of LDS it takes several times as long (4 rows of 151936 logits: 10.0 us against 8.5).
+template <int D>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  constexpr int kRowRor8 = 0x128, kQuadReverse = 0x1B;
+  const int i = static_cast<int>(v);
+  if constexpr (D == 1) return dpp_mov<kDppXor1>(i);
+  if constexpr (D == 2) return dpp_mov<kDppXor2>(i);
+  if constexpr (D == 4) return dpp_mov<kQuadReverse>(dpp_mov<kDppHalfMirror>(i));  // 7 away, then 3
+  if constexpr (D == 8) return dpp_mov<kRowRor8>(i);
+  if constexpr (D == 16) {  // (rows 0, 0, 2, 2 and 1, 1, 3, 3)
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  }
+  if constexpr (D == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
 }
-// One step of a bitonic network over the lanes: the larger of a lane and the one d away goes to the lower lane where `down`.
-__device__ __forceinline__ uint64_t bitonic(uint64_t v, int d, bool down) {
-  const uint64_t o = shfl_xor_u64(v, d);
-  const bool low = (threadIdx.x & d) == 0;
-  return (v > o) == (low == down) ? v : o;
+// f(D) for D = FROM, FROM / 2 .. 1
+template <int FROM, typename F>
+__device__ __forceinline__ void each_distance(F&& f) {
+  f(std::integral_constant<int, FROM>{});
+  if constexpr (FROM > 1) each_distance<FROM / 2>(f);
+}
+// Steps of a bitonic network over the lanes: the larger of a lane and the one D away goes to the lower lane where `down`.
+template <int FROM>
+__device__ __forceinline__ uint64_t bitonic(uint64_t v, bool down) {
+  each_distance<FROM>([&](auto d) __attribute__((always_inline)) {
+    constexpr int D = decltype(d)::value;
+    const uint64_t o = static_cast<uint64_t>(lane_xor<D>(static_cast<uint32_t>(v >> 32))) << 32 | lane_xor<D>(static_cast<uint32_t>(v));
+    const bool low = (threadIdx.x & D) == 0;
+    v = (v > o) == (low == down) ? v : o;
+  });
+  return v;
 }
 // The 64 best of a falling list (one per lane) and 64 more keys in any order, as a falling list.
 __device__ __forceinline__ uint64_t merge64(uint64_t list, uint64_t more) {
   const int lane = threadIdx.x & 63;
-  for (int k = 2; k <= 64; k <<= 1)  // `more` rising
-    for (int d = k >> 1; d > 0; d >>= 1) more = bitonic(more, d, (lane & k) != 0);
-  list = list > more ? list : more;
-  for (int d = 32; d > 0; d >>= 1) list = bitonic(list, d, true);
-  return list;
+  more = bitonic<1>(more, (lane & 2) != 0);  // `more` rising
+  more = bitonic<2>(more, (lane & 4) != 0);
+  more = bitonic<4>(more, (lane & 8) != 0);
+  more = bitonic<8>(more, (lane & 16) != 0);
+  more = bitonic<16>(more, (lane & 32) != 0);
+  more = bitonic<32>(more, false);
+  return bitonic<32>(list > more ? list : more, true);
 }
 // The same for two falling lists.
 __device__ __forceinline__ uint64_t merge_lists(uint64_t a, uint64_t b) {
   const int r = 63 - (threadIdx.x & 63);
   const uint32_t lo = __shfl(static_cast<int>(b), r), hi = __shfl(static_cast<int>(b >> 32), r);
   const uint64_t o = static_cast<uint64_t>(hi) << 32 | lo;
-  a = a > o ? a : o;
-  for (int d = 32; d > 0; d >>= 1) a = bitonic(a, d, true);
-  return a;
+  return bitonic<32>(a > o ? a : o, true);
+}
+// The values in falling order.
+__device__ __forceinline__ float sorted(float v) {
+  const int lane = threadIdx.x & 63;
+  auto steps = [&](auto from, bool down) __attribute__((always_inline)) {
+    each_distance<decltype(from)::value>([&](auto d) __attribute__((always_inline)) {
+      constexpr int D = decltype(d)::value;
+      const float o = __uint_as_float(lane_xor<D>(__float_as_uint(v)));
+      v = ((lane & D) == 0) == down ? fmaxf(v, o) : fminf(v, o);
+    });
+  };
+  steps(std::integral_constant<int, 1>{}, (lane & 2) == 0);
+  steps(std::integral_constant<int, 2>{}, (lane & 4) == 0);
+  steps(std::integral_constant<int, 4>{}, (lane & 8) == 0);
+  steps(std::integral_constant<int, 8>{}, (lane & 16) == 0);
+  steps(std::integral_constant<int, 16>{}, (lane & 32) == 0);
+  steps(std::integral_constant<int, 32>{}, true);
+  return v;
 }
 __device__ __forceinline__ uint64_t readlane_u64(uint64_t v, int l) {
   const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), l);
@@ -101,7 +147,7 @@ __device__ __forceinline__ PartSum add(const PartSum& a, const PartSum& b) {
 constexpr int kBeamWaves = 4, kBeamVecs = 4;  // waves per workgroup, 16-byte vectors per lane and step
 
 // One pass over logits [lo, hi) of a row by one wave.  A lane keeps its running maximum and sum.  A logit that may belong
-// to the n best (not below the last of the list) is put into a buffer in LDS; a full buffer is sorted and merged into the
+// to the n best (not below the last of the list) is put into a buffer in LDS; from 64 on it is sorted and merged into the
 // list.  The n-th largest of the lanes' own maxima is not above the n-th largest logit so far: taken as the bound after
 // the first step and whenever the steps have doubled, it lets few logits through.
 // The sum's terms are 2^(logit L - ref) with L = log2 e and ref = L times the maximum, rounded: one fused operation and the
@@ -118,12 +164,8 @@ __device__ __forceinline__ RowPart row_pass(const void* row, int lo, int hi, int
   int held = 0, step = 0;
   auto flush = [&]() {
     __builtin_amdgcn_wave_barrier();
-    uint64_t k = lane < held ? buffer[lane] : 0;
-    p.list = merge64(p.list, k);
-    if (held > 64) {
-      k = lane + 64 < held ? buffer[lane + 64] : 0;
-      p.list = merge64(p.list, k);
-    }
+#pragma unroll 1
+    for (int c = 0; c < held; c += 64) p.list = merge64(p.list, c + lane < held ? buffer[c + lane] : 0);
     __builtin_amdgcn_wave_barrier();
     held = 0;
     const uint64_t last = readlane_u64(p.list, n - 1);
@@ -205,12 +247,7 @@ __device__ __forceinline__ RowPart row_pass(const void* row, int lo, int hi, int
     p.max = mx;
     p.sum = sum;
     if ((step & (step + 1)) == 0) {  // after 1, 2, 4, 8 .. steps
-      float s = mx == mx ? mx : -inf;
-      for (int k = 2; k <= 64; k <<= 1)
-        for (int d = k >> 1; d > 0; d >>= 1) {
-          const float o = __shfl_xor(s, d);
-          s = ((lane & d) == 0) == ((lane & k) == 0) ? fmaxf(s, o) : fminf(s, o);
-        }
+      float s = sorted(mx == mx ? mx : -inf);
       s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s), n - 1));
       if (s > bound) {
         bound = s;
@@ -230,19 +267,9 @@ __device__ __forceinline__ RowPart row_pass(const void* row, int lo, int hi, int
         if (CLEAN && !(x == x)) x = -inf;
         const bool take = x >= bound && (x > bound || i + e <= bound_index) && i + e < hi;
         const uint64_t who = __ballot(take);
-        if (who == 0) continue;
-        if (held + __popcll(who) > 128) {
-          flush();
-          const bool still = take && x >= bound && (x > bound || i + e <= bound_index);
-          const uint64_t left = __ballot(still);
-          const int place = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(left >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(left), 0));
-          if (still) buffer[place] = top_key(x, i + e);
-          held = __popcll(left);
-        } else {
-          const int place = held + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
-          if (take) buffer[place] = top_key(x, i + e);
-          held += __popcll(who);
-        }
+        const int place = held + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
+        if (take) buffer[place] = top_key(x, i + e);  // (below 64 + 64 EV)
+        held += __popcll(who);
       }
       if (held >= 64) flush();
     }
@@ -254,7 +281,7 @@ __device__ __forceinline__ RowPart row_pass(const void* row, int lo, int hi, int
 // Part blockIdx.x of row blockIdx.y, a quarter of it per wave: its m best keys and its sum.
 template <int DT>
 __global__ __launch_bounds__(64 * kBeamWaves) void beam_row_kernel(BeamArgs a, int m, int part, uint64_t* keys, PartSum* sums) {
-  __shared__ uint64_t buffer[kBeamWaves][128];
+  __shared__ uint64_t buffer[kBeamWaves][64 + 64 * (DT == kBF16 ? 8 : 4)];
   __shared__ PartSum ps[kBeamWaves];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t r = blockIdx.y;
@@ -296,7 +323,7 @@ struct Offer {
 
 // One workgroup per request: a wave per beam merges its parts' lists into the beam's m best offers; the offers' ranks
 // among all beams' are then counted.  Bound by latency: the chains of sorting steps and of the 64-bit exponentials and
-// logarithm, 7 to 12 us.
+// logarithm, 6 to 12 us; all that a beam needs is read at once (4 beams 6.2 us against 6.8).
 __global__ __launch_bounds__(512) void beam_merge_kernel(BeamArgs a, int m, int parts, const uint64_t* keys, const PartSum* sums) {
   extern __shared__ __attribute__((aligned(16))) char lds_beam[];
   Offer* const offers = reinterpret_cast<Offer*>(lds_beam);
@@ -306,24 +333,31 @@ __global__ __launch_bounds__(512) void beam_merge_kernel(BeamArgs a, int m, int 
   const double inf = __builtin_inf();
   for (int k = wave; k < K; k += 8) {
     const int64_t r = b * K + k;
+    const uint64_t* const kr = keys + r * parts * m;
+    const PartSum* const sr = sums + r * parts;
+    // (under way together, also where they turn out not to be wanted)
     const float score = a.scores[r];
-    const bool live = fabsf(score) < __builtin_inff(), done = a.finished && a.finished[r];
+    const uint8_t fin = a.finished ? a.finished[r] : 0;
+    const uint64_t first = lane < parts * m ? kr[lane] : 0, second = lane + 64 < parts * m ? kr[lane + 64] : 0;
+    const PartSum own = lane < parts ? sr[lane] : PartSum{-inf, 0.0};
+    const bool live = fabsf(score) < __builtin_inff(), done = fin != 0;
     double value = -inf;
     int64_t token = lane;
     if (live && done) {
       token = lane == 0 ? a.pad : (lane <= a.pad ? lane - 1 : lane);
       if (lane == 0) value = score;
     } else if (live) {
-      const uint64_t* kr = keys + r * parts * m;
-      uint64_t list = 0;
-      for (int c = 0; c < parts * m; c += 64) list = merge64(list, c + lane < parts * m ? kr[c + lane] : 0);
-      double ref = -inf, s = 0.0;
-      for (int c = lane; c < parts; c += 64) ref = fmax(ref, sums[r * parts + c].ref);
-      for (int d = 32; d > 0; d >>= 1) ref = fmax(ref, __shfl_xor(ref, d));
-      for (int c = lane; c < parts; c += 64) {
-        const PartSum q = sums[r * parts + c];
-        s += q.ref == ref ? q.sum : q.sum * exp(q.ref - ref);
+      uint64_t list = 0, next = first;
+#pragma unroll 1
+      for (int c = 0; c < parts * m; c += 64) {
+        list = merge64(list, next);
+        next = c == 0 ? second : c + 64 + lane < parts * m ? kr[c + 64 + lane] : 0;
       }
+      double ref = own.ref, s = 0.0;
+      for (int c = lane + 64; c < parts; c += 64) ref = fmax(ref, sr[c].ref);
+      for (int d = 32; d > 0; d >>= 1) ref = fmax(ref, __shfl_xor(ref, d));
+      if (lane < parts) s = own.ref == ref ? own.sum : own.sum * exp(own.ref - ref);
+      for (int c = lane + 64; c < parts; c += 64) s += sr[c].ref == ref ? sr[c].sum : sr[c].sum * exp(sr[c].ref - ref);
       s = wave_sum_d<64>(s);
       const double lse = ref + log(s);
       if (fabs(lse) < inf) {
@@ -338,6 +372,7 @@ __global__ __launch_bounds__(512) void beam_merge_kernel(BeamArgs a, int m, int 
     const Offer o = offers[c];
     int rank = 0;
     if (c % m >= n) continue;
+#pragma unroll 8
     for (int j = 0; j < count; ++j) {
       const Offer q = offers[j];
       rank += before(q.value, q.flat, o.value, o.flat);
