@@ -303,6 +303,8 @@ struct SsmLds {
 
 // FULL: y and the final state of a segment from its carried-in state; otherwise the segment's end state from zero.
 // VEC: whole 32-column slices and 32-state steps, and 32-bit offsets inside a chunk.
+// (Two waves per SIMD also where float32 operands with 128 states then spill 32 registers: 14 sequences of 600 rows and 24
+// heads 179 us, with one wave and no spill 186; 256 states need the registers of one.)
 template <int DT, int NS, bool FULL, bool VEC>
 __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_kernel(SsmArgs a, SsmGrid gr) {
   using TT = Tile<DT>;
