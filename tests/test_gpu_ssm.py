@@ -4,8 +4,8 @@ Tolerances are bounds, elementwise.  ``u`` = 2^-24 is half a float32 step, ``e``
 (2^-8 relative for bfloat16).  ``mass`` is the sum of the magnitudes of a result's contributions.  A sum of n terms in
 float32 is off by at most n u mass; chunked products add their decays' errors (an exponential of a few ulps for every
 chunk passed).  With bfloat16 operands each contribution is rounded to bfloat16 once on the way (the decayed score inside
-a chunk, the state read across chunks: e mass in all), and states are sums of products whose scaled operand is held as two
-bfloat16 halves: 2^-16 relative.  The result is rounded once: e |y|.
+a chunk, the state read across chunks: e mass in all); states are sums of products whose scaled operand is held whole, as
+three bfloat16 parts.  The result is rounded once: e |y|.
 """
 import pytest
 import torch
@@ -225,8 +225,7 @@ def _check_scan(c, y, h):
     got = y.reshape(M, c["H"], c["P"])
     for lo, hi in spans:
         _within(got[lo:hi], want[lo:hi], tol[lo:hi], "scan rows %d..%d" % (lo, hi))
-    split = 2.0 ** -16 if c["dtype"] == torch.bfloat16 else 0.0
-    _within(h, want_h, (split + count * U) * mass_h + 1e-36, "scan state")
+    _within(h, want_h, count * U * mass_h + 1e-36, "scan state")
 
 
 SCANS = [  # B, L, H, P, G, N
