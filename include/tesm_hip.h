@@ -531,7 +531,8 @@ int tesm_hip_causal_conv(const tesm_hip_conv* p, void* stream);
  *   state[p,n] = a * state[p,n] + d * x[t,h,p] * B[t,g,n],
  *   y[t,h,p] = sum_n state[p,n] C[t,g,n] + D[h] x[t,h,p],  times silu(z[t,h,p]) with z.
  * Rows and seq_starts as in tesm_hip_causal_conv.  h0 / h_out: (S, H, P, N) float32, the states before and
- * after each sequence (NULL h0: zeros; h_out is another buffer).  N <= 256; ws: selective_scan_ws_bytes. */
+ * after each sequence (NULL h0: zeros; h_out is another buffer).  y must not overlap the operands.  N <= 256,
+ * H * P and the row pitches below 2^24, fewer than 65536 sequences; ws: selective_scan_ws_bytes. */
 typedef struct tesm_hip_ssm {
   int dt;                     /* x, dts, Bm, Cm, z, y */
   int64_t B, L, H, P, G, N, S;
@@ -594,7 +595,8 @@ int tesm_hip_selective_scan_step(const tesm_hip_ssm_step* p, void* stream);
  * written in falling order, equal ones by k * V + v.  Offers that are no number (a NaN logit; a row with
  * a +infinite logit or none above -infinity) and all offers of a beam whose score is not finite count as
  * -infinity.  A beam with finished != 0 offers token pad alone, at its own score.  finished_out: the
- * parent was finished, or the token is eos (eos < 0: no such token).  K, n <= 64, n <= K * V. */
+ * parent was finished, or the token is eos (eos < 0: no such token).  The outputs must not overlap the
+ * inputs.  K, n <= 64, n <= K * V, B * K < 65536, V < 2^30. */
 typedef struct tesm_hip_beam {
   int dt;                     /* logits */
   int64_t B, K, V, n;
