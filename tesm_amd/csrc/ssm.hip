@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "ssm.h"
+#include "ssm_chunk.h"
 
 namespace tesm {
 
@@ -66,7 +67,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // 585 + 270 us, 2.1 TB/s.
 // ---------------------------------------------------------------------------
 constexpr int kCols = 128;  // columns per workgroup
-constexpr int kQ = 32;      // rows per chunk
 
 template <int DT>
 struct Tile;
@@ -312,7 +312,9 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
   using Frag = typename TT::Frag;
   using Lds = SsmLds<DT, NS, FULL>;
   constexpr int EV = TT::EV, NB = TT::NB, WP = Lds::WP, UX = Lds::UX, UB = Lds::UB;
-  constexpr int XR = kQ * UX / 256, BR = kQ * UB >= 256 ? kQ * UB / 256 : 1;  // units per thread
+  using XU = ChunkUnits<UX>;
+  using BU = ChunkUnits<UB>;
+  constexpr int XR = XU::kEach, BR = BU::kEach;  // units per thread
   extern __shared__ __attribute__((aligned(16))) char lds_s[];
   E* const stages = reinterpret_cast<E*>(lds_s);
   E* const Ws = stages + NB * Lds::kStage;
@@ -380,7 +382,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
   const uint32_t px = static_cast<uint32_t>(a.ld_x * es), pb = static_cast<uint32_t>(a.ld_b * es), pc = static_cast<uint32_t>(a.ld_c * es);
   const uint32_t pz = static_cast<uint32_t>(a.ld_z * es), py = static_cast<uint32_t>(a.ld_y * es);
   auto load_rows = [&](const char* at, uint32_t pitch, int last, auto whole, int r, int col, int count, bool in) __attribute__((always_inline)) {
-    const uint32_t off = static_cast<uint32_t>(whole.value ? r : min(r, last)) * pitch;
+    const uint32_t off = static_cast<uint32_t>(chunk_source(whole.value, r, last)) * pitch;
     if constexpr (VEC) return load16(at + (off + static_cast<uint32_t>(col * sizeof(E))));
     return in ? load_unit<DT>(at + off, 0, col, count) : make_uint4(0, 0, 0, 0);
   };
@@ -389,11 +391,11 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
     const int last = sg.r1 - 1 - row0;
 #pragma unroll
     for (int i = 0; i < XR; ++i)
-      xr[i] = load_rows(xat, px, last, whole, tid / UX + i * (256 / UX), xcol, xcol - xp + P, xin);
+      xr[i] = load_rows(xat, px, last, whole, XU::row(tid, i), xcol, xcol - xp + P, xin);
 #pragma unroll
     for (int i = 0; i < BR; ++i) {
-      br[i] = load_rows(bat, pb, last, whole, tid / UB + i * (256 / UB), bc, N, bin);
-      if constexpr (FULL) cr[i] = load_rows(cat, pc, last, whole, tid / UB + i * (256 / UB), bc, N, bin);
+      br[i] = load_rows(bat, pb, last, whole, BU::row(tid, i), bc, N, bin);
+      if constexpr (FULL) cr[i] = load_rows(cat, pc, last, whole, BU::row(tid, i), bc, N, bin);
     }
     if (FULL && a.z && active) {  // the gate of this lane's outputs
 #pragma unroll
@@ -480,20 +482,20 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
     if (left < kQ) {
 #pragma unroll
       for (int i = 0; i < XR; ++i)
-        if (tid / UX + i * (256 / UX) >= left) xr[i] = make_uint4(0, 0, 0, 0);
+        if (XU::row(tid, i) >= left) xr[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < BR; ++i)
-        if (tid / UB + i * (256 / UB) >= left) {
+        if (BU::row(tid, i) >= left) {
           br[i] = make_uint4(0, 0, 0, 0);
           if constexpr (FULL) cr[i] = make_uint4(0, 0, 0, 0);
         }
     }
 #pragma unroll
-    for (int i = 0; i < XR; ++i) *reinterpret_cast<uint4*>(X + TT::template unit<UX>(tid / UX + i * (256 / UX), tid % UX)) = xr[i];
+    for (int i = 0; i < XR; ++i) *reinterpret_cast<uint4*>(X + TT::template unit<UX>(XU::row(tid, i), tid % UX)) = xr[i];
 #pragma unroll
     for (int i = 0; i < BR; ++i) {
-      if (kQ * UB < 256 && tid >= kQ * UB) break;
-      const int at = TT::template unit<UB>(tid / UB + i * (256 / UB), tid % UB);
+      if (!BU::stages(tid)) break;
+      const int at = TT::template unit<UB>(BU::row(tid, i), tid % UB);
       *reinterpret_cast<uint4*>(Bs + at) = br[i];
       if constexpr (FULL) *reinterpret_cast<uint4*>(Cs + at) = cr[i];
     }
