@@ -130,16 +130,19 @@ __device__ __forceinline__ void st4(void* p, int64_t i, const float (&v)[4]) {
 // rounds to bf16 is rounded again afterwards).  Built on the hardware exp2 / reciprocal.
 // ---------------------------------------------------------------------------
 // e^x = 2^(x log2 e), with x * log2 e split into a rounded product and its error term so that
-// the argument error stays below an ulp of 2^t for |x| up to ~88.
+// the argument error stays below an ulp of 2^t for |x| up to ~88.  Beyond, 2^t is +0 or infinite and is the result: the
+// error term, of either sign and infinite itself where t overflows, would make NaN of it.
 __device__ __forceinline__ float fast_exp(float x) {
   constexpr float kL2e = 1.44269504088896340736f;
+  constexpr int kPlusZero = 1 << 6, kPlusInfinity = 1 << 9;
   const float t = x * kL2e;
   const float err = __builtin_fmaf(x, kL2e, -t) + x * 1.925963033500e-8f;  // log2(e) - kL2e
   const float r = __builtin_amdgcn_exp2f(t);
-  return __builtin_fmaf(r, err * 0.69314718055994531f, r);
+  const float v = __builtin_fmaf(r, err * 0.69314718055994531f, r);
+  return __builtin_amdgcn_classf(r, kPlusZero | kPlusInfinity) ? r : v;
 }
 
-// 1 / (1 + e^-x); saturates to 0 / 1 without NaN for large |x|.
+// 1 / (1 + e^-x); saturates to 0 / 1 without NaN for large |x|, infinite ones among them.
 __device__ __forceinline__ float sigmoidf_(float x) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-x)); }
 
 // tanh: odd Taylor polynomial below |x| = 0.25 (truncation < 1e-8 relative), otherwise

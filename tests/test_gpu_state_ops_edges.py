@@ -3,8 +3,10 @@ Tolerances are those of the operators' own tests (``test_gpu_ssm``, ``test_gpu_b
 import pytest
 import torch
 
-from hip_helpers import need_gpu
-from test_gpu_ssm import _check_scan, _run_scan, _scan_case
+from hip_helpers import DEV, TOL, need_gpu, normwise, to_np
+from oracle import tesm_torch as ot
+from tesm_amd import TESM_SISO, hip_ops
+from test_gpu_ssm import HALF, U, _check_scan, _dev, _randn, _run_scan, _scan_case, _silu, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +33,139 @@ def test_scan_of_few_states_in_whole_chunks(dtype, N, L):
 def test_scan_of_few_states_packed_in_whole_chunks(N):
     c = _scan_case(N, 1, 1056, 2, 24, 2, N, torch.bfloat16, starts=[0, 32, 96, 96, 1056])
     _check_scan(c, *_run_scan(c))
+
+
+# ---------------------------------------------------------------------------
+# activations and gates far from zero.  e^-v overflows below v = -88.7: silu(v) is 0 there.  Elsewhere silu is off by 8 u of
+# its value, with bfloat16 operands by |v| u more (the exponent is one rounded product); a reciprocal below 2^-126 may
+# come out as 0, which is off by at most 89 * 2^-126 < 2^-119.
+# ---------------------------------------------------------------------------
+FAR = [80.0, 85.0, 87.0, 88.0, 89.0, 92.0, 95.0, 100.0, 110.0, 200.0, 500.0, 1000.0, 1e4, 1e9, 1e30, 3e38]
+
+
+def _far(dtype):
+    v = torch.tensor(FAR)
+    more = torch.cat([torch.linspace(-130.0, -80.0, 400), torch.linspace(-2e4, -130.0, 400)])
+    return torch.cat([v, -v, more]).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("C", [1, 5, None])
+def test_conv_of_far_values(dtype, C):
+    v = _far(dtype)
+    x = v[:, None, None].expand(-1, 1, C).contiguous() if C else v.view(1, 1, -1)
+    w = torch.tensor([0.0, 1.0], dtype=dtype).expand(x.shape[2], 2)
+    y, _ = hip_ops.causal_conv(_dev(x), _dev(w))
+    want = _silu(x.double())
+    _within(y, want, ((8 + x.double().abs().clamp(max=1e3)) * U + HALF[dtype]) * want.abs() + 2.0 ** -119, "conv")
+    top = torch.full((1, 1, 8), float("inf"), dtype=dtype)
+    assert bool((hip_ops.causal_conv(_dev(top), _dev(torch.ones(8, 2, dtype=dtype)))[0] == float("inf")).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scan_gate_of_far_values(dtype):
+    # (values whose gate is a normal number or below 2^-126 by far: the scan's bound has no term for what lies between)
+    v = torch.tensor([f for f in FAR if f < 87 or f > 90]).to(dtype)
+    v = torch.cat([v[v < 1e31], -v])
+    c = _scan_case(101, 1, 70, 2, 40, 1, 16, dtype)
+    c["z"] = v[torch.arange(c["z"].numel()) % v.numel()].view(c["z"].shape).contiguous()
+    _check_scan(c, *_run_scan(c))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bias", [True, False])
+def test_scan_of_masked_step_sizes(dtype, bias):
+    """Step sizes masked by the type's lowest value, by -infinity or by large negative numbers are 0: those rows leave
+    the state as it is."""
+    c = _scan_case(102, 2, 75, 3, 32, 1, 32, dtype, bias=bias)
+    for i, low in enumerate((torch.finfo(dtype).min, float("-inf"), -1e30, -1e4, -95.0)):
+        c["dt"][:, 3 + i::7] = low
+    c["dt"][1, 40:] = torch.finfo(dtype).min
+    _check_scan(c, *_run_scan(c))
+
+
+def _check_step(c, W):
+    """One token with the filter (0, .., 0, 1), so that the convolved values are silu(row), against 64 bits."""
+    B, H, P, G, N, dtype = (c[k] for k in ("B", "H", "P", "G", "N", "dtype"))
+    width = H * P + 2 * G * N
+    w = torch.zeros(width, W, dtype=dtype)
+    w[:, -1] = 1
+    hd = _dev(c["h"]).clone()
+    y, _ = hip_ops.selective_scan_step(_dev(c["row"]), _dev(c["dt"]), _dev(c["A"]), hd, _dev(w), None,
+                                       torch.zeros(B, W - 1, width, dtype=dtype, device=DEV), n_groups=G, z=_dev(c["z"]))
+    v = _silu(c["row"].double())
+    dv = (8 + c["row"].double().abs().clamp(max=1e3)) * U * v.abs() + 2.0 ** -119
+    cut = [H * P, G * N, G * N]
+    (x, b, cc), (dx, db, dc) = v.split(cut, 1), dv.split(cut, 1)
+    x, dx = (t.reshape(B, H, P) for t in (x, dx))
+    b, cc, db, dc = (t.reshape(B, G, N).repeat_interleave(H // G, 1)[:, :, None] for t in (b, cc, db, dc))
+    raw = c["dt"].double()
+    d = torch.where(raw < -30, raw.exp(), torch.nn.functional.softplus(raw, threshold=700))
+    a = (d * c["A"].double()).exp()[..., None, None]
+    add = (d[..., None] * x)[..., None] * b
+    hn = a * c["h"].double() + add
+    mass = (a * c["h"].double()).abs() + add.abs()
+    dh = d[..., None, None] * (dx[..., None] * b.abs() + x.abs()[..., None] * db) + 48 * U * mass
+    _within(hd, hn, dh + 1e-36, "step state")
+    gate = _silu(c["z"].double())
+    dg = (8 + c["z"].double().abs().clamp(max=1e3)) * U * gate.abs() + 2.0 ** -119
+    core = (hn * cc).sum(-1)
+    ym = (hn.abs() * cc.abs()).sum(-1)
+    tol = gate.abs() * ((dh * cc.abs() + hn.abs() * dc).sum(-1) + (N + 16) * U * ym) + dg * ym
+    _within(y, core * gate, tol + HALF[dtype] * (core * gate).abs() + 1e-36, "step y")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N", [16, 33])
+def test_step_of_far_values(dtype, N):
+    g = torch.Generator().manual_seed(103)
+    B, H, P, G = 3, 4, 40, 2
+    c = dict(B=B, H=H, P=P, G=G, N=N, dtype=dtype)
+    width = H * P + 2 * G * N
+    c["row"] = _randn(g, B, width, dtype=dtype)
+    low = -_far(dtype)[:len(FAR)]
+    c["row"][:, ::3] = low[torch.arange(c["row"][:, ::3].numel()) % len(FAR)].view(B, -1)
+    c["dt"] = _randn(g, B, H, dtype=dtype)
+    c["dt"][0, 1], c["dt"][1, 2], c["dt"][2, 0], c["dt"][2, 3] = torch.finfo(dtype).min, float("-inf"), -95.0, 120.0
+    c["A"] = -(0.3 + 4 * torch.rand(H, generator=g))
+    v = _far(dtype)
+    v = v[v < 1e31]
+    c["z"] = v[torch.arange(B * H * P) % v.numel()].view(B, H, P).contiguous()
+    c["h"] = _randn(g, B, H, P, N)
+    _check_step(c, 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_output_gate_of_far_values(dtype):
+    """Gates below -88.7 are 0 like those whose sigmoid is lost beside the other addend."""
+    g = torch.Generator().manual_seed(104)
+    M, dm, D = 32, 64, 64
+    codes = [hip_ops.quant_act(_randn(g, M, D, dtype=dtype).to(DEV)) for _ in range(2)]
+    packed = []
+    for _ in range(2):
+        w = _randn(g, dm, D).to(DEV)
+        s, cw = hip_ops.absmean_scale(w)
+        packed += [hip_ops.pack_weight(w, s), cw]
+    low = -_far(dtype)[:len(FAR)][torch.arange(M * dm) % len(FAR)].view(M, dm).to(DEV)
+    local = _randn(g, M, dm, dtype=dtype).to(DEV)
+    for quantize in (True, False):
+        y, _ = hip_ops.output_gate(*codes, *packed, local, low, D, quantize=quantize)
+        want, _ = hip_ops.output_gate(*codes, *packed, local, torch.full_like(low, -80.0), D, quantize=quantize)
+        # sigmoid(-80) = 1.8e-35: no bit of a sum of ordinary numbers
+        assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("decay_bias", [-95.0, -110.0, -1000.0])
+def test_layer_of_closed_decay_gates(dtype, decay_bias):
+    cfg = dict(d_model=64, d_state=32, ent_rank=8, entanglement_window=8, entanglement_threshold=0.08,
+               entanglement_scale=0.2, decay_init_bias=decay_bias, max_seq_len=64)
+    torch.manual_seed(0)
+    ref = ot.TESM_SISO(**cfg).eval()
+    torch.manual_seed(0)
+    m = TESM_SISO(**cfg).to(DEV).to(dtype).eval()
+    u = torch.randn(2, 40, 64, generator=torch.Generator().manual_seed(1))
+    y, _ = m(u.to(DEV).to(dtype))
+    want, _ = ref.to(dtype)(u.to(dtype))
+    assert bool(y.isfinite().all())
+    assert normwise(to_np(y), to_np(want)) <= TOL[dtype]
