@@ -145,14 +145,17 @@ __device__ __forceinline__ PartSum add(const PartSum& a, const PartSum& b) {
 }
 
 constexpr int kBeamWaves = 4, kBeamVecs = 4;  // waves per workgroup, 16-byte vectors per lane and step
+constexpr float kFar = 1.0e6f;
 
 // One pass over logits [lo, hi) of a row by one wave.  A lane keeps its running maximum and sum.  A logit that may belong
 // to the n best (not below the last of the list) is put into a buffer in LDS; from 64 on it is sorted and merged into the
 // list.  The n-th largest of the lanes' own maxima is not above the n-th largest logit so far: taken as the bound after
 // the first step and whenever the steps have doubled, it lets few logits through.
 // The sum's terms are 2^(logit L - ref) with L = log2 e and ref = L times the maximum, rounded: one fused operation and the
-// exponential.  Where a logit is NaN, +infinite or beyond 2e38 this form's sum is NaN or too
-// small, and the pass is made again with CLEAN: terms 2^((logit - max) L), a NaN counts as -infinity.
+// exponential.  The largest logit's own term is then 2^d, d the rounding of ref: within a sixteenth of 0 for maxima up to
+// kFar either way, but up to 64 at 1e9.  A lane whose maximum is below -kFar takes ref from -kFar, and its terms may all be
+// 0; sum_is_off tells where that matters.  There, and where a logit is NaN or the maximum above kFar, the pass is made again
+// with CLEAN: terms 2^((logit - max) L), a NaN counts as -infinity.
 template <int DT, bool CLEAN>
 __device__ __forceinline__ RowPart row_pass(const void* row, int lo, int hi, int n, uint64_t* buffer) {
   constexpr int EV = DT == kBF16 ? 8 : 4, ES = 16 / EV, STEP = 64 * EV * kBeamVecs;
@@ -226,8 +229,8 @@ __device__ __forceinline__ RowPart row_pass(const void* row, int lo, int hi, int
       ref = fmaxf(mx, -FLT_MAX);
       scale = p.max == mx ? 1.0f : __builtin_amdgcn_exp2f((fmaxf(p.max, -FLT_MAX) - ref) * kLog2e);
     } else {
-      ref = fmaxf(mx, -2.0e38f) * kLog2e;
-      scale = __builtin_amdgcn_exp2f(fmaxf(p.max, -2.0e38f) * kLog2e - ref);
+      ref = fmaxf(mx, -kFar) * kLog2e;
+      scale = __builtin_amdgcn_exp2f(fmaxf(p.max, -kFar) * kLog2e - ref);
     }
     float sum = p.sum * scale;
 #pragma unroll
@@ -278,6 +281,13 @@ __device__ __forceinline__ RowPart row_pass(const void* row, int lo, int hi, int
   return p;
 }
 
+// Whether a lane's sum of the first form does not hold its largest terms, and the part's sum (`top`: its largest logit) needs
+// them: terms 200 below the largest are lost in it anyway (a lane that met masked logits alone).
+__device__ __forceinline__ bool sum_is_off(const RowPart& p, float top) {
+  if (p.max > kFar || !(p.sum == p.sum)) return true;
+  return p.sum < 0.5f && p.max > -__builtin_inff() && p.max >= top - 200.0f;
+}
+
 // Part blockIdx.x of row blockIdx.y, a quarter of it per wave: its m best keys and its sum.
 template <int DT>
 __global__ __launch_bounds__(64 * kBeamWaves) void beam_row_kernel(BeamArgs a, int m, int part, uint64_t* keys, PartSum* sums) {
@@ -291,14 +301,18 @@ __global__ __launch_bounds__(64 * kBeamWaves) void beam_row_kernel(BeamArgs a, i
   const int each = part / kBeamWaves, V = static_cast<int>(a.V);
   const int lo = min(static_cast<int>(blockIdx.x) * part + wave * each, V), hi = min(lo + each, V);
   RowPart p = row_pass<DT, false>(row, lo, hi, m, buffer[wave]);
-  // a lane that saw a finite logit has a sum of 1 or more: the largest one's own term
-  const bool again = __any(!(p.sum > 0.5f) && p.max > -__builtin_inff()) || __any(!(p.sum == p.sum));
-  if (again) p = row_pass<DT, true>(row, lo, hi, m, buffer[wave]);
+  float mx = wave_max<64>(p.max);
+  const bool again = __any(sum_is_off(p, mx));
+  if (again) {
+    p = row_pass<DT, true>(row, lo, hi, m, buffer[wave]);
+    mx = wave_max<64>(p.max);
+  }
   // over the lanes, then the waves
-  const float mx = wave_max<64>(p.max), top = fmaxf(mx, again ? -FLT_MAX : -2.0e38f), own = fmaxf(p.max, again ? -FLT_MAX : -2.0e38f);
+  const float top = fmaxf(mx, again ? -FLT_MAX : -kFar), own = fmaxf(p.max, again ? -FLT_MAX : -kFar);
   const float scale = p.max == mx ? 1.0f : __builtin_amdgcn_exp2f(again ? (own - top) * kLog2e : own * kLog2e - top * kLog2e);
   const float s = wave_sum_f<64>(p.sum * scale);
-  const double ref = again ? static_cast<double>(mx) : static_cast<double>(mx * kLog2e) * 0.69314718055994530942;
+  // (a part of -infinities alone keeps such a reference)
+  const double ref = again || mx == -__builtin_inff() ? static_cast<double>(mx) : static_cast<double>(top * kLog2e) * 0.69314718055994530942;
   if (lane == 0) ps[wave] = {ref, s};
   buffer[wave][lane] = p.list;
   __syncthreads();

@@ -6,6 +6,7 @@ import torch
 from hip_helpers import DEV, TOL, need_gpu, normwise, to_np
 from oracle import tesm_torch as ot
 from tesm_amd import TESM_SISO, hip_ops
+from test_gpu_beam import INF, _case, check_select
 from test_gpu_ssm import HALF, U, _check_scan, _dev, _randn, _run_scan, _scan_case, _silu, _within
 
 pytestmark = pytest.mark.gpu
@@ -169,3 +170,36 @@ def test_layer_of_closed_decay_gates(dtype, decay_bias):
     want, _ = ref.to(dtype)(u.to(dtype))
     assert bool(y.isfinite().all())
     assert normwise(to_np(y), to_np(want)) <= TOL[dtype]
+
+
+# ---------------------------------------------------------------------------
+# beam selection: logits of any magnitude
+# ---------------------------------------------------------------------------
+MASKS = [-1e4, -1e6, -1.1e6, -1e9, -3e9, -1e10, -1e20, -1e30, -3e38]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("allowed", [1, 40, 3000])
+def test_select_of_masked_rows(dtype, mask, allowed):
+    """A few allowed tokens among ones masked by a large negative number: anywhere in the row, all in one part of it."""
+    logits, scores, g = _case(200 + allowed, 4, 3, 20000, dtype)
+    keep = torch.zeros(20000, dtype=torch.bool)
+    keep[torch.randperm(20000, generator=g)[:allowed]] = True
+    logits[:2, :, ~keep] = mask
+    logits[2, :, allowed:] = mask
+    logits[3, :2, :-allowed] = mask
+    check_select(logits, scores, 8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("top", [3e9, -3e9, 1e10, -1e10, 1e20, -1e20, 3e38, -3e38])
+def test_select_of_rows_far_from_zero(dtype, top):
+    """Rows whose largest logits are far from zero, equal or spread over a few steps of the type."""
+    logits, scores, g = _case(210, 4, 2, 9000, dtype)
+    step = abs(top) * torch.finfo(dtype).eps
+    logits[0] = top
+    logits[1] = (top + step * torch.randint(-3, 1, logits[1].shape, generator=g).double()).to(dtype)
+    logits[2, :, ::5] = top
+    logits[3, 0], logits[3, 1, 100:] = top, -INF
+    check_select(logits, scores, 6)
