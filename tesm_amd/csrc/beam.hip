@@ -311,8 +311,11 @@ __global__ __launch_bounds__(64 * kBeamWaves) void beam_row_kernel(BeamArgs a, i
   const float top = fmaxf(mx, again ? -FLT_MAX : -kFar), own = fmaxf(p.max, again ? -FLT_MAX : -kFar);
   const float scale = p.max == mx ? 1.0f : __builtin_amdgcn_exp2f(again ? (own - top) * kLog2e : own * kLog2e - top * kLog2e);
   const float s = wave_sum_f<64>(p.sum * scale);
-  // (a part of -infinities alone keeps such a reference)
-  const double ref = again || mx == -__builtin_inff() ? static_cast<double>(mx) : static_cast<double>(top * kLog2e) * 0.69314718055994530942;
+  // The first form's terms are exp(logit - top) times 2^(top L - r) in the float L, r the rounded product: in 64 bits the
+  // product of two floats is exact, and what the sum has too much is taken off its reference (r ln 2 would be off by 1.3e-8
+  // top, L's own error).  A part of -infinities alone keeps such a reference.
+  const double t = top, over = t * static_cast<double>(kLog2e) - static_cast<double>(top * kLog2e);
+  const double ref = again || mx == -__builtin_inff() ? static_cast<double>(mx) : t - 0.69314718055994530942 * over;
   if (lane == 0) ps[wave] = {ref, s};
   buffer[wave][lane] = p.list;
   __syncthreads();

@@ -203,3 +203,15 @@ def test_select_of_rows_far_from_zero(dtype, top):
     logits[2, :, ::5] = top
     logits[3, 0], logits[3, 1, 100:] = top, -INF
     check_select(logits, scores, 6)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [500, 20000])
+@pytest.mark.parametrize("offset", [100.0, 1000.0, 10000.0, 1.1e6, 1e7])
+def test_select_of_shifted_rows(dtype, V, offset):
+    """A beam's offers do not depend on an offset of its logits: the scores keep their bound at every offset."""
+    logits, scores, _ = _case(220, 4, 4, V, torch.float32)
+    logits[:, 1] += offset
+    logits[:, 2] -= offset
+    logits[1, 3, ::2] += offset
+    check_select(logits.to(dtype), scores, 8)
