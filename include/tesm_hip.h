@@ -531,7 +531,9 @@ int tesm_hip_causal_conv(const tesm_hip_conv* p, void* stream);
  *   state[p,n] = a * state[p,n] + d * x[t,h,p] * B[t,g,n],
  *   y[t,h,p] = sum_n state[p,n] C[t,g,n] + D[h] x[t,h,p],  times silu(z[t,h,p]) with z.
  * Rows and seq_starts as in tesm_hip_causal_conv.  h0 / h_out: (S, H, P, N) float32, the states before and
- * after each sequence (NULL h0: zeros; h_out is another buffer).  y must not overlap the operands.  N <= 256,
+ * after each sequence (NULL h0: zeros; h_out is another buffer).  Outputs that overlap an operand or each other
+ * are refused, as they are by tesm_hip_causal_conv and tesm_hip_selective_scan_step (columns of the same wider
+ * rows do not overlap).  N <= 256,
  * H * P and the row pitches below 2^24, fewer than 65536 sequences; ws: selective_scan_ws_bytes. */
 typedef struct tesm_hip_ssm {
   int dt;                     /* x, dts, Bm, Cm, z, y */

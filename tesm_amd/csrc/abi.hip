@@ -16,6 +16,7 @@
 #include "global.h"
 #include "mimo.h"
 #include "norm.h"
+#include "rows_overlap.h"
 #include "scan.h"
 #include "ssm.h"
 #include "tesm_hip_internal.h"
@@ -1906,8 +1907,83 @@ int tesm_hip_ffn_forward(const tesm_hip_ffn* pp, void* ws, int64_t ws_bytes, voi
   return run_linear(s.hq, p.down_proj, p.M, p.d_model, p.d_inter, p.y, p.dt, p.ld_y, st);
 }
 
+}  // extern "C"
+
+namespace tesm {
+namespace {
+struct NamedSpan {
+  const char* name;
+  RowSpan rows;
+};
+RowSpan span(const void* p, int64_t n, int64_t pitch, int64_t width, int64_t size) { return {p, n, pitch * size, width * size}; }
+RowSpan dense(const void* p, int64_t count, int64_t size) { return {p, p ? 1 : 0, count * size, count * size}; }
+
+// Workgroups read the inputs while others already write: no output may share memory with an input or another output.
+int check_overlaps(const char* who, std::initializer_list<NamedSpan> outputs, std::initializer_list<NamedSpan> inputs) {
+  for (const NamedSpan* o = outputs.begin(); o != outputs.end(); ++o) {
+    for (const NamedSpan& i : inputs)
+      if (rows_share(o->rows, i.rows)) return fail(kErrInvalidArg, std::string(who) + ": " + o->name + " overlaps " + i.name);
+    for (const NamedSpan* q = o + 1; q != outputs.end(); ++q)
+      if (rows_share(o->rows, q->rows)) return fail(kErrInvalidArg, std::string(who) + ": " + o->name + " overlaps " + q->name);
+  }
+  return kOk;
+}
+
+int64_t size_of(int dt) { return dt == kBF16 ? 2 : 4; }
+// (sizes whose products fit 64 bits; others are refused behind, or beyond any memory)
+bool plain_sizes(std::initializer_list<int64_t> sizes, std::initializer_list<int64_t> pitches) {
+  for (int64_t v : sizes)
+    if (v < 0 || v >= (1LL << 31)) return false;
+  for (int64_t v : pitches)
+    if (v < 0 || v >= (1LL << 28)) return false;
+  return true;
+}
+
+int check_overlaps(const tesm_hip_conv& p) {
+  if (!plain_sizes({p.B, p.L, p.C, p.W, p.S}, {p.ld_x, p.ld_y}) || p.B * p.L >= (1LL << 31) || p.C >= (1LL << 23) || p.S >= (1LL << 24) || p.W > kConvMaxW)
+    return kOk;
+  const int64_t M = p.B * p.L, e = size_of(p.dt), we = size_of(p.w_dt), states = p.S * (p.W - 1) * p.C;
+  return check_overlaps("causal conv", {{"y", span(p.y, M, p.ld_y, p.C, e)}, {"state_out", dense(p.state_out, states, e)}},
+                        {{"x", span(p.x, M, p.ld_x, p.C, e)}, {"state", dense(p.state, states, e)},
+                         {"weight", dense(p.weight, p.C * p.W, we)}, {"bias", dense(p.bias, p.C, we)},
+                         {"seq_starts", dense(p.seq_starts, p.S + 1, 4)}});
+}
+
+int check_overlaps(const tesm_hip_ssm& p) {
+  if (!plain_sizes({p.B, p.L, p.H, p.P, p.G, p.N, p.S}, {p.ld_x, p.ld_dt, p.ld_b, p.ld_c, p.ld_y, p.ld_z}) || p.B * p.L >= (1LL << 31) ||
+      p.H * p.P >= (1LL << 24) || p.N > kSsmMaxN || p.S >= (1LL << 24))
+    return kOk;
+  const int64_t M = p.B * p.L, e = size_of(p.dt), hp = p.H * p.P, gn = p.G * p.N, states = p.S * hp * p.N;
+  return check_overlaps("selective scan", {{"y", span(p.y, M, p.ld_y, hp, e)}, {"h_out", dense(p.h_out, states, 4)}},
+                        {{"x", span(p.x, M, p.ld_x, hp, e)}, {"dt", span(p.dts, M, p.ld_dt, p.H, e)},
+                         {"B", span(p.Bm, M, p.ld_b, gn, e)}, {"C", span(p.Cm, M, p.ld_c, gn, e)},
+                         {"z", span(p.z, M, p.ld_z, hp, e)}, {"h0", dense(p.h0, states, 4)}, {"A", dense(p.A, p.H, 4)},
+                         {"D", dense(p.D, p.H, 4)}, {"dt_bias", dense(p.dt_bias, p.H, 4)},
+                         {"seq_starts", dense(p.seq_starts, p.S + 1, 4)}});
+}
+
+int check_overlaps(const tesm_hip_ssm_step& p) {
+  if (!plain_sizes({p.B, p.H, p.P, p.G, p.N, p.W}, {p.ld_row, p.ld_dt, p.ld_z, p.ld_y}) || p.H * p.P >= (1LL << 24) || p.N > kSsmMaxN ||
+      p.G > p.H || p.W > kConvMaxW)
+    return kOk;
+  const int64_t e = size_of(p.dt), we = size_of(p.w_dt), hp = p.H * p.P, C = hp + 2 * p.G * p.N;
+  const int64_t window = p.conv_weight && p.W > 1 ? p.B * (p.W - 1) * C : 0;
+  return check_overlaps("selective scan step",
+                        {{"y", span(p.y, p.B, p.ld_y, hp, e)}, {"state", dense(p.state, p.B * hp * p.N, 4)},
+                         {"conv_state_out", dense(p.conv_state_out, window, e)}},
+                        {{"row", span(p.row, p.B, p.ld_row, C, e)}, {"conv_state", dense(p.conv_state, window, e)},
+                         {"dt", span(p.dts, p.B, p.ld_dt, p.H, e)}, {"z", span(p.z, p.B, p.ld_z, hp, e)},
+                         {"conv_weight", dense(p.conv_weight, C * p.W, we)}, {"conv_bias", dense(p.conv_bias, C, we)},
+                         {"A", dense(p.A, p.H, 4)}, {"D", dense(p.D, p.H, 4)}, {"dt_bias", dense(p.dt_bias, p.H, 4)}});
+}
+}  // namespace
+}  // namespace tesm
+
+extern "C" {
+
 int tesm_hip_causal_conv(const tesm_hip_conv* p, void* stream) {
   TESM_REQUIRE(p != nullptr, kErrInvalidArg, "causal conv: null descriptor");
+  if (int rc = check_overlaps(*p)) return rc;
   if (int rc = check_ptrs("causal conv", {{p->x, "x"}, {p->weight, "weight"}, {p->bias, "bias"},
                                           {p->seq_starts, "seq_starts"}, {p->state, "state"}, {p->y, "y"},
                                           {p->state_out, "state_out"}}))
@@ -1975,6 +2051,7 @@ int64_t tesm_hip_selective_scan_ws_bytes(const tesm_hip_ssm* p) {
 
 int tesm_hip_selective_scan(const tesm_hip_ssm* p, void* ws, int64_t ws_bytes, void* stream) {
   TESM_REQUIRE(p != nullptr, kErrInvalidArg, "selective scan: null descriptor");
+  if (int rc = check_overlaps(*p)) return rc;
   if (int rc = check_ptrs("selective scan",
                           {{p->x, "x"}, {p->dts, "dt"}, {p->A, "A"}, {p->Bm, "B"}, {p->Cm, "C"}, {p->D, "D"},
                            {p->z, "z"}, {p->dt_bias, "dt_bias"}, {p->seq_starts, "seq_starts"}, {p->h0, "h0"},
@@ -1985,6 +2062,7 @@ int tesm_hip_selective_scan(const tesm_hip_ssm* p, void* ws, int64_t ws_bytes, v
 
 int tesm_hip_selective_scan_step(const tesm_hip_ssm_step* p, void* stream) {
   TESM_REQUIRE(p != nullptr, kErrInvalidArg, "selective scan step: null descriptor");
+  if (int rc = check_overlaps(*p)) return rc;
   if (int rc = check_ptrs("selective scan step",
                           {{p->row, "row"}, {p->conv_weight, "conv_weight"}, {p->conv_bias, "conv_bias"},
                            {p->conv_state, "conv_state"}, {p->conv_state_out, "conv_state_out"}, {p->dts, "dt"},

@@ -529,10 +529,11 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     ``y[b, t, c] = silu(bias[c] + sum_j weight[c, j] x[b, t - W + 1 + j, c])`` (``silu=False``: no activation) for x
     (B, L, C) and ``weight`` (C, W), 2 <= W <= 8, summed in float32.  With ``seq_starts`` (S + 1, on the device, not
     decreasing) x is (1, rows, C) and holds S sequences one behind the other, sequence s in rows
-    ``seq_starts[s] .. seq_starts[s + 1] - 1`` (starts past the rows count as their end); rows in front of the first and behind the last one stay as they are in
-    ``out`` (zero without ``out``).  ``state`` (S, W - 1, C): the rows before each sequence, oldest first, zeros by
-    default.  The state returned holds each sequence's last W - 1 rows.  ``out`` must not overlap x.  x, state and y
-    share a dtype; weight and bias share one (float32 or bfloat16) of their own.
+    ``seq_starts[s] .. seq_starts[s + 1] - 1`` (starts past the rows count as their end); rows in front of the first and
+    behind the last one stay as they are in ``out`` (zero without ``out``).  ``state`` (S, W - 1, C): the rows before each
+    sequence, oldest first, zeros by default.  The state returned holds each sequence's last W - 1 rows.  ``out`` may be
+    columns beside x in wider rows, but an output that overlaps an input is refused.  x, state and y share a dtype; weight
+    and bias share one (float32 or bfloat16) of their own.
     """
     if x.dim() != 3 or weight.dim() != 2 or weight.shape[0] != x.shape[2]:
         raise ValueError("causal_conv: x must be (B, L, C) and weight (C, W)")
@@ -633,7 +634,8 @@ def selective_scan_step(row: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, st
     without ``conv_weight`` the row is used as it is.  ``state`` (B, H, P, N) float32 is updated in place;
     ``conv_state`` (B, W - 1, H * P + 2 * G * N) is read, and the state after the token is returned in a tensor of its
     own (``conv_state_out``, which must not be ``conv_state``; captured graphs alternate between two).  dt (B, H),
-    z (B, H, P); the rest as in ``selective_scan``.  ``out`` must not overlap the other arguments.  B < 65536, P <= 4096.
+    z (B, H, P); the rest as in ``selective_scan``.  An output that overlaps another argument
+    is refused.  B < 65536, P <= 4096.
     """
     if state.dim() != 4 or row.dim() != 2 or row.shape[0] != state.shape[0] or dt.shape != state.shape[:2] or \
             (z is not None and z.shape != state.shape[:3]):

@@ -215,3 +215,41 @@ def test_select_of_shifted_rows(dtype, V, offset):
     logits[:, 2] -= offset
     logits[1, 3, ::2] += offset
     check_select(logits.to(dtype), scores, 8)
+
+
+# ---------------------------------------------------------------------------
+# outputs beside their inputs in one buffer, and on top of them
+# ---------------------------------------------------------------------------
+def test_outputs_in_columns_beside_the_inputs():
+    g = torch.Generator().manual_seed(230)
+    B, L, H, P, G, N = 2, 70, 4, 32, 1, 32
+    C = H * P
+    wide = torch.zeros(B, L, 3 * C, device=DEV)
+    x, w = _randn(g, B, L, C).to(DEV), _randn(g, C, 4).to(DEV)
+    wide[..., :C] = x
+    y, new = hip_ops.causal_conv(wide[..., :C], w, out=wide[..., C:2 * C])
+    want, want_new = hip_ops.causal_conv(x, w)
+    assert torch.equal(y, want) and torch.equal(new, want_new) and torch.equal(wide[..., :C], x)
+    with pytest.raises(RuntimeError, match="y overlaps x"):
+        hip_ops.causal_conv(wide[..., :C], w, out=wide[..., C - 1:2 * C - 1])
+
+    c = _scan_case(231, B, L, H, P, G, N, torch.float32)
+    wide[..., :C] = _dev(c["x"]).flatten(2)
+    args = [_dev(c[k]) for k in ("dt", "A", "B", "C")]
+    y, h = hip_ops.selective_scan(wide[..., :C].unflatten(-1, (H, P)), *args, out=wide[..., 2 * C:].unflatten(-1, (H, P)))
+    want, want_h = hip_ops.selective_scan(_dev(c["x"]), *args)
+    assert torch.equal(y, want) and torch.equal(h, want_h)
+    with pytest.raises(RuntimeError, match="y overlaps x"):
+        hip_ops.selective_scan(wide[..., :C].unflatten(-1, (H, P)), *args, out=wide[..., 8:C + 8].unflatten(-1, (H, P)))
+
+    width = C + 2 * G * N
+    both = torch.zeros(B, width + C, device=DEV)
+    both[:, :width] = _randn(g, B, width).to(DEV)
+    row, dt, h = both[:, :width].clone(), _dev(c["dt"][:, 0]), torch.zeros(B, H, P, N, device=DEV)
+    y, _ = hip_ops.selective_scan_step(both[:, :width], dt, args[1], h, out=both[:, width:].unflatten(-1, (H, P)))
+    want, _ = hip_ops.selective_scan_step(row, dt, args[1], torch.zeros_like(h))
+    assert torch.equal(y, want)
+    keep = both.clone()
+    with pytest.raises(RuntimeError, match="y overlaps row"):
+        hip_ops.selective_scan_step(both[:, :width], dt, args[1], h, out=both[:, :C].unflatten(-1, (H, P)))
+    assert torch.equal(both, keep)
