@@ -617,7 +617,7 @@ int64_t tesm_hip_beam_select_ws_bytes(const tesm_hip_beam* p);
 int tesm_hip_beam_select(const tesm_hip_beam* p, void* ws, int64_t ws_bytes, void* stream);
 
 /* Rows of `count` tensors moved to their new beams, in place, no reference counterpart: row b * K + k of
- * each becomes the old row b * K + parents[b,k].  The tensors must not overlap.  A parent outside [0, K)
+ * each becomes the old row b * K + parents[b,k].  Tensors that overlap are refused.  A parent outside [0, K)
  * leaves its row as it is and sets TESM_STATUS_BAD_PARENT.  K <= 64. */
 typedef struct tesm_hip_rows {
   void* p;

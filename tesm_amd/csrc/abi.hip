@@ -8,7 +8,9 @@
 #include <cstring>
 #include <initializer_list>
 #include <mutex>
+#include <new>
 #include <string>
+#include <vector>
 
 #include "beam.h"
 #include "decode.h"
@@ -1976,6 +1978,22 @@ int check_overlaps(const tesm_hip_ssm_step& p) {
                          {"conv_weight", dense(p.conv_weight, C * p.W, we)}, {"conv_bias", dense(p.conv_bias, C, we)},
                          {"A", dense(p.A, p.H, 4)}, {"D", dense(p.D, p.H, 4)}, {"dt_bias", dense(p.dt_bias, p.H, 4)}});
 }
+
+int check_overlaps(const tesm_hip_rows* t, int64_t count, int64_t B, int64_t K) {
+  if (!t || count <= 0 || B < 0 || K < 0 || B >= (1 << 16) || K > kBeamMaxN) return kOk;
+  bool shared;
+  try {
+    std::vector<RowSpan> rows;
+    for (int64_t i = 0; i < count; ++i)
+      if (t[i].bytes > 0 && t[i].bytes < (1LL << 36) && t[i].pitch < (1LL << 40) && (B * K <= 1 || t[i].pitch >= t[i].bytes))
+        rows.push_back({t[i].p, B * K, t[i].pitch, t[i].bytes});
+    shared = any_rows_share(rows);
+  } catch (const std::bad_alloc&) {
+    return fail(kErrInvalidArg, "reorder rows: no memory for a table of that many tensors");
+  }
+  TESM_REQUIRE(!shared, kErrInvalidArg, "reorder rows: two of the tensors overlap");
+  return kOk;
+}
 }  // namespace
 }  // namespace tesm
 
@@ -2100,6 +2118,7 @@ int tesm_hip_beam_select(const tesm_hip_beam* p, void* ws, int64_t ws_bytes, voi
 int tesm_hip_reorder_rows(const tesm_hip_rows* t, int64_t count, const int64_t* parents, int64_t B, int64_t K,
                           void* stream) {
   static_assert(sizeof(tesm_hip_rows) == sizeof(ReorderRows), "one layout");
+  if (int rc = check_overlaps(t, count, B, K)) return rc;
   if (int rc = check_ptrs("reorder rows", {{parents, "parents"}})) return rc;
   for (int64_t i = 0; t && i < count; ++i)
     if (int rc = check_ptr(t[i].p, "a tensor", "reorder rows")) return rc;

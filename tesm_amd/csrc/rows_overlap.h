@@ -1,7 +1,9 @@
 // Whether two arrays laid out in rows share memory: plain arithmetic on the host, before anything is queued.
 #pragma once
 
+#include <algorithm>
 #include <cstdint>
+#include <vector>
 
 namespace tesm {
 
@@ -39,6 +41,28 @@ inline bool rows_share(RowSpan a, RowSpan b) {
   }
   for (int64_t i = 0; i < a.n; ++i)
     if (hits(at + i * a.pitch)) return true;
+  return false;
+}
+
+// Whether any two of the arrays share memory (sorted by address here).  Only arrays whose ranges meet are compared, and
+// column slices of the same wider rows by their order inside a row.
+inline bool any_rows_share(std::vector<RowSpan>& v) {
+  auto at = [&](size_t i) { return reinterpret_cast<uintptr_t>(v[i].p); };
+  auto end = [&](size_t i) { return at(i) + static_cast<uintptr_t>((v[i].n - 1) * v[i].pitch + v[i].width); };
+  v.erase(std::remove_if(v.begin(), v.end(), [](const RowSpan& r) { return !r.p || r.n <= 0 || r.width <= 0; }), v.end());
+  std::sort(v.begin(), v.end(), [](const RowSpan& a, const RowSpan& b) { return reinterpret_cast<uintptr_t>(a.p) < reinterpret_cast<uintptr_t>(b.p); });
+  for (size_t i = 0, j; i < v.size(); i = j) {
+    uintptr_t past = end(i);
+    bool slices = true;  // one pitch, each behind the last, all inside one row
+    for (j = i + 1; j < v.size() && at(j) < past; ++j) {
+      slices = slices && v[j].pitch == v[i].pitch && at(j - 1) + static_cast<uintptr_t>(v[j - 1].width) <= at(j);
+      past = std::max(past, end(j));
+    }
+    if (j == i + 1 || (slices && at(j - 1) + static_cast<uintptr_t>(v[j - 1].width) <= at(i) + static_cast<uintptr_t>(v[i].pitch))) continue;
+    for (size_t a = i; a < j; ++a)
+      for (size_t b = a + 1; b < j; ++b)
+        if (rows_share(v[a], v[b])) return true;
+  }
   return false;
 }
 

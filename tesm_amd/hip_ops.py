@@ -740,7 +740,7 @@ def reorder_rows(tensors, parents: torch.Tensor) -> None:
     """Row ``b * K + k`` of every tensor becomes its old row ``b * K + parents[b, k]``, in place and in one launch.
 
     ``parents`` (B, K) int64, B < 65536, K <= 64; each tensor has B * K rows (its first dimension), each row contiguous; any
-    dtype.  The tensors must not overlap.  A parent outside 0 .. K - 1 leaves its row as it is and sets bit 1 of
+    dtype.  Tensors that overlap are refused.  A parent outside 0 .. K - 1 leaves its row as it is and sets bit 1 of
     ``device_status``.
     """
     if parents.dim() != 2 or parents.dtype != torch.int64:
@@ -767,11 +767,13 @@ def reorder_rows(tensors, parents: torch.Tensor) -> None:
             pitch *= t.element_size()
         if t.get_device() != index:
             require_device(parents, t)
-        table += (t.data_ptr(), pitch, nbytes)
-    if len(set(table[::3])) != len(tensors) and rows and all(table[2::3]):
+        if nbytes:  # (empty ones share whatever address they have)
+            table += (t.data_ptr(), pitch, nbytes)
+    count = len(table) // 3
+    if len(set(table[::3])) != count:
         raise ValueError("reorder_rows: a tensor is given twice")
     parents = parents.contiguous()
     require_device(parents)
     table = array.array("q", table)
-    on_device(dev.index, _lib.load().tesm_hip_reorder_rows, table.buffer_info()[0], len(tensors), parents.data_ptr(), B, K,
+    on_device(dev.index, _lib.load().tesm_hip_reorder_rows, table.buffer_info()[0], count, parents.data_ptr(), B, K,
               raw_stream(dev.index))

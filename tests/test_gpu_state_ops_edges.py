@@ -253,3 +253,19 @@ def test_outputs_in_columns_beside_the_inputs():
     with pytest.raises(RuntimeError, match="y overlaps row"):
         hip_ops.selective_scan_step(both[:, :width], dt, args[1], h, out=both[:, :C].unflatten(-1, (H, P)))
     assert torch.equal(both, keep)
+
+
+def test_reorder_of_column_slices_of_one_buffer():
+    g = torch.Generator().manual_seed(240)
+    wide = torch.randn(6, 100, generator=g)
+    parents = torch.tensor([[2, 0, 0], [1, 1, 2]])
+    rows = torch.tensor([2, 0, 0, 4, 4, 5])
+    dev = wide.to(DEV)
+    hip_ops.reorder_rows([dev[:, 40:90], dev[:, :17], torch.zeros(6, 0, device=DEV), dev[:, 17:30]], parents.to(DEV))
+    want = wide.clone()
+    for lo, hi in ((0, 30), (40, 90)):
+        want[:, lo:hi] = wide[rows, lo:hi]
+    assert torch.equal(dev.cpu(), want)
+    with pytest.raises(RuntimeError, match="overlap"):
+        hip_ops.reorder_rows([dev[:, 40:90], dev[:, :17], dev[:, 16:30]], parents.to(DEV))
+    assert torch.equal(dev.cpu(), want)

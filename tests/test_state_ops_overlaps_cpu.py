@@ -6,9 +6,10 @@ import os
 import subprocess
 
 import pytest
+import torch
 
 from conftest import ROOT
-from tesm_amd import _lib
+from tesm_amd import _lib, hip_ops
 
 CSRC = os.path.join(ROOT, "tesm_amd", "csrc")
 
@@ -60,6 +61,25 @@ int main() {
   }
   if (rows_share({nullptr, 3, 4, 4}, {memory, 3, 4, 4})) ++wrong;
   printf("%ld apart, %ld sharing, %ld wrong\n", seen[0], seen[1], wrong);
+  // several at once: column slices of one pitch, and arrays of their own
+  long many[2] = {0, 0};
+  for (int step = 0; step < 200000; ++step) {
+    std::vector<RowSpan> v(2 + rand() % 4);
+    const int64_t n = 1 + rand() % 5, pitch = 12 + rand() % 20;
+    for (RowSpan& r : v) {
+      r.n = n;
+      r.width = rand() % 7;
+      r.pitch = rand() % 4 ? pitch : r.width + rand() % 20;
+      r.p = memory + 200 + (rand() % 2 ? rand() % 30 : 200 * (rand() % 8) + rand() % 10);
+    }
+    bool want = false;
+    for (size_t a = 0; a < v.size(); ++a)
+      for (size_t b = a + 1; b < v.size(); ++b) want = want || every_byte(v[a], v[b]);
+    ++many[want];
+    if (any_rows_share(v) != want && wrong++ < 5) printf("several: %d\n", want);
+  }
+  printf("several: %ld apart, %ld sharing, %ld wrong\n", many[0], many[1], wrong);
+  if (many[0] < 10000 || many[1] < 10000) return 2;
   return wrong || seen[0] < 10000 || seen[1] < 10000;
 }
 """
@@ -164,3 +184,27 @@ def test_step_refuses_overlaps(out):
     # the token's outputs in the columns beside its inputs
     wide = WIDTH + H * P
     assert "overlaps" not in _step(ld_row=wide, ld_y=wide, row=AT << 1, y=(AT << 1) + 4 * WIDTH)
+
+
+def _reorder(rows, B=2, K=3):
+    t = (_lib.Rows * len(rows))(*[_lib.Rows(p=AT + at, pitch=pitch, bytes=n) for at, pitch, n in rows])
+    rc = _lib.load().tesm_hip_reorder_rows(ctypes.addressof(t), len(rows), AT << 1, B, K, None)
+    assert rc == 1
+    return _lib.load().tesm_hip_last_error().decode()
+
+
+def test_reorder_refuses_overlaps():
+    apart = [(0, 40, 40), (240, 64, 40), (280, 64, 24), (1000, 16, 16), (0, 8, 0)]
+    assert "overlap" not in _reorder(apart) and "overlap" not in _reorder(apart[::-1])
+    for more in ((0, 40, 40), (39, 8, 8), (276, 64, 8), (1090, 16, 16), (990, 4, 4)):
+        assert "overlap" in _reorder(apart + [more]), more
+        assert "overlap" in _reorder([more] + apart), more
+    assert "overlap" in _reorder([(0, 16, 16), (0, 16, 16)]) and "overlap" in _reorder([(0, 16, 16), (8, 16, 16)], 1, 1)
+
+
+def test_reorder_refuses_a_tensor_given_twice_beside_an_empty_one():
+    ok, par = torch.randn(6, 4), torch.zeros(2, 3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="twice"):
+        hip_ops.reorder_rows([ok, torch.zeros(6, 0), ok], par)
+    with pytest.raises(RuntimeError, match="ROCm device"):  # (two empty ones are none)
+        hip_ops.reorder_rows([ok, torch.zeros(6, 0), torch.zeros(6, 0)], par)
