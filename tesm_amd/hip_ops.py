@@ -512,7 +512,10 @@ def _sequences(seq_starts: Optional[torch.Tensor], B: int, what: str):
         raise ValueError(f"{what}: packed sequences lie in one row axis: with seq_starts the first dimension must be 1")
     if seq_starts.dim() != 1 or seq_starts.numel() < 1 or seq_starts.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{what}: seq_starts must be a 1-D int32 or int64 tensor of one entry more than sequences")
-    return seq_starts.to(torch.int32).contiguous(), seq_starts.numel() - 1
+    S = seq_starts.numel() - 1
+    if seq_starts.dtype == torch.int64:  # (starts past int32 are past the rows as well, and must not wrap)
+        seq_starts = seq_starts.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    return seq_starts.contiguous(), S
 
 
 def _same_dtype(what: str, dtype: torch.dtype, **ts) -> None:
