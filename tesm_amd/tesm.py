@@ -372,6 +372,8 @@ class TESM_SISO(nn.Module):
         desc.local_bias = local_bias.data_ptr()
         keep = (decay_bias, local_bias, [b.detach() for b in biases[1:]])
         keep += tuple(p.packed_weight() for p in lins[:4 + int(cross)])
+        # (the size counts the cross query's buffers where there is a cross state; every step sets its own)
+        desc.cross_state = desc.decay_bias if cross else None
         nbytes = int(_lib.load().tesm_hip_siso_decode_ws_bytes(ctypes.byref(desc)))
         if stamp is not None:
             self.__dict__["_decode_plan"] = (key, (desc, nbytes, keep))

@@ -5,8 +5,8 @@ import torch
 
 from hip_helpers import DEV, TOL, need_gpu, normwise, to_np
 from oracle import tesm_torch as ot
-from tesm_amd import TESM_SISO, hip_ops
-from test_gpu_beam import INF, _case, check_select
+from tesm_amd import TESM_SISO, hip_ops, tesm
+from test_gpu_beam import INF, _case, _model, check_select
 from test_gpu_ssm import HALF, U, _check_scan, _dev, _randn, _run_scan, _scan_case, _silu, _within
 
 pytestmark = pytest.mark.gpu
@@ -269,3 +269,20 @@ def test_reorder_of_column_slices_of_one_buffer():
     with pytest.raises(RuntimeError, match="overlap"):
         hip_ops.reorder_rows([dev[:, 40:90], dev[:, :17], dev[:, 16:30]], parents.to(DEV))
     assert torch.equal(dev.cpu(), want)
+
+
+# ---------------------------------------------------------------------------
+# beam search from one token
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("kw", [{}, dict(use_mimo=True, n_heads=2), dict(entanglement_window=0)])
+def test_beam_search_from_one_token_needs_no_earlier_prompt(kw):
+    """The decode step is then the first call of all: its workspace holds the cross-layer query's buffers."""
+    m = _model(torch.float32, **kw)
+    ids = torch.randint(0, 300, (3, 1), generator=torch.Generator().manual_seed(1)).to(DEV)
+    m(torch.zeros(8, 40, dtype=torch.int64, device=DEV))  # (a prompt leaves a workspace large enough for any step)
+    want = m.beam_search(ids, 4, 5)
+    torch.cuda.synchronize()
+    tesm._WORKSPACES.clear()
+    m = _model(torch.float32, **kw)
+    got = m.beam_search(ids, 4, 5)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
