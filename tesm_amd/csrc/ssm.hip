@@ -435,8 +435,11 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
       if (2 * k >= nh) break;
       const float raw = from_bits<DT>(dtr[k]) + biasr[k];
       const float d = row0 + (lane & 31) < sg.r1 ? (a.softplus ? softplusf_(raw) : raw) : 0.0f;
-      // in units of log 2, 64 bits split into two floats
-      const double c = half_scan_d(static_cast<double>(d) * static_cast<double>(Ar[k]) * 1.4426950408889634074);
+      // in units of log 2, 64 bits split into two floats.  A row below -2^16 clears the state like one of -2^16 (no growth that
+      // float32 holds makes up for either), which leaves the sums' last bits to the rows around it.
+      double each = static_cast<double>(d) * static_cast<double>(Ar[k]) * 1.4426950408889634074;
+      if (each < -0x1p16) each = -0x1p16;
+      const double c = half_scan_d(each);
       const double all = dh ? readlane_d(c, 63) : readlane_d(c, 31);
       if (2 * k + dh < nh) {
         float* sm = to + (2 * k + dh) * Lds::kSmall + (lane & 31);

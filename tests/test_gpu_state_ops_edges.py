@@ -286,3 +286,17 @@ def test_beam_search_from_one_token_needs_no_earlier_prompt(kw):
     m = _model(torch.float32, **kw)
     got = m.beam_search(ids, 4, 5)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ---------------------------------------------------------------------------
+# scan: rows that clear the state
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("step", [1e4, 1e8, 1e10, 1e12, 1e20, 1e30])
+def test_scan_of_step_sizes_that_clear_the_state(dtype, step):
+    """A huge step size with x = 0 leaves a state of 0: the rows behind it, in its chunk and later, know nothing of it."""
+    c = _scan_case(300, 1, 140, 3, 32, 1, 32, dtype, softplus=False, bias=False, gate=False)
+    c["dt"][0, ::9] = step
+    c["x"][0, ::9] = 0
+    c["A"][2] = -0.3
+    _check_scan(c, *_run_scan(c))
