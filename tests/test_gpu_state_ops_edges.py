@@ -1,11 +1,13 @@
 """The state operators where their range ends: narrow states, far values, masks, memory on either side of the outputs.
 Tolerances are those of the operators' own tests (``test_gpu_ssm``, ``test_gpu_beam``) unless a test derives another."""
+import ctypes
+
 import pytest
 import torch
 
 from hip_helpers import DEV, TOL, need_gpu, normwise, to_np
 from oracle import tesm_torch as ot
-from tesm_amd import TESM_SISO, hip_ops, tesm
+from tesm_amd import TESM_SISO, _lib, hip_ops, tesm
 from test_gpu_beam import INF, _case, _model, check_select
 from test_gpu_ssm import HALF, U, _check_scan, _dev, _randn, _run_scan, _scan_case, _silu, _within
 
@@ -300,3 +302,76 @@ def test_scan_of_step_sizes_that_clear_the_state(dtype, step):
     c["x"][0, ::9] = 0
     c["A"][2] = -0.3
     _check_scan(c, *_run_scan(c))
+
+
+# ---------------------------------------------------------------------------
+# memory on either side of the outputs
+# ---------------------------------------------------------------------------
+class Guarded:
+    """Buffers of exactly the sizes asked for, each inside a larger one filled with a byte that must stay."""
+    PAD, BYTE = 1 << 16, 0xA5
+
+    def __init__(self):
+        self.all = []
+
+    def bytes(self, n, fill=0):
+        whole = torch.full((n + 2 * self.PAD,), self.BYTE, dtype=torch.uint8, device=DEV)
+        whole[self.PAD:self.PAD + n] = fill
+        self.all.append((whole, n))
+        return whole[self.PAD:self.PAD + n]
+
+    def like(self, shape, dtype):
+        n = torch.Size(shape).numel() * dtype.itemsize
+        return self.bytes(n).view(dtype).view(shape)
+
+    def check(self):
+        for whole, n in self.all:
+            assert bool((whole[:self.PAD] == self.BYTE).all()) and bool((whole[self.PAD + n:] == self.BYTE).all())
+
+
+ORDERS = [[0, 1000] * 8, [900, 100, 1000, 0, 700, 699, 5, 5, 1000, 3], [-5, 2000, -7, 1 << 30, 12, -(1 << 30), 64, 1000],
+          [1000, 0], [0, 1000], [1000] * 5, [-3] * 5]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("starts", ORDERS)
+@pytest.mark.parametrize("H,P,G,N", [(2, 16, 1, 16), (4, 64, 2, 64)])
+def test_scan_of_any_starts_writes_its_own_memory_only(dtype, starts, H, P, G, N):
+    """What starts that are in no order give is not looked at; workspace, outputs and states are of the exact size."""
+    M, S, code = 1000, len(starts) - 1, hip_ops.dt_code(dtype)
+    c = _scan_case(72, 1, M, H, P, G, N, dtype, starts=starts)
+    mem, ins = Guarded(), {k: _dev(c[k]) for k in ("x", "dt", "A", "B", "C", "D", "z", "dt_bias", "h0")}
+    at = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    y, h = mem.like((M, H * P), dtype), mem.like((S, H, P, N), torch.float32)
+    p = {k: v.data_ptr() for k, v in ins.items()}
+    d = _lib.Ssm(code, 1, M, H, P, G, N, S, 1, p["x"], H * P, p["dt"], H, p["A"], p["B"], G * N, p["C"], G * N, p["D"], p["z"], H * P,
+                 p["dt_bias"], at.data_ptr(), p["h0"], y.data_ptr(), H * P, h.data_ptr())
+    lib = _lib.load()
+    nbytes = lib.tesm_hip_selective_scan_ws_bytes(ctypes.byref(d))
+    ws = mem.bytes(nbytes)
+    keep = {k: v.clone() for k, v in ins.items()}
+    _lib.check(lib.tesm_hip_selective_scan(ctypes.byref(d), ws.data_ptr() if nbytes else None, nbytes, hip_ops.raw_stream(0)))
+    torch.cuda.synchronize()
+    mem.check()
+    assert all(torch.equal(v, keep[k]) for k, v in ins.items())
+    if starts == sorted(starts) and starts[0] >= 0 and starts[-1] <= M:
+        _check_scan(c, y.view(1, M, H, P), h)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("starts", ORDERS)
+@pytest.mark.parametrize("C", [3, 40])
+def test_conv_of_any_starts_writes_its_own_memory_only(dtype, starts, C):
+    M, S, W, code = 1000, len(starts) - 1, 4, hip_ops.dt_code(dtype)
+    g = torch.Generator().manual_seed(73)
+    x, w, state = (_randn(g, *n, dtype=dtype).to(DEV) for n in ((M, C), (C, W), (S, W - 1, C)))
+    at = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    mem = Guarded()
+    y, new = mem.like((M, C), dtype), mem.like((S, W - 1, C), dtype)
+    d = _lib.Conv(code, code, 1, M, C, W, S, 1, x.data_ptr(), C, w.data_ptr(), None, at.data_ptr(), state.data_ptr(), y.data_ptr(), C,
+                  new.data_ptr())
+    keep = x.clone(), state.clone()
+    _lib.check(_lib.load().tesm_hip_causal_conv(ctypes.byref(d), hip_ops.raw_stream(0)))
+    torch.cuda.synchronize()
+    mem.check()
+    assert torch.equal(x, keep[0]) and torch.equal(state, keep[1])
