@@ -56,15 +56,19 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // A chunk's x, B and C come through registers, read one chunk ahead, into LDS (two chunks' worth for bfloat16, so that
 // one barrier separates a chunk's writes from its reads; float32 rows fill it with one).  Three of the waves form the
 // scores; the fourth meanwhile forms d and the sums c of the next chunk (in 64 bits: c is a difference's operand, and is
-// kept as a high and a low float).  Roundings with bfloat16 operands: W and the h that C reads go to bfloat16 once, like
-// the operands they meet (y is rounded to it as well); the state itself takes its addends in three parts, unrounded.
+// kept as a high and a low float).  With bfloat16 operands W and the h that C reads go into their products as two bfloat16
+// parts each, which leaves y the error of its own rounding; the state takes its addends in three parts, unrounded.  (One
+// rounded part each: y's error 1.9e-3 of it instead of 1.7e-3, with narrow states 2.3e-3, single values up to 30 times what
+// the formula in float32 leaves, for 72 us instead of 78 and 800 instead of 880.)
 //
-// Bound by the vector unit: per wave and chunk about 650 instructions, the exponentials and reciprocals among them at a
-// quarter of the rate, next to 72 matrix instructions (about a quarter of the time), at the two waves per SIMD that the
-// state's and the next operands' registers leave; with every operand in the cache it gained a seventh.  Chunks of 64 rows
+// Bound by the vector unit first: with 128 bfloat16 states a wave issues some 800 of its instructions per chunk, 91
+// matrix ones among them and the exponentials and reciprocals at a quarter of the rate.  Counters over 32768 rows: the
+// vector unit issues in 63 % of the cycles, the matrix unit works in 27 %, LDS conflicts take 10 %; a wave waits for an issue
+// slot in 29 % of its time and for memory, LDS or one of the two barriers per chunk in 22 %, which the two waves per SIMD that
+// the state's and the next operands' registers leave do not cover for each other.  Chunks of 64 rows
 // (one staged, with the work inside a chunk doubled) took 628 us where these took 520.  Measured, bfloat16 with 128
-// states: 4 x 2048 rows of 1536 columns 42 us + 30 for the states of the segments, 32768 rows of 8192 columns (1.76 GB)
-// 585 + 270 us, 2.1 TB/s.
+// states: 4 x 2048 rows of 1536 columns 50 us + 31 for the states of the segments, 32768 rows of 8192 columns (1.76 GB)
+// 676 + 271 us, 1.9 TB/s.
 // ---------------------------------------------------------------------------
 constexpr int kCols = 128;  // columns per workgroup
 
@@ -120,8 +124,27 @@ struct Tile<kBF16> {
       v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
-  static __device__ __forceinline__ void store4(E* p, const f32x4& v) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+  // Float32 values as two bfloat16 parts: the first cut off, the second what that leaves, rounded (2^-15 of the value off).
+  static constexpr int PARTS = 2;
+  static __device__ __forceinline__ uint2 cut(const f32x4& v, f32x4& rest) {
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      b[i] = __float_as_uint(v[i]);
+      rest[i] = v[i] - __uint_as_float(b[i] & 0xffff0000u);
+    }
+    return make_uint2(__builtin_amdgcn_perm(b[1], b[0], 0x07060302), __builtin_amdgcn_perm(b[3], b[2], 0x07060302));
+  }
+  static __device__ __forceinline__ void parts(const f32x4& lo, const f32x4& hi, Frag (&f)[PARTS]) {
+    f32x4 a, b;
+    const uint2 u = cut(lo, a), v = cut(hi, b);
+    f[0] = make_uint4(u.x, u.y, v.x, v.y);
+    f[1] = pack(a, b);
+  }
+  static __device__ __forceinline__ void store4(E* p, int part_pitch, const f32x4& v) {
+    f32x4 rest;
+    *reinterpret_cast<uint2*>(p) = cut(v, rest);
+    *reinterpret_cast<uint2*>(p + part_pitch) = make_uint2(pack_bf16x2(rest[0], rest[1]), pack_bf16x2(rest[2], rest[3]));
   }
 };
 template <>
@@ -163,7 +186,9 @@ struct Tile<kF32> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = f.v[i];
   }
-  static __device__ __forceinline__ void store4(E* p, const f32x4& v) {
+  static constexpr int PARTS = 1;
+  static __device__ __forceinline__ void parts(const f32x4& lo, const f32x4& hi, Frag (&f)[PARTS]) { f[0] = pack(lo, hi); }
+  static __device__ __forceinline__ void store4(E* p, int, const f32x4& v) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
   }
 };
@@ -297,14 +322,15 @@ struct SsmLds {
   static constexpr int kSmall = 6 * kQ;  // per head: c high, c low, d, exp(c_Q - c) d, exp(c), and exp(c_Q) at 5 kQ
   static constexpr int64_t bytes(int nh) {
     const int64_t e = sizeof(typename TT::E);
-    return TT::NB * kStage * e + (FULL ? nh * kQ * WP * e : 0) + 2 * nh * kSmall * 4;
+    return TT::NB * kStage * e + (FULL ? TT::PARTS * nh * kQ * WP * e : 0) + 2 * nh * kSmall * 4;
   }
 };
 
 // FULL: y and the final state of a segment from its carried-in state; otherwise the segment's end state from zero.
 // VEC: whole 32-column slices and 32-state steps, and 32-bit offsets inside a chunk.
-// (Two waves per SIMD also where float32 operands with 128 states then spill 32 registers: 14 sequences of 600 rows and 24
-// heads 179 us, with one wave and no spill 186; 256 states need the registers of one.)
+// (Two waves per SIMD also where float32 operands with 128 states then spill 37 registers, 40 with edges: 14 sequences of 600
+// rows and 24 heads 179 us, with one wave and no spill 186; 256 states need the registers of one and spill 4 to 10 with float32
+// operands.  The states' pass with float32 operands and 128 states spills 1 register, 15 with edges.)
 template <int DT, int NS, bool FULL, bool VEC>
 __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_kernel(SsmArgs a, SsmGrid gr) {
   using TT = Tile<DT>;
@@ -318,7 +344,9 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
   extern __shared__ __attribute__((aligned(16))) char lds_s[];
   E* const stages = reinterpret_cast<E*>(lds_s);
   E* const Ws = stages + NB * Lds::kStage;
-  float* const smalls = reinterpret_cast<float*>(Ws + (FULL ? gr.nh * kQ * WP : 0));
+  constexpr int PARTS = TT::PARTS;
+  const int wpart = gr.nh * kQ * WP;  // from W's first parts to its second
+  float* const smalls = reinterpret_cast<float*>(Ws + (FULL ? PARTS * wpart : 0));
 
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -471,7 +499,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
       load_dt(sg.r0 + kQ);
     }
     if constexpr (FULL) {  // the block of W above the diagonal that a 32-wide step reads: zero throughout
-      for (int e = tid; e < nh * 256; e += 256) Ws[((e >> 8) * kQ + ((e >> 4) & 15)) * WP + 16 + (e & 15)] = E(0);
+      for (int e = tid; e < PARTS * gr.nh * 256; e += 256) Ws[((e >> 8) * kQ + ((e >> 4) & 15)) * WP + 16 + (e & 15)] = E(0);
     }
   }
   int buf = 0;
@@ -547,7 +575,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
           for (int r = 0; r < 4; ++r)
             if (j0 + r > i) v[r] = 0.0f;
         }
-        TT::store4(Ws + (w * kQ + i) * WP + j0, v);
+        TT::store4(Ws + (w * kQ + i) * WP + j0, wpart, v);
       }
     }
     Frag xf[2];  // x of this wave's columns, 8 rows of a column per lane
@@ -557,7 +585,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
     }
     if constexpr (FULL) {
       f32x4 y[2][2];
-      // exp(c_i) C_i . h (bfloat16 operands: h is rounded here, once, for the product)
+      // exp(c_i) C_i . h
       auto across = [&]() __attribute__((always_inline)) {
         anew(h);
 #pragma unroll
@@ -566,12 +594,17 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
           for (int T = 0; T < 2; ++T) y[q][T] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-          const Frag h0 = TT::pack(h[s][0][0], h[s][1][0]), h1 = TT::pack(h[s][0][1], h[s][1][1]);
+          Frag h0[PARTS], h1[PARTS];
+          TT::parts(h[s][0][0], h[s][1][0], h0);
+          TT::parts(h[s][0][1], h[s][1][1], h1);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const Frag c = TT::template rows<UB>(Cs, 16 * q, m, g, s);
-            y[q][0] = TT::mma(h0, c, y[q][0]);
-            y[q][1] = TT::mma(h1, c, y[q][1]);
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
+              y[q][0] = TT::mma(h0[part], c, y[q][0]);
+              y[q][1] = TT::mma(h1[part], c, y[q][1]);
+            }
           }
         }
 #pragma unroll
@@ -586,11 +619,13 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
       if (active) {
         // + W x over the rows up to each
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const Frag w = TT::row(Ws + (hh * kQ + 16 * q + m) * WP + 8 * g);
-          y[q][0] = TT::mma(xf[0], w, y[q][0]);
-          y[q][1] = TT::mma(xf[1], w, y[q][1]);
-        }
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) {
+            const Frag w = TT::row(Ws + part * wpart + (hh * kQ + 16 * q + m) * WP + 8 * g);
+            y[q][0] = TT::mma(xf[0], w, y[q][0]);
+            y[q][1] = TT::mma(xf[1], w, y[q][1]);
+          }
         // An infinite or NaN x must not reach the rows before it through a weight 0.  Rows with one near have sums
         // that are not finite: they are formed again without such values, which are then added from their row on.
         bool odd = false;
@@ -609,7 +644,10 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
             for (int r = 0; r < 8; ++r) v[r] = fabsf(v[r]) < __builtin_inff() ? v[r] : 0.0f;
             const Frag f = TT::pack(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
 #pragma unroll
-            for (int q = 0; q < 2; ++q) y[q][T] = TT::mma(f, TT::row(Ws + (hh * kQ + 16 * q + m) * WP + 8 * g), y[q][T]);
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+              for (int part = 0; part < PARTS; ++part)
+                y[q][T] = TT::mma(f, TT::row(Ws + part * wpart + (hh * kQ + 16 * q + m) * WP + 8 * g), y[q][T]);
           }
 #pragma unroll 1
           for (int j = 0; j < kQ; ++j)
@@ -681,8 +719,8 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
       const f32x4 w0 = *reinterpret_cast<const f32x4*>(sm + 3 * kQ + 8 * g) * per;
       const f32x4 w1 = *reinterpret_cast<const f32x4*>(sm + 3 * kQ + 8 * g + 4) * per;
       // w x: float32, or as three bfloat16 parts that hold all its 24 bits, each a product of its own
-      constexpr int PARTS = DT == kBF16 ? 3 : 1;
-      Frag wx[PARTS][2];
+      constexpr int ADDENDS = DT == kBF16 ? 3 : 1;
+      Frag wx[ADDENDS][2];
 #pragma unroll
       for (int T = 0; T < 2; ++T) {
         float v[8];
@@ -691,9 +729,9 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
 #pragma unroll
         for (int r = 0; r < 4; ++r) v0[r] = v[r] * w0[r], v1[r] = v[4 + r] * w1[r];
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
+        for (int part = 0; part < ADDENDS; ++part) {
           wx[part][T] = TT::pack(v0, v1);
-          if (part + 1 == PARTS) break;
+          if (part + 1 == ADDENDS) break;
           TT::unpack(wx[part][T], v);
 #pragma unroll
           for (int r = 0; r < 4; ++r) v0[r] -= v[r], v1[r] -= v[4 + r];  // (an infinity's states become NaN)
@@ -705,7 +743,7 @@ __global__ __launch_bounds__(256, NS == 8 ? 1 : FULL ? 2 : 3) void ssm_chunk_ker
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) b[t2] = TT::template column<UB>(Bs, 0, m, g, s, t2);
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part)
+        for (int part = 0; part < ADDENDS; ++part)
 #pragma unroll
           for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll

@@ -582,9 +582,10 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     ``y = state C + D x``, times ``silu(z)`` with ``z``.  x, z: (B, L, H, P); dt: (B, L, H); B, C: (B, L, G, N),
     N <= 256; A, D, dt_bias: (H); ``state`` (S, H, P, N) float32: the states before each sequence (zeros by default).
     ``seq_starts`` and ``out`` as in ``causal_conv``.  x, dt, B, C, z and y share a dtype and may be column slices of
-    wider rows.  States and sums are float32; with bfloat16 operands the decayed scores and the state read by a chunk's
-    rows are rounded to bfloat16 for the products.  A NaN or an infinity in row t reaches no row before it; an infinite
-    x may leave NaN where the formula's state is infinite.  Fewer than 65536 sequences, H * P and row pitches below 2^24.
+    wider rows.  States and sums are float32; with bfloat16 operands the decayed scores and the states that rows read go
+    into their products as two bfloat16 parts (16 bits).  A NaN or an infinity in row t reaches no row before it; an infinite
+    x or state may leave NaN where the formula's value is infinite, and so may states beyond 2^118 in magnitude.  Fewer than
+    65536 sequences, H * P and row pitches below 2^24.
     """
     if x.dim() != 4 or dt.dim() != 3 or B.dim() != 4 or dt.shape != x.shape[:3] or B.shape[:2] != x.shape[:2] or \
             C.shape != B.shape or (z is not None and z.shape != x.shape):

@@ -9,7 +9,8 @@ from hip_helpers import DEV, TOL, need_gpu, normwise, to_np
 from oracle import tesm_torch as ot
 from tesm_amd import TESM_SISO, _lib, hip_ops, tesm
 from test_gpu_beam import INF, _case, _model, check_select
-from test_gpu_ssm import HALF, U, _check_scan, _dev, _randn, _run_scan, _scan_case, _silu, _within
+from test_gpu_ssm import (HALF, PACKED, SCANS, U, _check_scan, _dev, _randn, _run_scan, _scan_case, _silu, _within,
+                          scan_ref)
 
 pytestmark = pytest.mark.gpu
 
@@ -375,3 +376,32 @@ def test_conv_of_any_starts_writes_its_own_memory_only(dtype, starts, C):
     torch.cuda.synchronize()
     mem.check()
     assert torch.equal(x, keep[0]) and torch.equal(state, keep[1])
+
+
+# ---------------------------------------------------------------------------
+# scan: bfloat16 operands, products of float32 accuracy.  Rows hold what float32 operands' do and their own rounding, and on
+# the way 2^-14 of the contributions' magnitudes: 2^-15 for the second bfloat16 part of the decayed scores and of the state,
+# and below 2^-15 for the decays, whose sums, below 512, are each off by 2^-16 in the exponent of 2.
+# ---------------------------------------------------------------------------
+def _check_scan_closely(c, y):
+    nb, L = c["x"].shape[:2]
+    spans = [(i * L, i * L + L) for i in range(nb)] if c["starts"] is None else list(zip(c["starts"][:-1], c["starts"][1:]))
+    want, mass, _, _ = scan_ref(c, spans, nb * L)
+    longest = max([b - a for a, b in spans], default=0)
+    count = c["N"] + 3 * min(longest, 64) + 6 * (longest // 32 + 1) + 64
+    tol = (2.0 ** -14 + count * U) * mass + (HALF[torch.bfloat16] + 8 * U) * want.abs() + 1e-36
+    for lo, hi in spans:
+        _within(y.reshape(want.shape)[lo:hi], want[lo:hi], tol[lo:hi], "scan rows %d..%d" % (lo, hi))
+
+
+@pytest.mark.parametrize("B,L,H,P,G,N", SCANS)
+@pytest.mark.parametrize("full", [True, False])
+def test_scan_rounds_bfloat16_rows_once(B, L, H, P, G, N, full):
+    c = _scan_case(B + L + H + P + N, B, L, H, P, G, N, torch.bfloat16, init=full, gate=full, skip=full, bias=full)
+    _check_scan_closely(c, _run_scan(c)[0])
+
+
+@pytest.mark.parametrize("starts", PACKED + [[0, 1000, 1003, 1700]])
+def test_scan_rounds_bfloat16_rows_once_packed(starts):
+    c = _scan_case(310, 1, starts[-1] + 5, 4, 32, 2, 64, torch.bfloat16, starts=starts)
+    _check_scan_closely(c, _run_scan(c)[0])
