@@ -6,9 +6,12 @@
 //
 // Inside a beam the order of the offers is the order of the logits, so each row is reduced to its n largest logits and
 // its logsumexp in one pass (beam_row_kernel), and requests then merge their beams' lists, the offers compared in 64
-// bits (beam_merge_kernel).  Bound by reading the logits once, and next to that by arithmetic: 7 operations per logit, of
-// which the exponential takes four.  Measured, bfloat16, a quarter of the beams finished: 512 rows of 151936 logits (117 MB
-// read) 47 us + 12 for the merge, 2.5 TB/s; 4 rows 8.5 + 6.2 us.
+// bits (beam_merge_kernel).  The floor is reading the logits once.  A wave issues 14 vector and 7 scalar instructions per
+// logit (unpacking for the maximum, the sum and the test; the exponential, at a quarter of the rate; the list's upkeep);
+// counters over 512 rows: the vector unit issues in 43 % of the cycles, a wave waits for memory or LDS in 47 % of its time and
+// for an issue slot in 17 %, so that no one unit is the bound.  Measured, bfloat16, a quarter of the beams finished: 512 rows
+// of 151936 logits (117 MB read) 46 us + 11 for the merge, 2.5 TB/s, whatever part of a row is masked; float32 (none finished,
+// 311 MB) 72 us in all; 4 rows 8.5 + 6.3 us.
 #include <float.h>
 
 #include <type_traits>
@@ -340,7 +343,8 @@ struct Offer {
 
 // One workgroup per request: a wave per beam merges its parts' lists into the beam's m best offers; the offers' ranks
 // among all beams' are then counted.  Bound by latency: the chains of sorting steps and of the 64-bit exponentials and
-// logarithm, 6 to 12 us; all that a beam needs is read at once (4 beams 6.2 us against 6.8).
+// logarithm, 6 to 12 us; all that a beam needs is read at once (4 beams 6.2 us against 6.8).  The ranking compares all offers
+// with all: 64 beams and 64 candidates take 2.9 ms.
 __global__ __launch_bounds__(512) void beam_merge_kernel(BeamArgs a, int m, int parts, const uint64_t* keys, const PartSum* sums) {
   extern __shared__ __attribute__((aligned(16))) char lds_beam[];
   Offer* const offers = reinterpret_cast<Offer*>(lds_beam);

@@ -4,9 +4,11 @@
 // come from its state (W - 1 rows, oldest first) and are zero without one; the state out is the last W - 1 rows of
 // state and sequence together.  Sums in float32, one rounding to the layer type.
 //
-// Bound by HBM: each row is read once and written once.  A thread owns 16 bytes of channels, at any alignment, and walks
-// kConvRows rows with its filter and the last W - 1 rows in registers; the W - 1 rows before its own are read again, from
-// the cache.  The last thread of a row ends with the row, so it may form some of its neighbour's channels too (the same
+// Bound by HBM up to 4 taps, with float32 rows up to 8: each row is read once and written once.  A thread owns 16 bytes of
+// channels, at any alignment, and walks kConvRows rows with its filter and the last W - 1 rows in registers, as float32: for
+// 8 bfloat16 channels and 5 to 8 taps these do not fit the 128 registers that four waves per SIMD leave, and 22 to 220 of them
+// spill.  The W - 1 rows before a thread's own are read again, from the cache.  Measured, 8192 rows of 1792 channels with 4, 5,
+// 6, 7 and 8 taps: bfloat16 15, 21, 39, 72 and 101 us (a copy of the same 29 MB 11.3), float32 22, 24, 25, 26 and 27.  The last thread of a row ends with the row, so it may form some of its neighbour's channels too (the same
 // values).  The states out are written by threads behind those of the rows, in the same launch.
 #include "ssm.h"
 
