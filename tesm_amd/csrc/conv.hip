@@ -101,7 +101,7 @@ struct ConvVec<kF32, 4> {
 // silu of a bfloat16 result: the exponent's rounding (2^-24 |v| log2 e) is far below the result's.
 template <int DT>
 __device__ __forceinline__ float conv_silu(float v) {
-  if constexpr (DT == kF32) return v * sigmoidf_(v);
+  if constexpr (DT == kF32) return siluf_(v);
   return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
 }
 

@@ -73,6 +73,8 @@ struct SsmStepArgs {
 };
 int launch_selective_scan_step(const SsmStepArgs& a, hipStream_t st);
 
+__device__ __forceinline__ float siluf_(float v) { return v * __builtin_amdgcn_rcpf(1.0f + fast_exp(-v)); }
+
 // The real rows [a, b) of packed sequence s, whatever the array holds: inside [0, M), b >= a.
 __device__ __forceinline__ void seq_rows(const int32_t* starts, int64_t s, int64_t M, int64_t& a, int64_t& b) {
   const int64_t lo = starts[s], hi = starts[s + 1];

@@ -25,8 +25,6 @@ __device__ __forceinline__ float softplusf_(float v) {
   p = __builtin_fmaf(p, s2, 1.0f);
   return (v < 0.0f ? 0.0f : v) + (v == -__builtin_inff() || v == __builtin_inff() ? 0.0f : 2.0f * s * p);
 }
-__device__ __forceinline__ float siluf_(float v) { return v * sigmoidf_(v); }
-
 // silu for a bfloat16 result: the exponent's rounding (2^-24 |v| log2 e) is far below the result's, so it is taken as it is.
 template <int DT>
 __device__ __forceinline__ float gatef_(float v) {
