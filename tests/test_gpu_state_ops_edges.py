@@ -157,6 +157,12 @@ def test_output_gate_of_far_values(dtype):
         want, _ = hip_ops.output_gate(*codes, *packed, local, torch.full_like(low, -80.0), D, quantize=quantize)
         # sigmoid(-80) = 1.8e-35: no bit of a sum of ordinary numbers
         assert torch.equal(y, want)
+        # and gates far above 0 are 1 like those of 80, infinite ones aside; NaN stays NaN
+        high = -low
+        high[0, 0] = float("nan")
+        y, _ = hip_ops.output_gate(*codes, *packed, local, high, D, quantize=quantize)
+        want, _ = hip_ops.output_gate(*codes, *packed, local, torch.full_like(low, 80.0), D, quantize=quantize)
+        assert bool(y[0, 0].isnan()) and torch.equal(y.flatten()[1:], want.flatten()[1:])
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
