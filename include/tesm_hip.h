@@ -60,13 +60,14 @@ int tesm_hip_stream_copy(void* dst, const void* src, int64_t bytes, void* stream
 /* Device status word of the library's bounded waits on the current device, no reference
  * counterpart (the reference's kernels never wait on one another), and of the indices that only the
  * device sees (bit 1, TESM_STATUS_BAD_PARENT).  Bit 0 (TESM_STATUS_SCAN_GAVE_UP):
- * a single-pass scan's look-back poll gave up; the states of that span are NaN.  The kernels still
+ * a single-pass scan's poll (tesm_hip_scan, tesm_hip_gated_scan) gave up; the states of that span are NaN.  The kernels still
  * return, so a caller that wants certainty checks this word after its work.  Synchronises with the
  * device (a diagnostic, not for the hot path); clear != 0 zeroes the word after reading it.
  * tesm_hip_debug_scan_spin_limit sets the poll limit of later scans (default 1 << 20 rounds; a
  * negative limit gives up at once, which tests use to exercise the report). */
 #define TESM_STATUS_SCAN_GAVE_UP 1u
 #define TESM_STATUS_BAD_PARENT 2u /* tesm_hip_reorder_rows met a parent outside [0, K); that row stayed as it was */
+#define TESM_STATUS_BAD_TARGET 4u /* tesm_hip_token_log_probs met a target that is no token; its log probability is NaN */
 int tesm_hip_device_status(uint32_t* status, int clear);
 int tesm_hip_debug_scan_spin_limit(int limit);
 
@@ -627,6 +628,162 @@ typedef struct tesm_hip_rows {
 
 int tesm_hip_reorder_rows(const tesm_hip_rows* t, int64_t count, const int64_t* parents, int64_t B, int64_t K,
                           void* stream);
+
+/* Gated linear recurrence, no reference counterpart (tesm_hip_scan takes decays and updates as they are).  Per channel c, over
+ * rows t of a sequence:
+ *   a = sigmoid(decay[t,c] + bias[c]),  h[t,c] = a h[t-1,c] + sigmoid(write[t,c]) tanh(value[t,c]).
+ * The rows are B sequences of L (S = B), or with seq_starts S sequences packed one behind the other in one row axis (B = 1, L
+ * rows): sequence s is rows seq_starts[s] .. seq_starts[s+1]-1 (starts outside the rows count as the nearest, one below an
+ * earlier one as that one); rows in front of the first and behind the last are neither read nor written.  h0 / h_out: (S, C) float32,
+ * the states before and after each sequence (NULL h0: zeros).  States are float32; results repeat bit for bit.  carries:
+ * (tesm_hip_gated_scan_slots, C) float32, what the backward call needs (NULL: not kept).  Fewer than 2^31 rows, C and S
+ * below 2^24.  Outputs must not overlap operands or each other (columns of the same wider rows do not overlap). */
+typedef struct tesm_hip_gates {
+  int dt;                     /* value, write, decay, and the arrays of their shape */
+  int64_t B, L, C, S;
+  const void* value;          /* row r, channel c at value[r * ld_value + c] */
+  int64_t ld_value;
+  const void* write;
+  int64_t ld_write;
+  const void* decay;
+  int64_t ld_decay;
+  const float* bias;          /* optional (C) */
+  const int32_t* seq_starts;  /* optional (S + 1) */
+  const float* h0;            /* optional (S, C) */
+} tesm_hip_gates;
+
+typedef struct tesm_hip_recurrence {
+  tesm_hip_gates in;
+  void* h;                    /* rows as value */
+  int64_t ld_h;
+  float* h_out;               /* (S, C) */
+  float* carries;             /* optional */
+} tesm_hip_recurrence;
+
+int64_t tesm_hip_gated_scan_slots(const tesm_hip_gates* p);
+int64_t tesm_hip_gated_scan_ws_bytes(const tesm_hip_recurrence* p);
+int tesm_hip_gated_scan(const tesm_hip_recurrence* p, void* ws, int64_t ws_bytes, void* stream);
+
+/* Its backward pass: from the gradients of h and (optional) of h_out those of value, write, decay, (optional) bias and h0.  in and
+ * carries are the forward call's. */
+typedef struct tesm_hip_recurrence_grad {
+  tesm_hip_gates in;
+  const float* carries;
+  const void* grad;           /* rows as value */
+  int64_t ld_grad;
+  const float* grad_state;    /* optional (S, C) */
+  void* d_value;              /* rows as value */
+  int64_t ld_d_value;
+  void* d_write;
+  int64_t ld_d_write;
+  void* d_decay;
+  int64_t ld_d_decay;
+  float* d_bias;              /* optional (C) */
+  float* d_h0;                /* optional (S, C) */
+} tesm_hip_recurrence_grad;
+
+int64_t tesm_hip_gated_scan_backward_ws_bytes(const tesm_hip_recurrence_grad* p);
+int tesm_hip_gated_scan_backward(const tesm_hip_recurrence_grad* p, void* ws, int64_t ws_bytes, void* stream);
+
+/* One token of the recurrence for B sequences: state (B, C) float32 is updated in place, h holds it in dt.  B < 65536. */
+typedef struct tesm_hip_recurrence_step {
+  int dt;
+  int64_t B, C;
+  const void* value;
+  int64_t ld_value;
+  const void* write;
+  int64_t ld_write;
+  const void* decay;
+  int64_t ld_decay;
+  const float* bias;          /* optional (C) */
+  float* state;
+  void* h;
+  int64_t ld_h;
+} tesm_hip_recurrence_step;
+
+int tesm_hip_gated_scan_step(const tesm_hip_recurrence_step* p, void* stream);
+
+/* Products of float matrices with what stands around them, no reference counterpart (the reference's projections are ternary).
+ * up given: the gated pair of a feed-forward block, y = act(x weight^T) * (x up^T).  up NULL: y = act(x weight^T + bias) +
+ * residual.  act: 0 none (not for a pair), 1 silu, 2 gelu (z (1 + erf(z / sqrt 2)) / 2).  Sums are float32, rounded to dt once;
+ * float32 operands go through the matrix units in three bfloat16 parts (an infinity among them gives NaN).  z (and z_up): x
+ * weight^T (+ bias) and x up^T rounded to dt, for the backward call (NULL: not kept).  M < 2^31, N, K < 2^24. */
+typedef struct tesm_hip_dense {
+  int dt;
+  int act;
+  int64_t M, K, N;
+  const void* x;              /* (M, ld_x) */
+  int64_t ld_x;
+  const void* weight;         /* (N, ld_weight) */
+  int64_t ld_weight;
+  const void* up;             /* optional (N, ld_up) */
+  int64_t ld_up;
+  const void* bias;           /* optional (N), no pair */
+  const void* residual;       /* optional (M, ld_residual), no pair */
+  int64_t ld_residual;
+  void* y;                    /* (M, ld_y) */
+  int64_t ld_y;
+  void* z;                    /* optional (M, N) */
+  void* z_up;                 /* optional (M, N) */
+} tesm_hip_dense;
+
+int64_t tesm_hip_dense_ws_bytes(const tesm_hip_dense* p);
+int tesm_hip_dense_forward(const tesm_hip_dense* p, void* ws, int64_t ws_bytes, void* stream);
+
+/* Its backward pass: from the gradient of y those of x, weight, up and bias that are asked for (the residual's is y's own).  of: the
+ * forward call's descriptor (bias, residual and y are not used); z and z_up what it kept (z not needed with act 0).  The
+ * gradients in front of the products go into them rounded to bfloat16, for float32 in three parts. */
+typedef struct tesm_hip_dense_grad {
+  tesm_hip_dense of;
+  const void* grad;           /* (M, ld_grad) */
+  int64_t ld_grad;
+  void* d_x;                  /* optional (M, K) */
+  void* d_weight;             /* optional (N, K) */
+  void* d_up;                 /* (N, K), with d_weight of a pair */
+  void* d_bias;               /* optional (N) */
+} tesm_hip_dense_grad;
+
+int64_t tesm_hip_dense_backward_ws_bytes(const tesm_hip_dense_grad* p);
+int tesm_hip_dense_backward(const tesm_hip_dense_grad* p, void* ws, int64_t ws_bytes, void* stream);
+
+/* Log probabilities of given tokens, no reference counterpart.  Per row r: log_probs[r] = logits[r,t] - logsumexp(logits[r,:]) for
+ * t = targets[r] (0 where t is ignore), entropy[r] of the row's distribution, and the log probabilities and tokens of its top
+ * largest logits in falling order, equal ones by token (a NaN logit counts as the lowest).  -infinity is a masked token; a row with a
+ * NaN or +infinite logit, or none above -infinity, gives NaN.  Any other target outside [0, V) gives NaN and sets
+ * TESM_STATUS_BAD_TARGET.  kept: (rows, 4) float32 for the backward call (NULL: not kept).  top <= 64, V < 2^30. */
+typedef struct tesm_hip_logp {
+  int dt;                     /* logits */
+  int64_t rows, V, top;
+  const void* logits;         /* (rows, ld) */
+  int64_t ld;
+  const int64_t* targets;     /* (rows) */
+  int64_t ignore;
+  float* log_probs;           /* (rows) */
+  float* entropy;             /* (rows) */
+  float* top_log_probs;       /* (rows, top) */
+  int64_t* top_tokens;        /* (rows, top) */
+  float* kept;
+} tesm_hip_logp;
+
+int64_t tesm_hip_token_log_probs_ws_bytes(const tesm_hip_logp* p);
+int tesm_hip_token_log_probs(const tesm_hip_logp* p, void* ws, int64_t ws_bytes, void* stream);
+
+/* The gradient of the logits from those of log_probs and entropy (NULL: 0). */
+typedef struct tesm_hip_logp_grad {
+  int dt;                     /* logits, d_logits */
+  int64_t rows, V;
+  const void* logits;
+  int64_t ld;
+  const int64_t* targets;
+  int64_t ignore;
+  const float* kept;
+  const float* grad_log_probs; /* optional (rows) */
+  const float* grad_entropy;  /* optional (rows) */
+  void* d_logits;             /* (rows, ld_d) */
+  int64_t ld_d;
+} tesm_hip_logp_grad;
+
+int tesm_hip_token_log_probs_backward(const tesm_hip_logp_grad* p, void* stream);
 
 #ifdef __cplusplus
 }

@@ -205,6 +205,75 @@ class Rows(ctypes.Structure):
     _fields_ = [("p", P), ("pitch", I64), ("bytes", I64)]
 
 
+class Gates(ctypes.Structure):
+    """``tesm_hip_gates``."""
+    _fields_ = [
+        ("dt", I32),
+        ("B", I64), ("L", I64), ("C", I64), ("S", I64),
+        ("value", P), ("ld_value", I64), ("write", P), ("ld_write", I64), ("decay", P), ("ld_decay", I64),
+        ("bias", P), ("seq_starts", P), ("h0", P),
+    ]
+
+
+class Recurrence(ctypes.Structure):
+    """``tesm_hip_recurrence``."""
+    _fields_ = [("in", Gates), ("h", P), ("ld_h", I64), ("h_out", P), ("carries", P)]
+
+
+class RecurrenceGrad(ctypes.Structure):
+    """``tesm_hip_recurrence_grad``."""
+    _fields_ = [
+        ("in", Gates), ("carries", P), ("grad", P), ("ld_grad", I64), ("grad_state", P),
+        ("d_value", P), ("ld_d_value", I64), ("d_write", P), ("ld_d_write", I64), ("d_decay", P), ("ld_d_decay", I64),
+        ("d_bias", P), ("d_h0", P),
+    ]
+
+
+class RecurrenceStep(ctypes.Structure):
+    """``tesm_hip_recurrence_step``."""
+    _fields_ = [
+        ("dt", I32),
+        ("B", I64), ("C", I64),
+        ("value", P), ("ld_value", I64), ("write", P), ("ld_write", I64), ("decay", P), ("ld_decay", I64),
+        ("bias", P), ("state", P), ("h", P), ("ld_h", I64),
+    ]
+
+
+class Dense(ctypes.Structure):
+    """``tesm_hip_dense``."""
+    _fields_ = [
+        ("dt", I32), ("act", I32),
+        ("M", I64), ("K", I64), ("N", I64),
+        ("x", P), ("ld_x", I64), ("weight", P), ("ld_weight", I64), ("up", P), ("ld_up", I64), ("bias", P),
+        ("residual", P), ("ld_residual", I64), ("y", P), ("ld_y", I64), ("z", P), ("z_up", P),
+    ]
+
+
+class DenseGrad(ctypes.Structure):
+    """``tesm_hip_dense_grad``."""
+    _fields_ = [("of", Dense), ("grad", P), ("ld_grad", I64), ("d_x", P), ("d_weight", P), ("d_up", P), ("d_bias", P)]
+
+
+class Logp(ctypes.Structure):
+    """``tesm_hip_logp``."""
+    _fields_ = [
+        ("dt", I32),
+        ("rows", I64), ("V", I64), ("top", I64),
+        ("logits", P), ("ld", I64), ("targets", P), ("ignore", I64),
+        ("log_probs", P), ("entropy", P), ("top_log_probs", P), ("top_tokens", P), ("kept", P),
+    ]
+
+
+class LogpGrad(ctypes.Structure):
+    """``tesm_hip_logp_grad``."""
+    _fields_ = [
+        ("dt", I32),
+        ("rows", I64), ("V", I64),
+        ("logits", P), ("ld", I64), ("targets", P), ("ignore", I64), ("kept", P),
+        ("grad_log_probs", P), ("grad_entropy", P), ("d_logits", P), ("ld_d", I64),
+    ]
+
+
 class Taps(ctypes.Structure):
     """``tesm_hip_taps``."""
     _fields_ = [("q_u", P), ("s_u", P), ("q_cs", P), ("s_cs", P), ("q_te", P), ("s_te", P), ("q_c", P), ("s_c", P),
@@ -255,6 +324,19 @@ _SIGNATURES = {
     "tesm_hip_beam_select_ws_bytes": ([ctypes.POINTER(Beam)], I64),
     "tesm_hip_beam_select": ([ctypes.POINTER(Beam), P, I64, P], I32),
     "tesm_hip_reorder_rows": ([P, I64, P, I64, I64, P], I32),
+    "tesm_hip_gated_scan_slots": ([ctypes.POINTER(Gates)], I64),
+    "tesm_hip_gated_scan_ws_bytes": ([ctypes.POINTER(Recurrence)], I64),
+    "tesm_hip_gated_scan": ([ctypes.POINTER(Recurrence), P, I64, P], I32),
+    "tesm_hip_gated_scan_backward_ws_bytes": ([ctypes.POINTER(RecurrenceGrad)], I64),
+    "tesm_hip_gated_scan_backward": ([ctypes.POINTER(RecurrenceGrad), P, I64, P], I32),
+    "tesm_hip_gated_scan_step": ([ctypes.POINTER(RecurrenceStep), P], I32),
+    "tesm_hip_dense_ws_bytes": ([ctypes.POINTER(Dense)], I64),
+    "tesm_hip_dense_forward": ([ctypes.POINTER(Dense), P, I64, P], I32),
+    "tesm_hip_dense_backward_ws_bytes": ([ctypes.POINTER(DenseGrad)], I64),
+    "tesm_hip_dense_backward": ([ctypes.POINTER(DenseGrad), P, I64, P], I32),
+    "tesm_hip_token_log_probs_ws_bytes": ([ctypes.POINTER(Logp)], I64),
+    "tesm_hip_token_log_probs": ([ctypes.POINTER(Logp), P, I64, P], I32),
+    "tesm_hip_token_log_probs_backward": ([ctypes.POINTER(LogpGrad), P], I32),
     "tesm_hip_mimo_coef": ([P, P, I32, I64, I64, I64, P, P, P], I32),
     "tesm_hip_mimo_prefill_ws_bytes": ([ctypes.POINTER(MimoLayer)], I64),
     "tesm_hip_mimo_prefill": ([ctypes.POINTER(MimoLayer), P, I64, P], I32),

@@ -14,10 +14,13 @@
 
 #include "beam.h"
 #include "decode.h"
+#include "dense.h"
 #include "entangle.h"
 #include "global.h"
+#include "logp.h"
 #include "mimo.h"
 #include "norm.h"
+#include "recur.h"
 #include "rows_overlap.h"
 #include "scan.h"
 #include "ssm.h"
@@ -682,7 +685,12 @@ int tesm_hip_device_status(uint32_t* status, int clear) {
   if (int rc = scan_status(&v, clear)) return rc;
   unsigned r = 0;
   if (int rc = reorder_status(&r, clear)) return rc;
-  if (status) *status = v | r;
+  v |= r;
+  if (int rc = recur_status(&r, clear)) return rc;
+  v |= r;
+  if (int rc = logp_status(&r, clear)) return rc;
+  v |= r;
+  if (status) *status = v;
   return kOk;
 }
 
@@ -695,6 +703,7 @@ int tesm_hip_debug_taps(const tesm_hip_taps* t) {
 
 int tesm_hip_debug_scan_spin_limit(int limit) {
   scan_set_spin_limit(limit);
+  recur_set_spin_limit(limit);
   return kOk;
 }
 
@@ -2124,6 +2133,303 @@ int tesm_hip_reorder_rows(const tesm_hip_rows* t, int64_t count, const int64_t* 
     if (int rc = check_ptr(t[i].p, "a tensor", "reorder rows")) return rc;
   return launch_reorder_rows(reinterpret_cast<const ReorderRows*>(t), count, parents, B, K,
                              static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"
+
+namespace tesm {
+namespace {
+RecurArgs recur_args(const tesm_hip_gates& p) {
+  RecurArgs a;
+  a.dt = p.dt;
+  a.B = p.B, a.L = p.L, a.C = p.C, a.S = p.S;
+  a.value = p.value, a.ld_v = p.ld_value;
+  a.write = p.write, a.ld_w = p.ld_write;
+  a.decay = p.decay, a.ld_d = p.ld_decay;
+  a.bias = p.bias;
+  a.seq_starts = p.seq_starts;
+  a.h0 = p.h0;
+  return a;
+}
+RecurArgs recur_args(const tesm_hip_recurrence& p) {
+  RecurArgs a = recur_args(p.in);
+  a.h = p.h, a.ld_h = p.ld_h;
+  a.h_out = p.h_out;
+  a.carries = p.carries;
+  return a;
+}
+RecurBwdArgs recur_args(const tesm_hip_recurrence_grad& p) {
+  RecurBwdArgs a;
+  a.in = recur_args(p.in);
+  a.in.carries = const_cast<float*>(p.carries);
+  a.grad = p.grad, a.ld_g = p.ld_grad;
+  a.grad_state = p.grad_state;
+  a.d_value = p.d_value, a.ld_dv = p.ld_d_value;
+  a.d_write = p.d_write, a.ld_dw = p.ld_d_write;
+  a.d_decay = p.d_decay, a.ld_dd = p.ld_d_decay;
+  a.d_bias = p.d_bias;
+  a.d_h0 = p.d_h0;
+  return a;
+}
+bool plain_sizes(const tesm_hip_gates& p, std::initializer_list<int64_t> pitches) {
+  return plain_sizes({p.B, p.L, p.C, p.S}, {p.ld_value, p.ld_write, p.ld_decay}) && plain_sizes({}, pitches) &&
+         p.B * p.L < (1LL << 31) && p.C < (1LL << 24) && p.S < (1LL << 24);
+}
+std::vector<NamedSpan> gate_spans(const tesm_hip_gates& p) {
+  const int64_t M = p.B * p.L, e = size_of(p.dt);
+  return {{"value", span(p.value, M, p.ld_value, p.C, e)}, {"write", span(p.write, M, p.ld_write, p.C, e)},
+          {"decay", span(p.decay, M, p.ld_decay, p.C, e)}, {"bias", dense(p.bias, p.C, 4)},
+          {"seq_starts", dense(p.seq_starts, p.S + 1, 4)}, {"h0", dense(p.h0, p.S * p.C, 4)}};
+}
+int check_overlaps(const char* who, const std::vector<NamedSpan>& outputs, const std::vector<NamedSpan>& inputs) {
+  for (size_t o = 0; o < outputs.size(); ++o) {
+    for (const NamedSpan& i : inputs)
+      if (rows_share(outputs[o].rows, i.rows)) return fail(kErrInvalidArg, std::string(who) + ": " + outputs[o].name + " overlaps " + i.name);
+    for (size_t q = o + 1; q < outputs.size(); ++q)
+      if (rows_share(outputs[o].rows, outputs[q].rows))
+        return fail(kErrInvalidArg, std::string(who) + ": " + outputs[o].name + " overlaps " + outputs[q].name);
+  }
+  return kOk;
+}
+int check_gate_ptrs(const char* who, const tesm_hip_gates& p) {
+  return check_ptrs(who, {{p.value, "value"}, {p.write, "write"}, {p.decay, "decay"}, {p.bias, "bias"}, {p.seq_starts, "seq_starts"},
+                          {p.h0, "h0"}});
+}
+
+DenseArgs dense_args(const tesm_hip_dense& p) {
+  DenseArgs a;
+  a.dt = p.dt, a.act = p.act;
+  a.M = p.M, a.K = p.K, a.N = p.N;
+  a.x = p.x, a.ld_x = p.ld_x;
+  a.w = p.weight, a.ld_w = p.ld_weight;
+  a.w2 = p.up, a.ld_w2 = p.ld_up;
+  a.bias = p.bias;
+  a.residual = p.residual, a.ld_r = p.ld_residual;
+  a.y = p.y, a.ld_y = p.ld_y;
+  a.z = p.z, a.z2 = p.z_up;
+  return a;
+}
+DenseBwdArgs dense_args(const tesm_hip_dense_grad& p) {
+  DenseBwdArgs a;
+  a.in = dense_args(p.of);
+  a.grad = p.grad, a.ld_g = p.ld_grad;
+  a.dx = p.d_x, a.dw = p.d_weight, a.dw2 = p.d_up;
+  a.dbias = p.d_bias;
+  return a;
+}
+bool plain_sizes(const tesm_hip_dense& p, std::initializer_list<int64_t> pitches) {
+  return plain_sizes({p.M, p.N, p.K}, {p.ld_x, p.ld_weight, p.ld_up, p.ld_residual, p.ld_y}) && plain_sizes({}, pitches) &&
+         p.N < (1LL << 24) && p.K < (1LL << 24);
+}
+std::vector<NamedSpan> dense_spans(const tesm_hip_dense& p) {
+  const int64_t e = size_of(p.dt);
+  return {{"x", span(p.x, p.M, p.ld_x, p.K, e)}, {"weight", span(p.weight, p.N, p.ld_weight, p.K, e)},
+          {"up", span(p.up, p.N, p.ld_up, p.K, e)}, {"bias", dense(p.bias, p.N, e)},
+          {"residual", span(p.residual, p.M, p.ld_residual, p.N, e)}};
+}
+int check_dense_ptrs(const char* who, const tesm_hip_dense& p) {
+  return check_ptrs(who, {{p.x, "x"}, {p.weight, "weight"}, {p.up, "up"}, {p.bias, "bias"}, {p.residual, "residual"}, {p.y, "y"},
+                          {p.z, "z"}, {p.z_up, "z_up"}});
+}
+
+LogpArgs logp_args(const tesm_hip_logp& p) {
+  LogpArgs a;
+  a.dt = p.dt;
+  a.rows = p.rows, a.V = p.V, a.top = p.top;
+  a.logits = p.logits, a.ld = p.ld;
+  a.targets = p.targets, a.ignore = p.ignore;
+  a.logp = p.log_probs, a.entropy = p.entropy;
+  a.top_logp = p.top_log_probs, a.top_tokens = p.top_tokens;
+  a.kept = p.kept;
+  return a;
+}
+
+// Host memory for a check's table may run out: an error, not an exception through the C entry.
+template <typename F>
+int guarded(const char* who, F&& f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return fail(kErrInvalidArg, std::string(who) + ": no host memory");
+  }
+}
+}  // namespace
+}  // namespace tesm
+
+extern "C" {
+
+int64_t tesm_hip_gated_scan_slots(const tesm_hip_gates* p) { return p ? recur_slots(recur_args(*p)) : -1; }
+
+int64_t tesm_hip_gated_scan_ws_bytes(const tesm_hip_recurrence* p) { return p ? recur_ws_bytes(recur_args(*p)) : -1; }
+
+int tesm_hip_gated_scan(const tesm_hip_recurrence* p, void* ws, int64_t ws_bytes, void* stream) {
+  const char* who = "gated scan";
+  TESM_REQUIRE(p != nullptr, kErrInvalidArg, "gated scan: null descriptor");
+  return guarded(who, [&]() -> int {
+    const tesm_hip_gates& g = p->in;
+    if (plain_sizes(g, {p->ld_h})) {
+      const int64_t M = g.B * g.L, slots = recur_slots(recur_args(g));
+      if (int rc = check_overlaps(who, {{"h", span(p->h, M, p->ld_h, g.C, size_of(g.dt))}, {"h_out", dense(p->h_out, g.S * g.C, 4)},
+                                        {"carries", dense(p->carries, std::max<int64_t>(slots, 0) * g.C, 4)},
+                                        {"workspace", dense(ws, std::max<int64_t>(ws_bytes, 0), 1)}},
+                                  gate_spans(g)))
+        return rc;
+    }
+    if (int rc = check_gate_ptrs(who, g)) return rc;
+    if (int rc = check_ptrs(who, {{p->h, "h"}, {p->h_out, "h_out"}, {p->carries, "carries"}, {ws, "workspace"}})) return rc;
+    return launch_gated_scan(recur_args(*p), ws, ws_bytes, static_cast<hipStream_t>(stream));
+  });
+}
+
+int64_t tesm_hip_gated_scan_backward_ws_bytes(const tesm_hip_recurrence_grad* p) {
+  return p ? recur_bwd_ws_bytes(recur_args(p->in), p->d_bias != nullptr) : -1;
+}
+
+int tesm_hip_gated_scan_backward(const tesm_hip_recurrence_grad* p, void* ws, int64_t ws_bytes, void* stream) {
+  const char* who = "gated scan backward";
+  TESM_REQUIRE(p != nullptr, kErrInvalidArg, "gated scan backward: null descriptor");
+  return guarded(who, [&]() -> int {
+    const tesm_hip_gates& g = p->in;
+    if (plain_sizes(g, {p->ld_grad, p->ld_d_value, p->ld_d_write, p->ld_d_decay})) {
+      const int64_t M = g.B * g.L, e = size_of(g.dt), slots = recur_slots(recur_args(g));
+      std::vector<NamedSpan> in = gate_spans(g);
+      in.push_back({"grad", span(p->grad, M, p->ld_grad, g.C, e)});
+      in.push_back({"grad_state", dense(p->grad_state, g.S * g.C, 4)});
+      in.push_back({"carries", dense(p->carries, std::max<int64_t>(slots, 0) * g.C, 4)});
+      if (int rc = check_overlaps(who, {{"d_value", span(p->d_value, M, p->ld_d_value, g.C, e)},
+                                        {"d_write", span(p->d_write, M, p->ld_d_write, g.C, e)},
+                                        {"d_decay", span(p->d_decay, M, p->ld_d_decay, g.C, e)}, {"d_bias", dense(p->d_bias, g.C, 4)},
+                                        {"d_h0", dense(p->d_h0, g.S * g.C, 4)}, {"workspace", dense(ws, std::max<int64_t>(ws_bytes, 0), 1)}},
+                                  in))
+        return rc;
+    }
+    if (int rc = check_gate_ptrs(who, g)) return rc;
+    if (int rc = check_ptrs(who, {{p->carries, "carries"}, {p->grad, "grad"}, {p->grad_state, "grad_state"}, {p->d_value, "d_value"},
+                                  {p->d_write, "d_write"}, {p->d_decay, "d_decay"}, {p->d_bias, "d_bias"}, {p->d_h0, "d_h0"},
+                                  {ws, "workspace"}}))
+      return rc;
+    return launch_gated_scan_bwd(recur_args(*p), ws, ws_bytes, static_cast<hipStream_t>(stream));
+  });
+}
+
+int tesm_hip_gated_scan_step(const tesm_hip_recurrence_step* p, void* stream) {
+  const char* who = "gated scan step";
+  TESM_REQUIRE(p != nullptr, kErrInvalidArg, "gated scan step: null descriptor");
+  if (plain_sizes({p->B, p->C}, {p->ld_value, p->ld_write, p->ld_decay, p->ld_h}) && p->C < (1LL << 24)) {
+    const int64_t e = size_of(p->dt);
+    if (int rc = check_overlaps(who, {{"h", span(p->h, p->B, p->ld_h, p->C, e)}, {"state", dense(p->state, p->B * p->C, 4)}},
+                                {{"value", span(p->value, p->B, p->ld_value, p->C, e)}, {"write", span(p->write, p->B, p->ld_write, p->C, e)},
+                                 {"decay", span(p->decay, p->B, p->ld_decay, p->C, e)}, {"bias", dense(p->bias, p->C, 4)}}))
+      return rc;
+  }
+  if (int rc = check_ptrs(who, {{p->value, "value"}, {p->write, "write"}, {p->decay, "decay"}, {p->bias, "bias"}, {p->state, "state"},
+                                {p->h, "h"}}))
+    return rc;
+  RecurStepArgs a;
+  a.dt = p->dt;
+  a.B = p->B, a.C = p->C;
+  a.value = p->value, a.ld_v = p->ld_value;
+  a.write = p->write, a.ld_w = p->ld_write;
+  a.decay = p->decay, a.ld_d = p->ld_decay;
+  a.bias = p->bias;
+  a.state = p->state;
+  a.h = p->h, a.ld_h = p->ld_h;
+  return launch_gated_scan_step(a, static_cast<hipStream_t>(stream));
+}
+
+int64_t tesm_hip_dense_ws_bytes(const tesm_hip_dense* p) { return p ? dense_ws_bytes(dense_args(*p)) : -1; }
+
+int tesm_hip_dense_forward(const tesm_hip_dense* p, void* ws, int64_t ws_bytes, void* stream) {
+  const char* who = "dense product";
+  TESM_REQUIRE(p != nullptr, kErrInvalidArg, "dense product: null descriptor");
+  return guarded(who, [&]() -> int {
+    TESM_REQUIRE(!p->up || (!p->bias && !p->residual), kErrInvalidArg, "dense product: a gated pair takes no bias and no residual");
+    if (plain_sizes(*p, {})) {
+      const int64_t e = size_of(p->dt), n = p->M * p->N;
+      if (int rc = check_overlaps(who, {{"y", span(p->y, p->M, p->ld_y, p->N, e)}, {"z", dense(p->z, n, e)}, {"z_up", dense(p->z_up, n, e)},
+                                        {"workspace", dense(ws, std::max<int64_t>(ws_bytes, 0), 1)}},
+                                  dense_spans(*p)))
+        return rc;
+    }
+    if (int rc = check_dense_ptrs(who, *p)) return rc;
+    if (int rc = check_ptrs(who, {{ws, "workspace"}})) return rc;
+    return launch_dense(dense_args(*p), ws, ws_bytes, static_cast<hipStream_t>(stream));
+  });
+}
+
+int64_t tesm_hip_dense_backward_ws_bytes(const tesm_hip_dense_grad* p) { return p ? dense_bwd_ws_bytes(dense_args(*p)) : -1; }
+
+int tesm_hip_dense_backward(const tesm_hip_dense_grad* p, void* ws, int64_t ws_bytes, void* stream) {
+  const char* who = "dense backward";
+  TESM_REQUIRE(p != nullptr, kErrInvalidArg, "dense backward: null descriptor");
+  return guarded(who, [&]() -> int {
+    TESM_REQUIRE(!p->of.up || !p->d_bias, kErrInvalidArg, "dense backward: a gated pair has no bias");
+    if (plain_sizes(p->of, {p->ld_grad})) {
+      const int64_t e = size_of(p->of.dt), mn = p->of.M * p->of.N, nk = p->of.N * p->of.K;
+      std::vector<NamedSpan> in = dense_spans(p->of);
+      in.push_back({"grad", span(p->grad, p->of.M, p->ld_grad, p->of.N, e)});
+      in.push_back({"z", dense(p->of.z, mn, e)});
+      in.push_back({"z_up", dense(p->of.z_up, mn, e)});
+      if (int rc = check_overlaps(who, {{"d_x", dense(p->d_x, p->of.M * p->of.K, e)}, {"d_weight", dense(p->d_weight, nk, e)},
+                                        {"d_up", dense(p->d_up, nk, e)}, {"d_bias", dense(p->d_bias, p->of.N, e)},
+                                        {"workspace", dense(ws, std::max<int64_t>(ws_bytes, 0), 1)}},
+                                  in))
+        return rc;
+    }
+    if (int rc = check_dense_ptrs(who, p->of)) return rc;
+    if (int rc = check_ptrs(who, {{p->grad, "grad"}, {p->d_x, "d_x"}, {p->d_weight, "d_weight"}, {p->d_up, "d_up"}, {p->d_bias, "d_bias"},
+                                  {ws, "workspace"}}))
+      return rc;
+    return launch_dense_bwd(dense_args(*p), ws, ws_bytes, static_cast<hipStream_t>(stream));
+  });
+}
+
+int64_t tesm_hip_token_log_probs_ws_bytes(const tesm_hip_logp* p) { return p ? logp_ws_bytes(logp_args(*p)) : -1; }
+
+int tesm_hip_token_log_probs(const tesm_hip_logp* p, void* ws, int64_t ws_bytes, void* stream) {
+  const char* who = "token log probs";
+  TESM_REQUIRE(p != nullptr, kErrInvalidArg, "token log probs: null descriptor");
+  return guarded(who, [&]() -> int {
+    if (plain_sizes({p->rows, p->V, p->top}, {}) && p->ld >= 0 && p->ld < (1LL << 31) && p->top <= kLogpMaxTop) {
+      const int64_t top = p->rows * p->top;
+      if (int rc = check_overlaps(who, {{"log_probs", dense(p->log_probs, p->rows, 4)}, {"entropy", dense(p->entropy, p->rows, 4)},
+                                        {"top_log_probs", dense(p->top_log_probs, top, 4)}, {"top_tokens", dense(p->top_tokens, top, 8)},
+                                        {"kept", dense(p->kept, 4 * p->rows, 4)}, {"workspace", dense(ws, std::max<int64_t>(ws_bytes, 0), 1)}},
+                                  {{"logits", span(p->logits, p->rows, p->ld, p->V, size_of(p->dt))}, {"targets", dense(p->targets, p->rows, 8)}}))
+        return rc;
+    }
+    if (int rc = check_ptrs(who, {{p->logits, "logits"}, {p->targets, "targets"}, {p->log_probs, "log_probs"}, {p->entropy, "entropy"},
+                                  {p->top_log_probs, "top_log_probs"}, {p->top_tokens, "top_tokens"}, {p->kept, "kept"}, {ws, "workspace"}}))
+      return rc;
+    return launch_token_logp(logp_args(*p), ws, ws_bytes, static_cast<hipStream_t>(stream));
+  });
+}
+
+int tesm_hip_token_log_probs_backward(const tesm_hip_logp_grad* p, void* stream) {
+  const char* who = "token log probs backward";
+  TESM_REQUIRE(p != nullptr, kErrInvalidArg, "token log probs backward: null descriptor");
+  return guarded(who, [&]() -> int {
+    if (plain_sizes({p->rows, p->V}, {}) && p->ld >= 0 && p->ld < (1LL << 31) && p->ld_d >= 0 && p->ld_d < (1LL << 31)) {
+      const int64_t e = size_of(p->dt);
+      if (int rc = check_overlaps(who, {{"d_logits", span(p->d_logits, p->rows, p->ld_d, p->V, e)}},
+                                  {{"logits", span(p->logits, p->rows, p->ld, p->V, e)}, {"targets", dense(p->targets, p->rows, 8)},
+                                   {"kept", dense(p->kept, 4 * p->rows, 4)}, {"grad_log_probs", dense(p->grad_log_probs, p->rows, 4)},
+                                   {"grad_entropy", dense(p->grad_entropy, p->rows, 4)}}))
+        return rc;
+    }
+    if (int rc = check_ptrs(who, {{p->logits, "logits"}, {p->targets, "targets"}, {p->kept, "kept"}, {p->grad_log_probs, "grad_log_probs"},
+                                  {p->grad_entropy, "grad_entropy"}, {p->d_logits, "d_logits"}}))
+      return rc;
+    LogpBwdArgs a;
+    a.dt = p->dt;
+    a.rows = p->rows, a.V = p->V;
+    a.logits = p->logits, a.ld = p->ld;
+    a.targets = p->targets, a.ignore = p->ignore;
+    a.kept = p->kept;
+    a.grad_logp = p->grad_log_probs, a.grad_entropy = p->grad_entropy;
+    a.grad_logits = p->d_logits, a.ld_g = p->ld_d;
+    return launch_token_logp_bwd(a, static_cast<hipStream_t>(stream));
+  });
 }
 
 }  // extern "C"

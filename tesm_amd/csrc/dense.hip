@@ -1,0 +1,559 @@
+// The dense operators around the matrix product (dense_mfma.hip): operands brought into its form, few rows, gradients of the
+// activations, sums over rows.
+//
+// Operands.  bfloat16 matrices whose rows start on 16 bytes and hold a multiple of 8 values are read where they lie; others are laid
+// out so in the workspace first, padded with zeros.  float32 matrices are laid out as three bfloat16 parts, x = x0 + x1 + x2 with
+// x0 = bf16(x), x1 = bf16(x - x0), x2 = x - x0 - x1 (8 bits each, together all 24 of x), and a product takes the six of their nine products
+// that reach above 2^-26 of it, smallest first, all into one float32 sum: bfloat16 products run at 16 times the
+// float32 rate, so six of them are 2.7 times as fast as one in float32.  An infinite operand gives NaN where the formula may
+// give an infinity.
+//
+// Gradients.  z (and z2), what stands before the activation, is kept by the forward pass in the operands' type.  The gradient in
+// front of the products goes into them in bfloat16 (float32: in three parts).
+#include "dense_mfma.h"
+
+namespace tesm {
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(2)));
+
+constexpr int64_t kSkinnyRows = 32;  // up to here weights are streamed once, past the matrix product's tiles
+
+int64_t up8(int64_t v) { return round_up(v, 8); }
+int64_t size_of_dt(int dt) { return dt == kBF16 ? 2 : 4; }
+
+// ---------------------------------------------------------------------------
+// float32 as three bfloat16 parts
+// ---------------------------------------------------------------------------
+struct Parts3 {
+  uint16_t p[3];
+};
+__device__ __forceinline__ Parts3 split3(float x) {
+  uint16_t h = f32_to_bf16(x);
+  if ((h & 0x7f80u) == 0x7f80u) {
+    if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) return {{h, 0, 0}};  // an infinity or NaN
+    h = static_cast<uint16_t>(__float_as_uint(x) >> 16);                       // (the largest values would round to infinity)
+  }
+  const float r = x - bf16_to_f32(h);
+  const uint16_t m = f32_to_bf16(r);
+  return {{h, m, f32_to_bf16(r - bf16_to_f32(m))}};
+}
+// Eight values to PARTS parts, `stride` apart.
+template <int PARTS>
+__device__ __forceinline__ void store_parts(uint16_t* to, int64_t stride, const float (&v)[8]) {
+  if constexpr (PARTS == 1) {
+    *reinterpret_cast<uint4*>(to) =
+        make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  } else {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const Parts3 a = split3(v[2 * q]), b = split3(v[2 * q + 1]);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) w[p][q] = a.p[p] | static_cast<uint32_t>(b.p[p]) << 16;
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(to + p * stride) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+  }
+}
+// Eight values at element i, of which `n` exist (the others are 0); whole ones by one or two loads where `vec`.
+template <int DT>
+__device__ __forceinline__ void load_eight(const void* p, int64_t i, int n, bool vec, float (&v)[8]) {
+  if (vec && n >= 8) {
+    if constexpr (DT == kBF16) {
+      const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        v[2 * q] = __uint_as_float(u[q] << 16);
+        v[2 * q + 1] = __uint_as_float(u[q] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const float4 f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i)[q];
+        v[4 * q] = f.x, v[4 * q + 1] = f.y, v[4 * q + 2] = f.z, v[4 * q + 3] = f.w;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? ld<DT>(p, i + e) : 0.0f;
+  }
+}
+
+// A matrix of R rows and C values per row into its parts, rows of Cp values.
+template <int DT>
+__global__ __launch_bounds__(256) void lay_out_kernel(const void* src, int64_t ld, int64_t R, int64_t C, int64_t Cp, int vec, uint16_t* dst) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, units = Cp / 8;
+  if (i >= R * units) return;
+  const int64_t r = i / units, c = i % units * 8;
+  float v[8];
+  load_eight<DT>(src, r * ld + c, static_cast<int>(C - c < 8 ? C - c : 8), vec != 0, v);
+  store_parts<DT == kBF16 ? 1 : 3>(dst + r * Cp + c, R * Cp, v);
+}
+
+// ---------------------------------------------------------------------------
+// few rows: the weights are read once, straight into the matrix unit's operands
+// ---------------------------------------------------------------------------
+// A workgroup owns 16 columns; its 8 waves share the contraction (chunks of 32 values, float32 of 16, taken in turn) and add
+// their sums through LDS in order.  Lane l holds 16 bytes of weight row l % 16 and of x row l % 16.  Bound by the weights' bytes, and
+// for small ones by latency.
+constexpr int kSkinnyWaves = 8;
+
+template <int DT>
+__device__ __forceinline__ any16 chunk_at(const void* p, int64_t row, int64_t ld, int64_t k, int64_t K) {
+  constexpr int EV = DT == kBF16 ? 8 : 4;
+  const char* q = static_cast<const char*>(p) + (row * ld + k) * (16 / EV);
+  if (k + EV <= K) return *reinterpret_cast<const any16*>(q);
+  any16 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < EV; ++e)
+    if (k + e < K) {
+      if constexpr (DT == kBF16)
+        v[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(q)[e]) << 16 * (e & 1);
+      else
+        v[e] = reinterpret_cast<const uint32_t*>(q)[e];
+    }
+  return v;
+}
+template <int DT>
+__device__ __forceinline__ f32x4 chunk_mma(const any16& w, const any16& x, f32x4 c) {
+  if constexpr (DT == kBF16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, make_uint4(w[0], w[1], w[2], w[3])),
+                                                   __builtin_bit_cast(b16x8, make_uint4(x[0], x[1], x[2], x[3])), c, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[j]), __uint_as_float(x[j]), c, 0, 0, 0);
+    return c;
+  }
+}
+
+template <int KIND, int DT, int MT>
+__global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_product_kernel(DenseArgs d, ProductArgs a) {
+  constexpr int NP = KIND == kProdGated ? 2 : 1, EV = DT == kBF16 ? 8 : 4, CK = 4 * EV, U = 4;
+  __shared__ float sums[kSkinnyWaves][NP][MT][16][17];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16, n = n0 + r < d.N ? n0 + r : d.N - 1;
+  int64_t m[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) m[i] = i * 16 + r < d.M ? i * 16 + r : d.M - 1;
+  f32x4 acc[NP][MT];
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[p][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int64_t chunks = (d.K + CK - 1) / CK;
+  for (int64_t c0 = wave; c0 < chunks; c0 += kSkinnyWaves * U) {
+    any16 w[U][NP], x[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // (chunks behind the end are zeros)
+      const int64_t k = (c0 + u * kSkinnyWaves) * CK + g * EV;
+      w[u][0] = chunk_at<DT>(d.w, n, d.ld_w, k, d.K);
+      if constexpr (NP == 2) w[u][1] = chunk_at<DT>(d.w2, n, d.ld_w2, k, d.K);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) x[u][i] = chunk_at<DT>(d.x, m[i], d.ld_x, k, d.K);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[p][i] = chunk_mma<DT>(w[u][p], x[u][i], acc[p][i]);
+  }
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sums[wave][p][i][4 * g + e][r] = acc[p][i][e];
+  __syncthreads();
+  const int col = threadIdx.x & 15, row = threadIdx.x >> 4;  // 32 rows of 16 columns
+  if (row >= 16 * MT || row >= d.M || n0 + col >= d.N) return;
+  float v[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int q = 0; q < kSkinnyWaves; ++q) v[p] += sums[q][p][row >> 4][col][row & 15];
+  store_one<KIND, DT>(a, a.out, row, n0 + col, v[0], v[1]);
+}
+
+// ---------------------------------------------------------------------------
+// in front of the backward products
+// ---------------------------------------------------------------------------
+// dg = dh u act'(g) and du = dh act(g) beside each other in rows of 2 Np values.
+template <int DT>
+__global__ __launch_bounds__(256) void gated_grad_kernel(const void* grad, int64_t ld_g, const void* z, const void* z2, int64_t M, int64_t N,
+                                                         int64_t Np, int act, int vec, uint16_t* dst) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, units = Np / 8;
+  if (i >= M * units) return;
+  const int64_t m = i / units, c = i % units * 8;
+  const int n = static_cast<int>(N - c < 8 ? N - c : 8);
+  float d[8], g[8], u[8];
+  load_eight<DT>(grad, m * ld_g + c, n, vec != 0, d);
+  load_eight<DT>(z, m * N + c, n, vec != 0, g);
+  load_eight<DT>(z2, m * N + c, n, vec != 0, u);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float v, s;
+    act_both(g[e], act, v, s);
+    g[e] = e < n ? d[e] * u[e] * s : 0.0f;
+    u[e] = e < n ? d[e] * v : 0.0f;
+  }
+  constexpr int P = DT == kBF16 ? 1 : 3;
+  store_parts<P>(dst + m * 2 * Np + c, M * 2 * Np, g);
+  store_parts<P>(dst + m * 2 * Np + Np + c, M * 2 * Np, u);
+}
+
+constexpr int kSumRows = 64;  // rows per workgroup
+// dz = dy act'(z) into its parts (dst), and the sums of kSumRows rows of it (sums); either may be left out.
+template <int DT>
+__global__ __launch_bounds__(256) void linear_grad_kernel(const void* grad, int64_t ld_g, const void* z, int64_t M, int64_t N, int64_t Np,
+                                                          int act, int vec, uint16_t* dst, float* sums) {
+  __shared__ float part[8][32][9];
+  const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
+  const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + cx) * 8, m0 = static_cast<int64_t>(blockIdx.y) * kSumRows;
+  float s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[e] = 0.0f;
+  if (c < Np) {
+    const int n = static_cast<int>(N - c < 8 ? N - c : 8);
+    const int64_t end = m0 + kSumRows < M ? m0 + kSumRows : M;
+#pragma unroll 4
+    for (int64_t m = m0 + ry; m < end; m += 8) {
+      float d[8];
+      load_eight<DT>(grad, m * ld_g + c, n, vec != 0, d);
+      if (act != kActNone) {
+        float v[8];
+        load_eight<DT>(z, m * N + c, n, vec != 0, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float a, b;
+          act_both(v[e], act, a, b);
+          d[e] = e < n ? d[e] * b : 0.0f;
+        }
+      }
+      if (dst) store_parts<DT == kBF16 ? 1 : 3>(dst + m * Np + c, M * Np, d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += d[e];
+    }
+  }
+  if (!sums) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) part[ry][cx][e] = s[e];
+  __syncthreads();
+  const int col = threadIdx.x;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + col;
+  if (at >= N) return;
+  float x = 0.0f;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) x += part[q][col >> 3][col & 7];
+  sums[blockIdx.y * N + at] = x;
+}
+// The sums of all workgroups' rows: 16 runs of them side by side, joined in order.
+template <int DT>
+__global__ __launch_bounds__(1024) void column_sum_kernel(const float* sums, int64_t count, int64_t N, void* out) {
+  __shared__ float part[16][64];
+  const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  float x = 0.0f;
+  if (n < N) {
+    const int64_t each = (count + 15) / 16, lo = run * each, hi = lo + each < count ? lo + each : count;
+#pragma unroll 8
+    for (int64_t s = lo; s < hi; ++s) x += sums[s * N + n];
+  }
+  part[run][lane] = x;
+  __syncthreads();
+  if (run == 0 && n < N) {
+    for (int q = 1; q < 16; ++q) x += part[q][lane];
+    st<DT>(out, n, x);
+  }
+}
+
+// The runs of a split contraction added in order.
+template <int DT>
+__global__ __launch_bounds__(256) void join_splits_kernel(const float* part, int splits, int64_t M, int64_t N, int64_t cut, int64_t fold,
+                                                          void* out, void* out2) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, all = M * N;
+  if (i >= all) return;
+  float x = 0.0f;
+  for (int s = 0; s < splits; ++s) x += part[s * all + i];
+  if (!out2 || i < cut * N)
+    st<DT>(out, i, x);
+  else if (i >= fold * N)
+    st<DT>(out2, i - fold * N, x);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+struct Space {  // a workspace handed out in pieces (base null: only measured)
+  char* base = nullptr;
+  int64_t used = 0;
+  template <typename T>
+  T* take(int64_t count) {
+    T* p = reinterpret_cast<T*>(base + used);
+    used += round_up(std::max<int64_t>(count, 1) * static_cast<int64_t>(sizeof(T)), 256);
+    return base ? p : nullptr;
+  }
+};
+
+struct Matrix {
+  const uint16_t* p = nullptr;
+  int64_t part = 0;  // values from part to part
+  int64_t ld = 0, ext = 0;
+};
+bool lies_ready(int dt, const void* p, int64_t ld, int64_t C) { return dt == kBF16 && aligned(p, 16) && ld % 8 == 0 && C % 8 == 0; }
+
+// The matrix as the product reads it, laid out in `s` unless `ready`.
+int bring(Space& s, bool run, int dt, const void* p, int64_t ld, int64_t R, int64_t C, bool ready, hipStream_t st, Matrix& out) {
+  if (ready) {
+    out = {static_cast<const uint16_t*>(p), 0, ld, C};
+    return kOk;
+  }
+  const int64_t Cp = up8(C);
+  uint16_t* dst = s.take<uint16_t>(R * Cp * (dt == kBF16 ? 1 : 3));
+  out = {dst, R * Cp, Cp, Cp};
+  const int64_t threads = R * Cp / 8;
+  if (!run || threads == 0) return kOk;
+  TESM_REQUIRE(threads < (1LL << 38), kErrUnsupported, "dense product: operand too large");
+  const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
+  const int vec = aligned(p, 16) && (ld * size_of_dt(dt)) % 16 == 0;
+  if (dt == kBF16)
+    lay_out_kernel<kBF16><<<blocks, 256, 0, TESM_LOGGED(st, lay_out_kernel<kBF16>)>>>(p, ld, R, C, Cp, vec, dst);
+  else
+    lay_out_kernel<kF32><<<blocks, 256, 0, TESM_LOGGED(st, lay_out_kernel<kF32>)>>>(p, ld, R, C, Cp, vec, dst);
+  return kOk;
+}
+
+// The pairs of parts that count, smallest products first.
+constexpr int kOrder[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
+void add_pairs(ProductArgs& a, int dt, const Matrix& A, int64_t a_off, const Matrix& B, const Matrix* B2) {
+  const int n = dt == kBF16 ? 1 : 6;
+  for (int i = 0; i < n; ++i) {
+    const int pa = dt == kBF16 ? 0 : kOrder[i][0], pb = dt == kBF16 ? 0 : kOrder[i][1];
+    a.A[a.pairs] = A.p + a_off + pa * A.part;
+    a.B[a.pairs] = B.p + pb * B.part;
+    a.B2[a.pairs] = B2 ? B2->p + pb * B2->part : nullptr;
+    ++a.pairs;
+  }
+}
+
+int dense_check(const DenseArgs& a, const char* who) {
+  const std::string w = std::string(who) + ": ";
+  TESM_REQUIRE(a.dt == kF32 || a.dt == kBF16, kErrInvalidArg, w + "dtype must be 0 or 1");
+  TESM_REQUIRE(a.act >= kActNone && a.act <= kActGelu, kErrInvalidArg, w + "no such activation");
+  TESM_REQUIRE(a.M >= 0 && a.N >= 0 && a.K >= 1 && a.M < (1LL << 31) && a.N < (1LL << 24) && a.K < (1LL << 24), kErrInvalidArg,
+               w + "bad sizes");
+  return kOk;
+}
+
+ProductArgs epilogue_of(const DenseArgs& d) {
+  ProductArgs a;
+  a.M = d.M, a.N = d.N, a.K = d.K;
+  a.act = d.act;
+  a.bias = d.bias;
+  a.residual = d.residual, a.ld_r = d.ld_r;
+  a.out = d.y, a.ldo = d.ld_y;
+  a.z = d.z, a.z2 = d.z2;
+  const int64_t e = size_of_dt(d.dt);
+  auto whole = [&](const void* p, int64_t ld) { return !p || (aligned(p, 16) && ld * e % 16 == 0); };
+  a.vec = d.N % 8 == 0 && whole(d.y, d.ld_y) && whole(d.residual, d.ld_r) && whole(d.bias, 0) && whole(d.z, d.N) && whole(d.z2, d.N);
+  return a;
+}
+
+template <int KIND>
+int run_skinny(const DenseArgs& d, hipStream_t st) {
+  const ProductArgs a = epilogue_of(d);
+  const unsigned blocks = static_cast<unsigned>((d.N + 15) / 16);
+  constexpr int T = 64 * kSkinnyWaves;
+#define TESM_SKINNY(DT, MT) skinny_product_kernel<KIND, DT, MT><<<blocks, T, 0, TESM_LOGGED(st, skinny_product_kernel<KIND, DT, MT>)>>>(d, a)
+  if (d.dt == kBF16) {
+    if (d.M <= 16)
+      TESM_SKINNY(kBF16, 1);
+    else
+      TESM_SKINNY(kBF16, 2);
+  } else {
+    if (d.M <= 16)
+      TESM_SKINNY(kF32, 1);
+    else
+      TESM_SKINNY(kF32, 2);
+  }
+#undef TESM_SKINNY
+  return check_launch("dense product of few rows");
+}
+
+int forward(const DenseArgs& d, Space s, bool run, int64_t* need, hipStream_t st) {
+  if (d.M <= kSkinnyRows) {
+    if (need) *need = 0;
+    if (!run || d.M == 0 || d.N == 0) return kOk;
+    return d.w2 ? run_skinny<kProdGated>(d, st) : run_skinny<kProdLinear>(d, st);
+  }
+  Matrix x, w, w2;
+  const bool ready = lies_ready(d.dt, d.w, d.ld_w, d.K) && (!d.w2 || (lies_ready(d.dt, d.w2, d.ld_w2, d.K) && d.ld_w == d.ld_w2));
+  if (int rc = bring(s, run, d.dt, d.x, d.ld_x, d.M, d.K, lies_ready(d.dt, d.x, d.ld_x, d.K), st, x)) return rc;
+  if (int rc = bring(s, run, d.dt, d.w, d.ld_w, d.N, d.K, ready, st, w)) return rc;
+  if (d.w2)
+    if (int rc = bring(s, run, d.dt, d.w2, d.ld_w2, d.N, d.K, ready, st, w2)) return rc;
+  if (need) *need = s.used;
+  if (!run || d.N == 0) return kOk;
+  ProductArgs a = epilogue_of(d);
+  a.pairs = 0;
+  add_pairs(a, d.dt, x, 0, w, d.w2 ? &w2 : nullptr);
+  a.lda = x.ld, a.ldb = w.ld;
+  return launch_product(d.w2 ? kProdGated : kProdLinear, d.dt, false, false, a, st);
+}
+
+// A product whose results are gradients, its contraction split where there are few tiles.
+int grad_product(Space& s, bool run, int dt, bool adown, ProductArgs a, hipStream_t st) {
+  a.splits = a.K ? product_splits(a.M, a.N, a.K, a.pairs) : 0;  // (nothing to add up: zeros)
+  const int64_t e = size_of_dt(dt);
+  if (a.splits == 1) {
+    a.ldo = a.N;
+    a.vec = a.N * e % 16 == 0 && a.N % 8 == 0 && aligned(a.out, 16) && (!a.out2 || aligned(a.out2, 16));
+    return run ? launch_product(kProdStore, dt, adown, true, a, st) : kOk;
+  }
+  float* part = s.take<float>(a.splits * a.M * a.N);
+  if (!run) return kOk;
+  ProductArgs b = a;
+  b.out = part, b.out2 = nullptr;
+  b.ldo = a.N;
+  b.vec = a.N % 8 == 0;
+  if (a.splits)
+    if (int rc = launch_product(kProdPartial, kF32, adown, true, b, st)) return rc;
+  const unsigned blocks = static_cast<unsigned>((a.M * a.N + 255) / 256);
+  if (dt == kBF16)
+    join_splits_kernel<kBF16><<<blocks, 256, 0, TESM_LOGGED(st, join_splits_kernel<kBF16>)>>>(part, a.splits, a.M, a.N, a.cut, a.fold, a.out, a.out2);
+  else
+    join_splits_kernel<kF32><<<blocks, 256, 0, TESM_LOGGED(st, join_splits_kernel<kF32>)>>>(part, a.splits, a.M, a.N, a.cut, a.fold, a.out, a.out2);
+  return check_launch("dense product, joined");
+}
+
+
+int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_t st) {
+  const DenseArgs& d = b.in;
+  const int dt = d.dt;
+  const int64_t M = d.M, N = d.N, K = d.K, Np = up8(N), e = size_of_dt(dt);
+  const bool gated = d.w2 != nullptr, products = b.dx || b.dw || b.dw2;
+  Matrix dz;
+  const bool grad_whole = aligned(b.grad, 16) && b.ld_g * e % 16 == 0;
+  const int vec = grad_whole && (!d.z || (aligned(d.z, 16) && N * e % 16 == 0)) && (!d.z2 || aligned(d.z2, 16));
+  if (gated) {
+    uint16_t* dst = s.take<uint16_t>(M * 2 * Np * (dt == kBF16 ? 1 : 3));
+    dz = {dst, M * 2 * Np, 2 * Np, 2 * Np};
+    const int64_t threads = M * Np / 8;
+    if (run && threads && products) {
+      TESM_REQUIRE(threads < (1LL << 38), kErrUnsupported, "dense backward: too large");
+      const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
+      if (dt == kBF16)
+        gated_grad_kernel<kBF16><<<blocks, 256, 0, TESM_LOGGED(st, gated_grad_kernel<kBF16>)>>>(b.grad, b.ld_g, d.z, d.z2, M, N, Np, d.act, vec, dst);
+      else
+        gated_grad_kernel<kF32><<<blocks, 256, 0, TESM_LOGGED(st, gated_grad_kernel<kF32>)>>>(b.grad, b.ld_g, d.z, d.z2, M, N, Np, d.act, vec, dst);
+    }
+  } else {
+    const bool direct = d.act == kActNone && lies_ready(dt, b.grad, b.ld_g, N);
+    uint16_t* dst = nullptr;
+    if (direct)
+      dz = {static_cast<const uint16_t*>(b.grad), 0, b.ld_g, N};
+    else {
+      dst = s.take<uint16_t>(M * Np * (dt == kBF16 ? 1 : 3));
+      dz = {dst, M * Np, Np, Np};
+    }
+    const int64_t rows = (M + kSumRows - 1) / kSumRows;
+    float* sums = b.dbias ? s.take<float>(rows * N) : nullptr;
+    if (run && M && N && (sums || (dst && products))) {
+      TESM_REQUIRE(rows < 65536, kErrUnsupported, "dense backward: too many rows");
+      const dim3 grid(static_cast<unsigned>((Np + 255) / 256), static_cast<unsigned>(rows));
+      if (dt == kBF16)
+        linear_grad_kernel<kBF16><<<grid, 256, 0, TESM_LOGGED(st, linear_grad_kernel<kBF16>)>>>(b.grad, b.ld_g, d.z, M, N, Np, d.act, vec, dst, sums);
+      else
+        linear_grad_kernel<kF32><<<grid, 256, 0, TESM_LOGGED(st, linear_grad_kernel<kF32>)>>>(b.grad, b.ld_g, d.z, M, N, Np, d.act, vec, dst, sums);
+    }
+    if (run && b.dbias && N) {
+      const unsigned blocks = static_cast<unsigned>((N + 63) / 64);
+      if (dt == kBF16)
+        column_sum_kernel<kBF16><<<blocks, 1024, 0, TESM_LOGGED(st, column_sum_kernel<kBF16>)>>>(sums, M ? rows : 0, N, b.dbias);
+      else
+        column_sum_kernel<kF32><<<blocks, 1024, 0, TESM_LOGGED(st, column_sum_kernel<kF32>)>>>(sums, M ? rows : 0, N, b.dbias);
+    }
+  }
+  if (b.dx && M) {
+    Matrix w, w2;
+    const bool ready = lies_ready(dt, d.w, d.ld_w, K) && (!gated || (lies_ready(dt, d.w2, d.ld_w2, K) && d.ld_w == d.ld_w2));
+    if (int rc = bring(s, run, dt, d.w, d.ld_w, N, K, ready, st, w)) return rc;
+    if (gated)
+      if (int rc = bring(s, run, dt, d.w2, d.ld_w2, N, K, ready, st, w2)) return rc;
+    ProductArgs a;
+    a.M = M, a.N = K, a.K = N;
+    a.pairs = 0;
+    add_pairs(a, dt, dz, 0, w, nullptr);
+    if (gated) add_pairs(a, dt, dz, Np, w2, nullptr);
+    a.lda = dz.ld, a.ldb = w.ld, a.ext_b = w.ext;
+    a.out = b.dx;
+    if (int rc = grad_product(s, run, dt, false, a, st)) return rc;
+  }
+  if ((b.dw || b.dw2) && N) {
+    Matrix x;
+    if (int rc = bring(s, run, dt, d.x, d.ld_x, M, K, lies_ready(dt, d.x, d.ld_x, K), st, x)) return rc;
+    ProductArgs a;
+    a.M = gated ? Np + N : N, a.N = K, a.K = M;
+    a.pairs = 0;
+    add_pairs(a, dt, dz, 0, x, nullptr);
+    a.lda = dz.ld, a.ext_a = dz.ext, a.ldb = x.ld, a.ext_b = x.ext;
+    a.out = b.dw, a.out2 = b.dw2;
+    a.cut = N, a.fold = Np;
+    if (int rc = grad_product(s, run, dt, true, a, st)) return rc;
+  }
+  if (need) *need = s.used;
+  return run ? check_launch("dense backward") : kOk;
+}
+
+}  // namespace
+
+int64_t dense_ws_bytes(const DenseArgs& a) {
+  int64_t need = 0;
+  if (dense_check(a, "dense product") != kOk || forward(a, Space{}, false, &need, nullptr) != kOk) return -1;
+  return need;
+}
+int64_t dense_bwd_ws_bytes(const DenseBwdArgs& b) {
+  int64_t need = 0;
+  if (dense_check(b.in, "dense backward") != kOk || backward(b, Space{}, false, &need, nullptr) != kOk) return -1;
+  return need;
+}
+
+int launch_dense(const DenseArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
+  const char* who = a.w2 ? "gated linear" : "fused linear";
+  const std::string w = std::string(who) + ": ";
+  if (int rc = dense_check(a, who)) return rc;
+  if (a.M == 0 || a.N == 0) return kOk;
+  TESM_REQUIRE(a.x && a.w && a.y, kErrInvalidArg, w + "need x, the weights and the output");
+  TESM_REQUIRE(a.ld_x >= a.K && a.ld_w >= a.K && (!a.w2 || a.ld_w2 >= a.K) && a.ld_y >= a.N && (!a.residual || a.ld_r >= a.N),
+               kErrInvalidArg, w + "a row pitch below the row's values");
+  TESM_REQUIRE(!a.w2 || (a.act != kActNone && (a.z != nullptr) == (a.z2 != nullptr)), kErrInvalidArg,
+               w + "need an activation, and both kept products or none");
+  const int64_t need = dense_ws_bytes(a);
+  TESM_REQUIRE(need == 0 || (ws && ws_bytes >= need && aligned(ws, 16)), kErrWorkspace, w + "workspace too small or not 16-byte aligned");
+  return forward(a, Space{static_cast<char*>(ws), 0}, true, nullptr, st);
+}
+
+int launch_dense_bwd(const DenseBwdArgs& b, void* ws, int64_t ws_bytes, hipStream_t st) {
+  const DenseArgs& a = b.in;
+  const char* who = a.w2 ? "gated linear backward" : "fused linear backward";
+  const std::string w = std::string(who) + ": ";
+  if (int rc = dense_check(a, who)) return rc;
+  TESM_REQUIRE(a.M == 0 || a.N == 0 || (b.grad && b.ld_g >= a.N), kErrInvalidArg, w + "need the gradient");
+  TESM_REQUIRE(a.M == 0 || a.N == 0 || ((!b.dx || (a.w && a.ld_w >= a.K && (!a.w2 || a.ld_w2 >= a.K))) &&
+                                        (!(b.dw || b.dw2) || (a.x && a.ld_x >= a.K))),
+               kErrInvalidArg, w + "need the operands that the gradients asked for are made of");
+  TESM_REQUIRE(!a.w2 || (b.dw != nullptr) == (b.dw2 != nullptr), kErrInvalidArg, w + "both weights' gradients or none");
+  TESM_REQUIRE(a.M == 0 || a.N == 0 || a.act == kActNone || (a.z && (!a.w2 || a.z2)), kErrInvalidArg,
+               w + "need what the forward call kept");
+  const int64_t need = dense_bwd_ws_bytes(b);
+  TESM_REQUIRE(need == 0 || (ws && ws_bytes >= need && aligned(ws, 16)), kErrWorkspace, w + "workspace too small or not 16-byte aligned");
+  return backward(b, Space{static_cast<char*>(ws), 0}, true, nullptr, st);
+}
+
+}  // namespace tesm

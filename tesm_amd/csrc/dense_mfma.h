@@ -1,0 +1,87 @@
+// The matrix product that the dense operators share: bfloat16 operands, float32 sums on v_mfma_f32_32x32x16_bf16.
+#pragma once
+
+#include "dense.h"
+#include "linear_dev.h"
+
+namespace tesm {
+
+constexpr int kMaxParts = 12;
+
+// out[m, n] = sum over pairs p and k of A_p[m, k] B_p[n, k].  An operand lies with k along its rows (m or n picks the row), or, where
+// its layout is "down", with k picking the row.  All pairs share extents and pitches.  Rows start on 16 bytes; the contiguous
+// extent is a multiple of 8.
+struct ProductArgs {
+  int64_t M = 0, N = 0, K = 0;
+  int pairs = 1;
+  const uint16_t* A[kMaxParts] = {};
+  const uint16_t* B[kMaxParts] = {};
+  const uint16_t* B2[kMaxParts] = {};  // the second weight of a gated pair
+  int64_t lda = 0, ldb = 0;
+  int64_t ext_a = 0, ext_b = 0;  // values per row of an operand that lies down, a multiple of 8 (not below M, N)
+  int splits = 1;  // the contraction in this many runs of steps, each to its own float32 result at out + split * M * N
+  // epilogue
+  int act = kActNone;
+  const void* bias = nullptr;
+  const void* residual = nullptr;
+  int64_t ld_r = 0;
+  void* out = nullptr;
+  int64_t ldo = 0;
+  void* out2 = nullptr;   // rows from `fold` on go to out2, counted from `fold`; rows in [cut, fold) nowhere
+  int64_t cut = 0, fold = 0;
+  void* z = nullptr;
+  void* z2 = nullptr;
+  int vec = 0;  // every array of the epilogue takes 16-byte accesses at columns that are multiples of 8
+};
+
+enum ProductKind : int { kProdGated = 0, kProdLinear = 1, kProdStore = 2, kProdPartial = 3 };
+enum ProductLayout : int { kAlong = 0, kDown = 1 };
+
+// dt: type of the results (kProdPartial: float32).  adown, bdown: operand layouts.
+int launch_product(ProductKind kind, int dt, bool adown, bool bdown, ProductArgs a, hipStream_t st);
+// How many runs the contraction of such a product should be split into (1: none).
+int product_splits(int64_t M, int64_t N, int64_t K, int pairs);
+
+__device__ __forceinline__ float act_silu(float z) { return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f)); }
+__device__ __forceinline__ float act_value(float z, int act) {
+  if (act == kActSilu) return act_silu(z);
+  if (act == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752440f));
+  return z;
+}
+// act(z) and act'(z)
+__device__ __forceinline__ void act_both(float z, int act, float& v, float& d) {
+  if (act == kActSilu) {
+    const float p = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f));
+    v = z * p;
+    d = __builtin_fmaf(v, 1.0f - p, p);
+  } else if (act == kActGelu) {
+    const float p = 0.5f * (1.0f + erff(z * 0.70710678118654752440f));
+    v = z * p;
+    d = __builtin_fmaf(z * 0.39894228040143267794f, __builtin_amdgcn_exp2f(z * z * -0.72134752044448170368f), p);
+  } else {
+    v = z;
+    d = 1.0f;
+  }
+}
+
+// One value (two products v, v2 of a gated pair) to its places.
+template <int KIND, int DT>
+__device__ __forceinline__ void store_one(const ProductArgs& a, void* out, int64_t m, int64_t n, float v, float v2) {
+  if constexpr (KIND == kProdGated) {
+    if (a.z) {
+      st<DT>(a.z, m * a.N + n, v);
+      st<DT>(a.z2, m * a.N + n, v2);
+    }
+    st<DT>(out, m * a.ldo + n, act_value(v, a.act) * v2);
+  } else if constexpr (KIND == kProdLinear) {
+    if (a.bias) v += ld<DT>(a.bias, n);
+    if (a.z) st<DT>(a.z, m * a.N + n, v);
+    v = act_value(v, a.act);
+    if (a.residual) v += ld<DT>(a.residual, m * a.ld_r + n);
+    st<DT>(out, m * a.ldo + n, v);
+  } else {
+    st<DT>(out, m * a.ldo + n, v);
+  }
+}
+
+}  // namespace tesm

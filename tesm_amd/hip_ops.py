@@ -781,3 +781,10 @@ def reorder_rows(tensors, parents: torch.Tensor) -> None:
     table = array.array("q", table)
     on_device(dev.index, _lib.load().tesm_hip_reorder_rows, table.buffer_info()[0], count, parents.data_ptr(), B, K,
               raw_stream(dev.index))
+
+
+# ---------------------------------------------------------------------------
+# operators that learn (they need the helpers above)
+# ---------------------------------------------------------------------------
+from .learn_ops import (fused_linear, fused_linear_backward, gated_linear, gated_linear_backward, gated_scan,  # noqa: E402,F401
+                        gated_scan_backward, gated_scan_step, token_log_probs, token_log_probs_backward)

@@ -337,6 +337,18 @@ class TESMLMHeadModel(nn.Module):
             n += 1
         return chosen[:, :n].view(B, num_beams, n), scores
 
+    @torch.no_grad()
+    def score(self, input_ids: torch.Tensor, top: int = 0):
+        """How likely the model finds the tokens of ``input_ids`` (B, L) one after the other: ``(log_probs (B, L - 1), entropy
+        (B, L - 1), top_log_probs, top_tokens (B, L - 1, top))`` of token t + 1 after the first t + 1, as
+        ``hip_ops.token_log_probs`` gives them; the configuration's ``label_ignore_index`` marks tokens that are not scored."""
+        ignore = self.tesm_config.label_ignore_index
+        logits = self(input_ids.clamp(min=0))[0].logits
+        # (the last row has no target; leaving it out of the logits would copy them)
+        targets = torch.nn.functional.pad(input_ids[:, 1:], (0, 1), value=ignore)
+        out = hip_ops.token_log_probs(logits, targets, top=top, ignore_index=ignore)
+        return tuple(t[:, :-1] if t is not None else None for t in out)
+
     def forward(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None,
                 inference_params: Optional[dict] = None, prev_states=None, logits_to_keep: int = 0,
                 sparse_logits: bool = False, **kwargs):
