@@ -42,10 +42,25 @@ int launch_product(ProductKind kind, int dt, bool adown, bool bdown, ProductArgs
 // How many runs the contraction of such a product should be split into (1: none).
 int product_splits(int64_t M, int64_t N, int64_t K, int pairs);
 
-__device__ __forceinline__ float act_silu(float z) { return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f)); }
+// The normal distribution's Phi(z) = (1 + erf(z / sqrt 2)) / 2 and e = exp(-z^2 / 2), with erfc(x) = P(t) exp(-x^2), t = 1 / (1 + p x),
+// the polynomial of Abramowitz and Stegun 7.1.26 (1.5e-7 off at most).  The library's erff takes three times as long: 8192 x 16384
+// results of K = 4096 1101 us with it.
+__device__ __forceinline__ float normal_phi(float z, float& e) {
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(z), 0.3275911f * 0.70710678118654752440f, 1.0f));
+  float p = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
+  p = __builtin_fmaf(t, p, 1.421413741f);
+  p = __builtin_fmaf(t, p, -0.284496736f);
+  p = __builtin_fmaf(t, p, 0.254829592f);
+  e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170368f);
+  const float tail = 0.5f * p * t * e;
+  return z < 0.0f ? tail : 1.0f - tail;
+}
 __device__ __forceinline__ float act_value(float z, int act) {
-  if (act == kActSilu) return act_silu(z);
-  if (act == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752440f));
+  if (act == kActSilu) return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f));
+  if (act == kActGelu) {
+    float e;
+    return z * normal_phi(z, e);
+  }
   return z;
 }
 // act(z) and act'(z)
@@ -55,9 +70,10 @@ __device__ __forceinline__ void act_both(float z, int act, float& v, float& d) {
     v = z * p;
     d = __builtin_fmaf(v, 1.0f - p, p);
   } else if (act == kActGelu) {
-    const float p = 0.5f * (1.0f + erff(z * 0.70710678118654752440f));
+    float e;
+    const float p = normal_phi(z, e);
     v = z * p;
-    d = __builtin_fmaf(z * 0.39894228040143267794f, __builtin_amdgcn_exp2f(z * z * -0.72134752044448170368f), p);
+    d = __builtin_fmaf(z * 0.39894228040143267794f, e, p);
   } else {
     v = z;
     d = 1.0f;

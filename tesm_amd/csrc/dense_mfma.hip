@@ -1,9 +1,11 @@
 // Products of bfloat16 matrices for the dense operators.
 //
 // A workgroup owns BM x BN results: WM x WN waves of TM x TN tiles of 32 x 32, with a gated pair two accumulators per tile and
-// two weight tiles.  Weights are the MFMA's first operand, so that a lane holds 4 consecutive columns of one row.  Operand tiles of BK values of k go
-// straight from memory to LDS in NS stages; a fragment's LDS reads are issued one k-step ahead of its MFMAs; one barrier per
-// tile, before its last k-step but one, where the next tile has landed and the previous one's stage is refilled.
+// two weight tiles.  Weights are the MFMA's first operand, so that a lane holds 4 consecutive columns of one row.  Operand tiles of
+// BK values of k go straight from memory to LDS in NS stages.  A fragment's LDS reads are issued one k-step ahead of its MFMAs, one
+// after each MFMA, and so are the loads of a later tile in a tile's last k-step: issued together behind the barrier, they held
+// up all waves at once (8192 x 16384 x 4096 1097 us, one after each MFMA 1040).  One barrier per tile, before its last k-step, where the
+// next tile has landed.
 //
 // A tile with k along its rows has rows of BK values, 16-byte chunk q of row r at q ^ (r / (16 / CPR)) % CPR (CPR chunks per
 // row): 16 rows' reads of one chunk fall on 256 different bytes.  A tile with k down its rows has BK rows of BM (BN) values; its
@@ -11,6 +13,11 @@
 // gets column i of the 4 rows), with the 64-byte block index of row k turned by k % 4 so that 4 rows fall on different banks.
 // What lies behind the end of the contraction is read as zeros (an offset beyond the buffer's range), what lies behind the last
 // row or column repeats the last one and is never stored.
+//
+// Bound by the matrix unit and the power it draws: counters over 8192 x 16384 x 4096 showed it busy in 60 % of the cycles of the first form,
+// LDS in 25 %, without bank conflicts, at clocks between 1.6 (all along) and 2.1 GHz.
+#include <type_traits>
+
 #include "dense_mfma.h"
 
 namespace tesm {
@@ -23,11 +30,16 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kRange = 0x80000000u;  // bytes from a tile's first value that a load can reach; offsets from here on give zeros
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, kRange, 0x00027000);
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x4 buffer_at(uint64_t p) {
+  return i32x4{static_cast<int>(p), static_cast<int>(p >> 32) & 0xffff, static_cast<int>(kRange), 0x00027000};
 }
-__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t buf, char* dst, uint32_t off) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (__attribute__((address_space(3))) void*)(dst), 16, off, 0, 0, 0);
+// 64 lanes x 16 bytes from the buffer's first value + `off` (each lane's own) to LDS in lane order.  In assembly, since the compiler
+// lets every transposing LDS read wait for all such loads, which would leave none of them ahead; the instruction writes no
+// register, and what waits for it is wait_vmcnt.  (Nothing else in this file uses m0, which the compiler sets anew where it does.)
+__device__ __forceinline__ void to_lds(i32x4 buf, char* dst, uint32_t off) {
+  const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(dst)));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(buf));
 }
 
 template <int KIND, int WM_, int WN_, int TM_, int TN_, int BK_, int NS_>
@@ -42,7 +54,11 @@ struct Shape {
   static constexpr int STEPS = BK / 16;
   static constexpr int PITCH = TN * 32 * 4 + 16, SLAB = NP * 32 * PITCH;
   static constexpr int SMEM = NS * STAGE > NW * SLAB ? NS * STAGE : NW * SLAB;
-  static_assert(NS >= 3 && STEPS >= 2 && SMEM <= 160 * 1024, "stages");
+  static_assert(NS >= 2 && STEPS >= 2 && SMEM <= 160 * 1024, "stages");
+  // With two stages a tile's own stage is refilled before its last k-step, whose fragments are in registers by then; with more of
+  // them the previous tile's, so that no wave has to wait for its LDS reads in front of the barrier.
+  static constexpr bool OWN = NS == 2;
+  static constexpr int AHEAD = OWN ? 2 : NS - 1;  // tiles between the one in work and the one asked for
 };
 
 // Where lane `lane` of a 1 KB block reads: the offset from the tile's first value, and the value of k (within the tile).
@@ -82,16 +98,25 @@ struct Frag {
       turn = 0;
     }
   }
-  __device__ __forceinline__ b16x8 read(const char* tile, int i, int s) const {
+  // What a read gives: put together where it is used, since a copy behind the read would wait for it.
+  struct Down {
+    s16x4 lo, hi;
+  };
+  using Value = std::conditional_t<DOWN, Down, b16x8>;
+  __device__ __forceinline__ Value read(const char* tile, int i, int s) const {
     if constexpr (!DOWN) {
       return *reinterpret_cast<const b16x8*>(tile + at[i] + ((turn ^ (2 * s)) * 16));
     } else {
       const char* p = tile + at[i] + s * 16 * BX * 2;
-      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
-      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * BX * 2));
-      typedef short s16x8 __attribute__((ext_vector_type(8)));
-      return __builtin_bit_cast(b16x8, s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+      return {__builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p)),
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * BX * 2))};
     }
+  }
+  static __device__ __forceinline__ b16x8 value(const Value& v) {
+    if constexpr (!DOWN)
+      return v;
+    else
+      return __builtin_bit_cast(b16x8, __builtin_shufflevector(v.lo, v.hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };
 
@@ -187,31 +212,42 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(ProductArgs a) {
     first = static_cast<int>(static_cast<int64_t>(all) * blockIdx.y / a.splits);
     steps = static_cast<int>(static_cast<int64_t>(all) * (blockIdx.y + 1) / a.splits) - first;
   }
+  // The next tile to ask for: its values' addresses, kept in scalar registers.  A new pair's addresses are waited for where they
+  // are read: left to the loop, that wait would hold up every tile's LDS reads (they share a counter).
   int pair = first / nk, kt = first % nk;
-  auto issue = [&](char* stage, bool live) {
-    const int64_t left = a.K - static_cast<int64_t>(kt) * BK;
-    const bool whole = left >= BK && live;
-    const int end = live ? static_cast<int>(left < BK ? left : BK) : 0;
-    const __amdgpu_buffer_rsrc_t ba = buffer_at(a.A[pair] + a_first + kt * a_step);
-    const __amdgpu_buffer_rsrc_t bb = buffer_at(a.B[pair] + b_first + kt * b_step);
-#pragma unroll
-    for (int i = 0; i < DA; ++i) to_lds(ba, stage + (wave + i * S::NW) * 1024, whole || k_a[i] < end ? off_a[i] : kRange);
-#pragma unroll
-    for (int i = 0; i < DB; ++i) to_lds(bb, stage + S::A_BYTES + (wave + i * S::NW) * 1024, whole || k_b[i] < end ? off_b[i] : kRange);
-    if constexpr (NP == 2) {
-      const __amdgpu_buffer_rsrc_t b2 = buffer_at(a.B2[pair] + b_first + kt * b_step);
-#pragma unroll
-      for (int i = 0; i < DB; ++i)
-        to_lds(b2, stage + S::A_BYTES + S::B_BYTES + (wave + i * S::NW) * 1024, whole || k_b[i] < end ? off_b[i] : kRange);
+  uint64_t at_a, at_b, at_b2 = 0;
+  auto begin = [&]() {
+    at_a = reinterpret_cast<uint64_t>(a.A[pair] + a_first + kt * a_step);
+    at_b = reinterpret_cast<uint64_t>(a.B[pair] + b_first + kt * b_step);
+    if constexpr (NP == 2) at_b2 = reinterpret_cast<uint64_t>(a.B2[pair] + b_first + kt * b_step);
+    asm volatile("" : "+s"(at_a), "+s"(at_b), "+s"(at_b2));
+  };
+  begin();
+  // Load number i of the D that the wave asks for per tile; the last one moves on to the next tile.
+  auto issue = [&](char* stage, bool live, int i) __attribute__((always_inline)) {
+    const int end = live ? static_cast<int>(a.K - static_cast<int64_t>(kt) * BK) : 0;  // values of k from here on are zeros
+    if (i < DA) {
+      to_lds(buffer_at(at_a), stage + (wave + i * S::NW) * 1024, k_a[i] < end ? off_a[i] : kRange);
+    } else {
+      const int p = (i - DA) / DB, j = (i - DA) % DB;
+      to_lds(buffer_at(p ? at_b2 : at_b), stage + S::A_BYTES + p * S::B_BYTES + (wave + j * S::NW) * 1024,
+             k_b[j] < end ? off_b[j] : kRange);
     }
+    if (i < S::D - 1) return;
+    at_a += a_step * 2;
+    at_b += b_step * 2;
+    if constexpr (NP == 2) at_b2 += b_step * 2;
     if (++kt == nk) {  // (behind the last pair the first one's values are never asked for: `live` is off)
       kt = 0;
       pair = pair + 1 < a.pairs ? pair + 1 : 0;
+      begin();
     }
   };
 
-  Frag<BK, S::BM, ADOWN, TM> fa;
-  Frag<BK, S::BN, BDOWN, TN> fb;
+  using FragA = Frag<BK, S::BM, ADOWN, TM>;
+  using FragB = Frag<BK, S::BN, BDOWN, TN>;
+  FragA fa;
+  FragB fb;
   fa.init(wm * TM * 32, lane);
   fb.init(wn * TN * 32, lane);
   f32x16 acc[NP][TM][TN];
@@ -221,49 +257,58 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(ProductArgs a) {
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) acc[p][i][j] = f32x16{};
-  b16x8 ra[2][TM], rb[2][NP][TN];
-  auto read = [&](const char* stage, int s, b16x8 (&x)[TM], b16x8 (&y)[NP][TN]) {
-#pragma unroll
-    for (int p = 0; p < NP; ++p)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) y[p][j] = fb.read(stage + S::A_BYTES + p * S::B_BYTES, j, s);
-#pragma unroll
-    for (int i = 0; i < TM; ++i) x[i] = fa.read(stage, i, s);
+  typename FragA::Value ra[2][TM];
+  typename FragB::Value rb[2][NP][TN];
+  constexpr int NR = NP * TN + TM, NM = NP * TN * TM;  // fragment reads and MFMAs per k-step
+  auto read = [&](const char* stage, int s, int r, typename FragA::Value (&x)[TM], typename FragB::Value (&y)[NP][TN]) __attribute__((always_inline)) {
+    if (r < NP * TN)
+      y[r / TN][r % TN] = fb.read(stage + S::A_BYTES + (r / TN) * S::B_BYTES, r % TN, s);
+    else
+      x[r - NP * TN] = fa.read(stage, r - NP * TN, s);
   };
-  auto mma = [&](const b16x8 (&x)[TM], const b16x8 (&y)[NP][TN]) {
+  auto mma = [&](int q, const typename FragA::Value (&x)[TM], const typename FragB::Value (&y)[NP][TN]) __attribute__((always_inline)) {
+    const int i = q % TM, j = q / TM % TN, p = q / (TM * TN);
+    acc[p][i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(FragB::value(y[p][j]), FragA::value(x[i]), acc[p][i][j], 0, 0, 0);
+  };
+  // k-step s of the tile in `cur`: between its MFMAs the next step's fragments are read and, in the last step, the tile NS - 1
+  // ahead is asked for, one instruction after each, so that neither the LDS nor the memory unit is asked for all at once.
+  auto step_of = [&](const char* cur, const char* next, char* refill, int s, bool live) __attribute__((always_inline)) {
+    const bool last = s == S::STEPS - 1;
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
+    for (int q = 0; q < NM; ++q) {
+      mma(q, ra[s & 1], rb[s & 1]);
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
+      for (int r = q * NR / NM; r < (q + 1) * NR / NM; ++r) read(last ? next : cur, last ? 0 : s + 1, r, ra[(s + 1) & 1], rb[(s + 1) & 1]);
+      if (last) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) acc[p][i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[p][j], x[i], acc[p][i][j], 0, 0, 0);
+        for (int i = q * S::D / NM; i < (q + 1) * S::D / NM; ++i) issue(refill, live, i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
 #pragma unroll
-  for (int s = 0; s < NS - 1; ++s) issue(smem + s * S::STAGE, s < steps);
-  wait_vmcnt<(NS - 2) * S::D>();
+  for (int s = 0; s < S::AHEAD; ++s)
+#pragma unroll
+    for (int i = 0; i < S::D; ++i) issue(smem + s * S::STAGE, s < steps, i);
+  wait_vmcnt<(S::AHEAD - 1) * S::D>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  read(smem, 0, ra[0], rb[0]);
+#pragma unroll
+  for (int r = 0; r < NR; ++r) read(smem, 0, r, ra[0], rb[0]);
   int st = 0;
   for (int step = 0; step < steps; ++step) {
     const char* cur = smem + st * S::STAGE;
     const int nx = st + 1 == NS ? 0 : st + 1, pv = st == 0 ? NS - 1 : st - 1;
 #pragma unroll
     for (int s = 0; s < S::STEPS; ++s) {
-      if (s == S::STEPS - 1)
-        read(smem + nx * S::STAGE, 0, ra[(s + 1) & 1], rb[(s + 1) & 1]);
-      else
-        read(cur, s + 1, ra[(s + 1) & 1], rb[(s + 1) & 1]);
-      if (s == S::STEPS - 2) {
-        wait_vmcnt<(NS - 3) * S::D>();  // this wave's part of the next tile has landed
+      if (s == S::STEPS - 1) {
+        wait_vmcnt<(S::AHEAD - 2) * S::D>();  // this wave's part of the next tile has landed
+        if (S::OWN) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();   // ... every wave's, and every wave is done with the tile before this one
         asm volatile("" ::: "memory");
-        issue(smem + pv * S::STAGE, step + NS - 1 < steps);
       }
-      __builtin_amdgcn_sched_barrier(0);
-      mma(ra[s & 1], rb[s & 1]);
-      __builtin_amdgcn_sched_barrier(0);
+      step_of(cur, smem + nx * S::STAGE, smem + (S::OWN ? st : pv) * S::STAGE, s, step + S::AHEAD < steps);
     }
     st = nx;
   }
@@ -357,28 +402,60 @@ int run_product(const ProductArgs& a, hipStream_t st) {
   return check_launch("dense product");
 }
 
+// Tile sizes.  Large: 256 x 256 results (a gated pair: 256 x 128 of each product) on 8 waves of 128 x 64, one workgroup per CU.
+// Mid: 128 x 128 (128 x 64) on 4 waves of 64 x 64, two workgroups per CU.  Small: the same tiles with four stages, one per CU, for
+// grids that have no second one anyway.  In us per round of the CUs, with k thousand values of the contraction: 25 k + 8, 15 k + 5 (9 k +
+// 5 where half the places stay empty) and 7.6 k + 4; a split adds the float32 results it writes and reads again.  Measured,
+// bfloat16: 8192 x 16384 x 4096 879 us large (1.25 Pflop/s; the library's product 1.29), mid 1075, small 1240; 8192 x 4096 x 768 58,
+// 69, 83; 8192 x 768 x 2048 47, 31, 39; 4096 x 768 x 8192 147, 77, 66.  Operands that lie down: 8192 x 16384 x 4096 864 us with one, 860
+// with both (the library 950 and 1080).  Tiles of 32 values of k instead of 64 cost 20 % where rows run along k (64-byte
+// pieces), stages of 128 x 256 with 8 waves of 64 x 64 another 10 %.
+enum Config : int { kLarge, kMid, kSmall };
+struct Plan {
+  Config config = kSmall;
+  int splits = 1;
+};
+Plan plan_product(ProductKind kind, int64_t M, int64_t N, int64_t K, int pairs, bool split) {
+  const int64_t cus = std::max(device_limits().cus, 1);
+  auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + (kind == kProdGated ? bn / 2 : bn) - 1) / (kind == kProdGated ? bn / 2 : bn)); };
+  const double k = static_cast<double>(K) * pairs / 1000.0;
+  Plan best;
+  double least = 1e30;
+  const int64_t steps = (K + 63) / 64 * pairs;
+  for (int s = 1; s <= (split ? 16 : 1) && (s == 1 || s * 4 <= steps); ++s) {
+    const double ks = k / s, joined = s == 1 ? 0.0 : 6.0 + 2.0 * s * 4.0 * static_cast<double>(M) * static_cast<double>(N) / 5.0e6;
+    const int64_t large = tiles(256, 256) * s, mid = tiles(128, 128) * s;
+    const int64_t rest = mid % (2 * cus);
+    const double cost[3] = {static_cast<double>((large + cus - 1) / cus) * (25.4 * ks + 8.0),
+                            static_cast<double>(mid / (2 * cus)) * (15.3 * ks + 5.0) + (rest == 0 ? 0.0 : rest <= cus ? 9.4 * ks + 5.0 : 15.3 * ks + 5.0),
+                            static_cast<double>((mid + cus - 1) / cus) * (7.6 * ks + 4.0)};
+    for (int c = 0; c < 3; ++c)
+      if (cost[c] + joined < least) {
+        least = cost[c] + joined;
+        best = {static_cast<Config>(c), s};
+      }
+  }
+  return best;
+}
+
 template <int KIND, int DT, bool ADOWN, bool BDOWN>
 int pick(const ProductArgs& a, hipStream_t st) {
-  auto tiles = [&](int64_t bm, int64_t bn) { return ((a.M + bm - 1) / bm) * ((a.N + bn - 1) / bn) * (KIND == kProdPartial ? a.splits : 1); };
-  const int64_t cus = std::max(device_limits().cus, 1);
+  // (a split product was planned by product_splits, with the same numbers)
+  const Plan p = plan_product(static_cast<ProductKind>(KIND), a.M, a.N, a.K, a.pairs, KIND == kProdPartial);
   if constexpr (KIND == kProdGated) {
-    if (4 * tiles(256, 128) >= 3 * cus) return run_product<KIND, DT, ADOWN, BDOWN, 4, 2, 2, 2, 32, 4>(a, st);
-    return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 1, 32, 4>(a, st);
+    if (p.config == kLarge) return run_product<KIND, DT, ADOWN, BDOWN, 4, 2, 2, 2, 64, 2>(a, st);
+    if (p.config == kMid) return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 1, 64, 2>(a, st);
+    return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 1, 64, 4>(a, st);
   } else {
-    if (4 * tiles(256, 256) >= 3 * cus) return run_product<KIND, DT, ADOWN, BDOWN, 2, 4, 4, 2, 32, 4>(a, st);
-    return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 2, 32, 4>(a, st);
+    if (p.config == kLarge) return run_product<KIND, DT, ADOWN, BDOWN, 2, 4, 4, 2, 64, 2>(a, st);
+    if (p.config == kMid) return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 2, 64, 2>(a, st);
+    return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 2, 64, 4>(a, st);
   }
 }
 
 }  // namespace
 
-int product_splits(int64_t M, int64_t N, int64_t K, int pairs) {
-  const int64_t cus = std::max(device_limits().cus, 1);
-  const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128), steps = (K + 31) / 32 * pairs;
-  if (tiles >= cus) return 1;
-  const int64_t want = std::min<int64_t>(2 * cus / tiles, steps / 16);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, 16)));
-}
+int product_splits(int64_t M, int64_t N, int64_t K, int pairs) { return plan_product(kProdPartial, M, N, K, pairs, true).splits; }
 
 int launch_product(ProductKind kind, int dt, bool adown, bool bdown, ProductArgs a, hipStream_t st) {
   if (a.M == 0 || a.N == 0) return kOk;

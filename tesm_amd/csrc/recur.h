@@ -5,7 +5,7 @@
 
 namespace tesm {
 
-constexpr int kRecurRows = 128;  // rows per tile: kept carries are one row of states per tile
+constexpr int kRecurRows = 64;   // rows per tile: kept carries are one row of states per tile
 
 struct RecurArgs {
   int dt = 0;

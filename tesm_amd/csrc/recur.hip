@@ -6,25 +6,29 @@
 //   d value_t = g_t sigmoid(write_t) (1 - tanh^2), d h_0 = c_1.
 // Both are first-order recurrences x <- A x + U, and runs of them compose: (A, U) then (A', U') is (A' A, A' U + U').
 //
-// One pass over the data.  A tile is 128 rows of one sequence by 64 or 128 channels; each of 8 waves takes 16 rows, a lane one or
+// One pass over the data.  A tile is 64 rows of one sequence by 64 or 128 channels; each of 8 waves takes 8 rows, a lane one or
 // two channels; inputs are read once and stay in registers as gates.  Waves scan their rows from zero, their (A, U) meet in
 // LDS, and tiles of one sequence and channel group hand on their state in a chain: a tile publishes its (A, U); from these
 // and the state in front of its group of 16 tiles every tile forms its own carry, always in the same order, so results
 // repeat bit for bit; the last tile of a group publishes the state behind it.  Tiles are taken by ticket, predecessors first, so that
-// whatever a tile waits for is already running.  The forward pass can keep every tile's carry (1/128 of a float32 copy of the
+// whatever a tile waits for is already running.  The forward pass can keep every tile's carry (1/64 of a float32 copy of the
 // states); the backward pass then forms the states again in registers and walks the chain from the end.
 //
-// Published values and flags go by agent-scope atomic accesses (coherent over the XCDs' caches); a wave waits for its
-// value stores before it sets its flag.  A poll gives up after kSpinLimit rounds: the states are then NaN and bit 0 of the
-// status word is set.
+// Published values go by agent-scope atomic accesses of 8 bytes (coherent over the XCDs' caches).  A value says by itself that it is
+// there, its bits are those of no number before: a flag beside it would cost the chain three more trips through memory (one for the
+// values to arrive before the flag, two for the reader).  A poll gives up after kSpinLimit rounds: the states are then NaN and bit 0 of
+// the status word is set.
+#include <type_traits>
+#include <utility>
+
 #include "recur.h"
 
 namespace tesm {
 
 namespace {
 
-constexpr int kWaves = 8, kRows = 16, kTile = kWaves * kRows, kGroup = 16;
-static_assert(kTile == kRecurRows && kGroup == 2 * kWaves, "a wave composes two earlier tiles");
+constexpr int kWaves = 8, kRows = 8, kTile = kWaves * kRows, kGroup = 16;
+static_assert(kTile == kRecurRows && kGroup == 2 * kWaves, "a wave looks after two earlier tiles");
 constexpr int kSpinLimit = 1 << 20;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -39,11 +43,16 @@ int g_spin_limit = kSpinLimit;
 struct Sig {
   float p, q;  // sigmoid(x), sigmoid(-x), each to a few ulp of itself
 };
+// (of x + b, given -b log2 e)
+__device__ __forceinline__ float sig(float x, float nb) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(__builtin_fmaf(x, -kLog2e, nb))); }
 __device__ __forceinline__ float sig(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -kLog2e)); }
-__device__ __forceinline__ Sig sig2(float x) {
-  const float e = __builtin_amdgcn_exp2f(x * -kLog2e), p = __builtin_amdgcn_rcpf(1.0f + e);
-  return {p, p < 0.5f ? 1.0f - p : e * p};
+// (where e overflows, p is 0; every use of q has p as a factor)
+__device__ __forceinline__ Sig sig_of(float e) {
+  const float p = __builtin_amdgcn_rcpf(1.0f + e);
+  return {p, fminf(e, 3.4e38f) * p};
 }
+__device__ __forceinline__ Sig sig2(float x, float nb) { return sig_of(__builtin_amdgcn_exp2f(__builtin_fmaf(x, -kLog2e, nb))); }
+__device__ __forceinline__ Sig sig2(float x) { return sig_of(__builtin_amdgcn_exp2f(x * -kLog2e)); }
 struct Tanh {
   float t, d;  // tanh(x), 1 - tanh^2(x)
 };
@@ -63,7 +72,7 @@ __device__ __forceinline__ Tanh tanh2(float x) {
   } else {
     p = -1.0f / 3.0f;
   }
-  const float small = __builtin_fmaf(x * x2, p, x);
+  const float small = x * __builtin_fmaf(x2, p, 1.0f);
   return {fabsf(x) < (DT == kF32 ? 0.25f : 0.03125f) ? small : big, 4.0f * r * (1.0f - r)};
 }
 
@@ -73,209 +82,230 @@ __device__ __forceinline__ Tanh tanh2(float x) {
 template <int DT, int CPT>
 struct Row {
   uint32_t w;  // one float32, one bfloat16 or two
-  __device__ __forceinline__ void load(const void* p, int64_t i) {
-    if constexpr (CPT == 2)
-      w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + i);
+  // (row: the same for all lanes; off: the lane's bytes in it)
+  __device__ __forceinline__ void load(const char* row, uint32_t off) {
+    if constexpr (DT == kBF16 && CPT == 1)
+      w = *reinterpret_cast<const uint16_t*>(row + off);
     else
-      w = ld_bits<DT>(p, i);
+      w = *reinterpret_cast<const uint32_t*>(row + off);
   }
   __device__ __forceinline__ float get(int j) const {
     if constexpr (CPT == 2) return __uint_as_float(j ? w & 0xffff0000u : w << 16);
     return from_bits<DT>(w);
   }
-  static __device__ __forceinline__ void store(void* p, int64_t i, const float (&v)[CPT]) {
+  static __device__ __forceinline__ void store(char* row, uint32_t off, const float (&v)[CPT]) {
     if constexpr (CPT == 2)
-      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p) + i) = pack_bf16x2(v[0], v[1]);
+      *reinterpret_cast<uint32_t*>(row + off) = pack_bf16x2(v[0], v[1]);
+    else if constexpr (DT == kBF16)
+      *reinterpret_cast<uint16_t*>(row + off) = f32_to_bf16(v[0]);
     else
-      st<DT>(p, i, v[0]);
+      *reinterpret_cast<float*>(row + off) = v[0];
   }
 };
+// The wave's first row of an array, and its rows' distance in bytes.
+struct RowsOf {
+  char* p;
+  int64_t step;
+};
+template <int DT>
+__device__ __forceinline__ RowsOf rows_of(const void* p, int64_t ld, int64_t row) {
+  constexpr int ES = DT == kBF16 ? 2 : 4;
+  return {const_cast<char*>(static_cast<const char*>(p)) + row * ld * ES, ld * ES};
+}
 
 // ---------------------------------------------------------------------------
 // the chain of a sequence's tiles
 // ---------------------------------------------------------------------------
 struct Chain {
-  int* flags = nullptr;     // (G, slots)
   unsigned* tickets = nullptr;  // a 256-byte line per channel group
-  unsigned long long* values = nullptr;  // (G, slots, 64 CPT): (A, U) of a tile, or the state behind a group's last one
+  unsigned long long* values = nullptr;  // (G, slots, 64 CPT): (A, U) of a tile, or the state behind a group's last one; kUnset before
   const int32_t* starts = nullptr;   // packed: S + 1 starts, inside the rows and not decreasing
-  int64_t slots = 0;
+  int slots = 0;
   int G = 0, tiles = 0;  // channel groups; tiles per sequence of a dense batch
   int spin_limit = 0;
 };
 constexpr int kTicketStride = 64;
+constexpr uint32_t kUnset = 0xffffffffu;  // as U: no value yet (a NaN is published with other bits)
 
-struct Place {
-  int64_t row0, len, seq, slot0;  // the sequence's first row and length, its number and first slot
-  int tile, tiles;
-  bool any;
+struct Place {  // (rows, sequences and slots are below 2^31)
+  int row0, len, seq, slot0;  // the sequence's first row and length, its number and first slot
+  int tile, tiles;            // tiles < 0: none
 };
 
 // The tile of slot `at` in walking order; `back`: from the end.
-__device__ __forceinline__ Place place_of(const RecurArgs& a, const Chain& c, int64_t at, bool back) {
+__device__ __forceinline__ Place place_of(const RecurArgs& a, const Chain& c, int at, bool back) {
   Place p;
   if (!c.starts) {
-    p.seq = at % a.B;
-    const int pos = static_cast<int>(at / a.B);
-    p.tile = back ? c.tiles - 1 - pos : pos;
+    const unsigned B = static_cast<unsigned>(a.B), pos = static_cast<unsigned>(at) / B;
+    p.seq = static_cast<int>(static_cast<unsigned>(at) - pos * B);
     p.tiles = c.tiles;
-    p.row0 = p.seq * a.L;
-    p.len = a.L;
+    p.tile = back ? c.tiles - 1 - static_cast<int>(pos) : static_cast<int>(pos);
+    p.len = static_cast<int>(a.L);
+    p.row0 = p.seq * p.len;
     p.slot0 = p.seq * c.tiles;
-    p.any = true;
     return p;
   }
-  const int64_t slot = back ? c.slots - 1 - at : at;
+  const int slot = back ? c.slots - 1 - at : at;
   // sequence s has the slots from start / kTile + s on, at least one
-  int64_t lo = 0, hi = a.S;
+  int lo = 0, hi = static_cast<int>(a.S);
   while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (c.starts[mid] / kTile + mid <= slot)
+    const int mid = (lo + hi) >> 1;
+    if (__builtin_amdgcn_readfirstlane(c.starts[mid]) / kTile + mid <= slot)
       lo = mid;
     else
       hi = mid;
   }
   p.seq = lo;
-  p.row0 = c.starts[lo];
-  p.len = c.starts[lo + 1] - p.row0;
+  p.row0 = __builtin_amdgcn_readfirstlane(c.starts[lo]);
+  p.len = __builtin_amdgcn_readfirstlane(c.starts[lo + 1]) - p.row0;
   p.slot0 = p.row0 / kTile + lo;
-  p.tile = static_cast<int>(slot - p.slot0);
-  p.tiles = static_cast<int>((p.len + kTile - 1) / kTile);
-  if (p.tiles < 1) p.tiles = 1;  // (an empty sequence hands its state through)
-  p.any = p.tile >= 0 && p.tile < p.tiles;
+  p.tile = slot - p.slot0;
+  p.tiles = p.len > 0 ? (p.len + kTile - 1) / kTile : 1;  // (an empty sequence hands its state through)
+  if (p.tile < 0 || p.tile >= p.tiles) p.tiles = -1;
   return p;
 }
 
-__device__ __forceinline__ unsigned long long pack2(float a, float u) {
-  return static_cast<unsigned long long>(__float_as_uint(u)) << 32 | __float_as_uint(a);
-}
 __device__ __forceinline__ float2 unpack2(unsigned long long v) {
   return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
 }
+__device__ __forceinline__ void publish(const Chain& c, int64_t at, float a, float u) {
+  const uint32_t bits = u == u ? __float_as_uint(u) : 0x7fc00000u;
+  __hip_atomic_store(c.values + at, static_cast<unsigned long long>(bits) << 32 | __float_as_uint(a), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ unsigned long long published(const Chain& c, int64_t at) {
+  return __hip_atomic_load(c.values + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ bool is_set(unsigned long long v) { return static_cast<uint32_t>(v >> 32) != kUnset; }
 
 template <int CPT>
 struct ChainTile {
-  float2 part[kWaves][64 * CPT];   // the waves' rows
+  float2 part[kWaves][64 * CPT];    // the waves' rows
   float2 before[kWaves][64 * CPT];  // the tiles in front, two per wave
   float base[64 * CPT];             // the state in front of the group
   int bad;
   unsigned ticket;
 };
 
-// Publishes a wave's values for slot `s`: the values first, then the flag.
-template <int CPT>
-__device__ __forceinline__ void publish(const Chain& c, int64_t s, int lane, const float2 (&v)[CPT]) {
-#pragma unroll
-  for (int j = 0; j < CPT; ++j)
-    __hip_atomic_store(c.values + (s * 64 + lane) * CPT + j, pack2(v[j].x, v[j].y), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  if (lane == 0) __hip_atomic_store(c.flags + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-// Waits for the flags of slots s and (with `two`) s2; whether they came.
-__device__ __forceinline__ bool await(const Chain& c, int64_t s, int64_t s2, bool two) {
-  bool ok = false;
-  for (int i = 0; i <= c.spin_limit && !ok; ++i) {
-    int f = __hip_atomic_load(c.flags + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (two) f &= __hip_atomic_load(c.flags + s2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    ok = __builtin_amdgcn_readfirstlane(f) != 0;
-    if (!ok) __builtin_amdgcn_s_sleep(1);
-  }
-  asm volatile("" ::: "memory");
-  return ok;
-}
-
-// The state entering the wave's rows.  part: the wave's (A, U).  In walking order: pos of the tile, order of the wave; slot(p):
-// the slot of position p; first: the sequence's own first state.  `entry` returns the tile's carry, `leave` the state behind the
-// tile (of use to the last wave in order).
-template <int CPT, typename Slot, typename First>
+// The state entering the wave's rows.  part: the wave's (A, U).  In walking order: pos of the tile, order of the wave; at(p): where
+// position p publishes this lane's values; first: the sequence's own first state.  `entry` returns the tile's carry, `leave`, to the
+// first wave in order, the state behind the tile.
+template <int CPT, typename At, typename First>
 __device__ __forceinline__ void chain_carry(const Chain& c, ChainTile<CPT>& sh, int lane, int order, int pos, int count,
-                                            const float2 (&part)[CPT], Slot&& slot, First&& first, float (&carry)[CPT],
+                                            const float2 (&part)[CPT], At&& at, First&& first, float (&carry)[CPT],
                                             float (&entry)[CPT], float (&leave)[CPT]) {
 #pragma unroll
   for (int j = 0; j < CPT; ++j) sh.part[order][lane * CPT + j] = part[j];
   if (order == 0 && lane == 0) sh.bad = 0;
   __syncthreads();
-  const int g0 = pos & ~(kGroup - 1);
-  const bool last_of_group = (pos & (kGroup - 1)) == kGroup - 1, more = pos + 1 < count;
+  const int g0 = pos & ~(kGroup - 1), front = pos - g0;
+  const bool last_of_group = front == kGroup - 1, more = pos + 1 < count;
   float2 all[CPT];
-#pragma unroll
-  for (int j = 0; j < CPT; ++j) {
-    all[j] = make_float2(1.0f, 0.0f);
-    for (int w = 0; w < kWaves; ++w) {
-      const float2 q = sh.part[w][lane * CPT + j];
-      all[j] = make_float2(q.x * all[j].x, __builtin_fmaf(q.x, all[j].y, q.y));
-    }
-  }
-  if (order == 0 && more && !last_of_group) publish<CPT>(c, slot(pos), lane, all);
-  // two tiles in front of this one, in order
-  const int p0 = g0 + 2 * order;
-  bool ok = true;
-  float2 b[CPT];
-#pragma unroll
-  for (int j = 0; j < CPT; ++j) b[j] = make_float2(1.0f, 0.0f);
-  if (p0 < pos) {
-    const bool two = p0 + 1 < pos;
-    const int64_t s0 = slot(p0), s1 = slot(two ? p0 + 1 : p0);
-    ok = await(c, s0, s1, two);
+  if (order == 0) {
 #pragma unroll
     for (int j = 0; j < CPT; ++j) {
-      const float2 x = unpack2(__hip_atomic_load(c.values + (s0 * 64 + lane) * CPT + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-      const float2 y = unpack2(__hip_atomic_load(c.values + (s1 * 64 + lane) * CPT + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-      b[j] = two ? make_float2(y.x * x.x, __builtin_fmaf(y.x, x.y, y.y)) : x;
+      all[j] = sh.part[0][lane * CPT + j];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) {
+        const float2 q = sh.part[w][lane * CPT + j];
+        all[j] = make_float2(q.x * all[j].x, __builtin_fmaf(q.x, all[j].y, q.y));
+      }
+      if (more && !last_of_group) publish(c, at(pos) + j, all[j].x, all[j].y);
     }
   }
+  // two tiles in front of this one, in order; the last wave has one, and the state in front of the group
+  const int p0 = g0 + 2 * order;
+  const bool one = p0 < pos, two = p0 + 1 < pos, base = order == kWaves - 1 && g0 > 0;
+  if (one || base) {
+    const int64_t at0 = at(one ? p0 : g0 - 1), at1 = at(two ? p0 + 1 : base ? g0 - 1 : p0);
+    unsigned long long x[CPT] = {}, y[CPT] = {};
+    bool ok = false;
+    // (polled by the first lane's value alone: all lanes' would be more traffic than the rows)
+    const int64_t look0 = at0 - lane * CPT, look1 = at1 - lane * CPT;
+    for (int i = 0; i <= c.spin_limit && !ok; ++i) {
+      bool set = true;
+      if (lane == 0) set = is_set(published(c, look0)) && is_set(published(c, look1));
+      if (!__all(set)) {
+        __builtin_amdgcn_s_sleep(2);
+        continue;
+      }
 #pragma unroll
-  for (int j = 0; j < CPT; ++j) sh.before[order][lane * CPT + j] = b[j];
-  if (order == kWaves - 1) {  // (it has the fewest tiles to wait for)
-    if (g0 == 0) {
+      for (int j = 0; j < CPT; ++j) {
+        x[j] = published(c, at0 + j);
+        y[j] = published(c, at1 + j);
+      }
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) sh.base[lane * CPT + j] = first(j);
-    } else {
-      const int64_t s = slot(g0 - 1);
-      ok = await(c, s, s, false) && ok;
+      for (int j = 0; j < CPT; ++j) set = set && is_set(x[j]) && is_set(y[j]);
+      ok = __all(set);
+    }
+    if (!ok && lane == 0) sh.bad = 1;
 #pragma unroll
-      for (int j = 0; j < CPT; ++j)
-        sh.base[lane * CPT + j] =
-            unpack2(__hip_atomic_load(c.values + (s * 64 + lane) * CPT + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)).y;
+    for (int j = 0; j < CPT; ++j) {
+      const float2 u = unpack2(x[j]), v = unpack2(y[j]);
+      if (one) sh.before[order][lane * CPT + j] = two ? make_float2(v.x * u.x, __builtin_fmaf(v.x, u.y, v.y)) : u;
+      if (base) sh.base[lane * CPT + j] = v.y;
     }
   }
-  if (!ok && lane == 0) sh.bad = 1;
+  if (order == kWaves - 1 && g0 == 0) {
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) sh.base[lane * CPT + j] = first(j);
+  }
   __syncthreads();
   const bool bad = sh.bad != 0;
   if (bad && order == 0 && lane == 0) __hip_atomic_fetch_or(&g_recur_status, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
   for (int j = 0; j < CPT; ++j) {
     float x = sh.base[lane * CPT + j];
-    if (pos != g0)
-      for (int w = 0; w < kWaves; ++w) {
-        const float2 q = sh.before[w][lane * CPT + j];
-        x = __builtin_fmaf(q.x, x, q.y);
-      }
+    for (int w = 0; w < (front + 1) / 2; ++w) {
+      const float2 q = sh.before[w][lane * CPT + j];
+      x = __builtin_fmaf(q.x, x, q.y);
+    }
     if (bad) x = __builtin_nanf("");
     entry[j] = x;
-    leave[j] = __builtin_fmaf(all[j].x, x, all[j].y);
+    if (order == 0) {
+      leave[j] = __builtin_fmaf(all[j].x, x, all[j].y);
+      if (more && last_of_group) publish(c, at(pos) + j, 0.0f, leave[j]);
+    }
     for (int w = 0; w < order; ++w) {
       const float2 q = sh.part[w][lane * CPT + j];
       x = __builtin_fmaf(q.x, x, q.y);
     }
     carry[j] = x;
   }
-  if (order == 0 && more && last_of_group) {
-    float2 v[CPT];
-#pragma unroll
-    for (int j = 0; j < CPT; ++j) v[j] = make_float2(0.0f, leave[j]);
-    publish<CPT>(c, slot(pos), lane, v);
-  }
 }
 
-// The workgroup's tile in walking order: by ticket where tiles wait for each other, else by its index.
+// The workgroup's tile in walking order: by ticket where tiles wait for each other, else by its index.  (Uniform: what follows
+// from it costs no vector operations.)
 template <int CPT>
-__device__ __forceinline__ int64_t take_ticket(const Chain& c, ChainTile<CPT>& sh, int g) {
-  if (!c.tickets) return blockIdx.x / c.G;
+__device__ __forceinline__ int take_ticket(const Chain& c, ChainTile<CPT>& sh, int g) {
+  if (!c.tickets) return static_cast<int>(blockIdx.x / static_cast<unsigned>(c.G));
   if (threadIdx.x == 0)
     sh.ticket = __hip_atomic_fetch_add(c.tickets + static_cast<int64_t>(g) * kTicketStride, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  return sh.ticket;
+  return __builtin_amdgcn_readfirstlane(static_cast<int>(sh.ticket));
+}
+
+// A wave's rows of a tile: the first one in the array, and how many there are.
+struct Part {
+  int row, n;
+};
+__device__ __forceinline__ Part part_of(const Place& p, int wave) {
+  const int t0 = p.tile * kTile + wave * kRows, left = p.tiles > 0 ? p.len - t0 : 0;
+  return {p.row0 + t0, left < 0 ? 0 : left < kRows ? left : kRows};
+}
+// Its inputs, rows behind the end read as the last one.
+template <int DT, int CPT, int ARRAYS, bool WHOLE>
+__device__ __forceinline__ void load_rows(const Part& q, const void* const (&&p)[ARRAYS], const int64_t (&&ld)[ARRAYS], uint32_t off,
+                                          Row<DT, CPT> (&to)[ARRAYS][kRows]) {
+  RowsOf r[ARRAYS];
+#pragma unroll
+  for (int k = 0; k < ARRAYS; ++k) r[k] = rows_of<DT>(p[k], ld[k], q.row);
+#pragma unroll
+  for (int i = 0; i < kRows; ++i)
+#pragma unroll
+    for (int k = 0; k < ARRAYS; ++k) {
+      to[k][i].load(r[k].p, off);
+      if (WHOLE || i + 1 < q.n) r[k].p += r[k].step;
+    }
 }
 
 template <int DT, int CPT>
@@ -284,161 +314,187 @@ __global__ __launch_bounds__(64 * kWaves) void recur_fwd_kernel(RecurArgs a, Cha
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = blockIdx.x % c.G;
   const Place p = place_of(a, c, take_ticket(c, sh, g), false);
-  if (!p.any) return;
+  if (p.tiles < 0) return;
   const int64_t mine = static_cast<int64_t>(g) * 64 * CPT + lane * CPT;
   const bool on = mine < a.C;
   const int64_t ch = on ? mine : a.C - CPT;
-  const int64_t t0 = static_cast<int64_t>(p.tile) * kTile + wave * kRows;
-  const int n = static_cast<int>(p.len - t0 < 0 ? 0 : p.len - t0 < kRows ? p.len - t0 : kRows);
-  float bias[CPT];
-#pragma unroll
-  for (int j = 0; j < CPT; ++j) bias[j] = a.bias ? a.bias[ch + j] : 0.0f;
+  constexpr int ES = DT == kBF16 ? 2 : 4;
+  const uint32_t off = static_cast<uint32_t>(ch * ES);
+  const Part q = part_of(p, wave);
   float A[kRows][CPT], U[kRows][CPT];
   float2 part[CPT];
 #pragma unroll
   for (int j = 0; j < CPT; ++j) part[j] = make_float2(1.0f, 0.0f);
-  if (n > 0) {
-    Row<DT, CPT> v[kRows], w[kRows], d[kRows];
+  // (whole parts apart: without a branch per row their rows are worked on side by side)
+  auto gates = [&](auto whole) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    Row<DT, CPT> raw[3][kRows];
+    load_rows<DT, CPT, 3, WHOLE>(q, {a.decay, a.write, a.value}, {a.ld_d, a.ld_w, a.ld_v}, off, raw);
+    float nb[CPT];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {  // (rows behind the end read the last one again)
-      const int64_t r = p.row0 + t0 + (i < n ? i : n - 1);
-      d[i].load(a.decay, r * a.ld_d + ch);
-      w[i].load(a.write, r * a.ld_w + ch);
-      v[i].load(a.value, r * a.ld_v + ch);
-    }
+    for (int j = 0; j < CPT; ++j) nb[j] = a.bias ? a.bias[ch + j] * -kLog2e : 0.0f;
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
 #pragma unroll
       for (int j = 0; j < CPT; ++j) {
-        A[i][j] = sig(d[i].get(j) + bias[j]);
-        U[i][j] = sig(w[i].get(j)) * tanh2<DT>(v[i].get(j)).t;
-        if (i < n) part[j] = make_float2(A[i][j] * part[j].x, __builtin_fmaf(A[i][j], part[j].y, U[i][j]));
+        A[i][j] = sig(raw[0][i].get(j), nb[j]);
+        U[i][j] = sig(raw[1][i].get(j)) * tanh2<DT>(raw[2][i].get(j)).t;
+        if (WHOLE || i < q.n) part[j] = make_float2(A[i][j] * part[j].x, __builtin_fmaf(A[i][j], part[j].y, U[i][j]));
       }
-  }
+  };
+  if (q.n == kRows)
+    gates(std::true_type{});
+  else if (q.n > 0)
+    gates(std::false_type{});
   float h[CPT], entry[CPT], leave[CPT];
   auto first = [&](int j) { return a.h0 ? a.h0[p.seq * a.C + ch + j] : 0.0f; };
-  auto slot = [&](int q) { return g * c.slots + p.slot0 + q; };
-  chain_carry<CPT>(c, sh, lane, wave, p.tile, p.tiles, part, slot, first, h, entry, leave);
+  auto at = [&](int k) { return ((static_cast<int64_t>(g) * c.slots + (p.slot0 + k)) * 64 + lane) * CPT; };
+  chain_carry<CPT>(c, sh, lane, wave, p.tile, p.tiles, part, at, first, h, entry, leave);
   if (!on) return;
-  if (wave == kWaves - 1) {
-    if (a.carries) {
+  if (wave == 0) {
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) a.carries[(p.slot0 + p.tile) * a.C + ch + j] = entry[j];
-    }
-    if (p.tile == p.tiles - 1) {
-#pragma unroll
-      for (int j = 0; j < CPT; ++j) a.h_out[p.seq * a.C + ch + j] = leave[j];
+    for (int j = 0; j < CPT; ++j) {
+      if (a.carries) a.carries[static_cast<int64_t>(p.slot0 + p.tile) * a.C + ch + j] = entry[j];
+      if (p.tile == p.tiles - 1) a.h_out[p.seq * a.C + ch + j] = leave[j];
     }
   }
+  auto states = [&](auto whole) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    RowsOf rh = rows_of<DT>(a.h, a.ld_h, q.row);
 #pragma unroll
-  for (int i = 0; i < kRows; ++i)
-    if (i < n) {
+    for (int i = 0; i < kRows; ++i) {
+      if (!WHOLE && i >= q.n) break;
 #pragma unroll
       for (int j = 0; j < CPT; ++j) h[j] = __builtin_fmaf(A[i][j], h[j], U[i][j]);
-      Row<DT, CPT>::store(a.h, (p.row0 + t0 + i) * a.ld_h + ch, h);
+      Row<DT, CPT>::store(rh.p, off, h);
+      rh.p += rh.step;
     }
+  };
+  if (q.n == kRows)
+    states(std::true_type{});
+  else
+    states(std::false_type{});
 }
 
 template <int DT, int CPT>
-__global__ __launch_bounds__(64 * kWaves) void recur_bwd_kernel(RecurBwdArgs b, Chain c, float* sums) {
+__global__ __launch_bounds__(64 * kWaves, 4) void recur_bwd_kernel(RecurBwdArgs b, Chain c, float* sums) {
   __shared__ ChainTile<CPT> sh;
   __shared__ float2 fwd[kWaves][64 * CPT];
   const RecurArgs& a = b.in;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int order = kWaves - 1 - wave;  // in walking order, from the end
   const int g = blockIdx.x % c.G;
   const Place p = place_of(a, c, take_ticket(c, sh, g), true);
-  if (!p.any) return;
+  if (p.tiles < 0) return;
   const int64_t mine = static_cast<int64_t>(g) * 64 * CPT + lane * CPT;
   const bool on = mine < a.C;
   const int64_t ch = on ? mine : a.C - CPT;
-  const int64_t t0 = static_cast<int64_t>(p.tile) * kTile + wave * kRows;
-  const int n = static_cast<int>(p.len - t0 < 0 ? 0 : p.len - t0 < kRows ? p.len - t0 : kRows);
-  float bias[CPT];
+  constexpr int ES = DT == kBF16 ? 2 : 4;
+  const uint32_t off = static_cast<uint32_t>(ch * ES);
+  const Part q = part_of(p, wave);
+  float kept[CPT];
 #pragma unroll
-  for (int j = 0; j < CPT; ++j) bias[j] = a.bias ? a.bias[ch + j] : 0.0f;
-  Row<DT, CPT> v[kRows], w[kRows], d[kRows], dh[kRows];
-  float A[kRows][CPT], U[kRows][CPT];
+  for (int j = 0; j < CPT; ++j) kept[j] = a.carries[static_cast<int64_t>(p.slot0 + p.tile) * a.C + ch + j];
+  // Per row: a, and what the gradient is multiplied with for value, write and decay; U: u.
+  Row<DT, CPT> dh[kRows];
+  float A[kRows][CPT], U[kRows][CPT], fv[kRows][CPT], fw[kRows][CPT], fd[kRows][CPT];
   float2 part[CPT], from[CPT];  // the rows backwards and forwards
 #pragma unroll
   for (int j = 0; j < CPT; ++j) part[j] = from[j] = make_float2(1.0f, 0.0f);
-  if (n > 0) {
+  auto gates = [&](auto whole) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    Row<DT, CPT> raw[4][kRows];
+    load_rows<DT, CPT, 4, WHOLE>(q, {a.decay, a.write, a.value, b.grad}, {a.ld_d, a.ld_w, a.ld_v, b.ld_g}, off, raw);
+    float nb[CPT];
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) nb[j] = a.bias ? a.bias[ch + j] * -kLog2e : 0.0f;
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      const int64_t r = p.row0 + t0 + (i < n ? i : n - 1);
-      d[i].load(a.decay, r * a.ld_d + ch);
-      w[i].load(a.write, r * a.ld_w + ch);
-      v[i].load(a.value, r * a.ld_v + ch);
-      dh[i].load(b.grad, r * b.ld_g + ch);
-    }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
+      dh[i] = raw[3][i];
 #pragma unroll
       for (int j = 0; j < CPT; ++j) {
-        A[i][j] = sig(d[i].get(j) + bias[j]);
-        U[i][j] = sig(w[i].get(j)) * tanh2<DT>(v[i].get(j)).t;
-        if (i < n) from[j] = make_float2(A[i][j] * from[j].x, __builtin_fmaf(A[i][j], from[j].y, U[i][j]));
+        const Sig f = sig2(raw[0][i].get(j), nb[j]), s = sig2(raw[1][i].get(j));
+        const Tanh t = tanh2<DT>(raw[2][i].get(j));
+        A[i][j] = f.p;
+        fd[i][j] = f.p * f.q;
+        U[i][j] = s.p * t.t;
+        fv[i][j] = s.p * t.d;
+        fw[i][j] = U[i][j] * s.q;
+        if (WHOLE || i < q.n) from[j] = make_float2(A[i][j] * from[j].x, __builtin_fmaf(A[i][j], from[j].y, U[i][j]));
       }
+    }
 #pragma unroll
     for (int i = kRows - 1; i >= 0; --i)
 #pragma unroll
       for (int j = 0; j < CPT; ++j)
-        if (i < n) part[j] = make_float2(A[i][j] * part[j].x, A[i][j] * (part[j].y + dh[i].get(j)));
-  }
+        if (WHOLE || i < q.n) part[j].y = A[i][j] * (part[j].y + dh[i].get(j));
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) part[j].x = from[j].x;
+  };
+  if (q.n == kRows)
+    gates(std::true_type{});
+  else if (q.n > 0)
+    gates(std::false_type{});
 #pragma unroll
   for (int j = 0; j < CPT; ++j) fwd[wave][lane * CPT + j] = from[j];
   // The chain's state is c; in front of it (behind the last row) stands the final state's gradient.
   float back[CPT], entry[CPT], leave[CPT];
-  const int pos = p.tiles - 1 - p.tile;
   auto first = [&](int j) { return b.grad_state ? b.grad_state[p.seq * a.C + ch + j] : 0.0f; };
-  auto slot = [&](int q) { return g * c.slots + p.slot0 + (p.tiles - 1 - q); };
-  chain_carry<CPT>(c, sh, lane, kWaves - 1 - wave, pos, p.tiles, part, slot, first, back, entry, leave);
+  auto at = [&](int k) { return ((static_cast<int64_t>(g) * c.slots + (p.slot0 + (p.tiles - 1 - k))) * 64 + lane) * CPT; };
+  chain_carry<CPT>(c, sh, lane, order, p.tiles - 1 - p.tile, p.tiles, part, at, first, back, entry, leave);
   // the states again, from the tile's kept carry
-  float h[kRows][CPT];  // in front of each row
   float db[CPT];
 #pragma unroll
   for (int j = 0; j < CPT; ++j) {
-    float x = a.carries[(p.slot0 + p.tile) * a.C + ch + j];
-    for (int q = 0; q < wave; ++q) {
-      const float2 f = fwd[q][lane * CPT + j];
-      x = __builtin_fmaf(f.x, x, f.y);
-    }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      h[i][j] = x;
-      if (n > 0) x = __builtin_fmaf(A[i][j], x, U[i][j]);
-    }
     db[j] = 0.0f;
-  }
-  if (n > 0) {
-#pragma unroll
-    for (int i = kRows - 1; i >= 0; --i)
-      if (i < n) {
-        float ov[CPT], ow[CPT], od[CPT];
-#pragma unroll
-        for (int j = 0; j < CPT; ++j) {
-          const Sig s = sig2(w[i].get(j));
-          const Tanh t = tanh2<DT>(v[i].get(j));
-          const float q = sig2(d[i].get(j) + bias[j]).q;
-          const float grad = back[j] + dh[i].get(j);
-          ov[j] = grad * s.p * t.d;
-          ow[j] = grad * U[i][j] * s.q;
-          od[j] = grad * h[i][j] * A[i][j] * q;
-          db[j] += od[j];
-          back[j] = A[i][j] * grad;
-        }
-        if (on) {
-          const int64_t r = p.row0 + t0 + i;
-          Row<DT, CPT>::store(b.d_value, r * b.ld_dv + ch, ov);
-          Row<DT, CPT>::store(b.d_write, r * b.ld_dw + ch, ow);
-          Row<DT, CPT>::store(b.d_decay, r * b.ld_dd + ch, od);
-        }
+    if (q.n > 0) {
+      float x = kept[j];
+      for (int w = 0; w < wave; ++w) {
+        const float2 f = fwd[w][lane * CPT + j];
+        x = __builtin_fmaf(f.x, x, f.y);
       }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        fd[i][j] *= x;
+        x = __builtin_fmaf(A[i][j], x, U[i][j]);
+      }
+    }
   }
-  if (on && wave == 0 && p.tile == 0 && b.d_h0) {
+  auto grads = [&](auto whole) __attribute__((always_inline)) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    const int64_t row = static_cast<int64_t>(q.row) + (WHOLE ? kRows : q.n) - 1;
+    RowsOf rv = rows_of<DT>(b.d_value, b.ld_dv, row), rw = rows_of<DT>(b.d_write, b.ld_dw, row), rd = rows_of<DT>(b.d_decay, b.ld_dd, row);
+#pragma unroll
+    for (int i = kRows - 1; i >= 0; --i) {
+      if (!WHOLE && i >= q.n) continue;
+      float ov[CPT], ow[CPT], od[CPT];
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) {
+        const float grad = back[j] + dh[i].get(j);
+        ov[j] = grad * fv[i][j];
+        ow[j] = grad * fw[i][j];
+        od[j] = grad * fd[i][j];
+        db[j] += od[j];
+        back[j] = A[i][j] * grad;
+      }
+      Row<DT, CPT>::store(rv.p, off, ov);
+      Row<DT, CPT>::store(rw.p, off, ow);
+      Row<DT, CPT>::store(rd.p, off, od);
+      rv.p -= rv.step, rw.p -= rw.step, rd.p -= rd.step;
+    }
+  };
+  if (on) {
+    if (q.n == kRows)
+      grads(std::true_type{});
+    else
+      grads(std::false_type{});
+  }
+  if (on && order == 0 && p.tile == 0 && b.d_h0) {
 #pragma unroll
     for (int j = 0; j < CPT; ++j) b.d_h0[p.seq * a.C + ch + j] = leave[j];
   }
-  if (sums) {
+  if (sums) {  // (the waves are past the carry's barrier: nobody reads `before` any more but this)
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < CPT; ++j) sh.before[wave][lane * CPT + j].x = db[j];
     __syncthreads();
@@ -446,8 +502,8 @@ __global__ __launch_bounds__(64 * kWaves) void recur_bwd_kernel(RecurBwdArgs b, 
 #pragma unroll
       for (int j = 0; j < CPT; ++j) {
         float x = 0.0f;
-        for (int q = 0; q < kWaves; ++q) x += sh.before[q][lane * CPT + j].x;
-        sums[(p.slot0 + p.tile) * a.C + ch + j] = x;
+        for (int w = 0; w < kWaves; ++w) x += sh.before[w][lane * CPT + j].x;
+        sums[static_cast<int64_t>(p.slot0 + p.tile) * a.C + ch + j] = x;
       }
     }
   }
@@ -472,9 +528,10 @@ __global__ __launch_bounds__(1024) void recur_bias_kernel(const float* sums, int
   }
 }
 
-// Workgroup 0 of a packed call brings the starts inside the rows and in order (a running maximum); the others clear words.
-__global__ __launch_bounds__(256) void recur_reset_kernel(uint32_t* words, int64_t n, const int32_t* starts, int64_t count, int64_t rows,
-                                                          int32_t* ordered) {
+// Clears the tickets and marks the values unset.  The last workgroup of a packed call brings the starts inside the rows and in
+// order (a running maximum).
+__global__ __launch_bounds__(256) void recur_reset_kernel(uint4* tickets, int64_t n_tickets, uint4* values, int64_t n_values, const int32_t* starts,
+                                                          int64_t count, int64_t rows, int32_t* ordered) {
   if (starts && blockIdx.x == gridDim.x - 1) {
     __shared__ int32_t top[256];
     int32_t run = 0;
@@ -498,7 +555,14 @@ __global__ __launch_bounds__(256) void recur_reset_kernel(uint32_t* words, int64
     return;
   }
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i < n) words[i] = 0;
+  if (i < n_tickets)
+    tickets[i] = make_uint4(0, 0, 0, 0);
+  else if (i < n_tickets + n_values)
+    values[i - n_tickets] = make_uint4(kUnset, kUnset, kUnset, kUnset);
+}
+__global__ __launch_bounds__(256) void recur_zero_kernel(float* p, int64_t n) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i < n) p[i] = 0.0f;
 }
 
 template <int DT>
@@ -533,8 +597,8 @@ bool in_pairs(int dt, int64_t C, std::initializer_list<std::pair<const void*, in
 }
 
 struct Plan {
-  int64_t slots = 0, words = 0;  // words to clear, at most: tickets, flags
-  int64_t at_values = 0, at_starts = 0, at_sums = 0, total = 0;
+  int64_t slots = 0;
+  int64_t at_values = 0, at_starts = 0, at_sums = 0, total = 0;  // tickets first
   bool chained = false;
 };
 int64_t up256(int64_t v) { return round_up(v, 256); }
@@ -544,8 +608,7 @@ Plan plan_of(const RecurArgs& a, bool sums) {
   const int64_t tiles = (a.L + kTile - 1) / kTile;
   p.slots = a.seq_starts ? a.B * a.L / kTile + a.S : a.B * std::max<int64_t>(tiles, 1);
   p.chained = a.seq_starts || tiles > 1;
-  if (p.chained) p.words = G * kTicketStride + G * p.slots;
-  p.at_values = up256(4 * p.words);
+  p.at_values = p.chained ? up256(4 * G * kTicketStride) : 0;
   p.at_starts = p.at_values + (p.chained ? up256(G * p.slots * 64 * 8) : 0);
   p.at_sums = p.at_starts + (a.seq_starts ? up256(4 * (a.S + 1)) : 0);
   p.total = p.at_sums + (sums ? up256(4 * p.slots * a.C) : 0);
@@ -555,30 +618,28 @@ Plan plan_of(const RecurArgs& a, bool sums) {
 Chain chain_of(const RecurArgs& a, const Plan& p, void* ws, int cpt) {
   Chain c;
   char* base = static_cast<char*>(ws);
-  c.slots = p.slots;
+  c.slots = static_cast<int>(p.slots);
   c.G = static_cast<int>((a.C + 64 * cpt - 1) / (64 * cpt));
   c.tiles = static_cast<int>(std::max<int64_t>(1, (a.L + kTile - 1) / kTile));
   c.spin_limit = g_spin_limit;
   if (p.chained) {
     c.tickets = reinterpret_cast<unsigned*>(base);
-    c.flags = reinterpret_cast<int*>(base) + static_cast<int64_t>(c.G) * kTicketStride;
     c.values = reinterpret_cast<unsigned long long*>(base + p.at_values);
   }
   if (a.seq_starts) c.starts = reinterpret_cast<int32_t*>(base + p.at_starts);
   return c;
 }
 
-int reset(const RecurArgs& a, const Plan& p, const Chain& c, void* ws, bool sums, hipStream_t st) {
+int reset(const RecurArgs& a, const Plan& p, const Chain& c, int cpt, float* sums, hipStream_t st) {
   if (!p.chained) return kOk;
-  // (sums lie behind the rest and are cleared with packed rows only: every slot of a dense batch is a tile)
-  const int64_t words = static_cast<int64_t>(c.G) * (kTicketStride + p.slots);
-  const unsigned blocks = static_cast<unsigned>((words + 255) / 256 + (a.seq_starts ? 1 : 0));
+  const int64_t n_tickets = static_cast<int64_t>(c.G) * kTicketStride / 4, n_values = c.G * p.slots * 64 * cpt / 2;
+  const unsigned blocks = static_cast<unsigned>((n_tickets + n_values + 255) / 256 + (a.seq_starts ? 1 : 0));
   recur_reset_kernel<<<blocks, 256, 0, TESM_LOGGED(st, recur_reset_kernel)>>>(
-      static_cast<uint32_t*>(ws), words, a.seq_starts, a.S + 1, a.B * a.L, const_cast<int32_t*>(c.starts));
-  if (sums && a.seq_starts) {
+      reinterpret_cast<uint4*>(c.tickets), n_tickets, reinterpret_cast<uint4*>(c.values), n_values, a.seq_starts, a.S + 1, a.B * a.L,
+      const_cast<int32_t*>(c.starts));
+  if (sums && a.seq_starts) {  // (slots of packed rows may hold no tile)
     const int64_t n = p.slots * a.C;
-    recur_reset_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, TESM_LOGGED(st, recur_reset_kernel)>>>(
-        reinterpret_cast<uint32_t*>(static_cast<char*>(ws) + p.at_sums), n, nullptr, 0, 0, nullptr);
+    recur_zero_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, TESM_LOGGED(st, recur_zero_kernel)>>>(sums, n);
   }
   return kOk;
 }
@@ -597,13 +658,13 @@ int launch_gated_scan(const RecurArgs& a, void* ws, int64_t ws_bytes, hipStream_
   TESM_REQUIRE(!rows || (a.ld_v >= a.C && a.ld_w >= a.C && a.ld_d >= a.C && a.ld_h >= a.C), kErrInvalidArg,
                "gated scan: a row pitch below the channels");
   const Plan p = plan_of(a, false);
-  TESM_REQUIRE(p.total == 0 || (ws && ws_bytes >= p.total && aligned(ws, 8)), kErrWorkspace,
-               "gated scan: workspace too small or not 8-byte aligned");
+  TESM_REQUIRE(p.total == 0 || (ws && ws_bytes >= p.total && aligned(ws, 16)), kErrWorkspace,
+               "gated scan: workspace too small or not 16-byte aligned");
   const bool pairs = in_pairs(a.dt, a.C, {{a.value, a.ld_v}, {a.write, a.ld_w}, {a.decay, a.ld_d}, {a.h, a.ld_h}});
   const Chain c = chain_of(a, p, ws, pairs ? 2 : 1);
   const int64_t blocks = p.slots * c.G;
   TESM_REQUIRE(blocks < (1LL << 31), kErrUnsupported, "gated scan: too many tiles for one call");
-  if (int rc = reset(a, p, c, ws, false, st)) return rc;
+  if (int rc = reset(a, p, c, pairs ? 2 : 1, nullptr, st)) return rc;
   constexpr int T = 64 * kWaves;
   const unsigned n = static_cast<unsigned>(blocks);
   if (a.dt == kF32)
@@ -626,8 +687,8 @@ int launch_gated_scan_bwd(const RecurBwdArgs& b, void* ws, int64_t ws_bytes, hip
                          b.ld_dd >= a.C),
                kErrInvalidArg, "gated scan backward: a row pitch below the channels");
   const Plan p = plan_of(a, b.d_bias != nullptr);
-  TESM_REQUIRE(p.total == 0 || (ws && ws_bytes >= p.total && aligned(ws, 8)), kErrWorkspace,
-               "gated scan backward: workspace too small or not 8-byte aligned");
+  TESM_REQUIRE(p.total == 0 || (ws && ws_bytes >= p.total && aligned(ws, 16)), kErrWorkspace,
+               "gated scan backward: workspace too small or not 16-byte aligned");
   const bool pairs = in_pairs(a.dt, a.C, {{a.value, a.ld_v}, {a.write, a.ld_w}, {a.decay, a.ld_d}, {b.grad, b.ld_g},
                                           {b.d_value, b.ld_dv}, {b.d_write, b.ld_dw}, {b.d_decay, b.ld_dd}});
   const Chain c = chain_of(a, p, ws, pairs ? 2 : 1);
@@ -635,7 +696,7 @@ int launch_gated_scan_bwd(const RecurBwdArgs& b, void* ws, int64_t ws_bytes, hip
   TESM_REQUIRE(blocks < (1LL << 31), kErrUnsupported, "gated scan backward: too many tiles for one call");
   float* sums = b.d_bias ? reinterpret_cast<float*>(static_cast<char*>(ws) + p.at_sums) : nullptr;
   if (blocks > 0) {
-    if (int rc = reset(a, p, c, ws, sums != nullptr, st)) return rc;
+    if (int rc = reset(a, p, c, pairs ? 2 : 1, sums, st)) return rc;
     constexpr int T = 64 * kWaves;
     const unsigned n = static_cast<unsigned>(blocks);
     if (a.dt == kF32)
