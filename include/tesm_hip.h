@@ -634,7 +634,8 @@ int tesm_hip_reorder_rows(const tesm_hip_rows* t, int64_t count, const int64_t* 
  *   a = sigmoid(decay[t,c] + bias[c]),  h[t,c] = a h[t-1,c] + sigmoid(write[t,c]) tanh(value[t,c]).
  * The rows are B sequences of L (S = B), or with seq_starts S sequences packed one behind the other in one row axis (B = 1, L
  * rows): sequence s is rows seq_starts[s] .. seq_starts[s+1]-1 (starts outside the rows count as the nearest, one below an
- * earlier one as that one); rows in front of the first and behind the last are neither read nor written.  h0 / h_out: (S, C) float32,
+ * earlier one as that one); rows in front of the first and behind the last are not read, and left as they are in the outputs or, with
+ * zero_rest, set to zero.  h0 / h_out: (S, C) float32,
  * the states before and after each sequence (NULL h0: zeros).  States are float32; results repeat bit for bit.  carries:
  * (tesm_hip_gated_scan_slots, C) float32, what the backward call needs (NULL: not kept).  Fewer than 2^31 rows, C and S
  * below 2^24.  Outputs must not overlap operands or each other (columns of the same wider rows do not overlap). */
@@ -650,6 +651,7 @@ typedef struct tesm_hip_gates {
   const float* bias;          /* optional (C) */
   const int32_t* seq_starts;  /* optional (S + 1) */
   const float* h0;            /* optional (S, C) */
+  int zero_rest;              /* with seq_starts and S >= 1 */
 } tesm_hip_gates;
 
 typedef struct tesm_hip_recurrence {

@@ -211,7 +211,7 @@ class Gates(ctypes.Structure):
         ("dt", I32),
         ("B", I64), ("L", I64), ("C", I64), ("S", I64),
         ("value", P), ("ld_value", I64), ("write", P), ("ld_write", I64), ("decay", P), ("ld_decay", I64),
-        ("bias", P), ("seq_starts", P), ("h0", P),
+        ("bias", P), ("seq_starts", P), ("h0", P), ("zero_rest", I32),
     ]
 
 

@@ -2149,6 +2149,7 @@ RecurArgs recur_args(const tesm_hip_gates& p) {
   a.bias = p.bias;
   a.seq_starts = p.seq_starts;
   a.h0 = p.h0;
+  a.zero_rest = p.zero_rest;
   return a;
 }
 RecurArgs recur_args(const tesm_hip_recurrence& p) {

@@ -10,7 +10,7 @@
 // A tile with k along its rows has rows of BK values, 16-byte chunk q of row r at q ^ (r / (16 / CPR)) % CPR (CPR chunks per
 // row): 16 rows' reads of one chunk fall on 256 different bytes.  A tile with k down its rows has BK rows of BM (BN) values; its
 // fragments come through the transposing read of 4 x 16 values (lane i of 16 gives the address of 4 columns of row i / 4 and
-// gets column i of the 4 rows), with the 64-byte block index of row k turned by k % 4 so that 4 rows fall on different banks.
+// gets column i of the 4 rows), with the 64-byte blocks of row k turned by k so that 4 rows fall on different banks.
 // What lies behind the end of the contraction is read as zeros (an offset beyond the buffer's range), what lies behind the last
 // row or column repeats the last one and is never stored.
 //
@@ -61,6 +61,14 @@ struct Shape {
   static constexpr int AHEAD = OWN ? 2 : NS - 1;  // tiles between the one in work and the one asked for
 };
 
+// How far the 64-byte blocks of row k of a tile that lies down are turned: 4 rows' blocks then fall on different banks (of 256
+// bytes: rows of 128 are two to that).
+template <int BX>
+__device__ __forceinline__ int turn_of(int k) {
+  static_assert(BX >= 64, "rows of two blocks at least");
+  return BX == 64 ? (k >> 1) & 1 : k & 3;
+}
+
 // Where lane `lane` of a 1 KB block reads: the offset from the tile's first value, and the value of k (within the tile).
 template <int BK, int BX, bool DOWN>
 __device__ __forceinline__ void load_place(int block, int lane, int64_t ld, int64_t extent, uint32_t& off, int& k) {
@@ -73,7 +81,7 @@ __device__ __forceinline__ void load_place(int block, int lane, int64_t ld, int6
   } else {
     constexpr int UPR = BX / 8, RPB = 64 / UPR;
     k = block * RPB + lane / UPR;
-    const int u = (lane % UPR) ^ ((k & 3) << 2);
+    const int u = (lane % UPR) ^ (turn_of<BX>(k) << 2);
     const int64_t x = u * 8 < extent ? u * 8 : extent - 8;
     off = static_cast<uint32_t>(k * ld * 2 + x * 2);
   }
@@ -94,7 +102,7 @@ struct Frag {
       const int row = 8 * (lane >> 5) + kk;
 #pragma unroll
       for (int i = 0; i < T; ++i)
-        at[i] = row * BX * 2 + ((((x0 >> 5) + i) ^ kk) * 4 + low) * 16 + 8 * (i16 & 1);
+        at[i] = row * BX * 2 + ((((x0 >> 5) + i) ^ turn_of<BX>(kk)) * 4 + low) * 16 + 8 * (i16 & 1);
       turn = 0;
     }
   }
@@ -404,13 +412,14 @@ int run_product(const ProductArgs& a, hipStream_t st) {
 
 // Tile sizes.  Large: 256 x 256 results (a gated pair: 256 x 128 of each product) on 8 waves of 128 x 64, one workgroup per CU.
 // Mid: 128 x 128 (128 x 64) on 4 waves of 64 x 64, two workgroups per CU.  Small: the same tiles with four stages, one per CU, for
-// grids that have no second one anyway.  In us per round of the CUs, with k thousand values of the contraction: 25 k + 8, 15 k + 5 (9 k +
-// 5 where half the places stay empty) and 7.6 k + 4; a split adds the float32 results it writes and reads again.  Measured,
+// grids that have no second one anyway.  Tiny: 64 x 64 on 4 waves, two per CU.  In us per round of the CUs, with k thousand values of
+// the contraction: 25 k + 8, 15 k + 5 (9 k + 5 where half the places stay empty), 7.6 k + 4 and 5.5 k + 4 (4 k + 3.5); a split adds the
+// float32 results it writes and reads again.  Measured,
 // bfloat16: 8192 x 16384 x 4096 879 us large (1.25 Pflop/s; the library's product 1.29), mid 1075, small 1240; 8192 x 4096 x 768 58,
-// 69, 83; 8192 x 768 x 2048 47, 31, 39; 4096 x 768 x 8192 147, 77, 66.  Operands that lie down: 8192 x 16384 x 4096 864 us with one, 860
+// 69, 83; 8192 x 768 x 2048 47, 31, 39; 4096 x 768 x 8192 147, 77, 66; 512 x 768 x 2048 43, 23, 19, tiny 11; 1024 x 2048 x 768 23, 13, 11, 10.  Operands that lie down: 8192 x 16384 x 4096 864 us with one, 860
 // with both (the library 950 and 1080).  Tiles of 32 values of k instead of 64 cost 20 % where rows run along k (64-byte
 // pieces), stages of 128 x 256 with 8 waves of 64 x 64 another 10 %.
-enum Config : int { kLarge, kMid, kSmall };
+enum Config : int { kLarge, kMid, kSmall, kTiny };
 struct Plan {
   Config config = kSmall;
   int splits = 1;
@@ -426,10 +435,12 @@ Plan plan_product(ProductKind kind, int64_t M, int64_t N, int64_t K, int pairs, 
     const double ks = k / s, joined = s == 1 ? 0.0 : 6.0 + 2.0 * s * 4.0 * static_cast<double>(M) * static_cast<double>(N) / 5.0e6;
     const int64_t large = tiles(256, 256) * s, mid = tiles(128, 128) * s;
     const int64_t rest = mid % (2 * cus);
-    const double cost[3] = {static_cast<double>((large + cus - 1) / cus) * (25.4 * ks + 8.0),
+    const int64_t tiny = tiles(64, kind == kProdGated ? 128 : 64) * s, few = tiny % (2 * cus);
+    const double cost[4] = {static_cast<double>((large + cus - 1) / cus) * (25.4 * ks + 8.0),
                             static_cast<double>(mid / (2 * cus)) * (15.3 * ks + 5.0) + (rest == 0 ? 0.0 : rest <= cus ? 9.4 * ks + 5.0 : 15.3 * ks + 5.0),
-                            static_cast<double>((mid + cus - 1) / cus) * (7.6 * ks + 4.0)};
-    for (int c = 0; c < 3; ++c)
+                            static_cast<double>((mid + cus - 1) / cus) * (7.6 * ks + 4.0),
+                            static_cast<double>(tiny / (2 * cus)) * (5.5 * ks + 4.0) + (few == 0 ? 0.0 : few <= cus ? 4.0 * ks + 3.5 : 5.5 * ks + 4.0)};
+    for (int c = 0; c < 4; ++c)
       if (cost[c] + joined < least) {
         least = cost[c] + joined;
         best = {static_cast<Config>(c), s};
@@ -445,11 +456,13 @@ int pick(const ProductArgs& a, hipStream_t st) {
   if constexpr (KIND == kProdGated) {
     if (p.config == kLarge) return run_product<KIND, DT, ADOWN, BDOWN, 4, 2, 2, 2, 64, 2>(a, st);
     if (p.config == kMid) return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 1, 64, 2>(a, st);
-    return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 1, 64, 4>(a, st);
+    if (p.config == kSmall) return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 1, 64, 4>(a, st);
+    return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 1, 1, 64, 3>(a, st);
   } else {
     if (p.config == kLarge) return run_product<KIND, DT, ADOWN, BDOWN, 2, 4, 4, 2, 64, 2>(a, st);
     if (p.config == kMid) return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 2, 64, 2>(a, st);
-    return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 2, 64, 4>(a, st);
+    if (p.config == kSmall) return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 2, 64, 4>(a, st);
+    return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 1, 1, 64, 4>(a, st);
   }
 }
 

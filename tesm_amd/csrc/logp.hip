@@ -25,13 +25,21 @@ constexpr double kLn2 = 0.69314718055994530942;
 struct LogpSum {
   double ref, sum, dot;
 };
-__device__ __forceinline__ LogpSum join(const LogpSum& a, const LogpSum& b) {
-  const double ref = fmax(a.ref, b.ref);  // (equal references may be infinite)
-  const double da = a.ref == ref ? 0.0 : a.ref - ref, db = b.ref == ref ? 0.0 : b.ref - ref;
-  // (a part of -infinities alone has an infinite distance and nothing to add; a NaN sum stays one)
-  const double fa = exp(da), fb = exp(db);
-  const double ma = fa == 0.0 ? 0.0 * a.sum : fa * (a.dot + da * a.sum), mb = fb == 0.0 ? 0.0 * b.sum : fb * (b.dot + db * b.sum);
-  return {ref, fa * a.sum + fb * b.sum, ma + mb};
+// The sums of groups of WIDTH lanes, on every lane of a group.  (Equal references may be infinite; a part of -infinities alone has an
+// infinite distance and nothing to add; a NaN sum stays one.)
+template <int WIDTH>
+__device__ __forceinline__ LogpSum join_lanes(const LogpSum& a) {
+  double ref = a.ref;
+#pragma unroll
+  for (int d = 1; d < WIDTH; d <<= 1) ref = fmax(ref, __shfl_xor(ref, d));
+  const double far = a.ref == ref ? 0.0 : a.ref - ref, f = exp(far);
+  double sum = f * a.sum, dot = f == 0.0 ? 0.0 * a.sum : f * (a.dot + far * a.sum);
+#pragma unroll
+  for (int d = 1; d < WIDTH; d <<= 1) {
+    sum += __shfl_xor(sum, d);
+    dot += __shfl_xor(dot, d);
+  }
+  return {ref, sum, dot};
 }
 
 // What a row's sums and list say, by one wave.
@@ -102,32 +110,43 @@ __global__ __launch_bounds__(64 * kLogpWaves) void logp_row_kernel(LogpArgs a, i
   if (wave) return;
   if constexpr (LIST)
     for (int w = 1; w < kLogpWaves; ++w) p.list = merge_lists(p.list, buffer[w][lane]);
-  LogpSum o = ps[0];
-  for (int w = 1; w < kLogpWaves; ++w) o = join(o, ps[w]);
+  const LogpSum o = join_lanes<kLogpWaves>(ps[lane % kLogpWaves]);
   if (parts == 1) return finish_row(a, r, o, p.list, DT);
   if constexpr (LIST)
     if (lane < m) keys[static_cast<int64_t>(blockIdx.x) * m + lane] = p.list;
   if (lane == 0) sums[blockIdx.x] = o;
 }
 
-// A wave per row joins its parts: their sums by a lane each, their lists in runs of 64 keys.
+// A workgroup per row joins its parts: a lane each for their sums, and, with lists, a wave each for runs of 64 keys, then merged in
+// pairs.
 template <int DT, bool LIST>
-__global__ __launch_bounds__(64) void logp_join_kernel(LogpArgs a, int m, int parts, const uint64_t* keys, const LogpSum* sums) {
+__global__ __launch_bounds__(64 * (LIST ? 8 : 1)) void logp_join_kernel(LogpArgs a, int m, int parts, const uint64_t* keys, const LogpSum* sums) {
   const int64_t r = blockIdx.x;
-  const int lane = threadIdx.x & 63;
-  uint64_t list = 0;
-  if constexpr (LIST) {
-    const uint64_t* kr = keys + r * parts * m;
-#pragma unroll 1
-    for (int c = 0; c < parts * m; c += 64) list = merge64(list, c + lane < parts * m ? kr[c + lane] : 0);
-  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const LogpSum* sr = sums + r * parts;
   LogpSum s = {-__builtin_inf(), 0.0, 0.0};
-  for (int c = lane; c < parts; c += 64) s = join(s, sr[c]);
+  if (wave == 0 && lane < parts) s = sr[lane];
+  uint64_t list = 0;
+  if constexpr (LIST) {
+    __shared__ uint64_t lists[8][64];
+    const uint64_t* kr = keys + r * parts * m;
+    const int count = parts * m;
 #pragma unroll 1
-  for (int d = 1; d < 64; d <<= 1) {  // (in the same order on every lane's side)
-    const LogpSum o = {__shfl_xor(s.ref, d), __shfl_xor(s.sum, d), __shfl_xor(s.dot, d)};
-    s = lane & d ? join(o, s) : join(s, o);
+    for (int c = wave * 64; c < count; c += 512) list = merge64(list, c + lane < count ? kr[c + lane] : 0);
+    const int waves = count < 512 ? (count + 63) / 64 : 8;
+#pragma unroll 1
+    for (int d = 1; d < waves; d <<= 1) {
+      lists[wave][lane] = list;
+      __syncthreads();
+      if (wave % (2 * d) == 0 && wave + d < waves) list = merge_lists(list, lists[wave + d][lane]);
+      __syncthreads();
+    }
+    if (wave) return;
+  }
+  s = join_lanes<64>(s);
+  for (int c = 64; c < parts; c += 64) {  // (more than 64 parts: joined 64 at a time)
+    const LogpSum more = join_lanes<64>(c + lane < parts ? sr[c + lane] : LogpSum{-__builtin_inf(), 0.0, 0.0});
+    s = join_lanes<2>(lane & 1 ? more : s);
   }
   finish_row(a, r, s, list, DT);
 }
@@ -247,7 +266,7 @@ int launch_token_logp(const LogpArgs& a, void* ws, int64_t ws_bytes, hipStream_t
   do {                                                                                                                          \
     logp_row_kernel<DT, LIST><<<blocks, T, 0, TESM_LOGGED(st, logp_row_kernel<DT, LIST>)>>>(a, m, parts, part, keys, sums);     \
     if (parts > 1)                                                                                                              \
-      logp_join_kernel<DT, LIST><<<static_cast<unsigned>(a.rows), 64, 0, TESM_LOGGED(st, logp_join_kernel<DT, LIST>)>>>(        \
+      logp_join_kernel<DT, LIST><<<static_cast<unsigned>(a.rows), LIST ? 512 : 64, 0, TESM_LOGGED(st, logp_join_kernel<DT, LIST>)>>>(        \
           a, m, parts, keys, sums);                                                                                             \
   } while (0)
   if (a.dt == kBF16) {

@@ -19,6 +19,7 @@ struct RecurArgs {
   const float* bias = nullptr;         // optional (C)
   const int32_t* seq_starts = nullptr;  // optional (S + 1)
   const float* h0 = nullptr;           // optional (S, C)
+  int zero_rest = 0;                   // rows of no sequence: outputs set to zero instead of left
   void* h = nullptr;
   int64_t ld_h = 0;
   float* h_out = nullptr;    // (S, C)

@@ -21,14 +21,15 @@
 #include <type_traits>
 #include <utility>
 
+#include "linear_dev.h"
 #include "recur.h"
 
 namespace tesm {
 
 namespace {
 
-constexpr int kWaves = 8, kRows = 8, kTile = kWaves * kRows, kGroup = 16;
-static_assert(kTile == kRecurRows && kGroup == 2 * kWaves, "a wave looks after two earlier tiles");
+constexpr int kWaves = 8, kGroup = 16;
+static_assert(kGroup == 2 * kWaves, "a wave looks after two earlier tiles");
 constexpr int kSpinLimit = 1 << 20;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -79,15 +80,27 @@ __device__ __forceinline__ Tanh tanh2(float x) {
 // ---------------------------------------------------------------------------
 // a lane's channels of a row
 // ---------------------------------------------------------------------------
-template <int DT, int CPT>
+// NT: past the caches, for arrays that are larger than they are and whose rows begin on cache lines.
+template <typename T>
+__device__ __forceinline__ T take(const char* p, bool nt) {
+  return nt ? __builtin_nontemporal_load(reinterpret_cast<const T*>(p)) : *reinterpret_cast<const T*>(p);
+}
+template <typename T>
+__device__ __forceinline__ void give(char* p, T v, bool nt) {
+  if (nt)
+    __builtin_nontemporal_store(v, reinterpret_cast<T*>(p));
+  else
+    *reinterpret_cast<T*>(p) = v;
+}
+template <int DT, int CPT, bool NT>
 struct Row {
   uint32_t w;  // one float32, one bfloat16 or two
   // (row: the same for all lanes; off: the lane's bytes in it)
   __device__ __forceinline__ void load(const char* row, uint32_t off) {
     if constexpr (DT == kBF16 && CPT == 1)
-      w = *reinterpret_cast<const uint16_t*>(row + off);
+      w = take<uint16_t>(row + off, NT);
     else
-      w = *reinterpret_cast<const uint32_t*>(row + off);
+      w = take<uint32_t>(row + off, NT);
   }
   __device__ __forceinline__ float get(int j) const {
     if constexpr (CPT == 2) return __uint_as_float(j ? w & 0xffff0000u : w << 16);
@@ -95,11 +108,11 @@ struct Row {
   }
   static __device__ __forceinline__ void store(char* row, uint32_t off, const float (&v)[CPT]) {
     if constexpr (CPT == 2)
-      *reinterpret_cast<uint32_t*>(row + off) = pack_bf16x2(v[0], v[1]);
+      give<uint32_t>(row + off, pack_bf16x2(v[0], v[1]), NT);
     else if constexpr (DT == kBF16)
-      *reinterpret_cast<uint16_t*>(row + off) = f32_to_bf16(v[0]);
+      give<uint16_t>(row + off, f32_to_bf16(v[0]), NT);
     else
-      *reinterpret_cast<float*>(row + off) = v[0];
+      give<float>(row + off, v[0], NT);
   }
 };
 // The wave's first row of an array, and its rows' distance in bytes.
@@ -122,6 +135,7 @@ struct Chain {
   const int32_t* starts = nullptr;   // packed: S + 1 starts, inside the rows and not decreasing
   int slots = 0;
   int G = 0, tiles = 0;  // channel groups; tiles per sequence of a dense batch
+  int kept = 0;          // kept carries per sequence of a dense batch
   int spin_limit = 0;
 };
 constexpr int kTicketStride = 64;
@@ -133,6 +147,7 @@ struct Place {  // (rows, sequences and slots are below 2^31)
 };
 
 // The tile of slot `at` in walking order; `back`: from the end.
+template <int ROWS>
 __device__ __forceinline__ Place place_of(const RecurArgs& a, const Chain& c, int at, bool back) {
   Place p;
   if (!c.starts) {
@@ -146,11 +161,11 @@ __device__ __forceinline__ Place place_of(const RecurArgs& a, const Chain& c, in
     return p;
   }
   const int slot = back ? c.slots - 1 - at : at;
-  // sequence s has the slots from start / kTile + s on, at least one
+  // sequence s has the slots from start / ROWS + s on, at least one
   int lo = 0, hi = static_cast<int>(a.S);
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (__builtin_amdgcn_readfirstlane(c.starts[mid]) / kTile + mid <= slot)
+    if (__builtin_amdgcn_readfirstlane(c.starts[mid]) / ROWS + mid <= slot)
       lo = mid;
     else
       hi = mid;
@@ -158,9 +173,9 @@ __device__ __forceinline__ Place place_of(const RecurArgs& a, const Chain& c, in
   p.seq = lo;
   p.row0 = __builtin_amdgcn_readfirstlane(c.starts[lo]);
   p.len = __builtin_amdgcn_readfirstlane(c.starts[lo + 1]) - p.row0;
-  p.slot0 = p.row0 / kTile + lo;
+  p.slot0 = p.row0 / ROWS + lo;
   p.tile = slot - p.slot0;
-  p.tiles = p.len > 0 ? (p.len + kTile - 1) / kTile : 1;  // (an empty sequence hands its state through)
+  p.tiles = p.len > 0 ? (p.len + ROWS - 1) / ROWS : 1;  // (an empty sequence hands its state through)
   if (p.tile < 0 || p.tile >= p.tiles) p.tiles = -1;
   return p;
 }
@@ -187,12 +202,12 @@ struct ChainTile {
 };
 
 // The state entering the wave's rows.  part: the wave's (A, U).  In walking order: pos of the tile, order of the wave; at(p): where
-// position p publishes this lane's values; first: the sequence's own first state.  `entry` returns the tile's carry, `leave`, to the
-// first wave in order, the state behind the tile.
+// position p publishes this lane's values; first: the sequence's own first state.  `leave` returns, to the first wave in order, the
+// state behind the tile.
 template <int CPT, typename At, typename First>
 __device__ __forceinline__ void chain_carry(const Chain& c, ChainTile<CPT>& sh, int lane, int order, int pos, int count,
                                             const float2 (&part)[CPT], At&& at, First&& first, float (&carry)[CPT],
-                                            float (&entry)[CPT], float (&leave)[CPT]) {
+                                            float (&leave)[CPT]) {
 #pragma unroll
   for (int j = 0; j < CPT; ++j) sh.part[order][lane * CPT + j] = part[j];
   if (order == 0 && lane == 0) sh.bad = 0;
@@ -260,7 +275,6 @@ __device__ __forceinline__ void chain_carry(const Chain& c, ChainTile<CPT>& sh, 
       x = __builtin_fmaf(q.x, x, q.y);
     }
     if (bad) x = __builtin_nanf("");
-    entry[j] = x;
     if (order == 0) {
       leave[j] = __builtin_fmaf(all[j].x, x, all[j].y);
       if (more && last_of_group) publish(c, at(pos) + j, 0.0f, leave[j]);
@@ -288,19 +302,20 @@ __device__ __forceinline__ int take_ticket(const Chain& c, ChainTile<CPT>& sh, i
 struct Part {
   int row, n;
 };
+template <int T>
 __device__ __forceinline__ Part part_of(const Place& p, int wave) {
-  const int t0 = p.tile * kTile + wave * kRows, left = p.tiles > 0 ? p.len - t0 : 0;
-  return {p.row0 + t0, left < 0 ? 0 : left < kRows ? left : kRows};
+  const int t0 = (p.tile * kWaves + wave) * T, left = p.tiles > 0 ? p.len - t0 : 0;
+  return {p.row0 + t0, left < 0 ? 0 : left < T ? left : T};
 }
 // Its inputs, rows behind the end read as the last one.
-template <int DT, int CPT, int ARRAYS, bool WHOLE>
+template <int DT, int CPT, bool NT, int T, bool WHOLE, int ARRAYS>
 __device__ __forceinline__ void load_rows(const Part& q, const void* const (&&p)[ARRAYS], const int64_t (&&ld)[ARRAYS], uint32_t off,
-                                          Row<DT, CPT> (&to)[ARRAYS][kRows]) {
+                                          Row<DT, CPT, NT> (&to)[ARRAYS][T]) {
   RowsOf r[ARRAYS];
 #pragma unroll
   for (int k = 0; k < ARRAYS; ++k) r[k] = rows_of<DT>(p[k], ld[k], q.row);
 #pragma unroll
-  for (int i = 0; i < kRows; ++i)
+  for (int i = 0; i < T; ++i)
 #pragma unroll
     for (int k = 0; k < ARRAYS; ++k) {
       to[k][i].load(r[k].p, off);
@@ -308,33 +323,33 @@ __device__ __forceinline__ void load_rows(const Part& q, const void* const (&&p)
     }
 }
 
-template <int DT, int CPT>
+template <int DT, int CPT, bool NT, int T>
 __global__ __launch_bounds__(64 * kWaves) void recur_fwd_kernel(RecurArgs a, Chain c) {
   __shared__ ChainTile<CPT> sh;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = blockIdx.x % c.G;
-  const Place p = place_of(a, c, take_ticket(c, sh, g), false);
+  const Place p = place_of<kWaves * T>(a, c, take_ticket(c, sh, g), false);
   if (p.tiles < 0) return;
   const int64_t mine = static_cast<int64_t>(g) * 64 * CPT + lane * CPT;
   const bool on = mine < a.C;
   const int64_t ch = on ? mine : a.C - CPT;
   constexpr int ES = DT == kBF16 ? 2 : 4;
   const uint32_t off = static_cast<uint32_t>(ch * ES);
-  const Part q = part_of(p, wave);
-  float A[kRows][CPT], U[kRows][CPT];
+  const Part q = part_of<T>(p, wave);
+  float A[T][CPT], U[T][CPT];
   float2 part[CPT];
 #pragma unroll
   for (int j = 0; j < CPT; ++j) part[j] = make_float2(1.0f, 0.0f);
   // (whole parts apart: without a branch per row their rows are worked on side by side)
   auto gates = [&](auto whole) __attribute__((always_inline)) {
     constexpr bool WHOLE = decltype(whole)::value;
-    Row<DT, CPT> raw[3][kRows];
-    load_rows<DT, CPT, 3, WHOLE>(q, {a.decay, a.write, a.value}, {a.ld_d, a.ld_w, a.ld_v}, off, raw);
+    Row<DT, CPT, NT> raw[3][T];
+    load_rows<DT, CPT, NT, T, WHOLE, 3>(q, {a.decay, a.write, a.value}, {a.ld_d, a.ld_w, a.ld_v}, off, raw);
     float nb[CPT];
 #pragma unroll
     for (int j = 0; j < CPT; ++j) nb[j] = a.bias ? a.bias[ch + j] * -kLog2e : 0.0f;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
+    for (int i = 0; i < T; ++i)
 #pragma unroll
       for (int j = 0; j < CPT; ++j) {
         A[i][j] = sig(raw[0][i].get(j), nb[j]);
@@ -342,74 +357,85 @@ __global__ __launch_bounds__(64 * kWaves) void recur_fwd_kernel(RecurArgs a, Cha
         if (WHOLE || i < q.n) part[j] = make_float2(A[i][j] * part[j].x, __builtin_fmaf(A[i][j], part[j].y, U[i][j]));
       }
   };
-  if (q.n == kRows)
+  if (q.n == T)
     gates(std::true_type{});
   else if (q.n > 0)
     gates(std::false_type{});
-  float h[CPT], entry[CPT], leave[CPT];
+  float h[CPT], leave[CPT];
   auto first = [&](int j) { return a.h0 ? a.h0[p.seq * a.C + ch + j] : 0.0f; };
   auto at = [&](int k) { return ((static_cast<int64_t>(g) * c.slots + (p.slot0 + k)) * 64 + lane) * CPT; };
-  chain_carry<CPT>(c, sh, lane, wave, p.tile, p.tiles, part, at, first, h, entry, leave);
+  chain_carry<CPT>(c, sh, lane, wave, p.tile, p.tiles, part, at, first, h, leave);
   if (!on) return;
-  if (wave == 0) {
+  if (wave == 0 && p.tile == p.tiles - 1) {
 #pragma unroll
-    for (int j = 0; j < CPT; ++j) {
-      if (a.carries) a.carries[static_cast<int64_t>(p.slot0 + p.tile) * a.C + ch + j] = entry[j];
-      if (p.tile == p.tiles - 1) a.h_out[p.seq * a.C + ch + j] = leave[j];
-    }
+    for (int j = 0; j < CPT; ++j) a.h_out[p.seq * a.C + ch + j] = leave[j];
+  }
+  // the state in front of every kRecurRows rows (an empty sequence has one such place)
+  const int t0 = (p.tile * kWaves + wave) * T;
+  if (a.carries && t0 % kRecurRows == 0 && (t0 < p.len || t0 == 0)) {
+    const int64_t slot0 = c.starts ? p.row0 / kRecurRows + p.seq : static_cast<int64_t>(p.seq) * c.kept;
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) a.carries[(slot0 + t0 / kRecurRows) * a.C + ch + j] = h[j];
   }
   auto states = [&](auto whole) __attribute__((always_inline)) {
     constexpr bool WHOLE = decltype(whole)::value;
     RowsOf rh = rows_of<DT>(a.h, a.ld_h, q.row);
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
+    for (int i = 0; i < T; ++i) {
       if (!WHOLE && i >= q.n) break;
 #pragma unroll
       for (int j = 0; j < CPT; ++j) h[j] = __builtin_fmaf(A[i][j], h[j], U[i][j]);
-      Row<DT, CPT>::store(rh.p, off, h);
+      Row<DT, CPT, NT>::store(rh.p, off, h);
       rh.p += rh.step;
     }
   };
-  if (q.n == kRows)
+  if (q.n == T)
     states(std::true_type{});
   else
     states(std::false_type{});
 }
 
-template <int DT, int CPT>
+template <int DT, int CPT, bool NT>
 __global__ __launch_bounds__(64 * kWaves, 4) void recur_bwd_kernel(RecurBwdArgs b, Chain c, float* sums) {
+  constexpr int T = kRecurRows / kWaves;
   __shared__ ChainTile<CPT> sh;
   __shared__ float2 fwd[kWaves][64 * CPT];
   const RecurArgs& a = b.in;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int order = kWaves - 1 - wave;  // in walking order, from the end
   const int g = blockIdx.x % c.G;
-  const Place p = place_of(a, c, take_ticket(c, sh, g), true);
-  if (p.tiles < 0) return;
+  const Place p = place_of<kRecurRows>(a, c, take_ticket(c, sh, g), true);
   const int64_t mine = static_cast<int64_t>(g) * 64 * CPT + lane * CPT;
   const bool on = mine < a.C;
   const int64_t ch = on ? mine : a.C - CPT;
+  if (p.tiles < 0) {  // (a slot without a tile: nothing to add to the bias's sums)
+    if (sums && wave == 0 && on) {
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) sums[static_cast<int64_t>(p.slot0 + p.tile) * a.C + ch + j] = 0.0f;
+    }
+    return;
+  }
   constexpr int ES = DT == kBF16 ? 2 : 4;
   const uint32_t off = static_cast<uint32_t>(ch * ES);
-  const Part q = part_of(p, wave);
+  const Part q = part_of<T>(p, wave);
   float kept[CPT];
 #pragma unroll
   for (int j = 0; j < CPT; ++j) kept[j] = a.carries[static_cast<int64_t>(p.slot0 + p.tile) * a.C + ch + j];
   // Per row: a, and what the gradient is multiplied with for value, write and decay; U: u.
-  Row<DT, CPT> dh[kRows];
-  float A[kRows][CPT], U[kRows][CPT], fv[kRows][CPT], fw[kRows][CPT], fd[kRows][CPT];
+  Row<DT, CPT, NT> dh[T];
+  float A[T][CPT], U[T][CPT], fv[T][CPT], fw[T][CPT], fd[T][CPT];
   float2 part[CPT], from[CPT];  // the rows backwards and forwards
 #pragma unroll
   for (int j = 0; j < CPT; ++j) part[j] = from[j] = make_float2(1.0f, 0.0f);
   auto gates = [&](auto whole) __attribute__((always_inline)) {
     constexpr bool WHOLE = decltype(whole)::value;
-    Row<DT, CPT> raw[4][kRows];
-    load_rows<DT, CPT, 4, WHOLE>(q, {a.decay, a.write, a.value, b.grad}, {a.ld_d, a.ld_w, a.ld_v, b.ld_g}, off, raw);
+    Row<DT, CPT, NT> raw[4][T];
+    load_rows<DT, CPT, NT, T, WHOLE, 4>(q, {a.decay, a.write, a.value, b.grad}, {a.ld_d, a.ld_w, a.ld_v, b.ld_g}, off, raw);
     float nb[CPT];
 #pragma unroll
     for (int j = 0; j < CPT; ++j) nb[j] = a.bias ? a.bias[ch + j] * -kLog2e : 0.0f;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
+    for (int i = 0; i < T; ++i) {
       dh[i] = raw[3][i];
 #pragma unroll
       for (int j = 0; j < CPT; ++j) {
@@ -424,24 +450,24 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recur_bwd_kernel(RecurBwdArgs 
       }
     }
 #pragma unroll
-    for (int i = kRows - 1; i >= 0; --i)
+    for (int i = T - 1; i >= 0; --i)
 #pragma unroll
       for (int j = 0; j < CPT; ++j)
         if (WHOLE || i < q.n) part[j].y = A[i][j] * (part[j].y + dh[i].get(j));
 #pragma unroll
     for (int j = 0; j < CPT; ++j) part[j].x = from[j].x;
   };
-  if (q.n == kRows)
+  if (q.n == T)
     gates(std::true_type{});
   else if (q.n > 0)
     gates(std::false_type{});
 #pragma unroll
   for (int j = 0; j < CPT; ++j) fwd[wave][lane * CPT + j] = from[j];
   // The chain's state is c; in front of it (behind the last row) stands the final state's gradient.
-  float back[CPT], entry[CPT], leave[CPT];
+  float back[CPT], leave[CPT];
   auto first = [&](int j) { return b.grad_state ? b.grad_state[p.seq * a.C + ch + j] : 0.0f; };
   auto at = [&](int k) { return ((static_cast<int64_t>(g) * c.slots + (p.slot0 + (p.tiles - 1 - k))) * 64 + lane) * CPT; };
-  chain_carry<CPT>(c, sh, lane, order, p.tiles - 1 - p.tile, p.tiles, part, at, first, back, entry, leave);
+  chain_carry<CPT>(c, sh, lane, order, p.tiles - 1 - p.tile, p.tiles, part, at, first, back, leave);
   // the states again, from the tile's kept carry
   float db[CPT];
 #pragma unroll
@@ -454,7 +480,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recur_bwd_kernel(RecurBwdArgs 
         x = __builtin_fmaf(f.x, x, f.y);
       }
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) {
+      for (int i = 0; i < T; ++i) {
         fd[i][j] *= x;
         x = __builtin_fmaf(A[i][j], x, U[i][j]);
       }
@@ -462,10 +488,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recur_bwd_kernel(RecurBwdArgs 
   }
   auto grads = [&](auto whole) __attribute__((always_inline)) {
     constexpr bool WHOLE = decltype(whole)::value;
-    const int64_t row = static_cast<int64_t>(q.row) + (WHOLE ? kRows : q.n) - 1;
+    const int64_t row = static_cast<int64_t>(q.row) + (WHOLE ? T : q.n) - 1;
     RowsOf rv = rows_of<DT>(b.d_value, b.ld_dv, row), rw = rows_of<DT>(b.d_write, b.ld_dw, row), rd = rows_of<DT>(b.d_decay, b.ld_dd, row);
 #pragma unroll
-    for (int i = kRows - 1; i >= 0; --i) {
+    for (int i = T - 1; i >= 0; --i) {
       if (!WHOLE && i >= q.n) continue;
       float ov[CPT], ow[CPT], od[CPT];
 #pragma unroll
@@ -477,14 +503,14 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recur_bwd_kernel(RecurBwdArgs 
         db[j] += od[j];
         back[j] = A[i][j] * grad;
       }
-      Row<DT, CPT>::store(rv.p, off, ov);
-      Row<DT, CPT>::store(rw.p, off, ow);
-      Row<DT, CPT>::store(rd.p, off, od);
+      Row<DT, CPT, NT>::store(rv.p, off, ov);
+      Row<DT, CPT, NT>::store(rw.p, off, ow);
+      Row<DT, CPT, NT>::store(rd.p, off, od);
       rv.p -= rv.step, rw.p -= rw.step, rd.p -= rd.step;
     }
   };
   if (on) {
-    if (q.n == kRows)
+    if (q.n == T)
       grads(std::true_type{});
     else
       grads(std::false_type{});
@@ -509,7 +535,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recur_bwd_kernel(RecurBwdArgs 
   }
 }
 
-// The bias gradient: tiles' sums (slots without rows hold zeros), 16 runs of slots per workgroup of 64 channels, joined in order.
+// The bias gradient: tiles' sums (zeros where a slot has no tile), 16 runs of slots per workgroup of 64 channels, joined in order.
 __global__ __launch_bounds__(1024) void recur_bias_kernel(const float* sums, int64_t slots, int64_t C, float* out) {
   __shared__ float part[16][64];
   const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
@@ -560,9 +586,23 @@ __global__ __launch_bounds__(256) void recur_reset_kernel(uint4* tickets, int64_
   else if (i < n_tickets + n_values)
     values[i - n_tickets] = make_uint4(kUnset, kUnset, kUnset, kUnset);
 }
-__global__ __launch_bounds__(256) void recur_zero_kernel(float* p, int64_t n) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i < n) p[i] = 0.0f;
+// The rows of no sequence set to zero in up to three arrays, a row per workgroup (starts in order).
+struct RestArgs {
+  void* p[3];
+  int64_t ld[3];
+  int64_t C, rows, S;
+  const int32_t* starts;
+};
+template <int DT>
+__global__ __launch_bounds__(256) void recur_rest_kernel(RestArgs a) {
+  const int64_t lo = a.starts[0], hi = a.starts[a.S];
+  for (int64_t i = blockIdx.x; i < lo + (a.rows - hi); i += gridDim.x) {
+    const int64_t r = i < lo ? i : hi + (i - lo);
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (a.p[k])
+        for (int64_t c = threadIdx.x; c < a.C; c += 256) st<DT>(a.p[k], r * a.ld[k] + c, 0.0f);
+  }
 }
 
 template <int DT>
@@ -596,17 +636,27 @@ bool in_pairs(int dt, int64_t C, std::initializer_list<std::pair<const void*, in
   return true;
 }
 
+// Whether a call's `arrays` arrays are more than the last cache holds, in rows of whole cache lines.  There the loads and stores go past
+// the caches (32768 x 8192 forward 519 us and 490, backward 877 and 827); elsewhere, the lines of rows that share one
+// are wanted again (11 sequences of 333 float32 channels backward 22 us and 27).
+bool past_caches(const RecurArgs& a, int arrays, std::initializer_list<int64_t> pitches) {
+  const int64_t e = a.dt == kBF16 ? 2 : 4;
+  for (int64_t ld : pitches)
+    if (ld * e % 128) return false;
+  return a.B * a.L * a.C * e * arrays > (256LL << 20);
+}
+
 struct Plan {
   int64_t slots = 0;
   int64_t at_values = 0, at_starts = 0, at_sums = 0, total = 0;  // tickets first
   bool chained = false;
 };
 int64_t up256(int64_t v) { return round_up(v, 256); }
-Plan plan_of(const RecurArgs& a, bool sums) {
+Plan plan_of(const RecurArgs& a, bool sums, int rows = kRecurRows) {
   Plan p;
   const int64_t G = 2 * ((a.C + 127) / 128);  // (64 channels each, or half as many of 128)
-  const int64_t tiles = (a.L + kTile - 1) / kTile;
-  p.slots = a.seq_starts ? a.B * a.L / kTile + a.S : a.B * std::max<int64_t>(tiles, 1);
+  const int64_t tiles = (a.L + rows - 1) / rows;
+  p.slots = a.seq_starts ? a.B * a.L / rows + a.S : a.B * std::max<int64_t>(tiles, 1);
   p.chained = a.seq_starts || tiles > 1;
   p.at_values = p.chained ? up256(4 * G * kTicketStride) : 0;
   p.at_starts = p.at_values + (p.chained ? up256(G * p.slots * 64 * 8) : 0);
@@ -615,12 +665,13 @@ Plan plan_of(const RecurArgs& a, bool sums) {
   return p;
 }
 
-Chain chain_of(const RecurArgs& a, const Plan& p, void* ws, int cpt) {
+Chain chain_of(const RecurArgs& a, const Plan& p, void* ws, int cpt, int rows = kRecurRows) {
   Chain c;
   char* base = static_cast<char*>(ws);
   c.slots = static_cast<int>(p.slots);
   c.G = static_cast<int>((a.C + 64 * cpt - 1) / (64 * cpt));
-  c.tiles = static_cast<int>(std::max<int64_t>(1, (a.L + kTile - 1) / kTile));
+  c.tiles = static_cast<int>(std::max<int64_t>(1, (a.L + rows - 1) / rows));
+  c.kept = static_cast<int>(std::max<int64_t>(1, (a.L + kRecurRows - 1) / kRecurRows));
   c.spin_limit = g_spin_limit;
   if (p.chained) {
     c.tickets = reinterpret_cast<unsigned*>(base);
@@ -630,18 +681,29 @@ Chain chain_of(const RecurArgs& a, const Plan& p, void* ws, int cpt) {
   return c;
 }
 
-int reset(const RecurArgs& a, const Plan& p, const Chain& c, int cpt, float* sums, hipStream_t st) {
+int reset(const RecurArgs& a, const Plan& p, const Chain& c, int cpt, RestArgs rest, hipStream_t st) {
   if (!p.chained) return kOk;
   const int64_t n_tickets = static_cast<int64_t>(c.G) * kTicketStride / 4, n_values = c.G * p.slots * 64 * cpt / 2;
   const unsigned blocks = static_cast<unsigned>((n_tickets + n_values + 255) / 256 + (a.seq_starts ? 1 : 0));
   recur_reset_kernel<<<blocks, 256, 0, TESM_LOGGED(st, recur_reset_kernel)>>>(
       reinterpret_cast<uint4*>(c.tickets), n_tickets, reinterpret_cast<uint4*>(c.values), n_values, a.seq_starts, a.S + 1, a.B * a.L,
       const_cast<int32_t*>(c.starts));
-  if (sums && a.seq_starts) {  // (slots of packed rows may hold no tile)
-    const int64_t n = p.slots * a.C;
-    recur_zero_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, TESM_LOGGED(st, recur_zero_kernel)>>>(sums, n);
+  if (a.seq_starts && a.zero_rest && a.B * a.L > 0) {
+    rest.C = a.C, rest.rows = a.B * a.L, rest.S = a.S;
+    rest.starts = c.starts;
+    const unsigned n = static_cast<unsigned>(std::min<int64_t>(a.B * a.L, 4096));
+    if (a.dt == kBF16)
+      recur_rest_kernel<kBF16><<<n, 256, 0, TESM_LOGGED(st, recur_rest_kernel<kBF16>)>>>(rest);
+    else
+      recur_rest_kernel<kF32><<<n, 256, 0, TESM_LOGGED(st, recur_rest_kernel<kF32>)>>>(rest);
   }
   return kOk;
+}
+
+// Two channels per lane once the tiles of 128 channels are four per CU; before that twice as many of 64 hide more of their
+// waits (4 x 2048 rows of 384 channels forward 11.0 us and 14.4, backward 15.7 and 18.7).
+bool many_tiles(const RecurArgs& a) {
+  return plan_of(a, false).slots * ((a.C + 127) / 128) >= 4 * static_cast<int64_t>(std::max(device_limits().cus, 1));
 }
 
 }  // namespace
@@ -652,27 +714,41 @@ int64_t recur_bwd_ws_bytes(const RecurArgs& a, bool bias) { return recur_check(a
 
 int launch_gated_scan(const RecurArgs& a, void* ws, int64_t ws_bytes, hipStream_t st) {
   if (int rc = recur_check(a)) return rc;
-  if (a.C == 0 || a.S == 0) return kOk;
+  if (a.C == 0) return kOk;
+  if (a.S == 0) {  // (no sequence: every row is of none)
+    TESM_REQUIRE(!a.zero_rest || a.B * a.L == 0, kErrUnsupported, "gated scan: zero_rest needs a sequence");
+    return kOk;
+  }
   const bool rows = a.B * a.L > 0;
   TESM_REQUIRE(a.h_out && (!rows || (a.value && a.write && a.decay && a.h)), kErrInvalidArg, "gated scan: need the gates, h and h_out");
   TESM_REQUIRE(!rows || (a.ld_v >= a.C && a.ld_w >= a.C && a.ld_d >= a.C && a.ld_h >= a.C), kErrInvalidArg,
                "gated scan: a row pitch below the channels");
-  const Plan p = plan_of(a, false);
-  TESM_REQUIRE(p.total == 0 || (ws && ws_bytes >= p.total && aligned(ws, 16)), kErrWorkspace,
+  const Plan small = plan_of(a, false);
+  TESM_REQUIRE(small.total == 0 || (ws && ws_bytes >= small.total && aligned(ws, 16)), kErrWorkspace,
                "gated scan: workspace too small or not 16-byte aligned");
-  const bool pairs = in_pairs(a.dt, a.C, {{a.value, a.ld_v}, {a.write, a.ld_w}, {a.decay, a.ld_d}, {a.h, a.ld_h}});
-  const Chain c = chain_of(a, p, ws, pairs ? 2 : 1);
+  const bool pairs = many_tiles(a) && in_pairs(a.dt, a.C, {{a.value, a.ld_v}, {a.write, a.ld_w}, {a.decay, a.ld_d}, {a.h, a.ld_h}});
+  const bool past = past_caches(a, 4, {a.ld_v, a.ld_w, a.ld_d, a.ld_h}), tall = past && pairs;
+  const int tile = tall ? 2 * kRecurRows : kRecurRows;
+  const Plan p = plan_of(a, false, tile);
+  const Chain c = chain_of(a, p, ws, pairs ? 2 : 1, tile);
   const int64_t blocks = p.slots * c.G;
   TESM_REQUIRE(blocks < (1LL << 31), kErrUnsupported, "gated scan: too many tiles for one call");
-  if (int rc = reset(a, p, c, pairs ? 2 : 1, nullptr, st)) return rc;
-  constexpr int T = 64 * kWaves;
+  if (int rc = reset(a, p, c, pairs ? 2 : 1, RestArgs{{a.h}, {a.ld_h}}, st)) return rc;
   const unsigned n = static_cast<unsigned>(blocks);
-  if (a.dt == kF32)
-    recur_fwd_kernel<kF32, 1><<<n, T, 0, TESM_LOGGED(st, recur_fwd_kernel<kF32, 1>)>>>(a, c);
-  else if (pairs)
-    recur_fwd_kernel<kBF16, 2><<<n, T, 0, TESM_LOGGED(st, recur_fwd_kernel<kBF16, 2>)>>>(a, c);
-  else
-    recur_fwd_kernel<kBF16, 1><<<n, T, 0, TESM_LOGGED(st, recur_fwd_kernel<kBF16, 1>)>>>(a, c);
+#define TESM_RECUR(DT, CPT, NT, T) recur_fwd_kernel<DT, CPT, NT, T><<<n, 64 * kWaves, 0, TESM_LOGGED(st, recur_fwd_kernel<DT, CPT, NT, T>)>>>(a, c)
+  if (a.dt == kF32) {
+    if (past)
+      TESM_RECUR(kF32, 1, true, 8);
+    else
+      TESM_RECUR(kF32, 1, false, 8);
+  } else if (tall) {
+    TESM_RECUR(kBF16, 2, true, 16);
+  } else if (pairs) {
+    TESM_RECUR(kBF16, 2, false, 8);
+  } else {
+    TESM_RECUR(kBF16, 1, false, 8);
+  }
+#undef TESM_RECUR
   return check_launch("gated scan");
 }
 
@@ -689,22 +765,31 @@ int launch_gated_scan_bwd(const RecurBwdArgs& b, void* ws, int64_t ws_bytes, hip
   const Plan p = plan_of(a, b.d_bias != nullptr);
   TESM_REQUIRE(p.total == 0 || (ws && ws_bytes >= p.total && aligned(ws, 16)), kErrWorkspace,
                "gated scan backward: workspace too small or not 16-byte aligned");
-  const bool pairs = in_pairs(a.dt, a.C, {{a.value, a.ld_v}, {a.write, a.ld_w}, {a.decay, a.ld_d}, {b.grad, b.ld_g},
+  const bool pairs = many_tiles(a) && in_pairs(a.dt, a.C, {{a.value, a.ld_v}, {a.write, a.ld_w}, {a.decay, a.ld_d}, {b.grad, b.ld_g},
                                           {b.d_value, b.ld_dv}, {b.d_write, b.ld_dw}, {b.d_decay, b.ld_dd}});
   const Chain c = chain_of(a, p, ws, pairs ? 2 : 1);
   const int64_t blocks = a.S ? p.slots * c.G : 0;
   TESM_REQUIRE(blocks < (1LL << 31), kErrUnsupported, "gated scan backward: too many tiles for one call");
   float* sums = b.d_bias ? reinterpret_cast<float*>(static_cast<char*>(ws) + p.at_sums) : nullptr;
   if (blocks > 0) {
-    if (int rc = reset(a, p, c, pairs ? 2 : 1, sums, st)) return rc;
-    constexpr int T = 64 * kWaves;
+    if (int rc = reset(a, p, c, pairs ? 2 : 1, RestArgs{{b.d_value, b.d_write, b.d_decay}, {b.ld_dv, b.ld_dw, b.ld_dd}}, st)) return rc;
     const unsigned n = static_cast<unsigned>(blocks);
-    if (a.dt == kF32)
-      recur_bwd_kernel<kF32, 1><<<n, T, 0, TESM_LOGGED(st, recur_bwd_kernel<kF32, 1>)>>>(b, c, sums);
-    else if (pairs)
-      recur_bwd_kernel<kBF16, 2><<<n, T, 0, TESM_LOGGED(st, recur_bwd_kernel<kBF16, 2>)>>>(b, c, sums);
-    else
-      recur_bwd_kernel<kBF16, 1><<<n, T, 0, TESM_LOGGED(st, recur_bwd_kernel<kBF16, 1>)>>>(b, c, sums);
+    const bool past = past_caches(a, 7, {a.ld_v, a.ld_w, a.ld_d, b.ld_g, b.ld_dv, b.ld_dw, b.ld_dd});
+#define TESM_RECUR(DT, CPT, NT) recur_bwd_kernel<DT, CPT, NT><<<n, 64 * kWaves, 0, TESM_LOGGED(st, recur_bwd_kernel<DT, CPT, NT>)>>>(b, c, sums)
+    if (a.dt == kF32) {
+      if (past)
+        TESM_RECUR(kF32, 1, true);
+      else
+        TESM_RECUR(kF32, 1, false);
+    } else if (pairs) {
+      if (past)
+        TESM_RECUR(kBF16, 2, true);
+      else
+        TESM_RECUR(kBF16, 2, false);
+    } else {
+      TESM_RECUR(kBF16, 1, false);
+    }
+#undef TESM_RECUR
   }
   if (b.d_bias) {
     const unsigned n = static_cast<unsigned>((a.C + 63) / 64);

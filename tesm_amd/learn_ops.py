@@ -84,7 +84,7 @@ class _GatedScan(torch.autograd.Function):
         return dv, dw, dd, db, ds, None
 
 
-def _gates(value, write, decay, bias, state, seq_starts, what):
+def _gates(value, write, decay, bias, state, seq_starts, what, zero_rest=False):
     """The call's checked operands: the descriptor, its tensors (kept alive by the caller) and the number of sequences."""
     if value.dim() != 3 or write.shape != value.shape or decay.shape != value.shape:
         raise ValueError(f"{what}: value, write and decay must all be (B, L, C)")
@@ -98,17 +98,17 @@ def _gates(value, write, decay, bias, state, seq_starts, what):
     (value, ld_v), (write, ld_w), (decay, ld_d) = _as_rows(value, 2), _as_rows(write, 2), _as_rows(decay, 2)
     require_device(value, write, decay, bias, state, seq_starts)
     d = _lib.Gates(code, B, L, C, S, value.data_ptr(), ld_v, write.data_ptr(), ld_w, decay.data_ptr(), ld_d, _ptr(bias),
-                   _ptr(seq_starts), _ptr(state))
+                   _ptr(seq_starts), _ptr(state), int(zero_rest and S > 0))
     return d, (value, write, decay, bias, state, seq_starts), S
 
 
 def _scan_forward(value, write, decay, bias, state, seq_starts, out, keep):
     what = "gated_scan"
-    g, held, S = _gates(value, write, decay, bias, state, seq_starts, what)
+    g, held, S = _gates(value, write, decay, bias, state, seq_starts, what, seq_starts is not None and out is None)
     B, L, C = value.shape
     dev = value.device
-    if out is None:
-        out = (torch.zeros if seq_starts is not None else torch.empty)((B, L, C), dtype=value.dtype, device=dev)
+    if out is None:  # (rows of no sequence are set to zero by the call, where it has a sequence)
+        out = (torch.empty if S else torch.zeros)((B, L, C), dtype=value.dtype, device=dev)
         ld = max(C, 1)
     else:
         require_device(value, out)
@@ -151,7 +151,7 @@ def gated_scan(value: torch.Tensor, write: torch.Tensor, decay: torch.Tensor, de
 
 def _scan_backward(grad, value, write, decay, bias, state, seq_starts, kept, grad_state, need_bias):
     what = "gated_scan_backward"
-    g, held, S = _gates(value, write, decay, bias, state, seq_starts, what)
+    g, held, S = _gates(value, write, decay, bias, state, seq_starts, what, seq_starts is not None)
     B, L, C = value.shape
     dev = value.device
     _like(what, "the gradient", grad, value.shape, value.dtype)
@@ -162,8 +162,7 @@ def _scan_backward(grad, value, write, decay, bias, state, seq_starts, kept, gra
     grad_state = grad_state.contiguous() if grad_state is not None else None
     kept = kept.contiguous()
     require_device(value, grad, grad_state, kept)
-    make = torch.zeros if seq_starts is not None else torch.empty
-    dv, dw, dd = make((3, B, L, C), dtype=value.dtype, device=dev).unbind()
+    dv, dw, dd = (torch.empty if S else torch.zeros)((3, B, L, C), dtype=value.dtype, device=dev).unbind()
     db = torch.empty((C,), dtype=torch.float32, device=dev) if need_bias else None
     ds = torch.empty((S, C), dtype=torch.float32, device=dev) if state is not None else None
     ld = max(C, 1)
