@@ -708,8 +708,9 @@ int tesm_hip_gated_scan_step(const tesm_hip_recurrence_step* p, void* stream);
 /* Products of float matrices with what stands around them, no reference counterpart (the reference's projections are ternary).
  * up given: the gated pair of a feed-forward block, y = act(x weight^T) * (x up^T).  up NULL: y = act(x weight^T + bias) +
  * residual.  act: 0 none (not for a pair), 1 silu, 2 gelu (z (1 + erf(z / sqrt 2)) / 2).  Sums are float32, rounded to dt once;
- * float32 operands go through the matrix units in three bfloat16 parts (an infinity among them gives NaN).  z (and z_up): x
- * weight^T (+ bias) and x up^T rounded to dt, for the backward call (NULL: not kept).  M < 2^31, N, K < 2^24. */
+ * float32 operands go through the matrix units in three bfloat16 parts (an infinity among them gives NaN).  z, for the
+ * backward call (NULL: not kept): x weight^T + bias, (M, N) in dt; of a pair, with z_up, x weight^T and x up^T, each (M, N) float32, or
+ * with bf16 operands M * N upper 16 bits followed by M * N next 8 bits.  M < 2^31, N, K < 2^24. */
 typedef struct tesm_hip_dense {
   int dt;
   int act;
@@ -725,8 +726,8 @@ typedef struct tesm_hip_dense {
   int64_t ld_residual;
   void* y;                    /* (M, ld_y) */
   int64_t ld_y;
-  void* z;                    /* optional (M, N) */
-  void* z_up;                 /* optional (M, N) */
+  void* z;                    /* optional */
+  void* z_up;                 /* optional, with z of a pair */
 } tesm_hip_dense;
 
 int64_t tesm_hip_dense_ws_bytes(const tesm_hip_dense* p);

@@ -2222,6 +2222,8 @@ bool plain_sizes(const tesm_hip_dense& p, std::initializer_list<int64_t> pitches
   return plain_sizes({p.M, p.N, p.K}, {p.ld_x, p.ld_weight, p.ld_up, p.ld_residual, p.ld_y}) && plain_sizes({}, pitches) &&
          p.N < (1LL << 24) && p.K < (1LL << 24);
 }
+// What a call keeps of one product, in bytes.
+int64_t kept_bytes(const tesm_hip_dense& p) { return p.M * p.N * (p.dt != kBF16 ? 4 : p.up ? 3 : 2); }
 std::vector<NamedSpan> dense_spans(const tesm_hip_dense& p) {
   const int64_t e = size_of(p.dt);
   return {{"x", span(p.x, p.M, p.ld_x, p.K, e)}, {"weight", span(p.weight, p.N, p.ld_weight, p.K, e)},
@@ -2346,8 +2348,8 @@ int tesm_hip_dense_forward(const tesm_hip_dense* p, void* ws, int64_t ws_bytes, 
   return guarded(who, [&]() -> int {
     TESM_REQUIRE(!p->up || (!p->bias && !p->residual), kErrInvalidArg, "dense product: a gated pair takes no bias and no residual");
     if (plain_sizes(*p, {})) {
-      const int64_t e = size_of(p->dt), n = p->M * p->N;
-      if (int rc = check_overlaps(who, {{"y", span(p->y, p->M, p->ld_y, p->N, e)}, {"z", dense(p->z, n, e)}, {"z_up", dense(p->z_up, n, e)},
+      const int64_t e = size_of(p->dt), kept = kept_bytes(*p);
+      if (int rc = check_overlaps(who, {{"y", span(p->y, p->M, p->ld_y, p->N, e)}, {"z", dense(p->z, kept, 1)}, {"z_up", dense(p->z_up, kept, 1)},
                                         {"workspace", dense(ws, std::max<int64_t>(ws_bytes, 0), 1)}},
                                   dense_spans(*p)))
         return rc;
@@ -2366,11 +2368,11 @@ int tesm_hip_dense_backward(const tesm_hip_dense_grad* p, void* ws, int64_t ws_b
   return guarded(who, [&]() -> int {
     TESM_REQUIRE(!p->of.up || !p->d_bias, kErrInvalidArg, "dense backward: a gated pair has no bias");
     if (plain_sizes(p->of, {p->ld_grad})) {
-      const int64_t e = size_of(p->of.dt), mn = p->of.M * p->of.N, nk = p->of.N * p->of.K;
+      const int64_t e = size_of(p->of.dt), kept = kept_bytes(p->of), nk = p->of.N * p->of.K;
       std::vector<NamedSpan> in = dense_spans(p->of);
       in.push_back({"grad", span(p->grad, p->of.M, p->ld_grad, p->of.N, e)});
-      in.push_back({"z", dense(p->of.z, mn, e)});
-      in.push_back({"z_up", dense(p->of.z_up, mn, e)});
+      in.push_back({"z", dense(p->of.z, kept, 1)});
+      in.push_back({"z_up", dense(p->of.z_up, kept, 1)});
       if (int rc = check_overlaps(who, {{"d_x", dense(p->d_x, p->of.M * p->of.K, e)}, {"d_weight", dense(p->d_weight, nk, e)},
                                         {"d_up", dense(p->d_up, nk, e)}, {"d_bias", dense(p->d_bias, p->of.N, e)},
                                         {"workspace", dense(ws, std::max<int64_t>(ws_bytes, 0), 1)}},

@@ -8,7 +8,8 @@
 // float32 rate, so six of them are 2.7 times as fast as one in float32.  An infinite operand gives NaN where the formula may
 // give an infinity.
 //
-// Gradients.  z (and z2), what stands before the activation, is kept by the forward pass in the operands' type.  The gradient in
+// Gradients.  What stands before the activation is kept by the forward pass: z in the operands' type (it reaches the gradients through
+// the activation's slope alone), a pair's z and z2 of bfloat16 operands in 24 bits.  The gradient in
 // front of the products goes into them in bfloat16 (float32: in three parts).
 #include "dense_mfma.h"
 
@@ -197,6 +198,27 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_product_kernel(Dense
 // ---------------------------------------------------------------------------
 // in front of the backward products
 // ---------------------------------------------------------------------------
+// Eight kept products of a pair.
+template <int DT>
+__device__ __forceinline__ void kept_eight(const void* z, int64_t all, int64_t i, int n, bool vec, float (&v)[8]) {
+  if constexpr (DT == kF32) {
+    load_eight<kF32>(z, i, n, vec, v);
+  } else {
+    const uint16_t* hi = static_cast<const uint16_t*>(z) + i;
+    const uint8_t* lo = static_cast<const uint8_t*>(z) + 2 * all + i;
+    if (vec && n >= 8) {
+      const uint4 h = *reinterpret_cast<const uint4*>(hi);
+      const uint2 l = *reinterpret_cast<const uint2*>(lo);
+      const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[2] = {l.x, l.y};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        v[e] = __uint_as_float((e & 1 ? hw[e / 2] & 0xffff0000u : hw[e / 2] << 16) | (lw[e / 4] >> 8 * (e & 3) & 0xffu) << 8);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < n ? __uint_as_float(static_cast<uint32_t>(hi[e]) << 16 | static_cast<uint32_t>(lo[e]) << 8) : 0.0f;
+    }
+  }
+}
 // dg = dh u act'(g) and du = dh act(g) beside each other in rows of 2 Np values.
 template <int DT>
 __global__ __launch_bounds__(256) void gated_grad_kernel(const void* grad, int64_t ld_g, const void* z, const void* z2, int64_t M, int64_t N,
@@ -207,8 +229,8 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const void* grad, int64
   const int n = static_cast<int>(N - c < 8 ? N - c : 8);
   float d[8], g[8], u[8];
   load_eight<DT>(grad, m * ld_g + c, n, vec != 0, d);
-  load_eight<DT>(z, m * N + c, n, vec != 0, g);
-  load_eight<DT>(z2, m * N + c, n, vec != 0, u);
+  kept_eight<DT>(z, M * N, m * N + c, n, vec != 0, g);
+  kept_eight<DT>(z2, M * N, m * N + c, n, vec != 0, u);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     float v, s;
@@ -266,13 +288,13 @@ __global__ __launch_bounds__(256) void linear_grad_kernel(const void* grad, int6
   for (int q = 0; q < 8; ++q) x += part[q][col >> 3][col & 7];
   sums[blockIdx.y * N + at] = x;
 }
-// The sums of all workgroups' rows: 16 runs of them side by side, joined in order.
+// The sums of all workgroups' rows, in 64 bits: 16 runs of them side by side, joined in order.
 template <int DT>
 __global__ __launch_bounds__(1024) void column_sum_kernel(const float* sums, int64_t count, int64_t N, void* out) {
-  __shared__ float part[16][64];
+  __shared__ double part[16][64];
   const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
   const int64_t n = static_cast<int64_t>(blockIdx.x) * 64 + lane;
-  float x = 0.0f;
+  double x = 0.0;
   if (n < N) {
     const int64_t each = (count + 15) / 16, lo = run * each, hi = lo + each < count ? lo + each : count;
 #pragma unroll 8
@@ -282,7 +304,7 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(const float* sums, int
   __syncthreads();
   if (run == 0 && n < N) {
     for (int q = 1; q < 16; ++q) x += part[q][lane];
-    st<DT>(out, n, x);
+    st<DT>(out, n, static_cast<float>(x));
   }
 }
 

@@ -158,12 +158,30 @@ __device__ __forceinline__ void store8(void* p, int64_t i, const float (&v)[8]) 
     q[1] = make_float4(v[4], v[5], v[6], v[7]);
   }
 }
+template <int DT>
+__device__ __forceinline__ void keep_eight(void* z, int64_t all, int64_t i, const float (&v)[8]) {
+  if constexpr (DT == kBF16) {
+    uint32_t b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = to_24(v[e]);
+    uint4 hi;
+    hi.x = __builtin_amdgcn_perm(b[1], b[0], 0x07060302), hi.y = __builtin_amdgcn_perm(b[3], b[2], 0x07060302);
+    hi.z = __builtin_amdgcn_perm(b[5], b[4], 0x07060302), hi.w = __builtin_amdgcn_perm(b[7], b[6], 0x07060302);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(z) + i) = hi;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] >>= 8;
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(z) + 2 * all + i) =
+        make_uint2(pack_low_bytes(b[0], b[1], b[2], b[3]), pack_low_bytes(b[4], b[5], b[6], b[7]));
+  } else {
+    store8<DT>(z, i, v);
+  }
+}
 template <int KIND, int DT>
 __device__ __forceinline__ void store_eight(const ProductArgs& a, void* out, int64_t m, int64_t n, float (&v)[8], float (&v2)[8]) {
   if constexpr (KIND == kProdGated) {
     if (a.z) {
-      store8<DT>(a.z, m * a.N + n, v);
-      store8<DT>(a.z2, m * a.N + n, v2);
+      keep_eight<DT>(a.z, a.M * a.N, m * a.N + n, v);
+      keep_eight<DT>(a.z2, a.M * a.N, m * a.N + n, v2);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = act_value(v[e], a.act) * v2[e];

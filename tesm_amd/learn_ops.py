@@ -248,6 +248,15 @@ def _dense(x, weight, up, bias, residual, act, what):
     return d, (x, weight, up, bias, residual), M, shape
 
 
+def _pair_dtype(dtype):
+    return torch.float32 if dtype == torch.float32 else torch.uint8
+
+
+def _pair_shape(M, N, dtype):
+    """What a pair keeps of each product: float32, or 3 bytes a value (and what keeps the second one's on 16 bytes)."""
+    return (M, N) if dtype == torch.float32 else ((3 * M * N + 15) // 16 * 16,)
+
+
 def _dense_forward(x, weight, up, bias, residual, act, keep, what):
     d, held, M, shape = _dense(x, weight, up, bias, residual, act, what)
     dev, N = x.device, shape[-1]
@@ -255,7 +264,7 @@ def _dense_forward(x, weight, up, bias, residual, act, keep, what):
     d.y, d.ld_y = y.data_ptr(), max(N, 1)
     kept = None
     if keep and up is not None:
-        kept = torch.empty((2, M, N), dtype=x.dtype, device=dev).unbind()
+        kept = torch.empty((2, *_pair_shape(M, N, x.dtype)), dtype=_pair_dtype(x.dtype), device=dev).unbind()
         d.z, d.z_up = kept[0].data_ptr(), kept[1].data_ptr()
     elif keep and act:
         kept = torch.empty((M, N), dtype=x.dtype, device=dev)
@@ -273,7 +282,7 @@ def _dense_backward(grad, x, weight, up, kept, act, need_x, need_w, need_b, what
     _like(what, "the gradient", grad, shape, x.dtype)
     kept = tuple(kept) if up is not None else (kept,) if act else ()
     for t in kept:
-        _like(what, "kept", t, (M, N), x.dtype)
+        _like(what, "kept", t, *((M, N), x.dtype) if up is None else (_pair_shape(M, N, x.dtype), _pair_dtype(x.dtype)))
         if not t.is_contiguous():
             raise ValueError(f"{what}: kept must be what the forward call returned")
     grad, ld_g = _as_rows(grad, len(shape) - 1)
@@ -318,7 +327,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
     x (.., K), w_gate and w_up (N, K) share a dtype; ``act`` is "silu" or "gelu" (the error function's form).  Sums and the
     activation are float32, the result is rounded once.  float32 operands go through the matrix units in three bfloat16 parts, to the
     error of a float32 sum; an infinity among them gives NaN.  Up to 32 rows the weights are streamed once.  ``keep=True`` also
-    returns what ``gated_linear_backward`` needs (both products, in x's dtype).
+    returns what ``gated_linear_backward`` needs (both products, in 24 bits where x is bfloat16).
     """
     code = _act_code(act, "gated_linear", pair=True)
     if _records("gated_linear", keep, x, w_gate, w_up):

@@ -123,11 +123,13 @@ def dense_ref(x, w, up, bias, residual, act, grad=None):
     if grad is None:
         return out
     d = grad.double()
-    # the kept products are rounded to the type, and so is the gradient in front of the products (float32: 2^-24, three parts)
-    kz = ez + half * z.abs() if act else torch.zeros_like(z)
+    # kept products are rounded, to the type or, a pair's, to 16 bits behind the point; and so is the gradient in front of the products
+    # (float32: 2^-24, three parts)
+    keep = 2.0 ** -16 if up is not None and dtype == torch.bfloat16 else half
+    kz = ez + keep * z.abs() if act else torch.zeros_like(z)
     eslope = 0.8 * kz + (24 * U * (1 + z.abs()) if act else 0)
     if up is not None:
-        kp = ep + half * p.abs()
+        kp = ep + keep * p.abs()
         dz = d * p * slope
         edz = d.abs() * ((p.abs() + kp) * eslope + kp * slope.abs()) + (half + 4 * U) * dz.abs()
         dp = d * val
