@@ -2318,26 +2318,28 @@ int tesm_hip_gated_scan_backward(const tesm_hip_recurrence_grad* p, void* ws, in
 int tesm_hip_gated_scan_step(const tesm_hip_recurrence_step* p, void* stream) {
   const char* who = "gated scan step";
   TESM_REQUIRE(p != nullptr, kErrInvalidArg, "gated scan step: null descriptor");
-  if (plain_sizes({p->B, p->C}, {p->ld_value, p->ld_write, p->ld_decay, p->ld_h}) && p->C < (1LL << 24)) {
-    const int64_t e = size_of(p->dt);
-    if (int rc = check_overlaps(who, {{"h", span(p->h, p->B, p->ld_h, p->C, e)}, {"state", dense(p->state, p->B * p->C, 4)}},
-                                {{"value", span(p->value, p->B, p->ld_value, p->C, e)}, {"write", span(p->write, p->B, p->ld_write, p->C, e)},
-                                 {"decay", span(p->decay, p->B, p->ld_decay, p->C, e)}, {"bias", dense(p->bias, p->C, 4)}}))
+  return guarded(who, [&]() -> int {
+    if (plain_sizes({p->B, p->C}, {p->ld_value, p->ld_write, p->ld_decay, p->ld_h}) && p->C < (1LL << 24)) {
+      const int64_t e = size_of(p->dt);
+      if (int rc = check_overlaps(who, {{"h", span(p->h, p->B, p->ld_h, p->C, e)}, {"state", dense(p->state, p->B * p->C, 4)}},
+                                  {{"value", span(p->value, p->B, p->ld_value, p->C, e)}, {"write", span(p->write, p->B, p->ld_write, p->C, e)},
+                                   {"decay", span(p->decay, p->B, p->ld_decay, p->C, e)}, {"bias", dense(p->bias, p->C, 4)}}))
+        return rc;
+    }
+    if (int rc = check_ptrs(who, {{p->value, "value"}, {p->write, "write"}, {p->decay, "decay"}, {p->bias, "bias"}, {p->state, "state"},
+                                  {p->h, "h"}}))
       return rc;
-  }
-  if (int rc = check_ptrs(who, {{p->value, "value"}, {p->write, "write"}, {p->decay, "decay"}, {p->bias, "bias"}, {p->state, "state"},
-                                {p->h, "h"}}))
-    return rc;
-  RecurStepArgs a;
-  a.dt = p->dt;
-  a.B = p->B, a.C = p->C;
-  a.value = p->value, a.ld_v = p->ld_value;
-  a.write = p->write, a.ld_w = p->ld_write;
-  a.decay = p->decay, a.ld_d = p->ld_decay;
-  a.bias = p->bias;
-  a.state = p->state;
-  a.h = p->h, a.ld_h = p->ld_h;
-  return launch_gated_scan_step(a, static_cast<hipStream_t>(stream));
+    RecurStepArgs a;
+    a.dt = p->dt;
+    a.B = p->B, a.C = p->C;
+    a.value = p->value, a.ld_v = p->ld_value;
+    a.write = p->write, a.ld_w = p->ld_write;
+    a.decay = p->decay, a.ld_d = p->ld_decay;
+    a.bias = p->bias;
+    a.state = p->state;
+    a.h = p->h, a.ld_h = p->ld_h;
+    return launch_gated_scan_step(a, static_cast<hipStream_t>(stream));
+  });
 }
 
 int64_t tesm_hip_dense_ws_bytes(const tesm_hip_dense* p) { return p ? dense_ws_bytes(dense_args(*p)) : -1; }

@@ -52,7 +52,7 @@ __device__ __forceinline__ Sig sig_of(float e) {
 }
 // The decay, of x + b, given nb = -b log2 e.  A state that is kept for n rows holds n times what a decay is off to one side, so this
 // reciprocal takes a Newton step, 1 - p (1 + e) = (1 - p) - p e being exact where p is near 1 (decays that keep 400 rows: the bias's
-// gradient is 1.6e-6 of itself off without it, 3.3e-7 with it; both passes of 4 x 32768 x 4096 take 1362 us instead of 1357).
+// gradient is 1.6e-6 of itself off without it, 3.3e-7 with it; both passes of 32768 x 8192 take 1362 us instead of 1357).
 __device__ __forceinline__ Sig decay_of(float x, float nb) {
   const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x, -kLog2e, nb));
   const float r = __builtin_amdgcn_rcpf(1.0f + e), most = fminf(e, 3.4e38f);
