@@ -4,7 +4,7 @@
 // Operands.  bfloat16 matrices whose rows start on 16 bytes and hold a multiple of 8 values are read where they lie; others are laid
 // out so in the workspace first, padded with zeros.  float32 matrices are laid out as three bfloat16 parts, x = x0 + x1 + x2 with
 // x0 = bf16(x), x1 = bf16(x - x0), x2 = x - x0 - x1 (8 bits each, together all 24 of x), and a product takes the six of their nine products
-// that reach above 2^-26 of it, smallest first, all into one float32 sum: bfloat16 products run at 16 times the
+// that reach above 2^-26 of it, smallest first; the largest has a float32 sum of its own: bfloat16 products run at 16 times the
 // float32 rate, so six of them are 2.7 times as fast as one in float32.  An infinite operand gives NaN where the formula may
 // give an infinity.
 //
@@ -19,7 +19,8 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(2)));  // at any alignment of its values
+typedef uint32_t any8 __attribute__((ext_vector_type(2), aligned(1)));
 
 constexpr int64_t kSkinnyRows = 32;  // up to here weights are streamed once, past the matrix product's tiles
 
@@ -59,13 +60,12 @@ __device__ __forceinline__ void store_parts(uint16_t* to, int64_t stride, const 
     for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(to + p * stride) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
   }
 }
-// Eight values at element i, of which `n` exist (the others are 0); whole ones by one or two loads where `vec`.
+// Eight values at element i, of which `n` exist (the others are 0); whole ones by one or two loads, at any alignment.
 template <int DT>
-__device__ __forceinline__ void load_eight(const void* p, int64_t i, int n, bool vec, float (&v)[8]) {
-  if (vec && n >= 8) {
+__device__ __forceinline__ void load_eight(const void* p, int64_t i, int n, float (&v)[8]) {
+  if (n >= 8) {
     if constexpr (DT == kBF16) {
-      const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+      const any16 u = *reinterpret_cast<const any16*>(static_cast<const uint16_t*>(p) + i);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         v[2 * q] = __uint_as_float(u[q] << 16);
@@ -74,8 +74,9 @@ __device__ __forceinline__ void load_eight(const void* p, int64_t i, int n, bool
     } else {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const float4 f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i)[q];
-        v[4 * q] = f.x, v[4 * q + 1] = f.y, v[4 * q + 2] = f.z, v[4 * q + 3] = f.w;
+        const any16 u = *reinterpret_cast<const any16*>(static_cast<const float*>(p) + i + 4 * q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * q + e] = __uint_as_float(u[e]);
       }
     }
   } else {
@@ -88,7 +89,6 @@ __device__ __forceinline__ void load_eight(const void* p, int64_t i, int n, bool
 struct LayOut {
   const void* src = nullptr;
   int64_t ld = 0, R = 0, C = 0, Cp = 0;
-  int vec = 0;
   uint16_t* dst = nullptr;
   unsigned block0 = 0;  // first workgroup
 };
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256) void lay_out_kernel(LayOuts t) {
   if (i >= a.R * units) return;
   const int64_t r = i / units, c = i % units * 8;
   float v[8];
-  load_eight<DT>(a.src, r * a.ld + c, static_cast<int>(a.C - c < 8 ? a.C - c : 8), a.vec != 0, v);
+  load_eight<DT>(a.src, r * a.ld + c, static_cast<int>(a.C - c < 8 ? a.C - c : 8), v);
   store_parts<DT == kBF16 ? 1 : 3>(a.dst + r * a.Cp + c, a.R * a.Cp, v);
 }
 
@@ -200,19 +200,18 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_product_kernel(Dense
 // ---------------------------------------------------------------------------
 // Eight kept products of a pair.
 template <int DT>
-__device__ __forceinline__ void kept_eight(const void* z, int64_t all, int64_t i, int n, bool vec, float (&v)[8]) {
+__device__ __forceinline__ void kept_eight(const void* z, int64_t all, int64_t i, int n, float (&v)[8]) {
   if constexpr (DT == kF32) {
-    load_eight<kF32>(z, i, n, vec, v);
+    load_eight<kF32>(z, i, n, v);
   } else {
     const uint16_t* hi = static_cast<const uint16_t*>(z) + i;
     const uint8_t* lo = static_cast<const uint8_t*>(z) + 2 * all + i;
-    if (vec && n >= 8) {
-      const uint4 h = *reinterpret_cast<const uint4*>(hi);
-      const uint2 l = *reinterpret_cast<const uint2*>(lo);
-      const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[2] = {l.x, l.y};
+    if (n >= 8) {
+      const any16 h = *reinterpret_cast<const any16*>(hi);
+      const any8 l = *reinterpret_cast<const any8*>(lo);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        v[e] = __uint_as_float((e & 1 ? hw[e / 2] & 0xffff0000u : hw[e / 2] << 16) | (lw[e / 4] >> 8 * (e & 3) & 0xffu) << 8);
+        v[e] = __uint_as_float((e & 1 ? h[e / 2] & 0xffff0000u : h[e / 2] << 16) | (l[e / 4] >> 8 * (e & 3) & 0xffu) << 8);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = e < n ? __uint_as_float(static_cast<uint32_t>(hi[e]) << 16 | static_cast<uint32_t>(lo[e]) << 8) : 0.0f;
@@ -222,15 +221,15 @@ __device__ __forceinline__ void kept_eight(const void* z, int64_t all, int64_t i
 // dg = dh u act'(g) and du = dh act(g) beside each other in rows of 2 Np values.
 template <int DT>
 __global__ __launch_bounds__(256) void gated_grad_kernel(const void* grad, int64_t ld_g, const void* z, const void* z2, int64_t M, int64_t N,
-                                                         int64_t Np, int act, int vec, uint16_t* dst) {
+                                                         int64_t Np, int act, uint16_t* dst) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, units = Np / 8;
   if (i >= M * units) return;
   const int64_t m = i / units, c = i % units * 8;
   const int n = static_cast<int>(N - c < 8 ? N - c : 8);
   float d[8], g[8], u[8];
-  load_eight<DT>(grad, m * ld_g + c, n, vec != 0, d);
-  kept_eight<DT>(z, M * N, m * N + c, n, vec != 0, g);
-  kept_eight<DT>(z2, M * N, m * N + c, n, vec != 0, u);
+  load_eight<DT>(grad, m * ld_g + c, n, d);
+  kept_eight<DT>(z, M * N, m * N + c, n, g);
+  kept_eight<DT>(z2, M * N, m * N + c, n, u);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     float v, s;
@@ -247,7 +246,7 @@ constexpr int kSumRows = 64;  // rows per workgroup
 // dz = dy act'(z) into its parts (dst), and the sums of kSumRows rows of it (sums); either may be left out.
 template <int DT>
 __global__ __launch_bounds__(256) void linear_grad_kernel(const void* grad, int64_t ld_g, const void* z, int64_t M, int64_t N, int64_t Np,
-                                                          int act, int vec, uint16_t* dst, float* sums) {
+                                                          int act, uint16_t* dst, float* sums) {
   __shared__ float part[8][32][9];
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
   const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + cx) * 8, m0 = static_cast<int64_t>(blockIdx.y) * kSumRows;
@@ -260,10 +259,10 @@ __global__ __launch_bounds__(256) void linear_grad_kernel(const void* grad, int6
 #pragma unroll 4
     for (int64_t m = m0 + ry; m < end; m += 8) {
       float d[8];
-      load_eight<DT>(grad, m * ld_g + c, n, vec != 0, d);
+      load_eight<DT>(grad, m * ld_g + c, n, d);
       if (act != kActNone) {
         float v[8];
-        load_eight<DT>(z, m * N + c, n, vec != 0, v);
+        load_eight<DT>(z, m * N + c, n, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           float a, b;
@@ -338,7 +337,7 @@ struct Space {  // a workspace handed out in pieces (base null: only measured)
 
 struct Matrix {
   const uint16_t* p = nullptr;
-  int64_t part = 0;  // values from part to part
+  int64_t part = 0;  // values from part to part of float32 operands
   int64_t ld = 0, ext = 0;
 };
 bool lies_ready(int dt, const void* p, int64_t ld, int64_t C) { return dt == kBF16 && aligned(p, 16) && ld % 8 == 0 && C % 8 == 0; }
@@ -350,9 +349,8 @@ Matrix bring(Space& s, LayOuts& todo, int dt, const void* p, int64_t ld, int64_t
   const int64_t Cp = round_up(C, 64);
   LayOut& m = todo.m[todo.count++];
   m.src = p, m.ld = ld, m.R = R, m.C = C, m.Cp = Cp;
-  m.vec = aligned(p, 16) && (ld * size_of_dt(dt)) % 16 == 0;
   m.dst = s.take<uint16_t>(R * Cp * (dt == kBF16 ? 1 : 3));
-  return {m.dst, R * Cp, Cp, Cp};
+  return {m.dst, dt == kBF16 ? 0 : R * Cp, Cp, Cp};
 }
 int lay_out(LayOuts& t, int dt, hipStream_t st) {
   int64_t blocks = 0;
@@ -370,17 +368,12 @@ int lay_out(LayOuts& t, int dt, hipStream_t st) {
   return kOk;
 }
 
-// The pairs of parts that count, smallest products first.
-constexpr int kOrder[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
-void add_pairs(ProductArgs& a, int dt, const Matrix& A, int64_t a_off, const Matrix& B, const Matrix* B2) {
-  const int n = dt == kBF16 ? 1 : 6;
-  for (int i = 0; i < n; ++i) {
-    const int pa = dt == kBF16 ? 0 : kOrder[i][0], pb = dt == kBF16 ? 0 : kOrder[i][1];
-    a.A[a.pairs] = A.p + a_off + pa * A.part;
-    a.B[a.pairs] = B.p + pb * B.part;
-    a.B2[a.pairs] = B2 ? B2->p + pb * B2->part : nullptr;
-    ++a.pairs;
-  }
+void add_pair(ProductArgs& a, const Matrix& A, int64_t a_off, const Matrix& B, const Matrix* B2) {
+  a.A[a.pairs] = A.p + a_off;
+  a.B[a.pairs] = B.p;
+  a.B2[a.pairs] = B2 ? B2->p : nullptr;
+  a.part_a = A.part, a.part_b = B.part;
+  ++a.pairs;
 }
 
 int dense_check(const DenseArgs& a, const char* who) {
@@ -443,14 +436,14 @@ int forward(const DenseArgs& d, Space s, bool run, int64_t* need, hipStream_t st
   if (int rc = lay_out(todo, d.dt, st)) return rc;
   ProductArgs a = epilogue_of(d);
   a.pairs = 0;
-  add_pairs(a, d.dt, x, 0, w, d.w2 ? &w2 : nullptr);
+  add_pair(a, x, 0, w, d.w2 ? &w2 : nullptr);
   a.lda = x.ld, a.ldb = w.ld;
   return launch_product(d.w2 ? kProdGated : kProdLinear, d.dt, false, false, a, st);
 }
 
 // A product whose results are gradients, its contraction split where there are few tiles.
 int grad_product(Space& s, bool run, int dt, bool adown, ProductArgs a, hipStream_t st) {
-  a.splits = a.K ? product_splits(a.M, a.N, a.K, a.pairs) : 0;  // (nothing to add up: zeros)
+  a.splits = a.K ? product_splits(a.M, a.N, a.K, a.pairs, a.part_a != 0) : 0;  // (nothing to add up: zeros)
   const int64_t e = size_of_dt(dt);
   if (a.splits == 1) {
     a.ldo = a.N;
@@ -477,22 +470,20 @@ int grad_product(Space& s, bool run, int dt, bool adown, ProductArgs a, hipStrea
 int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_t st) {
   const DenseArgs& d = b.in;
   const int dt = d.dt;
-  const int64_t M = d.M, N = d.N, K = d.K, Np = round_up(N, 64), e = size_of_dt(dt);  // (rows of whole cache lines)
+  const int64_t M = d.M, N = d.N, K = d.K, Np = round_up(N, 64);  // (rows of whole cache lines)
   const bool gated = d.w2 != nullptr, products = b.dx || b.dw || b.dw2;
   Matrix dz;
-  const bool grad_whole = aligned(b.grad, 16) && b.ld_g * e % 16 == 0;
-  const int vec = grad_whole && (!d.z || (aligned(d.z, 16) && N * e % 16 == 0)) && (!d.z2 || aligned(d.z2, 16));
   if (gated) {
     uint16_t* dst = s.take<uint16_t>(M * 2 * Np * (dt == kBF16 ? 1 : 3));
-    dz = {dst, M * 2 * Np, 2 * Np, 2 * Np};
+    dz = {dst, dt == kBF16 ? 0 : M * 2 * Np, 2 * Np, 2 * Np};
     const int64_t threads = M * Np / 8;
     if (run && threads && products) {
       TESM_REQUIRE(threads < (1LL << 38), kErrUnsupported, "dense backward: too large");
       const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
       if (dt == kBF16)
-        gated_grad_kernel<kBF16><<<blocks, 256, 0, TESM_LOGGED(st, gated_grad_kernel<kBF16>)>>>(b.grad, b.ld_g, d.z, d.z2, M, N, Np, d.act, vec, dst);
+        gated_grad_kernel<kBF16><<<blocks, 256, 0, TESM_LOGGED(st, gated_grad_kernel<kBF16>)>>>(b.grad, b.ld_g, d.z, d.z2, M, N, Np, d.act, dst);
       else
-        gated_grad_kernel<kF32><<<blocks, 256, 0, TESM_LOGGED(st, gated_grad_kernel<kF32>)>>>(b.grad, b.ld_g, d.z, d.z2, M, N, Np, d.act, vec, dst);
+        gated_grad_kernel<kF32><<<blocks, 256, 0, TESM_LOGGED(st, gated_grad_kernel<kF32>)>>>(b.grad, b.ld_g, d.z, d.z2, M, N, Np, d.act, dst);
     }
   } else {
     const bool direct = d.act == kActNone && lies_ready(dt, b.grad, b.ld_g, N);
@@ -501,7 +492,7 @@ int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_
       dz = {static_cast<const uint16_t*>(b.grad), 0, b.ld_g, N};
     else {
       dst = s.take<uint16_t>(M * Np * (dt == kBF16 ? 1 : 3));
-      dz = {dst, M * Np, Np, Np};
+      dz = {dst, dt == kBF16 ? 0 : M * Np, Np, Np};
     }
     const int64_t rows = (M + kSumRows - 1) / kSumRows;
     float* sums = b.dbias ? s.take<float>(rows * N) : nullptr;
@@ -509,9 +500,9 @@ int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_
       TESM_REQUIRE(rows < 65536, kErrUnsupported, "dense backward: too many rows");
       const dim3 grid(static_cast<unsigned>((Np + 255) / 256), static_cast<unsigned>(rows));
       if (dt == kBF16)
-        linear_grad_kernel<kBF16><<<grid, 256, 0, TESM_LOGGED(st, linear_grad_kernel<kBF16>)>>>(b.grad, b.ld_g, d.z, M, N, Np, d.act, vec, dst, sums);
+        linear_grad_kernel<kBF16><<<grid, 256, 0, TESM_LOGGED(st, linear_grad_kernel<kBF16>)>>>(b.grad, b.ld_g, d.z, M, N, Np, d.act, dst, sums);
       else
-        linear_grad_kernel<kF32><<<grid, 256, 0, TESM_LOGGED(st, linear_grad_kernel<kF32>)>>>(b.grad, b.ld_g, d.z, M, N, Np, d.act, vec, dst, sums);
+        linear_grad_kernel<kF32><<<grid, 256, 0, TESM_LOGGED(st, linear_grad_kernel<kF32>)>>>(b.grad, b.ld_g, d.z, M, N, Np, d.act, dst, sums);
     }
     if (run && b.dbias && N) {
       const unsigned blocks = static_cast<unsigned>((N + 63) / 64);
@@ -536,8 +527,8 @@ int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_
     ProductArgs a;
     a.M = M, a.N = K, a.K = N;
     a.pairs = 0;
-    add_pairs(a, dt, dz, 0, w, nullptr);
-    if (gated) add_pairs(a, dt, dz, Np, w2, nullptr);
+    add_pair(a, dz, 0, w, nullptr);
+    if (gated) add_pair(a, dz, Np, w2, nullptr);
     a.lda = dz.ld, a.ldb = w.ld, a.ext_b = w.ext;
     a.out = b.dx;
     if (int rc = grad_product(s, run, dt, false, a, st)) return rc;
@@ -546,7 +537,7 @@ int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_
     ProductArgs a;
     a.M = gated ? Np + N : N, a.N = K, a.K = M;
     a.pairs = 0;
-    add_pairs(a, dt, dz, 0, x, nullptr);
+    add_pair(a, dz, 0, x, nullptr);
     a.lda = dz.ld, a.ext_a = dz.ext, a.ldb = x.ld, a.ext_b = x.ext;
     a.out = b.dw, a.out2 = b.dw2;
     a.cut = N, a.fold = Np;

@@ -6,17 +6,19 @@
 
 namespace tesm {
 
-constexpr int kMaxParts = 12;
+constexpr int kMaxPairs = 2, kParts = 3;
 
 // out[m, n] = sum over pairs p and k of A_p[m, k] B_p[n, k].  An operand lies with k along its rows (m or n picks the row), or, where
 // its layout is "down", with k picking the row.  All pairs share extents and pitches.  Rows start on 16 bytes; the contiguous
-// extent is a multiple of 8.
+// extent is a multiple of 8.  With part_a set, operands are float32 values in three bfloat16 parts, part i lying i * part_a (part_b)
+// values behind the first.
 struct ProductArgs {
   int64_t M = 0, N = 0, K = 0;
   int pairs = 1;
-  const uint16_t* A[kMaxParts] = {};
-  const uint16_t* B[kMaxParts] = {};
-  const uint16_t* B2[kMaxParts] = {};  // the second weight of a gated pair
+  const uint16_t* A[kMaxPairs] = {};
+  const uint16_t* B[kMaxPairs] = {};
+  const uint16_t* B2[kMaxPairs] = {};  // the second weight of a gated pair
+  int64_t part_a = 0, part_b = 0;
   int64_t lda = 0, ldb = 0;
   int64_t ext_a = 0, ext_b = 0;  // values per row of an operand that lies down, a multiple of 8 (not below M, N)
   int splits = 1;  // the contraction in this many runs of steps, each to its own float32 result at out + split * M * N
@@ -40,7 +42,7 @@ enum ProductLayout : int { kAlong = 0, kDown = 1 };
 // dt: type of the results (kProdPartial: float32).  adown, bdown: operand layouts.
 int launch_product(ProductKind kind, int dt, bool adown, bool bdown, ProductArgs a, hipStream_t st);
 // How many runs the contraction of such a product should be split into (1: none).
-int product_splits(int64_t M, int64_t N, int64_t K, int pairs);
+int product_splits(int64_t M, int64_t N, int64_t K, int pairs, bool parts);
 
 // The normal distribution's Phi(z) = (1 + erf(z / sqrt 2)) / 2 and e = exp(-z^2 / 2), with erfc(x) = P(t) exp(-x^2), t = 1 / (1 + p x),
 // the polynomial of Abramowitz and Stegun 7.1.26 (1.5e-7 off at most).  The library's erff takes three times as long: 8192 x 16384

@@ -42,15 +42,19 @@ __device__ __forceinline__ void to_lds(i32x4 buf, char* dst, uint32_t off) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(buf));
 }
 
-template <int KIND, int WM_, int WN_, int TM_, int TN_, int BK_, int NS_>
+// The products of parts that count, smallest first; the last one has sums of its own, which the others' join at the end.
+constexpr int kOrder[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
+
+template <int KIND, int PARTS_, int WM_, int WN_, int TM_, int TN_, int BK_, int NS_>
 struct Shape {
+  static constexpr int PARTS = PARTS_, ORDERS = PARTS == 1 ? 1 : 6, SETS = PARTS == 1 ? 1 : 2;
   static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, BK = BK_, NS = NS_;
   static constexpr int NP = KIND == kProdGated ? 2 : 1;  // products
   static constexpr int NW = WM * WN, NT = NW * 64, BM = WM * TM * 32, BN = WN * TN * 32;
-  static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + NP * B_BYTES;
-  static constexpr int NA = A_BYTES / 1024, NB = B_BYTES / 1024, BLOCKS = NA + NP * NB;  // 1 KB per load instruction
+  static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = PARTS * (A_BYTES + NP * B_BYTES);
+  static constexpr int NA = A_BYTES / 1024, NB = B_BYTES / 1024, BLOCKS = PARTS * (NA + NP * NB);  // 1 KB per load instruction
   static constexpr int D = BLOCKS / NW;
-  static_assert(BLOCKS % NW == 0 && NA % NW == 0 && NB % NW == 0, "every wave loads as many blocks of each operand");
+  static_assert(BLOCKS % NW == 0 && PARTS * NA % NW == 0 && PARTS * NB % NW == 0, "every wave loads as many blocks of each operand");
   static constexpr int STEPS = BK / 16;
   static constexpr int PITCH = TN * 32 * 4 + 16, SLAB = NP * 32 * PITCH;
   static constexpr int SMEM = NS * STAGE > NW * SLAB ? NS * STAGE : NW * SLAB;
@@ -207,9 +211,9 @@ __device__ __forceinline__ void store_eight(const ProductArgs& a, void* out, int
   store8<DT>(out, m * a.ldo + n, v);
 }
 
-template <int KIND, int DT, bool ADOWN, bool BDOWN, int WM, int WN, int TM, int TN, int BK, int NS>
+template <int KIND, int DT, int PARTS, bool ADOWN, bool BDOWN, int WM, int WN, int TM, int TN, int BK, int NS>
 __global__ __launch_bounds__(WM* WN * 64) void product_kernel(ProductArgs a) {
-  using S = Shape<KIND, WM, WN, TM, TN, BK, NS>;
+  using S = Shape<KIND, PARTS, WM, WN, TM, TN, BK, NS>;
   __shared__ __attribute__((aligned(1024))) char smem[S::SMEM];
   constexpr int NP = S::NP;
   const int t = threadIdx.x;
@@ -221,14 +225,19 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(ProductArgs a) {
   xcd_tile_of<4>(blockIdx.x, ntm, ntn, tm, tn);
   const int64_t m0 = tm * S::BM, n0 = tn * S::BN;
 
-  // this wave's loads
-  constexpr int DA = S::NA / S::NW, DB = S::NB / S::NW;
+  // this wave's loads: block b of an operand is block b % NA of its part b / NA
+  constexpr int DA = PARTS * S::NA / S::NW, DB = PARTS * S::NB / S::NW;
   uint32_t off_a[DA], off_b[DB];
   int k_a[DA], k_b[DB];
 #pragma unroll
-  for (int i = 0; i < DA; ++i) load_place<BK, S::BM, ADOWN>(wave + i * S::NW, lane, a.lda, (ADOWN ? a.ext_a : a.M) - m0, off_a[i], k_a[i]);
+  for (int i = 0; i < DA; ++i)
+    load_place<BK, S::BM, ADOWN>((wave + i * S::NW) % S::NA, lane, a.lda, (ADOWN ? a.ext_a : a.M) - m0, off_a[i], k_a[i]);
 #pragma unroll
-  for (int i = 0; i < DB; ++i) load_place<BK, S::BN, BDOWN>(wave + i * S::NW, lane, a.ldb, (BDOWN ? a.ext_b : a.N) - n0, off_b[i], k_b[i]);
+  for (int i = 0; i < DB; ++i)
+    load_place<BK, S::BN, BDOWN>((wave + i * S::NW) % S::NB, lane, a.ldb, (BDOWN ? a.ext_b : a.N) - n0, off_b[i], k_b[i]);
+  auto part_of = [&](int block, int per, int64_t stride) __attribute__((always_inline)) {
+    return PARTS == 1 ? 0 : static_cast<uint64_t>(block / per) * static_cast<uint64_t>(stride) * 2;
+  };
   const int64_t a_first = ADOWN ? m0 : m0 * a.lda, b_first = BDOWN ? n0 : n0 * a.ldb;
   const int64_t a_step = ADOWN ? BK * a.lda : BK, b_step = BDOWN ? BK * a.ldb : BK;
   const int nk = static_cast<int>((a.K + BK - 1) / BK);
@@ -253,11 +262,11 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(ProductArgs a) {
   auto issue = [&](char* stage, bool live, int i) __attribute__((always_inline)) {
     const int end = live ? static_cast<int>(a.K - static_cast<int64_t>(kt) * BK) : 0;  // values of k from here on are zeros
     if (i < DA) {
-      to_lds(buffer_at(at_a), stage + (wave + i * S::NW) * 1024, k_a[i] < end ? off_a[i] : kRange);
+      to_lds(buffer_at(at_a + part_of(wave + i * S::NW, S::NA, a.part_a)), stage + (wave + i * S::NW) * 1024, k_a[i] < end ? off_a[i] : kRange);
     } else {
       const int p = (i - DA) / DB, j = (i - DA) % DB;
-      to_lds(buffer_at(p ? at_b2 : at_b), stage + S::A_BYTES + p * S::B_BYTES + (wave + j * S::NW) * 1024,
-             k_b[j] < end ? off_b[j] : kRange);
+      to_lds(buffer_at((p ? at_b2 : at_b) + part_of(wave + j * S::NW, S::NB, a.part_b)),
+             stage + PARTS * (S::A_BYTES + p * S::B_BYTES) + (wave + j * S::NW) * 1024, k_b[j] < end ? off_b[j] : kRange);
     }
     if (i < S::D - 1) return;
     at_a += a_step * 2;
@@ -276,25 +285,34 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(ProductArgs a) {
   FragB fb;
   fa.init(wm * TM * 32, lane);
   fb.init(wn * TN * 32, lane);
-  f32x16 acc[NP][TM][TN];
+  f32x16 sums[S::SETS][NP][TM][TN];
 #pragma unroll
-  for (int p = 0; p < NP; ++p)
+  for (int h = 0; h < S::SETS; ++h)
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int p = 0; p < NP; ++p)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[p][i][j] = f32x16{};
-  typename FragA::Value ra[2][TM];
-  typename FragB::Value rb[2][NP][TN];
-  constexpr int NR = NP * TN + TM, NM = NP * TN * TM;  // fragment reads and MFMAs per k-step
-  auto read = [&](const char* stage, int s, int r, typename FragA::Value (&x)[TM], typename FragB::Value (&y)[NP][TN]) __attribute__((always_inline)) {
-    if (r < NP * TN)
-      y[r / TN][r % TN] = fb.read(stage + S::A_BYTES + (r / TN) * S::B_BYTES, r % TN, s);
-    else
-      x[r - NP * TN] = fa.read(stage, r - NP * TN, s);
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) sums[h][p][i][j] = f32x16{};
+  typename FragA::Value ra[2][PARTS][TM];
+  typename FragB::Value rb[2][PARTS][NP][TN];
+  constexpr int NR = PARTS * (NP * TN + TM), NM = S::ORDERS * NP * TN * TM;  // fragment reads and MFMAs per k-step
+  auto read = [&](const char* stage, int s, int r, int to) __attribute__((always_inline)) {
+    // (what the first products need comes first)
+    const int h = PARTS == 1 ? 0 : r / (NP * TN + TM), q = PARTS == 1 ? r : r % (NP * TN + TM);
+    if (q < NP * TN) {
+      const int part = PARTS == 1 ? 0 : h == 0 ? 0 : h == 1 ? 2 : 1;
+      rb[to][part][q / TN][q % TN] = fb.read(stage + PARTS * S::A_BYTES + (q / TN) * PARTS * S::B_BYTES + part * S::B_BYTES, q % TN, s);
+    } else {
+      const int part = PARTS == 1 ? 0 : h == 0 ? 2 : h == 1 ? 0 : 1;
+      ra[to][part][q - NP * TN] = fa.read(stage + part * S::A_BYTES, q - NP * TN, s);
+    }
   };
-  auto mma = [&](int q, const typename FragA::Value (&x)[TM], const typename FragB::Value (&y)[NP][TN]) __attribute__((always_inline)) {
-    const int i = q % TM, j = q / TM % TN, p = q / (TM * TN);
-    acc[p][i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(FragB::value(y[p][j]), FragA::value(x[i]), acc[p][i][j], 0, 0, 0);
+  auto mma = [&](int q, int from) __attribute__((always_inline)) {
+    const int i = q % TM, j = q / TM % TN, p = q / (TM * TN) % NP, o = q / (TM * TN * NP);
+    const int pa = PARTS == 1 ? 0 : kOrder[o][0], pb = PARTS == 1 ? 0 : kOrder[o][1];
+    f32x16& c = sums[o == S::ORDERS - 1 ? 0 : 1 % S::SETS][p][i][j];
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(FragB::value(rb[from][pb][p][j]), FragA::value(ra[from][pa][i]), c, 0, 0, 0);
   };
   // k-step s of the tile in `cur`: between its MFMAs the next step's fragments are read and, in the last step, the tile NS - 1
   // ahead is asked for, one instruction after each, so that neither the LDS nor the memory unit is asked for all at once.
@@ -302,9 +320,9 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(ProductArgs a) {
     const bool last = s == S::STEPS - 1;
 #pragma unroll
     for (int q = 0; q < NM; ++q) {
-      mma(q, ra[s & 1], rb[s & 1]);
+      mma(q, s & 1);
 #pragma unroll
-      for (int r = q * NR / NM; r < (q + 1) * NR / NM; ++r) read(last ? next : cur, last ? 0 : s + 1, r, ra[(s + 1) & 1], rb[(s + 1) & 1]);
+      for (int r = q * NR / NM; r < (q + 1) * NR / NM; ++r) read(last ? next : cur, last ? 0 : s + 1, r, (s + 1) & 1);
       if (last) {
 #pragma unroll
         for (int i = q * S::D / NM; i < (q + 1) * S::D / NM; ++i) issue(refill, live, i);
@@ -321,7 +339,7 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(ProductArgs a) {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
-  for (int r = 0; r < NR; ++r) read(smem, 0, r, ra[0], rb[0]);
+  for (int r = 0; r < NR; ++r) read(smem, 0, r, 0);
   int st = 0;
   for (int step = 0; step < steps; ++step) {
     const char* cur = smem + st * S::STAGE;
@@ -356,7 +374,8 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(ProductArgs a) {
       for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x16& c = acc[p][i][j];
+          f32x16 c = sums[0][p][i][j];
+          if constexpr (PARTS > 1) c += sums[1][p][i][j];
           *reinterpret_cast<float4*>(slab + p * 32 * S::PITCH + (lane & 31) * S::PITCH + (32 * j + 8 * g + 4 * (lane >> 5)) * 4) =
               make_float4(c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]);
         }
@@ -412,9 +431,9 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(ProductArgs a) {
   }
 }
 
-template <int KIND, int DT, bool ADOWN, bool BDOWN, int WM, int WN, int TM, int TN, int BK, int NS>
+template <int KIND, int DT, int PARTS, bool ADOWN, bool BDOWN, int WM, int WN, int TM, int TN, int BK, int NS>
 int run_product(const ProductArgs& a, hipStream_t st) {
-  using S = Shape<KIND, WM, WN, TM, TN, BK, NS>;
+  using S = Shape<KIND, PARTS, WM, WN, TM, TN, BK, NS>;
   const int64_t tiles = ((a.M + S::BM - 1) / S::BM) * ((a.N + S::BN - 1) / S::BN);
   TESM_REQUIRE(tiles < (1LL << 31), kErrUnsupported, "dense product: too many tiles");
   // offsets from a tile's first value stay inside the buffer's range
@@ -423,8 +442,8 @@ int run_product(const ProductArgs& a, hipStream_t st) {
                    a.K / BK * a.pairs < (1LL << 30),
                kErrUnsupported, "dense product: rows too long");
   const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(KIND == kProdPartial ? a.splits : 1));
-  product_kernel<KIND, DT, ADOWN, BDOWN, WM, WN, TM, TN, BK, NS>
-      <<<grid, S::NT, 0, TESM_LOGGED(st, product_kernel<KIND, DT, ADOWN, BDOWN, WM, WN, TM, TN, BK, NS>)>>>(a);
+  product_kernel<KIND, DT, PARTS, ADOWN, BDOWN, WM, WN, TM, TN, BK, NS>
+      <<<grid, S::NT, 0, TESM_LOGGED(st, product_kernel<KIND, DT, PARTS, ADOWN, BDOWN, WM, WN, TM, TN, BK, NS>)>>>(a);
   return check_launch("dense product");
 }
 
@@ -436,28 +455,48 @@ int run_product(const ProductArgs& a, hipStream_t st) {
 // bfloat16: 8192 x 16384 x 4096 879 us large (1.25 Pflop/s; the library's product 1.29), mid 1075, small 1240; 8192 x 4096 x 768 58,
 // 69, 83; 8192 x 768 x 2048 47, 31, 39; 4096 x 768 x 8192 147, 77, 66; 512 x 768 x 2048 43, 23, 19, tiny 11; 1024 x 2048 x 768 23, 13, 11, 10.  Operands that lie down: 8192 x 16384 x 4096 864 us with one, 860
 // with both (the library 950 and 1080).  Tiles of 32 values of k instead of 64 cost 20 % where rows run along k (64-byte
-// pieces), stages of 128 x 256 with 8 waves of 64 x 64 another 10 %.
+// pieces), stages of 128 x 256 with 8 waves of 64 x 64 another 10 %, 128 x 192 on 4 waves is no faster than mid where it fills the CUs.
+//
+// Operands of three parts: all parts of a tile lie in a stage and meet there in six products, so that values are loaded and read from
+// LDS once, not twice (pairs of parts one after the other: 999 x 2 x 1030 x 515 36 us, now 28).  Large: 256 x 128 (128 x 128 of each) on 8
+// waves, mid: 128 x 128 (128 x 64), small: 64 x 64 (of each) with six (four) stages, one per CU, tiny: the same with three (two),
+// two per CU.  With what lays out the operands, large, mid and tiny: 4096 x 4096 x 4096 633, 725, 998 us (217 Tflop/s; the library's
+// float32 product 137), 2048 x 768 x 2048 115, 84, 74, small 74; 999 x 515 x 1030 79, 54, 37, small 32.
 enum Config : int { kLarge, kMid, kSmall, kTiny };
 struct Plan {
   Config config = kSmall;
   int splits = 1;
 };
-Plan plan_product(ProductKind kind, int64_t M, int64_t N, int64_t K, int pairs, bool split) {
+Plan plan_product(ProductKind kind, bool parts, int64_t M, int64_t N, int64_t K, int pairs, bool split) {
   const int64_t cus = std::max(device_limits().cus, 1);
-  auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + (kind == kProdGated ? bn / 2 : bn) - 1) / (kind == kProdGated ? bn / 2 : bn)); };
-  const double k = static_cast<double>(K) * pairs / 1000.0;
+  const bool gated = kind == kProdGated;
+  auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  // rounds of one workgroup per CU, of two (`half`: where only one is left)
+  auto ones = [&](int64_t n, double us) { return static_cast<double>((n + cus - 1) / cus) * us; };
+  auto twos = [&](int64_t n, double half, double us) {
+    const int64_t rest = n % (2 * cus);
+    return static_cast<double>(n / (2 * cus)) * us + (rest == 0 ? 0.0 : rest <= cus ? half : us);
+  };
+  const int64_t large = parts ? (gated ? tiles(128, 128) : tiles(256, 128)) : tiles(256, gated ? 128 : 256);
+  const int64_t mid = tiles(128, gated ? 64 : 128), tiny = tiles(64, 64);
+  const double all = static_cast<double>(K) * pairs / 1000.0;
+  const int64_t steps = (K + 63) / 64 * pairs;
   Plan best;
   double least = 1e30;
-  const int64_t steps = (K + 63) / 64 * pairs;
   for (int s = 1; s <= (split ? 16 : 1) && (s == 1 || s * 4 <= steps); ++s) {
-    const double ks = k / s, joined = s == 1 ? 0.0 : 6.0 + 2.0 * s * 4.0 * static_cast<double>(M) * static_cast<double>(N) / 5.0e6;
-    const int64_t large = tiles(256, 256) * s, mid = tiles(128, 128) * s;
-    const int64_t rest = mid % (2 * cus);
-    const int64_t tiny = tiles(64, kind == kProdGated ? 128 : 64) * s, few = tiny % (2 * cus);
-    const double cost[4] = {static_cast<double>((large + cus - 1) / cus) * (25.4 * ks + 8.0),
-                            static_cast<double>(mid / (2 * cus)) * (15.3 * ks + 5.0) + (rest == 0 ? 0.0 : rest <= cus ? 9.4 * ks + 5.0 : 15.3 * ks + 5.0),
-                            static_cast<double>((mid + cus - 1) / cus) * (7.6 * ks + 4.0),
-                            static_cast<double>(tiny / (2 * cus)) * (5.5 * ks + 4.0) + (few == 0 ? 0.0 : few <= cus ? 4.0 * ks + 3.5 : 5.5 * ks + 4.0)};
+    const double k = all / s, joined = s == 1 ? 0.0 : 6.0 + 2.0 * s * 4.0 * static_cast<double>(M) * static_cast<double>(N) / 5.0e6;
+    double cost[4];
+    if (parts) {
+      cost[kLarge] = ones(large * s, 72.0 * k + 5.0);
+      cost[kMid] = ones(mid * s, 39.0 * k + 4.0);
+      cost[kSmall] = ones(tiny * s, (gated ? 34.0 : 16.0) * k + 2.0);
+      cost[kTiny] = gated ? twos(tiny * s, 45.0 * k + 3.0, 52.0 * k + 2.0) : twos(tiny * s, 20.0 * k + 2.0, 24.0 * k + 2.0);
+    } else {
+      cost[kLarge] = ones(large * s, 25.4 * k + 8.0);
+      cost[kMid] = twos(mid * s, 9.4 * k + 5.0, 15.3 * k + 5.0);
+      cost[kSmall] = ones(mid * s, 7.6 * k + 4.0);
+      cost[kTiny] = twos(tiny * s, 4.0 * k + 3.5, 5.5 * k + 4.0);
+    }
     for (int c = 0; c < 4; ++c)
       if (cost[c] + joined < least) {
         least = cost[c] + joined;
@@ -469,24 +508,47 @@ Plan plan_product(ProductKind kind, int64_t M, int64_t N, int64_t K, int pairs, 
 
 template <int KIND, int DT, bool ADOWN, bool BDOWN>
 int pick(const ProductArgs& a, hipStream_t st) {
+  const bool parts = a.part_a != 0;
   // (a split product was planned by product_splits, with the same numbers)
-  const Plan p = plan_product(static_cast<ProductKind>(KIND), a.M, a.N, a.K, a.pairs, KIND == kProdPartial);
-  if constexpr (KIND == kProdGated) {
-    if (p.config == kLarge) return run_product<KIND, DT, ADOWN, BDOWN, 4, 2, 2, 2, 64, 2>(a, st);
-    if (p.config == kMid) return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 1, 64, 2>(a, st);
-    if (p.config == kSmall) return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 1, 64, 4>(a, st);
-    return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 1, 1, 64, 3>(a, st);
-  } else {
-    if (p.config == kLarge) return run_product<KIND, DT, ADOWN, BDOWN, 2, 4, 4, 2, 64, 2>(a, st);
-    if (p.config == kMid) return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 2, 64, 2>(a, st);
-    if (p.config == kSmall) return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 2, 2, 64, 4>(a, st);
-    return run_product<KIND, DT, ADOWN, BDOWN, 2, 2, 1, 1, 64, 4>(a, st);
+  const Plan p = plan_product(static_cast<ProductKind>(KIND), parts, a.M, a.N, a.K, a.pairs, KIND == kProdPartial);
+#define TESM_RUN(PARTS, ...) return run_product<KIND, DT, PARTS, ADOWN, BDOWN, __VA_ARGS__>(a, st)
+  if constexpr (DT == kF32) {
+    if (KIND != kProdPartial || parts) {
+      if constexpr (KIND == kProdGated) {
+        if (p.config == kLarge) TESM_RUN(3, 4, 2, 1, 2, 32, 2);
+        if (p.config == kMid) TESM_RUN(3, 2, 2, 2, 1, 32, 3);
+        if (p.config == kSmall) TESM_RUN(3, 2, 2, 1, 1, 32, 4);
+        TESM_RUN(3, 2, 2, 1, 1, 32, 2);
+      } else {
+        if (p.config == kLarge) TESM_RUN(3, 4, 2, 2, 2, 32, 2);
+        if (p.config == kMid) TESM_RUN(3, 2, 4, 2, 1, 32, 3);
+        if (p.config == kSmall) TESM_RUN(3, 2, 2, 1, 1, 32, 6);
+        TESM_RUN(3, 2, 2, 1, 1, 32, 3);
+      }
+    }
   }
+  if constexpr (DT == kBF16 || KIND == kProdPartial) {
+    if constexpr (KIND == kProdGated) {
+      if (p.config == kLarge) TESM_RUN(1, 4, 2, 2, 2, 64, 2);
+      if (p.config == kMid) TESM_RUN(1, 2, 2, 2, 1, 64, 2);
+      if (p.config == kSmall) TESM_RUN(1, 2, 2, 2, 1, 64, 4);
+      TESM_RUN(1, 2, 2, 1, 1, 64, 3);
+    } else {
+      if (p.config == kLarge) TESM_RUN(1, 2, 4, 4, 2, 64, 2);
+      if (p.config == kMid) TESM_RUN(1, 2, 2, 2, 2, 64, 2);
+      if (p.config == kSmall) TESM_RUN(1, 2, 2, 2, 2, 64, 4);
+      TESM_RUN(1, 2, 2, 1, 1, 64, 4);
+    }
+  }
+#undef TESM_RUN
+  return fail(kErrUnsupported, "dense product: no kernel for these operands");  // (float32 results of one part)
 }
 
 }  // namespace
 
-int product_splits(int64_t M, int64_t N, int64_t K, int pairs) { return plan_product(kProdPartial, M, N, K, pairs, true).splits; }
+int product_splits(int64_t M, int64_t N, int64_t K, int pairs, bool parts) {
+  return plan_product(kProdPartial, parts, M, N, K, pairs, true).splits;
+}
 
 int launch_product(ProductKind kind, int dt, bool adown, bool bdown, ProductArgs a, hipStream_t st) {
   if (a.M == 0 || a.N == 0) return kOk;
