@@ -450,8 +450,8 @@ int run_product(const ProductArgs& a, hipStream_t st) {
 // Tile sizes.  Large: 256 x 256 results (a gated pair: 256 x 128 of each product) on 8 waves of 128 x 64, one workgroup per CU.
 // Mid: 128 x 128 (128 x 64) on 4 waves of 64 x 64, two workgroups per CU.  Small: the same tiles with four stages, one per CU, for
 // grids that have no second one anyway.  Tiny: 64 x 64 on 4 waves, two per CU.  In us per round of the CUs, with k thousand values of
-// the contraction: 25 k + 8, 15 k + 5 (9 k + 5 where half the places stay empty), 7.6 k + 4 and 5.5 k + 4 (4 k + 3.5); a split adds the
-// float32 results it writes and reads again.  Measured,
+// the contraction: 25 k + 8, 15 k + 5 (9 k + 5 where half the places stay empty), 7.6 k + 4 and 5.5 k + 4 (4 k + 3.5; a pair, which has
+// 64 x 64 of each, 9 k + 4); a split adds the float32 results it writes and reads again.  Measured,
 // bfloat16: 8192 x 16384 x 4096 879 us large (1.25 Pflop/s; the library's product 1.29), mid 1075, small 1240; 8192 x 4096 x 768 58,
 // 69, 83; 8192 x 768 x 2048 47, 31, 39; 4096 x 768 x 8192 147, 77, 66; 512 x 768 x 2048 43, 23, 19, tiny 11; 1024 x 2048 x 768 23, 13, 11, 10.  Operands that lie down: 8192 x 16384 x 4096 864 us with one, 860
 // with both (the library 950 and 1080).  Tiles of 32 values of k instead of 64 cost 20 % where rows run along k (64-byte
@@ -495,7 +495,7 @@ Plan plan_product(ProductKind kind, bool parts, int64_t M, int64_t N, int64_t K,
       cost[kLarge] = ones(large * s, 25.4 * k + 8.0);
       cost[kMid] = twos(mid * s, 9.4 * k + 5.0, 15.3 * k + 5.0);
       cost[kSmall] = ones(mid * s, 7.6 * k + 4.0);
-      cost[kTiny] = twos(tiny * s, 4.0 * k + 3.5, 5.5 * k + 4.0);
+      cost[kTiny] = gated ? twos(tiny * s, 6.5 * k + 4.0, 9.0 * k + 4.0) : twos(tiny * s, 4.0 * k + 3.5, 5.5 * k + 4.0);
     }
     for (int c = 0; c < 4; ++c)
       if (cost[c] + joined < least) {

@@ -203,6 +203,14 @@ def test_products_of_other_layouts(dtype):
 
 @pytest.mark.parametrize("dtype", BOTH)
 @pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("M,K,N", [(1000, 500, 4000), (2000, 100, 4000), (2100, 1000, 1000), (1500, 1300, 2000), (777, 2500, 333)])
+def test_products_of_many_tiles(dtype, pair, M, K, N):
+    """Every tile size, whole and split contractions."""
+    check_dense(dense_case(M + K, M, K, N, dtype, pair=pair, bias=not pair), "gelu")
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("pair", [False, True])
 def test_products_of_nothing(dtype, pair):
     for M, N in [(0, 4), (5, 0), (0, 0)]:
         x, w, b = (torch.randn(*s, device=DEV).to(dtype) for s in ((M, 8), (N, 8), (N,)))
