@@ -54,6 +54,18 @@ def _workspace(nbytes: int, dev):
     return torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes > 0 else None
 
 
+def _rows(t: Optional[torch.Tensor], lead: int):
+    """``_as_rows`` for rows of the last dimension, contiguous ones at once (short calls are bound by the host)."""
+    if t is not None and t.is_contiguous():
+        return t, t.shape[-1] or 1
+    return _as_rows(t, lead)
+
+
+def _empty_as(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous, of t's shape and dtype."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _like(what: str, name: str, t: Optional[torch.Tensor], shape, dtype) -> None:
     if t is not None and (t.shape != torch.Size(shape) or t.dtype != dtype):
         raise ValueError(f"{what}: {name} must be a {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
@@ -95,7 +107,7 @@ def _gates(value, write, decay, bias, state, seq_starts, what, zero_rest=False):
     _like(what, "state", state, (S, C), torch.float32)
     bias = _f32(bias, C, "decay_bias", what)
     state = state.contiguous() if state is not None else None
-    (value, ld_v), (write, ld_w), (decay, ld_d) = _as_rows(value, 2), _as_rows(write, 2), _as_rows(decay, 2)
+    (value, ld_v), (write, ld_w), (decay, ld_d) = _rows(value, 2), _rows(write, 2), _rows(decay, 2)
     require_device(value, write, decay, bias, state, seq_starts)
     d = _lib.Gates(code, B, L, C, S, value.data_ptr(), ld_v, write.data_ptr(), ld_w, decay.data_ptr(), ld_d, _ptr(bias),
                    _ptr(seq_starts), _ptr(state), int(zero_rest and S > 0))
@@ -108,7 +120,7 @@ def _scan_forward(value, write, decay, bias, state, seq_starts, out, keep):
     B, L, C = value.shape
     dev = value.device
     if out is None:  # (rows of no sequence are set to zero by the call, where it has a sequence)
-        out = (torch.empty if S else torch.zeros)((B, L, C), dtype=value.dtype, device=dev)
+        out = _empty_as(value) if S else torch.zeros((B, L, C), dtype=value.dtype, device=dev)
         ld = max(C, 1)
     else:
         require_device(value, out)
@@ -158,7 +170,7 @@ def _scan_backward(grad, value, write, decay, bias, state, seq_starts, kept, gra
     _like(what, "grad_state", grad_state, (S, C), torch.float32)
     lib = _lib.load()
     _like(what, "kept", kept, (lib.tesm_hip_gated_scan_slots(ctypes.byref(g)), C), torch.float32)
-    grad, ld_g = _as_rows(grad, 2)
+    grad, ld_g = _rows(grad, 2)
     grad_state = grad_state.contiguous() if grad_state is not None else None
     kept = kept.contiguous()
     require_device(value, grad, grad_state, kept)
@@ -204,11 +216,11 @@ def gated_scan_step(value: torch.Tensor, write: torch.Tensor, decay: torch.Tenso
     if not state.is_contiguous():
         raise ValueError(f"{what}: state must be contiguous (it is updated in place)")
     decay_bias = _f32(decay_bias, C, "decay_bias", what)
-    (value, ld_v), (write, ld_w), (decay, ld_d) = _as_rows(value, 1), _as_rows(write, 1), _as_rows(decay, 1)
+    (value, ld_v), (write, ld_w), (decay, ld_d) = _rows(value, 1), _rows(write, 1), _rows(decay, 1)
     require_device(value, write, decay, decay_bias, state, out)
     dev = value.device
     if out is None:
-        out = torch.empty((B, C), dtype=value.dtype, device=dev)
+        out = _empty_as(value)
         ld = max(C, 1)
     else:
         ld = _out_rows(out, (B, C), value.dtype, 1, what)
@@ -239,8 +251,8 @@ def _dense(x, weight, up, bias, residual, act, what):
     if residual is not None and residual.shape != torch.Size(shape):
         raise ValueError(f"{what}: residual must be {shape}, got {tuple(residual.shape)}")
     M = math.prod(lead)
-    (x, ld_x), (residual, ld_r) = _as_rows(x, len(lead)), _as_rows(residual, len(lead))
-    (weight, ld_w), (up, ld_u) = _as_rows(weight, 1), _as_rows(up, 1)
+    (x, ld_x), (residual, ld_r) = _rows(x, len(lead)), _rows(residual, len(lead))
+    (weight, ld_w), (up, ld_u) = _rows(weight, 1), _rows(up, 1)
     bias = bias.contiguous() if bias is not None else None
     require_device(x, weight, up, bias, residual)
     d = _lib.Dense(code, act, M, K, N, x.data_ptr(), ld_x, weight.data_ptr(), ld_w, _ptr(up), ld_u, _ptr(bias), _ptr(residual), ld_r,
@@ -260,7 +272,7 @@ def _pair_shape(M, N, dtype):
 def _dense_forward(x, weight, up, bias, residual, act, keep, what):
     d, held, M, shape = _dense(x, weight, up, bias, residual, act, what)
     dev, N = x.device, shape[-1]
-    y = torch.empty(shape, dtype=x.dtype, device=dev)
+    y = x.new_empty(shape)
     d.y, d.ld_y = y.data_ptr(), max(N, 1)
     kept = None
     if keep and up is not None:
@@ -285,7 +297,7 @@ def _dense_backward(grad, x, weight, up, kept, act, need_x, need_w, need_b, what
         _like(what, "kept", t, *((M, N), x.dtype) if up is None else (_pair_shape(M, N, x.dtype), _pair_dtype(x.dtype)))
         if not t.is_contiguous():
             raise ValueError(f"{what}: kept must be what the forward call returned")
-    grad, ld_g = _as_rows(grad, len(shape) - 1)
+    grad, ld_g = _rows(grad, len(shape) - 1)
     require_device(x, grad, *kept)
     if kept:
         d.z = kept[0].data_ptr()
@@ -399,7 +411,7 @@ def _logits(logits, targets, what):
     if logits.shape[-1] < 1:
         raise ValueError(f"{what}: rows without logits")
     code = dt_code(logits.dtype)
-    logits, ld = _as_rows(logits, logits.dim() - 1)
+    logits, ld = _rows(logits, logits.dim() - 1)
     targets = targets.contiguous()
     require_device(logits, targets)
     return code, logits, ld, targets
