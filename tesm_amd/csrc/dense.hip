@@ -22,8 +22,6 @@ typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(2)));  // at any alignment of its values
 typedef uint32_t any8 __attribute__((ext_vector_type(2), aligned(1)));
 
-constexpr int64_t kSkinnyRows = 32;  // up to here weights are streamed once, past the matrix product's tiles
-
 int64_t size_of_dt(int dt) { return dt == kBF16 ? 2 : 4; }
 
 // ---------------------------------------------------------------------------
@@ -113,8 +111,8 @@ __global__ __launch_bounds__(256) void lay_out_kernel(LayOuts t) {
 // few rows: the weights are read once, straight into the matrix unit's operands
 // ---------------------------------------------------------------------------
 // A workgroup owns 16 columns; its 8 waves share the contraction (chunks of 32 values, float32 of 16, taken in turn) and add
-// their sums through LDS in order.  Lane l holds 16 bytes of weight row l % 16 and of x row l % 16.  Bound by the weights' bytes, and
-// for small ones by latency.
+// their sums through LDS in order.  Lane l holds 16 bytes of weight row l % 16 and of x row l % 16.  Bound by the weights' bytes (4096 x
+// 16384 bfloat16, 1 row: 23 us, 5.8 TB/s), for small ones by latency (768 x 2 x 2048: 4.9 us), above 16 rows by its reads of x.
 constexpr int kSkinnyWaves = 8;
 
 template <int DT>
@@ -185,14 +183,16 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_product_kernel(Dense
 #pragma unroll
       for (int e = 0; e < 4; ++e) sums[wave][p][i][4 * g + e][r] = acc[p][i][e];
   __syncthreads();
-  const int col = threadIdx.x & 15, row = threadIdx.x >> 4;  // 32 rows of 16 columns
-  if (row >= 16 * MT || row >= d.M || n0 + col >= d.N) return;
-  float v[2] = {0.0f, 0.0f};
+  const int col = threadIdx.x & 15;
+  if (n0 + col >= d.N) return;
+  for (int row = threadIdx.x >> 4; row < d.M; row += 4 * kSkinnyWaves) {
+    float v[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int p = 0; p < NP; ++p)
+    for (int p = 0; p < NP; ++p)
 #pragma unroll
-    for (int q = 0; q < kSkinnyWaves; ++q) v[p] += sums[q][p][row >> 4][col][row & 15];
-  store_one<KIND, DT>(a, a.out, row, n0 + col, v[0], v[1]);
+      for (int q = 0; q < kSkinnyWaves; ++q) v[p] += sums[q][p][row >> 4][col][row & 15];
+    store_one<KIND, DT>(a, a.out, row, n0 + col, v[0], v[1]);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -404,31 +404,46 @@ int run_skinny(const DenseArgs& d, hipStream_t st) {
   const ProductArgs a = epilogue_of(d);
   const unsigned blocks = static_cast<unsigned>((d.N + 15) / 16);
   constexpr int T = 64 * kSkinnyWaves;
+  const int64_t tiles = (d.M + 15) / 16;
 #define TESM_SKINNY(DT, MT) skinny_product_kernel<KIND, DT, MT><<<blocks, T, 0, TESM_LOGGED(st, skinny_product_kernel<KIND, DT, MT>)>>>(d, a)
   if (d.dt == kBF16) {
-    if (d.M <= 16)
+    if (tiles == 1)
       TESM_SKINNY(kBF16, 1);
     else
       TESM_SKINNY(kBF16, 2);
   } else {
-    if (d.M <= 16)
+    if (tiles == 1)
       TESM_SKINNY(kF32, 1);
-    else
+    else if (tiles == 2)
       TESM_SKINNY(kF32, 2);
+    else
+      TESM_SKINNY(kF32, 4);
   }
 #undef TESM_SKINNY
   return check_launch("dense product of few rows");
 }
 
+// Whether the weights are streamed once, past the matrix product's tiles.  float32 ones up to 64 rows, since tiles need them laid out
+// (768 x 2048: 64 rows 12.7 us, in tiles 21.6; 4096 x 16384: 198 and 216).  bfloat16 ones up to 32 rows, but not where the tiles read them where they lie and are expected to take
+// less time: streaming, every wave reads x besides, and comes to 4.7 TB/s of weights up to 16 rows and 3.2 above (768 x 2048: 1 row 3.8 us,
+// 32 rows 5.2, tiles 6.0; 4096 x 16384: 23, 45 and 22).
+bool streams(const DenseArgs& d, bool ready) {
+  if (d.dt == kF32) return d.M <= 64;
+  if (d.M > 32) return false;
+  const double us = 3.0 + 2.0 * static_cast<double>(d.N * d.K) * (d.w2 ? 2 : 1) / (d.M <= 16 ? 4.7e6 : 3.2e6);
+  return !ready || us <= product_us(d.w2 ? kProdGated : kProdLinear, d.M, d.N, d.K);
+}
+
 int forward(const DenseArgs& d, Space s, bool run, int64_t* need, hipStream_t st) {
-  if (d.M <= kSkinnyRows) {
+  const bool x_ready = lies_ready(d.dt, d.x, d.ld_x, d.K);
+  const bool ready = lies_ready(d.dt, d.w, d.ld_w, d.K) && (!d.w2 || (lies_ready(d.dt, d.w2, d.ld_w2, d.K) && d.ld_w == d.ld_w2));
+  if (streams(d, x_ready && ready)) {
     if (need) *need = 0;
     if (!run || d.M == 0 || d.N == 0) return kOk;
     return d.w2 ? run_skinny<kProdGated>(d, st) : run_skinny<kProdLinear>(d, st);
   }
-  const bool ready = lies_ready(d.dt, d.w, d.ld_w, d.K) && (!d.w2 || (lies_ready(d.dt, d.w2, d.ld_w2, d.K) && d.ld_w == d.ld_w2));
   LayOuts todo;
-  const Matrix x = bring(s, todo, d.dt, d.x, d.ld_x, d.M, d.K, lies_ready(d.dt, d.x, d.ld_x, d.K));
+  const Matrix x = bring(s, todo, d.dt, d.x, d.ld_x, d.M, d.K, x_ready);
   const Matrix w = bring(s, todo, d.dt, d.w, d.ld_w, d.N, d.K, ready);
   const Matrix w2 = d.w2 ? bring(s, todo, d.dt, d.w2, d.ld_w2, d.N, d.K, ready) : Matrix{};
   if (need) *need = s.used;

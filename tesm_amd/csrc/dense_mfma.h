@@ -44,6 +44,9 @@ int launch_product(ProductKind kind, int dt, bool adown, bool bdown, ProductArgs
 // How many runs the contraction of such a product should be split into (1: none).
 int product_splits(int64_t M, int64_t N, int64_t K, int pairs, bool parts);
 
+// How long a product of bfloat16 operands that lie ready is expected to take.
+double product_us(ProductKind kind, int64_t M, int64_t N, int64_t K);
+
 // The normal distribution's Phi(z) = (1 + erf(z / sqrt 2)) / 2 and e = exp(-z^2 / 2), with erfc(x) = P(t) exp(-x^2), t = 1 / (1 + p x),
 // the polynomial of Abramowitz and Stegun 7.1.26 (1.5e-7 off at most).  The library's erff takes three times as long: 8192 x 16384
 // results of K = 4096 1101 us with it.

@@ -466,6 +466,7 @@ enum Config : int { kLarge, kMid, kSmall, kTiny };
 struct Plan {
   Config config = kSmall;
   int splits = 1;
+  double us = 1e30;
 };
 Plan plan_product(ProductKind kind, bool parts, int64_t M, int64_t N, int64_t K, int pairs, bool split) {
   const int64_t cus = std::max(device_limits().cus, 1);
@@ -482,7 +483,6 @@ Plan plan_product(ProductKind kind, bool parts, int64_t M, int64_t N, int64_t K,
   const double all = static_cast<double>(K) * pairs / 1000.0;
   const int64_t steps = (K + 63) / 64 * pairs;
   Plan best;
-  double least = 1e30;
   for (int s = 1; s <= (split ? 16 : 1) && (s == 1 || s * 4 <= steps); ++s) {
     const double k = all / s, joined = s == 1 ? 0.0 : 6.0 + 2.0 * s * 4.0 * static_cast<double>(M) * static_cast<double>(N) / 5.0e6;
     double cost[4];
@@ -498,10 +498,7 @@ Plan plan_product(ProductKind kind, bool parts, int64_t M, int64_t N, int64_t K,
       cost[kTiny] = gated ? twos(tiny * s, 6.5 * k + 4.0, 9.0 * k + 4.0) : twos(tiny * s, 4.0 * k + 3.5, 5.5 * k + 4.0);
     }
     for (int c = 0; c < 4; ++c)
-      if (cost[c] + joined < least) {
-        least = cost[c] + joined;
-        best = {static_cast<Config>(c), s};
-      }
+      if (cost[c] + joined < best.us) best = {static_cast<Config>(c), s, cost[c] + joined};
   }
   return best;
 }
@@ -549,6 +546,8 @@ int pick(const ProductArgs& a, hipStream_t st) {
 int product_splits(int64_t M, int64_t N, int64_t K, int pairs, bool parts) {
   return plan_product(kProdPartial, parts, M, N, K, pairs, true).splits;
 }
+
+double product_us(ProductKind kind, int64_t M, int64_t N, int64_t K) { return plan_product(kind, false, M, N, K, 1, false).us; }
 
 int launch_product(ProductKind kind, int dt, bool adown, bool bdown, ProductArgs a, hipStream_t st) {
   if (a.M == 0 || a.N == 0) return kOk;

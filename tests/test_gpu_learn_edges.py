@@ -211,6 +211,14 @@ def test_products_of_many_tiles(dtype, pair, M, K, N):
 
 @pytest.mark.parametrize("dtype", BOTH)
 @pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("M,K,N", [(1, 512, 16384), (20, 512, 16384), (20, 516, 16384), (40, 70, 50), (64, 300, 33), (65, 300, 33)])
+def test_products_of_few_rows(dtype, pair, M, K, N):
+    """Weights streamed once, or in tiles where those are expected to take less time."""
+    check_dense(dense_case(M + N, M, K, N, dtype, pair=pair, bias=not pair, residual=not pair), "silu")
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("pair", [False, True])
 def test_products_of_nothing(dtype, pair):
     for M, N in [(0, 4), (5, 0), (0, 0)]:
         x, w, b = (torch.randn(*s, device=DEV).to(dtype) for s in ((M, 8), (N, 8), (N,)))
