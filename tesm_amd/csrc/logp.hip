@@ -9,6 +9,9 @@
 // The backward pass forms p again as 2^((x - m) L - d), m near the row's largest logit and d in two floats: the high one goes into
 // the exponent's fused operation, the low one into the row's two coefficients, so that an element costs one exponential and five
 // more operations.
+//
+// Bound by HBM: 8192 x 151936 bfloat16 forward 459 us, backward 939 (5.4 TB/s); one row with its 20 best by latency, 10 us and 5 to join
+// its parts.
 #include "logp.h"
 #include "row_pass.h"
 

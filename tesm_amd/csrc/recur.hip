@@ -18,6 +18,10 @@
 // there, its bits are those of no number before: a flag beside it would cost the chain three more trips through memory (one for the
 // values to arrive before the flag, two for the reader).  A poll gives up after kSpinLimit rounds: the states are then NaN and bit 0 of
 // the status word is set.
+//
+// Bound by HBM where there is much of it: 32768 x 8192 bfloat16 forward 484 us (4.4 TB/s; a copy's 5.9 would take 364), backward 872 (637).
+// The vector unit is busy for 58 to 63 % of that, the chain costs 7 %, the tickets 5 %; workgroups that stay and load their next
+// tile ahead took 610 and 1103 us.  Short calls by latency: 4 x 2048 x 384 11 and 16 us.
 #include <type_traits>
 #include <utility>
 
@@ -612,6 +616,7 @@ __global__ __launch_bounds__(256) void recur_rest_kernel(RestArgs a) {
   }
 }
 
+// One token: a channel per thread (64 x 8192 bfloat16 3.4 us, 2.5 TB/s).
 template <int DT>
 __global__ __launch_bounds__(256) void recur_step_kernel(RecurStepArgs a) {
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, b = blockIdx.y;

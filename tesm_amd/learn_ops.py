@@ -338,9 +338,9 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
 
     x (.., K), w_gate and w_up (N, K) share a dtype; ``act`` is "silu" or "gelu" (the error function's form).  Sums and the
     activation are float32, the result is rounded once.  float32 operands go through the matrix units in three bfloat16 parts, to the
-    error of a float32 sum; an infinity among them gives NaN.  Of few rows (up to 32, float32 64) the weights are
-    streamed once.  ``keep=True`` also
-    returns what ``gated_linear_backward`` needs (both products, in 24 bits where x is bfloat16).
+    error of a float32 sum; an infinity among them gives NaN.  Of few rows (up to 32, float32 64) the weights are streamed once.
+    Rows of more than 2^21 values may be refused.  ``keep=True`` also returns what ``gated_linear_backward`` needs (both products,
+    in 24 bits where x is bfloat16).
     """
     code = _act_code(act, "gated_linear", pair=True)
     if _records("gated_linear", keep, x, w_gate, w_up):
