@@ -150,7 +150,7 @@ def gated_scan(value: torch.Tensor, write: torch.Tensor, decay: torch.Tensor, de
     ``out`` (zero without ``out``).  A decay of -infinity forgets, one of +infinity with a write of -infinity leaves the state
     as it is; states are float32, finite ones, and results repeat bit for bit.
 
-    ``keep=True`` also returns what ``gated_scan_backward`` needs (float32, one row per 128).  ``out`` takes no gradients and must not
+    ``keep=True`` also returns what ``gated_scan_backward`` needs (float32, one row per 64).  ``out`` takes no gradients and must not
     overlap an operand.  Fewer than 2^31 rows, C below 2^24.
     """
     if _records("gated_scan", keep, value, write, decay, decay_bias, state):
