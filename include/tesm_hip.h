@@ -736,7 +736,8 @@ int tesm_hip_dense_forward(const tesm_hip_dense* p, void* ws, int64_t ws_bytes, 
 
 /* Its backward pass: from the gradient of y those of x, weight, up and bias that are asked for (the residual's is y's own).  of: the
  * forward call's descriptor (bias, residual and y are not used); z and z_up what it kept (z not needed with act 0).  The
- * gradients in front of the products go into them rounded to bfloat16, for float32 in three parts. */
+ * gradients in front of the products go into them in two bfloat16 parts (16 bits) where an activation or a pair made them, for float32 in
+ * three; gradients made with an infinite operand may be NaN. */
 typedef struct tesm_hip_dense_grad {
   tesm_hip_dense of;
   const void* grad;           /* (M, ld_grad) */

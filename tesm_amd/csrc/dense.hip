@@ -8,9 +8,10 @@
 // float32 rate, so six of them are 2.7 times as fast as one in float32.  An infinite operand gives NaN where the formula may
 // give an infinity.
 //
-// Gradients.  What stands before the activation is kept by the forward pass: z in the operands' type (it reaches the gradients through
-// the activation's slope alone), a pair's z and z2 of bfloat16 operands in 24 bits.  The gradient in
-// front of the products goes into them in bfloat16 (float32: in three parts).
+// Gradients.  What stands before the activation is kept by the forward pass.  The gradient in front of the products is float32; an
+// activation or a pair's factor leaves more bits in it than bfloat16 holds, and it goes into the products in two bfloat16 parts, 16 bits
+// (float32: in three).  In one part its rounding alone was as large as the results' own (8192 x 768 x 2 x 2048: gradients 2.3e-3 of
+// themselves off, the results' rounding 1.7e-3).
 #include "dense_mfma.h"
 
 namespace tesm {
@@ -40,22 +41,22 @@ __device__ __forceinline__ Parts3 split3(float x) {
   const uint16_t m = f32_to_bf16(r);
   return {{h, m, f32_to_bf16(r - bf16_to_f32(m))}};
 }
-// Eight values to PARTS parts, `stride` apart.
+// Eight values to PARTS parts, `stride` apart (two parts: the first 16 bits).
 template <int PARTS>
 __device__ __forceinline__ void store_parts(uint16_t* to, int64_t stride, const float (&v)[8]) {
   if constexpr (PARTS == 1) {
     *reinterpret_cast<uint4*>(to) =
         make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
   } else {
-    uint32_t w[3][4];
+    uint32_t w[PARTS][4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const Parts3 a = split3(v[2 * q]), b = split3(v[2 * q + 1]);
 #pragma unroll
-      for (int p = 0; p < 3; ++p) w[p][q] = a.p[p] | static_cast<uint32_t>(b.p[p]) << 16;
+      for (int p = 0; p < PARTS; ++p) w[p][q] = a.p[p] | static_cast<uint32_t>(b.p[p]) << 16;
     }
 #pragma unroll
-    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(to + p * stride) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+    for (int p = 0; p < PARTS; ++p) *reinterpret_cast<uint4*>(to + p * stride) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
   }
 }
 // Eight values at element i, of which `n` exist (the others are 0); whole ones by one or two loads, at any alignment.
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const void* grad, int64
     g[e] = e < n ? d[e] * u[e] * s : 0.0f;
     u[e] = e < n ? d[e] * v : 0.0f;
   }
-  constexpr int P = DT == kBF16 ? 1 : 3;
+  constexpr int P = DT == kBF16 ? 2 : 3;
   store_parts<P>(dst + m * 2 * Np + c, M * 2 * Np, g);
   store_parts<P>(dst + m * 2 * Np + Np + c, M * 2 * Np, u);
 }
@@ -270,7 +271,12 @@ __global__ __launch_bounds__(256) void linear_grad_kernel(const void* grad, int6
           d[e] = e < n ? d[e] * b : 0.0f;
         }
       }
-      if (dst) store_parts<DT == kBF16 ? 1 : 3>(dst + m * Np + c, M * Np, d);
+      if (dst) {  // (without an activation the gradient is as it came)
+        if (DT == kBF16 && act == kActNone)
+          store_parts<1>(dst + m * Np + c, M * Np, d);
+        else
+          store_parts<DT == kBF16 ? 2 : 3>(dst + m * Np + c, M * Np, d);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[e] += d[e];
     }
@@ -487,9 +493,10 @@ int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_
   const int dt = d.dt;
   const int64_t M = d.M, N = d.N, K = d.K, Np = round_up(N, 64);  // (rows of whole cache lines)
   const bool gated = d.w2 != nullptr, products = b.dx || b.dw || b.dw2;
+  const int parts = dt == kF32 ? 3 : gated || d.act != kActNone ? 2 : 1;  // of the gradient in front of the products
   Matrix dz;
   if (gated) {
-    uint16_t* dst = s.take<uint16_t>(M * 2 * Np * (dt == kBF16 ? 1 : 3));
+    uint16_t* dst = s.take<uint16_t>(M * 2 * Np * parts);
     dz = {dst, dt == kBF16 ? 0 : M * 2 * Np, 2 * Np, 2 * Np};
     const int64_t threads = M * Np / 8;
     if (run && threads && products) {
@@ -506,7 +513,7 @@ int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_
     if (direct)
       dz = {static_cast<const uint16_t*>(b.grad), 0, b.ld_g, N};
     else {
-      dst = s.take<uint16_t>(M * Np * (dt == kBF16 ? 1 : 3));
+      dst = s.take<uint16_t>(M * Np * parts);
       dz = {dst, dt == kBF16 ? 0 : M * Np, Np, Np};
     }
     const int64_t rows = (M + kSumRows - 1) / kSumRows;
@@ -530,6 +537,7 @@ int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_
   LayOuts todo;
   Matrix w, w2, x;
   const bool for_x = b.dx && M, for_w = (b.dw || b.dw2) && N;
+  const int sums_of = dt == kF32 ? 1 : parts;  // (float32 parts meet inside the product, two bfloat16 ones as products that are added up)
   if (for_x) {
     const bool ready = lies_ready(dt, d.w, d.ld_w, K) && (!gated || (lies_ready(dt, d.w2, d.ld_w2, K) && d.ld_w == d.ld_w2));
     w = bring(s, todo, dt, d.w, d.ld_w, N, K, ready);
@@ -542,8 +550,10 @@ int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_
     ProductArgs a;
     a.M = M, a.N = K, a.K = N;
     a.pairs = 0;
-    add_pair(a, dz, 0, w, nullptr);
-    if (gated) add_pair(a, dz, Np, w2, nullptr);
+    for (int p = 0; p < sums_of; ++p) {
+      add_pair(a, dz, p * M * dz.ld, w, nullptr);
+      if (gated) add_pair(a, dz, p * M * dz.ld + Np, w2, nullptr);
+    }
     a.lda = dz.ld, a.ldb = w.ld, a.ext_b = w.ext;
     a.out = b.dx;
     if (int rc = grad_product(s, run, dt, false, a, st)) return rc;
@@ -552,7 +562,7 @@ int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_
     ProductArgs a;
     a.M = gated ? Np + N : N, a.N = K, a.K = M;
     a.pairs = 0;
-    add_pair(a, dz, 0, x, nullptr);
+    for (int p = 0; p < sums_of; ++p) add_pair(a, dz, p * M * dz.ld, x, nullptr);
     a.lda = dz.ld, a.ext_a = dz.ext, a.ldb = x.ld, a.ext_b = x.ext;
     a.out = b.dw, a.out2 = b.dw2;
     a.cut = N, a.fold = Np;

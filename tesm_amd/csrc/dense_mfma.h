@@ -6,7 +6,7 @@
 
 namespace tesm {
 
-constexpr int kMaxPairs = 2, kParts = 3;
+constexpr int kMaxPairs = 4;
 
 // out[m, n] = sum over pairs p and k of A_p[m, k] B_p[n, k].  An operand lies with k along its rows (m or n picks the row), or, where
 // its layout is "down", with k picking the row.  All pairs share extents and pitches.  Rows start on 16 bytes; the contiguous

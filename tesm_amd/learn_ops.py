@@ -352,8 +352,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
 def gated_linear_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, kept, act: str = "silu",
                           need_x: bool = True, need_weights: bool = True):
     """The gradients ``(x, w_gate, w_up)`` of ``gated_linear``, called with the same operands and ``keep=True``; those not asked
-    for are None.  The gradients of the two products are rounded to x's dtype (float32: kept in three bfloat16 parts) before the
-    products with x and the weights, whose sums are float32."""
+    for are None.  The gradients of the two products go into those with x and the weights in 16 bits (float32: all 24), the sums are
+    float32, and the results are rounded once; where bfloat16 operands hold an infinity, gradients made with it may be NaN."""
     hip_ops._no_grad("gated_linear_backward", grad, x, w_gate, w_up)
     return _dense_backward(grad, x, w_gate, w_up, kept, _act_code(act, "gated_linear_backward", pair=True), need_x, need_weights, False,
                            "gated_linear_backward")[:3]

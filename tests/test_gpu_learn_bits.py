@@ -1,0 +1,41 @@
+"""Gradients and results that lose no more bits than their type's own rounding takes (bounds: ``learn_bits``)."""
+import pytest
+import torch
+
+from hip_helpers import DEV, need_gpu
+from learn_bits import dense_bounds
+from learn_refs import within
+from tesm_amd import hip_ops
+from test_gpu_learn import _dev, dense_case
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    need_gpu()
+    with torch.no_grad():
+        yield
+
+
+def gradients(c, act):
+    x, w, up, b, grad = (_dev(c[k]) for k in ("x", "w", "up", "bias", "grad"))
+    if up is not None:
+        _, kept = hip_ops.gated_linear(x, w, up, act=act, keep=True)
+        return dict(zip(("dx", "dw", "du"), hip_ops.gated_linear_backward(grad, x, w, up, kept=kept, act=act)))
+    _, kept = hip_ops.fused_linear(x, w, b, act=act, keep=True)
+    got = dict(zip(("dx", "dw", "db"), hip_ops.fused_linear_backward(grad, x, w, b, kept=kept, act=act)))
+    return got if b is not None else {k: got[k] for k in ("dx", "dw")}
+
+
+SIZES = [(40, 31, 70), (70, 40, 26), (130, 72, 136), (300, 64, 256)]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_gradients_of_a_pair(act, M, K, N):
+    c = dense_case(M + N, M, K, N, BF, pair=True)
+    r = dense_bounds(c, act)
+    for name, got in gradients(c, act).items():
+        within(got, *r[name], name)
