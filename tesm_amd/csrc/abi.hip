@@ -2223,7 +2223,7 @@ bool plain_sizes(const tesm_hip_dense& p, std::initializer_list<int64_t> pitches
          p.N < (1LL << 24) && p.K < (1LL << 24);
 }
 // What a call keeps of one product, in bytes.
-int64_t kept_bytes(const tesm_hip_dense& p) { return p.M * p.N * (p.dt != kBF16 ? 4 : p.up ? 3 : 2); }
+int64_t kept_bytes(const tesm_hip_dense& p) { return p.M * p.N * (p.dt != kBF16 ? 4 : 3); }
 std::vector<NamedSpan> dense_spans(const tesm_hip_dense& p) {
   const int64_t e = size_of(p.dt);
   return {{"x", span(p.x, p.M, p.ld_x, p.K, e)}, {"weight", span(p.weight, p.N, p.ld_weight, p.K, e)},

@@ -24,7 +24,7 @@ struct DenseArgs {
   int64_t ld_r = 0;
   void* y = nullptr;  // (M, ld_y)
   int64_t ld_y = 0;
-  void* z = nullptr;  // optional (M, N)
+  void* z = nullptr;  // optional (M, N): float32, or 24 bits (dense_mfma.h)
   void* z2 = nullptr;
 };
 

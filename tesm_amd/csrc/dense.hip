@@ -199,7 +199,7 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_product_kernel(Dense
 // ---------------------------------------------------------------------------
 // in front of the backward products
 // ---------------------------------------------------------------------------
-// Eight kept products of a pair.
+// Eight kept products.
 template <int DT>
 __device__ __forceinline__ void kept_eight(const void* z, int64_t all, int64_t i, int n, float (&v)[8]) {
   if constexpr (DT == kF32) {
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(256) void linear_grad_kernel(const void* grad, int6
       load_eight<DT>(grad, m * ld_g + c, n, d);
       if (act != kActNone) {
         float v[8];
-        load_eight<DT>(z, m * N + c, n, v);
+        kept_eight<DT>(z, M * N, m * N + c, n, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           float a, b;

@@ -85,10 +85,9 @@ __device__ __forceinline__ void act_both(float z, int act, float& v, float& d) {
   }
 }
 
-// What a pair keeps of bfloat16 operands' products for the backward pass: 24 bits of each, the upper 16 of all values, then the next 8
-// (`all` values further).  The gradients are products of the kept ones, and 16 bits would cost them as much as their own
-// rounding does (8192 x 768 x 2 x 2048: gradients off by 3.1e-3 of themselves instead of 2.4e-3).  float32 products are kept as they
-// are.
+// What is kept of bfloat16 operands' products for the backward pass: the upper 24 bits of each (16 of its significand), the first 16 of
+// all values, then the next 8 (`all` values further).  The gradients are products of a pair's kept ones and of an activation's slope at
+// them, and with 16 bits of each they would be further off than their own rounding takes them.  float32 products are kept as they are.
 __device__ __forceinline__ uint32_t to_24(float v) {
   const uint32_t b = __float_as_uint(v);
   return (b & 0x7f800000u) == 0x7f800000u ? b | (b & 0x007fffffu ? 0x00400000u : 0u) : b + 0x80u;  // (infinities and NaNs keep their kind)
@@ -115,7 +114,7 @@ __device__ __forceinline__ void store_one(const ProductArgs& a, void* out, int64
     st<DT>(out, m * a.ldo + n, act_value(v, a.act) * v2);
   } else if constexpr (KIND == kProdLinear) {
     if (a.bias) v += ld<DT>(a.bias, n);
-    if (a.z) st<DT>(a.z, m * a.N + n, v);
+    if (a.z) keep_one<DT>(a.z, a.M * a.N, m * a.N + n, v);
     v = act_value(v, a.act);
     if (a.residual) v += ld<DT>(a.residual, m * a.ld_r + n);
     st<DT>(out, m * a.ldo + n, v);

@@ -196,7 +196,7 @@ __device__ __forceinline__ void store_eight(const ProductArgs& a, void* out, int
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += b[e];
     }
-    if (a.z) store8<DT>(a.z, m * a.N + n, v);
+    if (a.z) keep_eight<DT>(a.z, a.M * a.N, m * a.N + n, v);
     if (a.act != kActNone) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = act_value(v[e], a.act);

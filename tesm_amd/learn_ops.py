@@ -260,12 +260,12 @@ def _dense(x, weight, up, bias, residual, act, what):
     return d, (x, weight, up, bias, residual), M, shape
 
 
-def _pair_dtype(dtype):
+def _kept_dtype(dtype):
     return torch.float32 if dtype == torch.float32 else torch.uint8
 
 
-def _pair_shape(M, N, dtype):
-    """What a pair keeps of each product: float32, or 3 bytes a value (and what keeps the second one's on 16 bytes)."""
+def _kept_shape(M, N, dtype):
+    """What is kept of each product: float32, or 3 bytes a value (and what keeps a pair's second one's on 16 bytes)."""
     return (M, N) if dtype == torch.float32 else ((3 * M * N + 15) // 16 * 16,)
 
 
@@ -276,10 +276,10 @@ def _dense_forward(x, weight, up, bias, residual, act, keep, what):
     d.y, d.ld_y = y.data_ptr(), max(N, 1)
     kept = None
     if keep and up is not None:
-        kept = torch.empty((2, *_pair_shape(M, N, x.dtype)), dtype=_pair_dtype(x.dtype), device=dev).unbind()
+        kept = torch.empty((2, *_kept_shape(M, N, x.dtype)), dtype=_kept_dtype(x.dtype), device=dev).unbind()
         d.z, d.z_up = kept[0].data_ptr(), kept[1].data_ptr()
     elif keep and act:
-        kept = torch.empty((M, N), dtype=x.dtype, device=dev)
+        kept = torch.empty(_kept_shape(M, N, x.dtype), dtype=_kept_dtype(x.dtype), device=dev)
         d.z = kept.data_ptr()
     lib, ref = _lib.load(), ctypes.byref(d)
     nbytes = lib.tesm_hip_dense_ws_bytes(ref)
@@ -294,7 +294,7 @@ def _dense_backward(grad, x, weight, up, kept, act, need_x, need_w, need_b, what
     _like(what, "the gradient", grad, shape, x.dtype)
     kept = tuple(kept) if up is not None else (kept,) if act else ()
     for t in kept:
-        _like(what, "kept", t, *((M, N), x.dtype) if up is None else (_pair_shape(M, N, x.dtype), _pair_dtype(x.dtype)))
+        _like(what, "kept", t, _kept_shape(M, N, x.dtype), _kept_dtype(x.dtype))
         if not t.is_contiguous():
             raise ValueError(f"{what}: kept must be what the forward call returned")
     grad, ld_g = _rows(grad, len(shape) - 1)
@@ -382,7 +382,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     """A projection with what follows it in one kernel: ``act(x weight^T + bias) + residual``, (.., N).
 
     x (.., K), weight (N, K), bias (N) and residual (.., N) share a dtype; ``act`` is None, "silu" or "gelu".  Precision and few
-    rows as in ``gated_linear``.  ``keep=True`` also returns what ``fused_linear_backward`` needs (None without an activation).
+    rows as in ``gated_linear``.  ``keep=True`` also returns what ``fused_linear_backward`` needs (the sum in front of the activation, in 24
+    bits where x is bfloat16; None without an activation).
     """
     code = _act_code(act, "fused_linear")
     if _records("fused_linear", keep, x, weight, bias, residual):

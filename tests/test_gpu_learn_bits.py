@@ -39,3 +39,12 @@ def test_gradients_of_a_pair(act, M, K, N):
     r = dense_bounds(c, act)
     for name, got in gradients(c, act).items():
         within(got, *r[name], name)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", None])
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_gradients_of_an_activation(act, M, K, N):
+    c = dense_case(M * N, M, K, N, BF, bias=True)
+    r = dense_bounds(c, act)
+    for name, got in gradients(c, act).items():
+        within(got, *r[name], name)

@@ -47,4 +47,12 @@ def test_a_gradient_rounded_in_front_of_the_products_is_seen(pair, act, M, K, N)
     two = lambda t: rounded(t) + rounded(t - rounded(t))
     assert not any(worst(c, act, front=two).values())
     one = worst(c, act, front=rounded)
-    assert all(one[k] > 0.05 for k in ("dx", "dw"))
+    assert one["dx"] and one["dw"]
+
+
+@pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_a_kept_value_rounded_to_its_type_is_seen(pair, M, K, N):
+    c = dense_case(M + N, M, K, N, BF, pair)
+    off = worst(c, "gelu", kept=rounded)
+    assert off["dx"] and off["dw"]  # (one value beyond its bound is enough)
