@@ -2369,6 +2369,7 @@ int tesm_hip_dense_backward(const tesm_hip_dense_grad* p, void* ws, int64_t ws_b
   TESM_REQUIRE(p != nullptr, kErrInvalidArg, "dense backward: null descriptor");
   return guarded(who, [&]() -> int {
     TESM_REQUIRE(!p->of.up || !p->d_bias, kErrInvalidArg, "dense backward: a gated pair has no bias");
+    TESM_REQUIRE(!p->of.up || p->of.act != kActNone, kErrInvalidArg, "dense backward: a gated pair has an activation");
     if (plain_sizes(p->of, {p->ld_grad})) {
       const int64_t e = size_of(p->of.dt), kept = kept_bytes(p->of), nk = p->of.N * p->of.K;
       std::vector<NamedSpan> in = dense_spans(p->of);

@@ -610,6 +610,7 @@ int launch_dense_bwd(const DenseBwdArgs& b, void* ws, int64_t ws_bytes, hipStrea
                                         (!(b.dw || b.dw2) || (a.x && a.ld_x >= a.K))),
                kErrInvalidArg, w + "need the operands that the gradients asked for are made of");
   TESM_REQUIRE(!a.w2 || (b.dw != nullptr) == (b.dw2 != nullptr), kErrInvalidArg, w + "both weights' gradients or none");
+  TESM_REQUIRE(!a.w2 || a.act != kActNone, kErrInvalidArg, w + "need an activation");
   TESM_REQUIRE(a.M == 0 || a.N == 0 || a.act == kActNone || (a.z && (!a.w2 || a.z2)), kErrInvalidArg,
                w + "need what the forward call kept");
   const int64_t need = dense_bwd_ws_bytes(b);
