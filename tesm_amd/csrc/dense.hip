@@ -243,55 +243,61 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const void* grad, int64
   store_parts<P>(dst + m * 2 * Np + Np + c, M * 2 * Np, u);
 }
 
-constexpr int kSumRows = 64;  // rows per workgroup
-// dz = dy act'(z) into its parts (dst), and the sums of kSumRows rows of it (sums); either may be left out.
+constexpr int kSumRows = 64;  // rows per sum
+// dz = dy act'(z) into its parts (dst), and the sums of kSumRows rows of it (sums); either may be left out.  A workgroup takes every
+// gridDim.y-th run of kSumRows rows.
 template <int DT>
 __global__ __launch_bounds__(256) void linear_grad_kernel(const void* grad, int64_t ld_g, const void* z, int64_t M, int64_t N, int64_t Np,
                                                           int act, uint16_t* dst, float* sums) {
   __shared__ float part[8][32][9];
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
-  const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + cx) * 8, m0 = static_cast<int64_t>(blockIdx.y) * kSumRows;
-  float s[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) s[e] = 0.0f;
-  if (c < Np) {
-    const int n = static_cast<int>(N - c < 8 ? N - c : 8);
-    const int64_t end = m0 + kSumRows < M ? m0 + kSumRows : M;
-#pragma unroll 4
-    for (int64_t m = m0 + ry; m < end; m += 8) {
-      float d[8];
-      load_eight<DT>(grad, m * ld_g + c, n, d);
-      if (act != kActNone) {
-        float v[8];
-        kept_eight<DT>(z, M * N, m * N + c, n, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float a, b;
-          act_both(v[e], act, a, b);
-          d[e] = e < n ? d[e] * b : 0.0f;
-        }
-      }
-      if (dst) {  // (without an activation the gradient is as it came)
-        if (DT == kBF16 && act == kActNone)
-          store_parts<1>(dst + m * Np + c, M * Np, d);
-        else
-          store_parts<DT == kBF16 ? 2 : 3>(dst + m * Np + c, M * Np, d);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += d[e];
-    }
-  }
-  if (!sums) return;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) part[ry][cx][e] = s[e];
-  __syncthreads();
+  const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + cx) * 8;
   const int col = threadIdx.x;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + col;
-  if (at >= N) return;
-  float x = 0.0f;
+  for (int64_t run = blockIdx.y; run * kSumRows < M; run += gridDim.y) {
+    const int64_t m0 = run * kSumRows;
+    float s[8];
 #pragma unroll
-  for (int q = 0; q < 8; ++q) x += part[q][col >> 3][col & 7];
-  sums[blockIdx.y * N + at] = x;
+    for (int e = 0; e < 8; ++e) s[e] = 0.0f;
+    if (c < Np) {
+      const int n = static_cast<int>(N - c < 8 ? N - c : 8);
+      const int64_t end = m0 + kSumRows < M ? m0 + kSumRows : M;
+#pragma unroll 4
+      for (int64_t m = m0 + ry; m < end; m += 8) {
+        float d[8];
+        load_eight<DT>(grad, m * ld_g + c, n, d);
+        if (act != kActNone) {
+          float v[8];
+          kept_eight<DT>(z, M * N, m * N + c, n, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float a, b;
+            act_both(v[e], act, a, b);
+            d[e] = e < n ? d[e] * b : 0.0f;
+          }
+        }
+        if (dst) {  // (without an activation the gradient is as it came)
+          if (DT == kBF16 && act == kActNone)
+            store_parts<1>(dst + m * Np + c, M * Np, d);
+          else
+            store_parts<DT == kBF16 ? 2 : 3>(dst + m * Np + c, M * Np, d);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += d[e];
+      }
+    }
+    if (!sums) continue;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[ry][cx][e] = s[e];
+    __syncthreads();
+    if (at < N) {
+      float x = 0.0f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) x += part[q][col >> 3][col & 7];
+      sums[run * N + at] = x;
+    }
+    __syncthreads();  // (`part` is written again)
+  }
 }
 // The sums of all workgroups' rows, in 64 bits: 16 runs of them side by side, joined in order.
 template <int DT>
@@ -519,8 +525,7 @@ int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_
     const int64_t rows = (M + kSumRows - 1) / kSumRows;
     float* sums = b.dbias ? s.take<float>(rows * N) : nullptr;
     if (run && M && N && (sums || (dst && products))) {
-      TESM_REQUIRE(rows < 65536, kErrUnsupported, "dense backward: too many rows");
-      const dim3 grid(static_cast<unsigned>((Np + 255) / 256), static_cast<unsigned>(rows));
+      const dim3 grid(static_cast<unsigned>((Np + 255) / 256), static_cast<unsigned>(std::min<int64_t>(rows, 65535)));
       if (dt == kBF16)
         linear_grad_kernel<kBF16><<<grid, 256, 0, TESM_LOGGED(st, linear_grad_kernel<kBF16>)>>>(b.grad, b.ld_g, d.z, M, N, Np, d.act, dst, sums);
       else
