@@ -638,7 +638,7 @@ int tesm_hip_reorder_rows(const tesm_hip_rows* t, int64_t count, const int64_t* 
  * zero_rest, set to zero.  h0 / h_out: (S, C) float32,
  * the states before and after each sequence (NULL h0: zeros).  States are float32; results repeat bit for bit.  carries:
  * (tesm_hip_gated_scan_slots, C) float32, what the backward call needs (NULL: not kept).  Fewer than 2^31 rows, C and S
- * below 2^24.  Outputs must not overlap operands or each other (columns of the same wider rows do not overlap). */
+ * below 2^24, and fewer than 2^23 tiles of 64 rows of a sequence by 64 channels.  Outputs must not overlap operands or each other (columns of the same wider rows do not overlap). */
 typedef struct tesm_hip_gates {
   int dt;                     /* value, write, decay, and the arrays of their shape */
   int64_t B, L, C, S;
@@ -711,7 +711,8 @@ int tesm_hip_gated_scan_step(const tesm_hip_recurrence_step* p, void* stream);
  * float32 operands go through the matrix units in three bfloat16 parts (an infinity among them gives NaN).  z, for the
  * backward call (NULL: not kept): x weight^T + bias; of a pair, with z_up, x weight^T and x up^T; each (M, N) float32, or
  * with bf16 operands M * N upper 16 bits followed by M * N next 8 bits.  M < 2^31, N, K < 2^24; above
- * 2^21 values per row or pitch, calls of many rows may be refused (32-bit offsets inside a tile). */
+ * 2^21 values per row or pitch, calls of many rows may be refused (32-bit offsets inside a tile), and so may matrices of 2^34 values
+ * in rows padded to 64. */
 typedef struct tesm_hip_dense {
   int dt;
   int act;
@@ -755,7 +756,8 @@ int tesm_hip_dense_backward(const tesm_hip_dense_grad* p, void* ws, int64_t ws_b
  * t = targets[r] (0 where t is ignore), entropy[r] of the row's distribution, and the log probabilities and tokens of its top
  * largest logits in falling order, equal ones by token (a NaN logit counts as the lowest).  -infinity is a masked token; a row with a
  * NaN or +infinite logit, or none above -infinity, gives NaN.  Any other target outside [0, V) gives NaN and sets
- * TESM_STATUS_BAD_TARGET.  kept: (rows, 4) float32 for the backward call (NULL: not kept).  top <= 64, V < 2^30. */
+ * TESM_STATUS_BAD_TARGET.  kept: (rows, 4) float32 for the backward call (NULL: not kept).  top <= 64, V < 2^30,
+ * fewer than 2^24 rows. */
 typedef struct tesm_hip_logp {
   int dt;                     /* logits */
   int64_t rows, V, top;

@@ -369,7 +369,7 @@ int lay_out(LayOuts& t, int dt, hipStream_t st) {
   for (int k = 0; k < t.count; ++k) {
     t.m[k].block0 = static_cast<unsigned>(blocks);
     blocks += (t.m[k].R * t.m[k].Cp / 8 + 255) / 256;
-    TESM_REQUIRE(blocks < (1LL << 31), kErrUnsupported, "dense product: operands too large");
+    TESM_REQUIRE(fits_grid(blocks, 256), kErrUnsupported, "dense product: operands too large for one call");
   }
   if (blocks == 0) return kOk;
   const unsigned n = static_cast<unsigned>(blocks);
@@ -485,6 +485,7 @@ int grad_product(Space& s, bool run, int dt, bool adown, ProductArgs a, hipStrea
   b.vec = a.N % 8 == 0;
   if (a.splits)
     if (int rc = launch_product(kProdPartial, kF32, adown, true, b, st)) return rc;
+  TESM_REQUIRE(fits_grid((a.M * a.N + 255) / 256, 256), kErrUnsupported, "dense product: too large for one call");
   const unsigned blocks = static_cast<unsigned>((a.M * a.N + 255) / 256);
   if (dt == kBF16)
     join_splits_kernel<kBF16><<<blocks, 256, 0, TESM_LOGGED(st, join_splits_kernel<kBF16>)>>>(part, a.splits, a.M, a.N, a.cut, a.fold, a.out, a.out2);
@@ -506,7 +507,7 @@ int backward(const DenseBwdArgs& b, Space s, bool run, int64_t* need, hipStream_
     dz = {dst, dt == kBF16 ? 0 : M * 2 * Np, 2 * Np, 2 * Np};
     const int64_t threads = M * Np / 8;
     if (run && threads && products) {
-      TESM_REQUIRE(threads < (1LL << 38), kErrUnsupported, "dense backward: too large");
+      TESM_REQUIRE(fits_grid((threads + 255) / 256, 256), kErrUnsupported, "dense backward: too large for one call");
       const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
       if (dt == kBF16)
         gated_grad_kernel<kBF16><<<blocks, 256, 0, TESM_LOGGED(st, gated_grad_kernel<kBF16>)>>>(b.grad, b.ld_g, d.z, d.z2, M, N, Np, d.act, dst);

@@ -435,7 +435,7 @@ template <int KIND, int DT, int PARTS, bool ADOWN, bool BDOWN, int WM, int WN, i
 int run_product(const ProductArgs& a, hipStream_t st) {
   using S = Shape<KIND, PARTS, WM, WN, TM, TN, BK, NS>;
   const int64_t tiles = ((a.M + S::BM - 1) / S::BM) * ((a.N + S::BN - 1) / S::BN);
-  TESM_REQUIRE(tiles < (1LL << 31), kErrUnsupported, "dense product: too many tiles");
+  TESM_REQUIRE(fits_grid(tiles, S::NT), kErrUnsupported, "dense product: too many tiles for one call");
   // offsets from a tile's first value stay inside the buffer's range
   TESM_REQUIRE(static_cast<int64_t>(ADOWN ? BK : S::BM) * a.lda * 2 + 1024 < static_cast<int64_t>(kRange) &&
                    static_cast<int64_t>(BDOWN ? BK : S::BN) * a.ldb * 2 + 1024 < static_cast<int64_t>(kRange) &&

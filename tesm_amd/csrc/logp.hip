@@ -260,7 +260,7 @@ int launch_token_logp(const LogpArgs& a, void* ws, int64_t ws_bytes, hipStream_t
   TESM_REQUIRE(need == 0 || (ws && ws_bytes >= need && aligned(ws, 8)), kErrWorkspace,
                "token log probs: workspace too small or not 8-byte aligned");
   const int parts = static_cast<int>(logp_parts(a)), part = static_cast<int>(logp_part(a)), m = static_cast<int>(a.top);
-  TESM_REQUIRE(a.rows * parts < (1LL << 31), kErrUnsupported, "token log probs: too many rows for one call");
+  TESM_REQUIRE(fits_grid(a.rows * parts, 64 * kLogpWaves), kErrUnsupported, "token log probs: too many rows for one call");
   uint64_t* keys = static_cast<uint64_t*>(ws);
   LogpSum* sums = reinterpret_cast<LogpSum*>(static_cast<char*>(ws) + up256(a.rows * parts * m * 8));
   const unsigned blocks = static_cast<unsigned>(a.rows * parts);
@@ -295,7 +295,7 @@ int launch_token_logp_bwd(const LogpBwdArgs& a, hipStream_t st) {
                "token log probs backward: need logits, targets, what the forward call kept and the output");
   const int64_t unit = 256 * 4 * (a.dt == kBF16 ? 8 : 4), many = (a.V + 4 * unit - 1) / (4 * unit);
   const int64_t part = round_up((a.V + many - 1) / many, unit), parts = (a.V + part - 1) / part;
-  TESM_REQUIRE(a.rows * parts < (1LL << 31), kErrUnsupported, "token log probs backward: too many rows for one call");
+  TESM_REQUIRE(fits_grid(a.rows * parts, 256), kErrUnsupported, "token log probs backward: too many rows for one call");
   const unsigned blocks = static_cast<unsigned>(a.rows * parts);
   const int p = static_cast<int>(parts);
 #define TESM_LOGP_BWD(DT, ENT) logp_bwd_kernel<DT, ENT><<<blocks, 256, 0, TESM_LOGGED(st, logp_bwd_kernel<DT, ENT>)>>>(a, p, part)

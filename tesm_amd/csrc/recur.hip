@@ -744,7 +744,7 @@ int launch_gated_scan(const RecurArgs& a, void* ws, int64_t ws_bytes, hipStream_
   const Plan p = plan_of(a, false, tile);
   const Chain c = chain_of(a, p, ws, pairs ? 2 : 1, tile);
   const int64_t blocks = p.slots * c.G;
-  TESM_REQUIRE(blocks < (1LL << 31), kErrUnsupported, "gated scan: too many tiles for one call");
+  TESM_REQUIRE(fits_grid(blocks, 64 * kWaves), kErrUnsupported, "gated scan: too many tiles for one call");
   if (int rc = reset(a, p, c, pairs ? 2 : 1, RestArgs{{a.h}, {a.ld_h}}, st)) return rc;
   const unsigned n = static_cast<unsigned>(blocks);
 #define TESM_RECUR(DT, CPT, NT, T) recur_fwd_kernel<DT, CPT, NT, T><<<n, 64 * kWaves, 0, TESM_LOGGED(st, recur_fwd_kernel<DT, CPT, NT, T>)>>>(a, c)
@@ -781,7 +781,7 @@ int launch_gated_scan_bwd(const RecurBwdArgs& b, void* ws, int64_t ws_bytes, hip
                                           {b.d_value, b.ld_dv}, {b.d_write, b.ld_dw}, {b.d_decay, b.ld_dd}});
   const Chain c = chain_of(a, p, ws, pairs ? 2 : 1);
   const int64_t blocks = a.S ? p.slots * c.G : 0;
-  TESM_REQUIRE(blocks < (1LL << 31), kErrUnsupported, "gated scan backward: too many tiles for one call");
+  TESM_REQUIRE(fits_grid(blocks, 64 * kWaves), kErrUnsupported, "gated scan backward: too many tiles for one call");
   float* sums = b.d_bias ? reinterpret_cast<float*>(static_cast<char*>(ws) + p.at_sums) : nullptr;
   if (blocks > 0) {
     if (int rc = reset(a, p, c, pairs ? 2 : 1, RestArgs{{b.d_value, b.d_write, b.d_decay}, {b.ld_dv, b.ld_dw, b.ld_dd}}, st)) return rc;

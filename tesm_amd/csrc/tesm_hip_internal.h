@@ -9,6 +9,9 @@ namespace tesm {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
+// Whether a grid's first axis can be launched: its threads are counted in 32 bits.
+inline bool fits_grid(int64_t blocks, int64_t threads) { return blocks * threads < (1LL << 32); }
+
 // zero_p / zero_n: an int range the kernel also clears (for a later kernel of the same stream).
 int launch_quant_act(const void* x, int dt, int64_t M, int64_t K, int64_t ldx, float eps, int layout, int8_t* q,
                      int64_t ldq, float* s_x, int32_t* rowsum, hipStream_t st, int* zero_p = nullptr,

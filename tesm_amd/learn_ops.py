@@ -151,7 +151,7 @@ def gated_scan(value: torch.Tensor, write: torch.Tensor, decay: torch.Tensor, de
     as it is; states are float32, finite ones, and results repeat bit for bit.
 
     ``keep=True`` also returns what ``gated_scan_backward`` needs (float32, one row per 64).  ``out`` takes no gradients and must not
-    overlap an operand.  Fewer than 2^31 rows, C below 2^24.
+    overlap an operand.  Fewer than 2^31 rows, C below 2^24, fewer than 2^23 tiles of 64 rows of a sequence by 64 channels.
     """
     if _records("gated_scan", keep, value, write, decay, decay_bias, state):
         if out is not None:
@@ -485,6 +485,7 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0
     own error at every offset of the logits.  With ``top`` (at most 64) the row's largest log probabilities and their tokens follow in
     falling order, equal ones by token (None without).  A logit of -infinity is a masked token.  Rows with a NaN or +infinite logit, or
     none above -infinity, give NaN, and so does any other target outside the vocabulary, which sets bit 2 of ``device_status``.
+    Fewer than 2^24 rows.
     Gradients flow through ``log_probs`` and ``entropy``.  ``keep=True`` also returns what ``token_log_probs_backward`` needs.
     """
     if _records("token_log_probs", keep, logits):

@@ -35,3 +35,22 @@ def test_projections_of_more_than_four_million_rows(dtype):
     for some in (slice(0, 100), slice(65535 * 64 - 50, M)):
         c = dict(x=x[some].cpu(), w=w.cpu(), up=None, bias=b.cpu(), residual=None, grad=grad[some].cpu())
         within(dx[some], *dense_bounds(c, "silu")["dx"], "dx")
+
+
+def test_grids_of_too_many_threads_are_refused():
+    """A launch counts its threads in 32 bits."""
+    n = 1 << 23
+    v = torch.zeros(n, 1, 2, dtype=BF, device=DEV)
+    with pytest.raises(RuntimeError, match="too many tiles"):
+        hip_ops.gated_scan(v, v, v)
+    h, _, kept = hip_ops.gated_scan(v[1:], v[1:], v[1:], keep=True)  # (one tile less)
+    assert not h.any()
+    with pytest.raises(RuntimeError, match="too many tiles"):
+        hip_ops.gated_scan_backward(v, v, v, v, kept=torch.zeros(n, 2, device=DEV))
+    x, t = torch.zeros(1 << 24, 2, dtype=BF, device=DEV), torch.zeros(1 << 24, dtype=torch.int64, device=DEV)
+    with pytest.raises(RuntimeError, match="too many rows"):
+        hip_ops.token_log_probs(x, t)
+    with pytest.raises(RuntimeError, match="too many rows"):
+        hip_ops.token_log_probs_backward(None, None, x, t, kept=torch.zeros(1 << 24, 4, device=DEV))
+    logp = hip_ops.token_log_probs(x[1:], t[1:])[0]
+    assert bool((logp + 0.6931472 <= 2.0 ** -22).all()) and bool((logp + 0.6931472 >= -2.0 ** -22).all())
