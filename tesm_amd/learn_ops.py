@@ -426,7 +426,8 @@ def _logp_forward(logits, targets, top, ignore_index, keep):
         raise ValueError(f"{what}: 0 to {min(64, max(V, 1))} alternatives, got {top}")
     code, x, ld, targets = _logits(logits, targets, what)
     dev, rows = x.device, targets.numel()
-    logp, entropy = torch.empty((2, *lead), dtype=torch.float32, device=dev).unbind()
+    logp = torch.empty(lead, dtype=torch.float32, device=dev)  # (no views of one buffer: autograd would refuse to change them in place)
+    entropy = torch.empty_like(logp)
     best = torch.empty((*lead, top), dtype=torch.float32, device=dev) if top else None
     tokens = torch.empty((*lead, top), dtype=torch.int64, device=dev) if top else None
     kept = torch.empty((rows, 4), dtype=torch.float32, device=dev) if keep else None

@@ -4,9 +4,9 @@ import torch
 
 from hip_helpers import DEV, need_gpu
 from learn_bits import dense_bounds
-from learn_refs import HALF, within
+from learn_refs import HALF, logp_ref, within
 from tesm_amd import hip_ops
-from test_gpu_learn import BOTH
+from test_gpu_learn import BOTH, _dev, logp_case
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -54,3 +54,16 @@ def test_grids_of_too_many_threads_are_refused():
         hip_ops.token_log_probs_backward(None, None, x, t, kept=torch.zeros(1 << 24, 4, device=DEV))
     logp = hip_ops.token_log_probs(x[1:], t[1:])[0]
     assert bool((logp + 0.6931472 <= 2.0 ** -22).all()) and bool((logp + 0.6931472 >= -2.0 ** -22).all())
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_log_probs_may_be_changed_in_place(dtype):
+    """A policy's loss: advantages times the log probabilities, in place."""
+    x, t, g, e = logp_case(3, 8, 300, dtype)
+    a = x.to(DEV).requires_grad_()
+    with torch.enable_grad():
+        logp, entropy, _, _ = hip_ops.token_log_probs(a, _dev(t))
+        logp *= _dev(g)
+        entropy.mul_(_dev(e))
+        (logp.sum() + entropy.sum()).backward()
+    within(a.grad, *logp_ref(x, t, 0, -100, g, e)["dx"], "dx")
