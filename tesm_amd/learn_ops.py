@@ -174,7 +174,8 @@ def _scan_backward(grad, value, write, decay, bias, state, seq_starts, kept, gra
     grad_state = grad_state.contiguous() if grad_state is not None else None
     kept = kept.contiguous()
     require_device(value, grad, grad_state, kept)
-    dv, dw, dd = (torch.empty if S else torch.zeros)((3, B, L, C), dtype=value.dtype, device=dev).unbind()
+    new = torch.empty if S else torch.zeros
+    dv, dw, dd = (new((B, L, C), dtype=value.dtype, device=dev) for _ in range(3))
     db = torch.empty((C,), dtype=torch.float32, device=dev) if need_bias else None
     ds = torch.empty((S, C), dtype=torch.float32, device=dev) if state is not None else None
     ld = max(C, 1)

@@ -6,7 +6,7 @@ from hip_helpers import DEV, need_gpu
 from learn_bits import dense_bounds
 from learn_refs import HALF, logp_ref, within
 from tesm_amd import hip_ops
-from test_gpu_learn import BOTH, _dev, logp_case
+from test_gpu_learn import BOTH, _dev, logp_case, scan_case
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -67,3 +67,14 @@ def test_log_probs_may_be_changed_in_place(dtype):
         entropy.mul_(_dev(e))
         (logp.sum() + entropy.sum()).backward()
     within(a.grad, *logp_ref(x, t, 0, -100, g, e)["dx"], "dx")
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_gradients_of_the_recurrence_hold_their_own_memory(dtype):
+    c = scan_case(4, 2, 90, 16, dtype)
+    args = [_dev(c[k]) for k in ("value", "write", "decay", "bias")]
+    h, last, kept = hip_ops.gated_scan(*args, state=_dev(c["state"]), keep=True)
+    grads = hip_ops.gated_scan_backward(_dev(c["grad"]), *args, kept=kept, state=_dev(c["state"]))
+    held = [t.untyped_storage() for t in (h, last, *grads)]
+    assert len({s.data_ptr() for s in held}) == len(held)
+    assert [s.nbytes() for s in held] == [t.numel() * t.element_size() for t in (h, last, *grads)]
