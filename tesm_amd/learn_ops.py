@@ -66,6 +66,11 @@ def _empty_as(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
+def _needed(what: str, name: str, *ts) -> None:
+    if not all(isinstance(t, torch.Tensor) for t in ts):
+        raise ValueError(f"{what}: needs {name}")
+
+
 def _like(what: str, name: str, t: Optional[torch.Tensor], shape, dtype) -> None:
     if t is not None and (t.shape != torch.Size(shape) or t.dtype != dtype):
         raise ValueError(f"{what}: {name} must be a {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
@@ -163,6 +168,8 @@ def gated_scan(value: torch.Tensor, write: torch.Tensor, decay: torch.Tensor, de
 
 def _scan_backward(grad, value, write, decay, bias, state, seq_starts, kept, grad_state, need_bias):
     what = "gated_scan_backward"
+    _needed(what, "the gradient of h", grad)
+    _needed(what, "kept, as the forward call with keep=True returned it", kept)
     g, held, S = _gates(value, write, decay, bias, state, seq_starts, what, seq_starts is not None)
     B, L, C = value.shape
     dev = value.device
@@ -207,6 +214,7 @@ def gated_scan_step(value: torch.Tensor, write: torch.Tensor, decay: torch.Tenso
     value, write, decay (B, C) share a dtype and may be column slices of wider rows.  ``out`` must not overlap an operand.  B < 65536.
     """
     what = "gated_scan_step"
+    _needed(what, "the state", state)
     if value.dim() != 2 or write.shape != value.shape or decay.shape != value.shape:
         raise ValueError(f"{what}: value, write and decay must all be (B, C)")
     hip_ops._no_grad(what, value, write, decay, decay_bias, state, out)
@@ -290,6 +298,12 @@ def _dense_forward(x, weight, up, bias, residual, act, keep, what):
 
 
 def _dense_backward(grad, x, weight, up, kept, act, need_x, need_w, need_b, what):
+    _needed(what, "the gradient of the result", grad)
+    if up is not None:
+        _needed(what, "kept, the two tensors that the forward call with keep=True returned",
+                *(kept if isinstance(kept, (tuple, list)) and len(kept) == 2 else (None,)))
+    elif act:
+        _needed(what, "kept, as the forward call with keep=True returned it", kept)
     d, held, M, shape = _dense(x, weight, up, None, None, act, what)
     dev, (N, K) = x.device, weight.shape
     _like(what, "the gradient", grad, shape, x.dtype)
@@ -443,6 +457,7 @@ def _logp_forward(logits, targets, top, ignore_index, keep):
 
 def _logp_backward(grad, grad_entropy, logits, targets, kept, ignore_index):
     what = "token_log_probs_backward"
+    _needed(what, "kept, as the forward call with keep=True returned it", kept)
     lead = targets.shape
     _like(what, "the log probabilities' gradient", grad, lead, torch.float32)
     _like(what, "the entropies' gradient", grad_entropy, lead, torch.float32)

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from tesm_amd import _lib
+from tesm_amd import _lib, hip_ops
 from test_learn_ops_cpu import _refused
 
 
@@ -17,3 +17,30 @@ def test_a_pair_without_an_activation_has_no_backward_pass(z, z_up):
     """Its kernel reads what the forward call kept, which that refuses to make."""
     b = _lib.DenseGrad(_pair(0, z, z_up), 1 << 25, 16, 1 << 26, None, None, None)
     assert "activation" in _refused("tesm_hip_dense_backward", ctypes.byref(b), None, 0, None)
+
+
+R = torch.randn
+
+
+@pytest.mark.parametrize("call", [
+    lambda: hip_ops.fused_linear_backward(R(3, 4), R(3, 8), R(4, 8), act="silu"),
+    lambda: hip_ops.gated_linear_backward(R(3, 4), R(3, 8), R(4, 8), R(4, 8), kept=None),
+    lambda: hip_ops.gated_linear_backward(R(3, 4), R(3, 8), R(4, 8), R(4, 8), kept=R(3, 4)),
+    lambda: hip_ops.gated_linear_backward(R(3, 4), R(3, 8), R(4, 8), R(4, 8), kept=(R(3, 4),)),
+    lambda: hip_ops.gated_linear_backward(R(3, 4), R(3, 8), R(4, 8), R(4, 8), kept=(R(3, 4), None)),
+    lambda: hip_ops.gated_scan_backward(R(2, 5, 6), R(2, 5, 6), R(2, 5, 6), R(2, 5, 6), kept=None),
+    lambda: hip_ops.token_log_probs_backward(R(3), None, R(3, 9), torch.zeros(3, dtype=torch.int64), kept=None),
+])
+def test_backward_passes_without_what_the_forward_pass_kept(call):
+    with torch.no_grad(), pytest.raises(ValueError, match="needs kept"):
+        call()
+
+
+@pytest.mark.parametrize("call,name", [
+    (lambda: hip_ops.fused_linear_backward(None, R(3, 8), R(4, 8)), "gradient"),
+    (lambda: hip_ops.gated_scan_backward(None, R(2, 5, 6), R(2, 5, 6), R(2, 5, 6), kept=R(2, 6)), "gradient"),
+    (lambda: hip_ops.gated_scan_step(R(2, 6), R(2, 6), R(2, 6), state=None), "state"),
+])
+def test_calls_without_what_they_need(call, name):
+    with torch.no_grad(), pytest.raises(ValueError, match="needs the " + name):
+        call()
