@@ -2,7 +2,7 @@
 
 Reached as ``hip_ops.gated_scan`` and so on.  Every operator has three forms:
 
-* the plain call, with autograd where an input requires a gradient (once differentiable);
+* the plain call, with autograd where an input requires a gradient (once differentiable; forward-mode tangents are refused);
 * ``keep=True`` (under ``torch.no_grad()``): the call also returns what its backward pass needs, as its last result;
 * ``.._backward``: that backward pass by hand, the form for captured graphs.  A stream that is being captured records no
   autograd graph of these operators: the call is refused there (a leaf's gradient would be accumulated on the stream that its
@@ -18,6 +18,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, hip_ops
@@ -36,12 +37,25 @@ def _act_code(act: Optional[str], what: str, pair: bool = False) -> int:
 
 def _records(what: str, keep: bool, *ts) -> bool:
     """Whether the call is one for autograd; refused where it cannot be."""
+    _no_tangents(what, *ts)
     if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in ts):
         return False
     if keep:
         raise RuntimeError(f"{what}: keep=True is for backward passes called by hand: run under torch.no_grad()")
     _no_capture(what)
     return True
+
+
+def _no_tangents(what: str, *ts) -> None:
+    """Forward-mode derivatives are refused: the results would have none, without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError(f"{what}: no forward-mode derivatives: an operand has a tangent")
+
+
+def _by_hand(what: str, *ts) -> None:
+    """A call without derivatives of its own."""
+    _no_tangents(what, *ts)
+    hip_ops._no_grad(what, *ts)
 
 
 def _no_capture(what: str) -> None:
@@ -203,7 +217,7 @@ def gated_scan_backward(grad: torch.Tensor, value: torch.Tensor, write: torch.Te
     ``grad`` (B, L, C): the gradient of h; ``grad_state`` (S, C) float32: that of the final states (zero by default).  The bias's
     and the state's are float32, None where there was none.  Rows of no sequence get zeros.
     """
-    hip_ops._no_grad("gated_scan_backward", grad, value, write, decay, decay_bias, state, grad_state)
+    _by_hand("gated_scan_backward", grad, value, write, decay, decay_bias, state, grad_state)
     return _scan_backward(grad, value, write, decay, decay_bias, state, seq_starts, kept, grad_state, decay_bias is not None)
 
 
@@ -217,7 +231,7 @@ def gated_scan_step(value: torch.Tensor, write: torch.Tensor, decay: torch.Tenso
     _needed(what, "the state", state)
     if value.dim() != 2 or write.shape != value.shape or decay.shape != value.shape:
         raise ValueError(f"{what}: value, write and decay must all be (B, C)")
-    hip_ops._no_grad(what, value, write, decay, decay_bias, state, out)
+    _by_hand(what, value, write, decay, decay_bias, state, out)
     _same_dtype(what, value.dtype, write=write, decay=decay)
     B, C = value.shape
     code = dt_code(value.dtype)
@@ -369,7 +383,7 @@ def gated_linear_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Ten
     """The gradients ``(x, w_gate, w_up)`` of ``gated_linear``, called with the same operands and ``keep=True``; those not asked
     for are None.  The gradients of the two products go into those with x and the weights in 16 bits (float32: all 24), the sums are
     float32, and the results are rounded once; where bfloat16 operands hold an infinity, gradients made with it may be NaN."""
-    hip_ops._no_grad("gated_linear_backward", grad, x, w_gate, w_up)
+    _by_hand("gated_linear_backward", grad, x, w_gate, w_up)
     return _dense_backward(grad, x, w_gate, w_up, kept, _act_code(act, "gated_linear_backward", pair=True), need_x, need_weights, False,
                            "gated_linear_backward")[:3]
 
@@ -411,7 +425,7 @@ def fused_linear_backward(grad: torch.Tensor, x: torch.Tensor, weight: torch.Ten
                           act: Optional[str] = None, need_x: bool = True, need_weight: bool = True):
     """The gradients ``(x, weight, bias)`` of ``fused_linear``, called with the same operands and ``keep=True`` (the residual's is
     ``grad`` itself); the bias's is None without one, those not asked for are.  Roundings as in ``gated_linear_backward``."""
-    hip_ops._no_grad("fused_linear_backward", grad, x, weight, bias)
+    _by_hand("fused_linear_backward", grad, x, weight, bias)
     dx, dw, _, db = _dense_backward(grad, x, weight, None, kept, _act_code(act, "fused_linear_backward"), need_x, need_weight,
                                     bias is not None, "fused_linear_backward")
     return dx, dw, db
@@ -515,5 +529,5 @@ def token_log_probs_backward(grad: Optional[torch.Tensor], grad_entropy: Optiona
                              targets: torch.Tensor, *, kept: torch.Tensor, ignore_index: int = -100):
     """The gradient of the logits of ``token_log_probs``, called with the same operands and ``keep=True``; ``grad`` and
     ``grad_entropy`` (..) float32 are those of its first two results (None: zero)."""
-    hip_ops._no_grad("token_log_probs_backward", grad, grad_entropy, logits)
+    _by_hand("token_log_probs_backward", grad, grad_entropy, logits)
     return _logp_backward(grad, grad_entropy, logits, targets, kept, ignore_index)

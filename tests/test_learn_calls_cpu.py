@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from tesm_amd import _lib, hip_ops
 from test_learn_ops_cpu import _refused
@@ -44,3 +45,31 @@ def test_backward_passes_without_what_the_forward_pass_kept(call):
 def test_calls_without_what_they_need(call, name):
     with torch.no_grad(), pytest.raises(ValueError, match="needs the " + name):
         call()
+
+
+def _calls_of(g, x, w, y):
+    t = torch.zeros(3, dtype=torch.int64)
+    return dict(
+        gated_scan=lambda: hip_ops.gated_scan(R(2, 5, 6), R(2, 5, 6), g),
+        gated_scan_backward=lambda: hip_ops.gated_scan_backward(g, R(2, 5, 6), R(2, 5, 6), R(2, 5, 6), kept=R(2, 6)),
+        gated_scan_step=lambda: hip_ops.gated_scan_step(g[:, 0], R(2, 6), R(2, 6), state=R(2, 6)),
+        gated_linear=lambda: hip_ops.gated_linear(R(3, 8), R(4, 8), w),
+        gated_linear_backward=lambda: hip_ops.gated_linear_backward(y, R(3, 8), R(4, 8), R(4, 8), kept=(R(3, 4), R(3, 4))),
+        fused_linear=lambda: hip_ops.fused_linear(x, R(4, 8)),
+        fused_linear_backward=lambda: hip_ops.fused_linear_backward(R(3, 4), x, R(4, 8)),
+        token_log_probs=lambda: hip_ops.token_log_probs(x, t),
+        token_log_probs_backward=lambda: hip_ops.token_log_probs_backward(R(3), None, x, t, kept=R(3, 4)))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_tangents_are_refused(grad):
+    """In a level of forward-mode derivatives operands without a tangent go on (here, to the refusal of host memory)."""
+    leaves = [R(*s) for s in ((2, 5, 6), (3, 8), (4, 8), (3, 4))]
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        duals = [forward_ad.make_dual(v, torch.ones_like(v)) for v in leaves]
+        for name, call in _calls_of(*duals).items():
+            with pytest.raises(RuntimeError, match=name + ": no forward-mode"):
+                call()
+        for call in _calls_of(*leaves).values():
+            with pytest.raises(RuntimeError, match="ROCm device"):
+                call()
