@@ -176,6 +176,7 @@ def gated_scan(value: torch.Tensor, write: torch.Tensor, decay: torch.Tensor, de
         if out is not None:
             raise RuntimeError("gated_scan: out takes no gradients: run under torch.no_grad()")
         return _GatedScan.apply(value, write, decay, decay_bias, state, seq_starts)
+    _by_hand("gated_scan", out)
     h, last, kept = _scan_forward(value, write, decay, decay_bias, state, seq_starts, out, keep)
     return (h, last, kept) if keep else (h, last)
 

@@ -73,3 +73,9 @@ def test_forward_mode_tangents_are_refused(grad):
         for call in _calls_of(*leaves).values():
             with pytest.raises(RuntimeError, match="ROCm device"):
                 call()
+
+
+def test_an_output_that_requires_a_gradient_is_refused():
+    g = R(2, 5, 6)
+    with pytest.raises(RuntimeError, match="under torch.no_grad"):
+        hip_ops.gated_scan(g, g, g, out=R(2, 5, 6, requires_grad=True))
