@@ -341,9 +341,11 @@ class TESMLMHeadModel(nn.Module):
     def score(self, input_ids: torch.Tensor, top: int = 0):
         """How likely the model finds the tokens of ``input_ids`` (B, L) one after the other: ``(log_probs (B, L - 1), entropy
         (B, L - 1), top_log_probs, top_tokens (B, L - 1, top))`` of token t + 1 after the first t + 1, as
-        ``hip_ops.token_log_probs`` gives them; the configuration's ``label_ignore_index`` marks tokens that are not scored."""
+        ``hip_ops.token_log_probs`` gives them; the configuration's ``label_ignore_index`` marks tokens that are not scored (one that
+        is no token, and any below 0, stands as token 0 in front of the others)."""
         ignore = self.tesm_config.label_ignore_index
-        logits = self(input_ids.clamp(min=0))[0].logits
+        tokens = input_ids.masked_fill(input_ids == ignore, 0) if ignore >= self.tesm_config.vocab_size else input_ids
+        logits = self(tokens.clamp(min=0))[0].logits
         # (the last row has no target; leaving it out of the logits would copy them)
         targets = torch.nn.functional.pad(input_ids[:, 1:], (0, 1), value=ignore)
         out = hip_ops.token_log_probs(logits, targets, top=top, ignore_index=ignore)

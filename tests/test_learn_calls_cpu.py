@@ -1,11 +1,12 @@
 """Calls of the operators that learn which have to be refused before any kernel runs, or answered without one."""
 import ctypes
+from types import SimpleNamespace
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from tesm_amd import _lib, hip_ops
+from tesm_amd import TESMLMHeadModel, _lib, hip_ops
 from test_learn_ops_cpu import _refused
 
 
@@ -79,3 +80,31 @@ def test_an_output_that_requires_a_gradient_is_refused():
     g = R(2, 5, 6)
     with pytest.raises(RuntimeError, match="under torch.no_grad"):
         hip_ops.gated_scan(g, g, g, out=R(2, 5, 6, requires_grad=True))
+
+
+class _Model:
+    """As much of a model as ``score`` sees: it keeps the ids that it is given."""
+
+    def __init__(self, ignore):
+        self.tesm_config = SimpleNamespace(label_ignore_index=ignore, vocab_size=11)
+
+    def __call__(self, ids):
+        self.ids = ids
+        return SimpleNamespace(logits=torch.zeros(*ids.shape, 11)), None
+
+
+@pytest.mark.parametrize("ignore", [-100, -1, 0, 10, 11, 1 << 40])
+def test_scores_read_no_embedding_behind_the_vocabulary(ignore, monkeypatch):
+    model, seen = _Model(ignore), {}
+
+    def log_probs(logits, targets, *, top, ignore_index):
+        seen.update(targets=targets, ignore=ignore_index)
+        return torch.zeros(targets.shape), torch.zeros(targets.shape), None, None
+
+    monkeypatch.setattr(hip_ops, "token_log_probs", log_probs)
+    ids = torch.tensor([[3, ignore, 10, 0], [ignore, 1, 2, ignore]])
+    TESMLMHeadModel.score(model, ids)
+    assert int(model.ids.min()) >= 0 and int(model.ids.max()) < 11
+    token = (ids >= 0) & (ids < 11)
+    assert torch.equal(model.ids, torch.where(token, ids, 0))
+    assert torch.equal(seen["targets"][:, :-1], ids[:, 1:]) and seen["ignore"] == ignore
