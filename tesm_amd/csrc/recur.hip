@@ -54,11 +54,12 @@ __device__ __forceinline__ Sig sig_of(float e) {
   const float p = __builtin_amdgcn_rcpf(1.0f + e);
   return {p, fminf(e, 3.4e38f) * p};
 }
-// The decay, of x + b, given nb = -b log2 e.  A state that is kept for n rows holds n times what a decay is off to one side, so this
+// The decay, of x + b: added first, since b log2 e and x log2 e, rounded apart, lose what is left where the two nearly cancel (biases of
+// 300: a decay 1e-5 of itself off).  A state that is kept for n rows holds n times what a decay is off to one side, so this
 // reciprocal takes a Newton step, 1 - p (1 + e) = (1 - p) - p e being exact where p is near 1 (decays that keep 400 rows: the bias's
 // gradient is 1.6e-6 of itself off without it, 3.3e-7 with it; both passes of 32768 x 8192 take 1362 us instead of 1357).
-__device__ __forceinline__ Sig decay_of(float x, float nb) {
-  const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x, -kLog2e, nb));
+__device__ __forceinline__ Sig decay_of(float x, float b) {
+  const float e = __builtin_amdgcn_exp2f((x + b) * -kLog2e);
   const float r = __builtin_amdgcn_rcpf(1.0f + e), most = fminf(e, 3.4e38f);
   const float p = __builtin_fmaf(r, __builtin_fmaf(-most, r, 1.0f - r), r);
   return {p, most * p};
@@ -355,14 +356,14 @@ __global__ __launch_bounds__(64 * kWaves) void recur_fwd_kernel(RecurArgs a, Cha
     constexpr bool WHOLE = decltype(whole)::value;
     Row<DT, CPT, NT> raw[3][T];
     load_rows<DT, CPT, NT, T, WHOLE, 3>(q, {a.decay, a.write, a.value}, {a.ld_d, a.ld_w, a.ld_v}, off, raw);
-    float nb[CPT];
+    float bias[CPT];
 #pragma unroll
-    for (int j = 0; j < CPT; ++j) nb[j] = a.bias ? a.bias[ch + j] * -kLog2e : 0.0f;
+    for (int j = 0; j < CPT; ++j) bias[j] = a.bias ? a.bias[ch + j] : 0.0f;
 #pragma unroll
     for (int i = 0; i < T; ++i)
 #pragma unroll
       for (int j = 0; j < CPT; ++j) {
-        A[i][j] = decay_of(raw[0][i].get(j), nb[j]).p;
+        A[i][j] = decay_of(raw[0][i].get(j), bias[j]).p;
         U[i][j] = sig(raw[1][i].get(j)) * tanh2<DT>(raw[2][i].get(j)).t;
         if (WHOLE || i < q.n) part[j] = make_float2(A[i][j] * part[j].x, __builtin_fmaf(A[i][j], part[j].y, U[i][j]));
       }
@@ -441,15 +442,15 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recur_bwd_kernel(RecurBwdArgs 
     constexpr bool WHOLE = decltype(whole)::value;
     Row<DT, CPT, NT> raw[4][T];
     load_rows<DT, CPT, NT, T, WHOLE, 4>(q, {a.decay, a.write, a.value, b.grad}, {a.ld_d, a.ld_w, a.ld_v, b.ld_g}, off, raw);
-    float nb[CPT];
+    float bias[CPT];
 #pragma unroll
-    for (int j = 0; j < CPT; ++j) nb[j] = a.bias ? a.bias[ch + j] * -kLog2e : 0.0f;
+    for (int j = 0; j < CPT; ++j) bias[j] = a.bias ? a.bias[ch + j] : 0.0f;
 #pragma unroll
     for (int i = 0; i < T; ++i) {
       dh[i] = raw[3][i];
 #pragma unroll
       for (int j = 0; j < CPT; ++j) {
-        const Sig f = decay_of(raw[0][i].get(j), nb[j]), s = sig2(raw[1][i].get(j));
+        const Sig f = decay_of(raw[0][i].get(j), bias[j]), s = sig2(raw[1][i].get(j));
         const Tanh t = tanh2<DT>(raw[2][i].get(j));
         A[i][j] = f.p;
         fd[i][j] = f.p * f.q;
@@ -622,7 +623,7 @@ __global__ __launch_bounds__(256) void recur_step_kernel(RecurStepArgs a) {
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, b = blockIdx.y;
   if (c >= a.C) return;
   const float d = ld<DT>(a.decay, b * a.ld_d + c), w = ld<DT>(a.write, b * a.ld_w + c), v = ld<DT>(a.value, b * a.ld_v + c);
-  const float h = __builtin_fmaf(decay_of(d, a.bias ? a.bias[c] * -kLog2e : 0.0f).p, a.state[b * a.C + c], sig(w) * tanh2<DT>(v).t);
+  const float h = __builtin_fmaf(decay_of(d, a.bias ? a.bias[c] : 0.0f).p, a.state[b * a.C + c], sig(w) * tanh2<DT>(v).t);
   a.state[b * a.C + c] = h;
   st<DT>(a.h, b * a.ld_h + c, h);
 }

@@ -4,9 +4,9 @@ import torch
 
 from hip_helpers import DEV, need_gpu
 from learn_bits import dense_bounds
-from learn_refs import within
+from learn_refs import scan_ref, within
 from tesm_amd import hip_ops
-from test_gpu_learn import _dev, dense_case
+from test_gpu_learn import _dev, check_scan, dense_case, run_scan, scan_case
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -48,3 +48,20 @@ def test_gradients_of_an_activation(act, M, K, N):
     r = dense_bounds(c, act)
     for name, got in gradients(c, act).items():
         within(got, *r[name], name)
+
+
+# ---------------------------------------------------------------------------
+# the recurrence's decays
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("far", [0.0, 40.0, 300.0, 5000.0])
+def test_decays_near_zero_from_far_biases(dtype, far):
+    """What counts is decay + bias, whose float32 sum is exact where they nearly cancel."""
+    c = scan_case(7, 2, 150, 12, dtype)
+    c["decay"] = ((c["decay"].float() - far).to(dtype))
+    c["bias"] = far + c["bias"]
+    check_scan(c, *run_scan(c))
+    state = _dev(c["state"])
+    r = scan_ref(c["value"][:, :1], c["write"][:, :1], c["decay"][:, :1], c["bias"], c["state"], None)
+    hip_ops.gated_scan_step(*(_dev(c[k][:, 0]) for k in ("value", "write", "decay")), _dev(c["bias"]), state=state)
+    within(state, *r["last"], "state")
