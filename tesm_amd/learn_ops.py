@@ -81,8 +81,9 @@ def _empty_as(t: torch.Tensor) -> torch.Tensor:
 
 
 def _needed(what: str, name: str, *ts) -> None:
-    if not all(isinstance(t, torch.Tensor) for t in ts):
-        raise ValueError(f"{what}: needs {name}")
+    for t in ts:
+        if t is None:
+            raise ValueError(f"{what}: needs {name}")
 
 
 def _like(what: str, name: str, t: Optional[torch.Tensor], shape, dtype) -> None:

@@ -3,8 +3,8 @@ import pytest
 import torch
 
 from hip_helpers import DEV, need_gpu
-from learn_bits import dense_bounds
-from learn_refs import scan_ref, within
+from learn_bits import dense_bounds, f32_bound, off_in_norm
+from learn_refs import act_ref, scan_ref, within
 from tesm_amd import hip_ops
 from test_gpu_learn import _dev, check_scan, dense_case, run_scan, scan_case
 
@@ -48,6 +48,24 @@ def test_gradients_of_an_activation(act, M, K, N):
     r = dense_bounds(c, act)
     for name, got in gradients(c, act).items():
         within(got, *r[name], name)
+
+
+# ---------------------------------------------------------------------------
+# float32 operands keep float32's precision
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("M,K,N", [(7, 100, 90), (40, 520, 72), (64, 1030, 300), (70, 104, 72), (200, 67, 130), (300, 500, 400), (999, 515, 1030),
+                                   (2100, 1000, 600), (1000, 500, 2000)])
+def test_float32_products(M, K, N):
+    c = dense_case(M + K, M, K, N, torch.float32, pair=True)
+    x, w, up, grad = (_dev(c[k]) for k in ("x", "w", "up", "grad"))
+    xd, wd, ud, gd = (t.double() for t in (x, w, up, grad))
+    assert off_in_norm(hip_ops.fused_linear(x, w), xd @ wd.t()) <= f32_bound(K)
+    dx, dw, _ = hip_ops.fused_linear_backward(grad, x, w)
+    assert off_in_norm(dx, gd @ wd) <= f32_bound(N)
+    assert off_in_norm(dw, gd.t() @ xd) <= f32_bound(M)
+    # a pair: both products, and 8 half steps for the activation (slope at most 1.1) and the product of the two
+    val = act_ref(xd @ wd.t(), "silu")[0]
+    assert off_in_norm(hip_ops.gated_linear(x, w, up), val * (xd @ ud.t())) <= 2.1 * f32_bound(K) + 8 * 2.0 ** -24
 
 
 # ---------------------------------------------------------------------------

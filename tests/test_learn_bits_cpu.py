@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from learn_bits import dense_bounds, rounded, share_beyond
+from learn_bits import dense_bounds, f32_bound, off_in_norm, rounded, share_beyond
 from learn_refs import act_ref
 
 BF = torch.bfloat16
@@ -56,3 +56,25 @@ def test_a_kept_value_rounded_to_its_type_is_seen(pair, M, K, N):
     c = dense_case(M + N, M, K, N, BF, pair)
     off = worst(c, "gelu", kept=rounded)
     assert off["dx"] and off["dw"]  # (one value beyond its bound is enough)
+
+
+def parts(x):
+    """float32 values as three of bfloat16."""
+    x0 = rounded(x)
+    x1 = rounded(x - x0)
+    return x0, x1, rounded(x - x0 - x1)
+
+
+ORDER = [(2, 0), (0, 2), (1, 1), (1, 0), (0, 1), (0, 0)]
+
+
+@pytest.mark.parametrize("M,K,N", [(70, 104, 72), (100, 70, 50), (300, 1030, 200), (64, 2100, 80)])
+def test_a_part_left_out_of_a_float32_product_is_seen(M, K, N):
+    """The six products of parts are within the bound, any five of them are not."""
+    g = torch.Generator().manual_seed(M)
+    x, w = torch.randn(M, K, generator=g).double(), torch.randn(N, K, generator=g).double()
+    xs, ws = parts(x), parts(w)
+    terms = {o: xs[o[0]] @ ws[o[1]].t() for o in ORDER}
+    assert off_in_norm(sum(terms.values()), x @ w.t()) < 2.0 ** -24
+    for left_out in ORDER:
+        assert off_in_norm(sum(v for o, v in terms.items() if o != left_out), x @ w.t()) > f32_bound(K), left_out
