@@ -5,7 +5,7 @@
 
 namespace tesm {
 
-// Rows per tile: kept carries are one row of states per tile.  (32, with three workgroups per CU backward instead of two, cost a tile's
+// Rows per tile, except for the forward pass's tallest ones: kept carries are one row of states per so many rows.  (32, with three workgroups per CU backward instead of two, cost a tile's
 // fixed time twice as often: 4 x 2048 x 384 15.5 and 19.0 us instead of 11.2 and 15.1, 32768 x 8192 backward 1033 instead of 885.)
 constexpr int kRecurRows = 64;
 
@@ -25,7 +25,7 @@ struct RecurArgs {
   void* h = nullptr;
   int64_t ld_h = 0;
   float* h_out = nullptr;    // (S, C)
-  float* carries = nullptr;  // optional (recur_slots, C): the state in front of every tile
+  float* carries = nullptr;  // optional (recur_slots, C): the state in front of every kRecurRows rows of a sequence
 };
 
 struct RecurBwdArgs {
@@ -58,7 +58,7 @@ struct RecurStepArgs {
   int64_t ld_h = 0;
 };
 
-int64_t recur_slots(const RecurArgs& a);  // tiles, and rows of the kept carries (-1: bad sizes)
+int64_t recur_slots(const RecurArgs& a);  // rows of the kept carries, and places of tiles of kRecurRows rows (-1: bad sizes)
 int64_t recur_ws_bytes(const RecurArgs& a);
 int64_t recur_bwd_ws_bytes(const RecurArgs& a, bool bias);
 int launch_gated_scan(const RecurArgs& a, void* ws, int64_t ws_bytes, hipStream_t st);

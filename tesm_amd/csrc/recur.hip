@@ -6,22 +6,24 @@
 //   d value_t = g_t sigmoid(write_t) (1 - tanh^2), d h_0 = c_1.
 // Both are first-order recurrences x <- A x + U, and runs of them compose: (A, U) then (A', U') is (A' A, A' U + U').
 //
-// One pass over the data.  A tile is 64 rows of one sequence by 64 or 128 channels; each of 8 waves takes 8 rows, a lane one or
-// two channels; inputs are read once and stay in registers as gates.  Waves scan their rows from zero, their (A, U) meet in
+// One pass over the data.  A tile is 64 rows of one sequence (forward, where long sequences are more than the caches hold, 128 bfloat16 rows) by
+// 64 or 128 channels; each of 8 waves takes 8 (16) rows, a lane one or two channels; inputs are read once and stay in registers as gates.  Waves scan their rows from zero, their (A, U) meet in
 // LDS, and tiles of one sequence and channel group hand on their state in a chain: a tile publishes its (A, U); from these
 // and the state in front of its group of 16 tiles every tile forms its own carry, always in the same order, so results
 // repeat bit for bit; the last tile of a group publishes the state behind it.  Tiles are taken by ticket, predecessors first, so that
-// whatever a tile waits for is already running.  The forward pass can keep every tile's carry (1/64 of a float32 copy of the
-// states); the backward pass then forms the states again in registers and walks the chain from the end.
+// whatever a tile waits for is already running.  The forward pass can keep the state in front of every 64 rows (1/64 of a
+// float32 copy of the states; a tile of 128 rows keeps two); the backward pass, whose tiles have 64 rows, then forms the states again in
+// registers and walks the chain from the end.
 //
 // Published values go by agent-scope atomic accesses of 8 bytes (coherent over the XCDs' caches).  A value says by itself that it is
 // there, its bits are those of no number before: a flag beside it would cost the chain three more trips through memory (one for the
 // values to arrive before the flag, two for the reader).  A poll gives up after kSpinLimit rounds: the states are then NaN and bit 0 of
 // the status word is set.
 //
-// Bound by HBM where there is much of it: 32768 x 8192 bfloat16 forward 484 us (4.4 TB/s; a copy's 5.9 would take 364), backward 872 (637).
-// The vector unit is busy for 58 to 63 % of that, the chain costs 7 %, the tickets 5 %; workgroups that stay and load their next
-// tile ahead took 610 and 1103 us.  Short calls by latency: 4 x 2048 x 384 11 and 16 us.
+// Bound by HBM where there is much of it: 32768 x 8192 bfloat16 forward 498 us (4.3 TB/s; a copy's 5.9 would take 364), backward 844 (637; accesses past the caches take as long);
+// 16384 x 4096 float32 231 us (182) and 353 (318).  The vector unit is busy for 58 to 63 % of the bfloat16 passes, the chain costs 7 %, the
+// tickets 5 %; workgroups that stay and load their next tile ahead took 610 and 1103 us.  Short calls by latency: 4 x 2048 x 384 12 and
+// 16 us.
 #include <type_traits>
 #include <utility>
 
@@ -91,27 +93,15 @@ __device__ __forceinline__ Tanh tanh2(float x) {
 // ---------------------------------------------------------------------------
 // a lane's channels of a row
 // ---------------------------------------------------------------------------
-// NT: past the caches, for arrays that are larger than they are and whose rows begin on cache lines.
-template <typename T>
-__device__ __forceinline__ T take(const char* p, bool nt) {
-  return nt ? __builtin_nontemporal_load(reinterpret_cast<const T*>(p)) : *reinterpret_cast<const T*>(p);
-}
-template <typename T>
-__device__ __forceinline__ void give(char* p, T v, bool nt) {
-  if (nt)
-    __builtin_nontemporal_store(v, reinterpret_cast<T*>(p));
-  else
-    *reinterpret_cast<T*>(p) = v;
-}
-template <int DT, int CPT, bool NT>
+template <int DT, int CPT>
 struct Row {
   uint32_t w;  // one float32, one bfloat16 or two
   // (row: the same for all lanes; off: the lane's bytes in it)
   __device__ __forceinline__ void load(const char* row, uint32_t off) {
     if constexpr (DT == kBF16 && CPT == 1)
-      w = take<uint16_t>(row + off, NT);
+      w = *reinterpret_cast<const uint16_t*>(row + off);
     else
-      w = take<uint32_t>(row + off, NT);
+      w = *reinterpret_cast<const uint32_t*>(row + off);
   }
   __device__ __forceinline__ float get(int j) const {
     if constexpr (CPT == 2) return __uint_as_float(j ? w & 0xffff0000u : w << 16);
@@ -119,11 +109,11 @@ struct Row {
   }
   static __device__ __forceinline__ void store(char* row, uint32_t off, const float (&v)[CPT]) {
     if constexpr (CPT == 2)
-      give<uint32_t>(row + off, pack_bf16x2(v[0], v[1]), NT);
+      *reinterpret_cast<uint32_t*>(row + off) = pack_bf16x2(v[0], v[1]);
     else if constexpr (DT == kBF16)
-      give<uint16_t>(row + off, f32_to_bf16(v[0]), NT);
+      *reinterpret_cast<uint16_t*>(row + off) = f32_to_bf16(v[0]);
     else
-      give<float>(row + off, v[0], NT);
+      *reinterpret_cast<float*>(row + off) = v[0];
   }
 };
 // The wave's first row of an array, and its rows' distance in bytes.
@@ -319,9 +309,9 @@ __device__ __forceinline__ Part part_of(const Place& p, int wave) {
   return {p.row0 + t0, left < 0 ? 0 : left < T ? left : T};
 }
 // Its inputs, rows behind the end read as the last one.
-template <int DT, int CPT, bool NT, int T, bool WHOLE, int ARRAYS>
+template <int DT, int CPT, int T, bool WHOLE, int ARRAYS>
 __device__ __forceinline__ void load_rows(const Part& q, const void* const (&&p)[ARRAYS], const int64_t (&&ld)[ARRAYS], uint32_t off,
-                                          Row<DT, CPT, NT> (&to)[ARRAYS][T]) {
+                                          Row<DT, CPT> (&to)[ARRAYS][T]) {
   RowsOf r[ARRAYS];
 #pragma unroll
   for (int k = 0; k < ARRAYS; ++k) r[k] = rows_of<DT>(p[k], ld[k], q.row);
@@ -334,7 +324,7 @@ __device__ __forceinline__ void load_rows(const Part& q, const void* const (&&p)
     }
 }
 
-template <int DT, int CPT, bool NT, int T>
+template <int DT, int CPT, int T>
 __global__ __launch_bounds__(64 * kWaves) void recur_fwd_kernel(RecurArgs a, Chain c) {
   __shared__ ChainTile<CPT> sh;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -354,8 +344,8 @@ __global__ __launch_bounds__(64 * kWaves) void recur_fwd_kernel(RecurArgs a, Cha
   // (whole parts apart: without a branch per row their rows are worked on side by side)
   auto gates = [&](auto whole) __attribute__((always_inline)) {
     constexpr bool WHOLE = decltype(whole)::value;
-    Row<DT, CPT, NT> raw[3][T];
-    load_rows<DT, CPT, NT, T, WHOLE, 3>(q, {a.decay, a.write, a.value}, {a.ld_d, a.ld_w, a.ld_v}, off, raw);
+    Row<DT, CPT> raw[3][T];
+    load_rows<DT, CPT, T, WHOLE, 3>(q, {a.decay, a.write, a.value}, {a.ld_d, a.ld_w, a.ld_v}, off, raw);
     float bias[CPT];
 #pragma unroll
     for (int j = 0; j < CPT; ++j) bias[j] = a.bias ? a.bias[ch + j] : 0.0f;
@@ -396,7 +386,7 @@ __global__ __launch_bounds__(64 * kWaves) void recur_fwd_kernel(RecurArgs a, Cha
       if (!WHOLE && i >= q.n) break;
 #pragma unroll
       for (int j = 0; j < CPT; ++j) h[j] = __builtin_fmaf(A[i][j], h[j], U[i][j]);
-      Row<DT, CPT, NT>::store(rh.p, off, h);
+      Row<DT, CPT>::store(rh.p, off, h);
       rh.p += rh.step;
     }
   };
@@ -406,7 +396,7 @@ __global__ __launch_bounds__(64 * kWaves) void recur_fwd_kernel(RecurArgs a, Cha
     states(std::false_type{});
 }
 
-template <int DT, int CPT, bool NT>
+template <int DT, int CPT>
 __global__ __launch_bounds__(64 * kWaves, 4) void recur_bwd_kernel(RecurBwdArgs b, Chain c, float* sums) {
   constexpr int T = kRecurRows / kWaves;
   __shared__ ChainTile<CPT> sh;
@@ -433,15 +423,15 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recur_bwd_kernel(RecurBwdArgs 
 #pragma unroll
   for (int j = 0; j < CPT; ++j) kept[j] = a.carries[static_cast<int64_t>(p.slot0 + p.tile) * a.C + ch + j];
   // Per row: a, and what the gradient is multiplied with for value, write and decay; U: u.
-  Row<DT, CPT, NT> dh[T];
+  Row<DT, CPT> dh[T];
   float A[T][CPT], U[T][CPT], fv[T][CPT], fw[T][CPT], fd[T][CPT];
   float2 part[CPT], from[CPT];  // the rows backwards and forwards
 #pragma unroll
   for (int j = 0; j < CPT; ++j) part[j] = from[j] = make_float2(1.0f, 0.0f);
   auto gates = [&](auto whole) __attribute__((always_inline)) {
     constexpr bool WHOLE = decltype(whole)::value;
-    Row<DT, CPT, NT> raw[4][T];
-    load_rows<DT, CPT, NT, T, WHOLE, 4>(q, {a.decay, a.write, a.value, b.grad}, {a.ld_d, a.ld_w, a.ld_v, b.ld_g}, off, raw);
+    Row<DT, CPT> raw[4][T];
+    load_rows<DT, CPT, T, WHOLE, 4>(q, {a.decay, a.write, a.value, b.grad}, {a.ld_d, a.ld_w, a.ld_v, b.ld_g}, off, raw);
     float bias[CPT];
 #pragma unroll
     for (int j = 0; j < CPT; ++j) bias[j] = a.bias ? a.bias[ch + j] : 0.0f;
@@ -514,9 +504,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recur_bwd_kernel(RecurBwdArgs 
         db[j] += od[j];
         back[j] = A[i][j] * grad;
       }
-      Row<DT, CPT, NT>::store(rv.p, off, ov);
-      Row<DT, CPT, NT>::store(rw.p, off, ow);
-      Row<DT, CPT, NT>::store(rd.p, off, od);
+      Row<DT, CPT>::store(rv.p, off, ov);
+      Row<DT, CPT>::store(rw.p, off, ow);
+      Row<DT, CPT>::store(rd.p, off, od);
       rv.p -= rv.step, rw.p -= rw.step, rd.p -= rd.step;
     }
   };
@@ -649,16 +639,6 @@ bool in_pairs(int dt, int64_t C, std::initializer_list<std::pair<const void*, in
   return true;
 }
 
-// Whether a call's `arrays` arrays are more than the last cache holds, in rows of whole cache lines.  There the loads and stores go past
-// the caches (32768 x 8192 forward 519 us and 490, backward 877 and 827); elsewhere, the lines of rows that share one
-// are wanted again (11 sequences of 333 float32 channels backward 22 us and 27).
-bool past_caches(const RecurArgs& a, int arrays, std::initializer_list<int64_t> pitches) {
-  const int64_t e = a.dt == kBF16 ? 2 : 4;
-  for (int64_t ld : pitches)
-    if (ld * e % 128) return false;
-  return a.B * a.L * a.C * e * arrays > (256LL << 20);
-}
-
 struct Plan {
   int64_t slots = 0;
   int64_t at_values = 0, at_starts = 0, at_sums = 0, total = 0;  // tickets first
@@ -740,7 +720,11 @@ int launch_gated_scan(const RecurArgs& a, void* ws, int64_t ws_bytes, hipStream_
   TESM_REQUIRE(small.total == 0 || (ws && ws_bytes >= small.total && aligned(ws, 16)), kErrWorkspace,
                "gated scan: workspace too small or not 16-byte aligned");
   const bool pairs = many_tiles(a) && in_pairs(a.dt, a.C, {{a.value, a.ld_v}, {a.write, a.ld_w}, {a.decay, a.ld_d}, {a.h, a.ld_h}});
-  const bool past = past_caches(a, 4, {a.ld_v, a.ld_w, a.ld_d, a.ld_h}), tall = past && pairs;
+  // Tiles of 128 rows where the call's four arrays are more than the last cache holds and sequences are long: half as many hand-overs, and
+  // twice the loads under way (us with 64 rows and with 128: 1 x 32768 x 8192 525 and 492, of 8190 channels 577 and 551; smaller arrays
+  // 4 x 2048 x 2048 37.1 and 37.5; short sequences, where half a tile may stay empty, 64 x 192 x 8192 185 and 208).
+  const int64_t all_rows = a.B * a.L;
+  const bool tall = pairs && all_rows * a.C * 2 * 4 > (256LL << 20) && all_rows >= 1024 * a.S;
   const int tile = tall ? 2 * kRecurRows : kRecurRows;
   const Plan p = plan_of(a, false, tile);
   const Chain c = chain_of(a, p, ws, pairs ? 2 : 1, tile);
@@ -748,19 +732,15 @@ int launch_gated_scan(const RecurArgs& a, void* ws, int64_t ws_bytes, hipStream_
   TESM_REQUIRE(fits_grid(blocks, 64 * kWaves), kErrUnsupported, "gated scan: too many tiles for one call");
   if (int rc = reset(a, p, c, pairs ? 2 : 1, RestArgs{{a.h}, {a.ld_h}}, st)) return rc;
   const unsigned n = static_cast<unsigned>(blocks);
-#define TESM_RECUR(DT, CPT, NT, T) recur_fwd_kernel<DT, CPT, NT, T><<<n, 64 * kWaves, 0, TESM_LOGGED(st, recur_fwd_kernel<DT, CPT, NT, T>)>>>(a, c)
-  if (a.dt == kF32) {
-    if (past)
-      TESM_RECUR(kF32, 1, true, 8);
-    else
-      TESM_RECUR(kF32, 1, false, 8);
-  } else if (tall) {
-    TESM_RECUR(kBF16, 2, true, 16);
-  } else if (pairs) {
-    TESM_RECUR(kBF16, 2, false, 8);
-  } else {
-    TESM_RECUR(kBF16, 1, false, 8);
-  }
+#define TESM_RECUR(DT, CPT, T) recur_fwd_kernel<DT, CPT, T><<<n, 64 * kWaves, 0, TESM_LOGGED(st, recur_fwd_kernel<DT, CPT, T>)>>>(a, c)
+  if (a.dt == kF32)
+    TESM_RECUR(kF32, 1, 8);
+  else if (tall)
+    TESM_RECUR(kBF16, 2, 16);
+  else if (pairs)
+    TESM_RECUR(kBF16, 2, 8);
+  else
+    TESM_RECUR(kBF16, 1, 8);
 #undef TESM_RECUR
   return check_launch("gated scan");
 }
@@ -787,21 +767,13 @@ int launch_gated_scan_bwd(const RecurBwdArgs& b, void* ws, int64_t ws_bytes, hip
   if (blocks > 0) {
     if (int rc = reset(a, p, c, pairs ? 2 : 1, RestArgs{{b.d_value, b.d_write, b.d_decay}, {b.ld_dv, b.ld_dw, b.ld_dd}}, st)) return rc;
     const unsigned n = static_cast<unsigned>(blocks);
-    const bool past = past_caches(a, 7, {a.ld_v, a.ld_w, a.ld_d, b.ld_g, b.ld_dv, b.ld_dw, b.ld_dd});
-#define TESM_RECUR(DT, CPT, NT) recur_bwd_kernel<DT, CPT, NT><<<n, 64 * kWaves, 0, TESM_LOGGED(st, recur_bwd_kernel<DT, CPT, NT>)>>>(b, c, sums)
-    if (a.dt == kF32) {
-      if (past)
-        TESM_RECUR(kF32, 1, true);
-      else
-        TESM_RECUR(kF32, 1, false);
-    } else if (pairs) {
-      if (past)
-        TESM_RECUR(kBF16, 2, true);
-      else
-        TESM_RECUR(kBF16, 2, false);
-    } else {
-      TESM_RECUR(kBF16, 1, false);
-    }
+#define TESM_RECUR(DT, CPT) recur_bwd_kernel<DT, CPT><<<n, 64 * kWaves, 0, TESM_LOGGED(st, recur_bwd_kernel<DT, CPT>)>>>(b, c, sums)
+    if (a.dt == kF32)
+      TESM_RECUR(kF32, 1);
+    else if (pairs)
+      TESM_RECUR(kBF16, 2);
+    else
+      TESM_RECUR(kBF16, 1);
 #undef TESM_RECUR
   }
   if (b.d_bias) {

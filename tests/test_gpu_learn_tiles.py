@@ -105,7 +105,7 @@ def test_projection_onto_a_vocabulary(dtype):
 
 
 # ---------------------------------------------------------------------------
-# recurrence: two channels per lane from 1024 tiles of 128 on, past the caches (and there 128 rows per tile forward) above 256 MiB
+# recurrence: two channels per lane from 1024 tiles of 128 on, 128 rows per tile forward above 256 MiB in long sequences
 # ---------------------------------------------------------------------------
 def scan_on_device(seed, B, L, C, dtype, starts=None):
     g = torch.Generator(device=DEV).manual_seed(seed)
@@ -138,38 +138,48 @@ PACKED = [5, 70, 70, 4001, 4129, 12345, 16990]  # (an empty one, one of 128 rows
 def test_scan_of_two_channels_per_lane():
     C = 1030
     check_channels(scan_on_device(1, 8, 1000, C, BF), [0, 1, 63, 64, 127, 128, 129, 766, 1023, 1024, C - 2, C - 1],
-                   ["recur_fwd_kernel<1,2,false,8>", "recur_bwd_kernel<1,2,false>"])
+                   ["recur_fwd_kernel<1,2,8>", "recur_bwd_kernel<1,2>"])
 
 
 def test_scan_of_two_channels_per_lane_packed():
     C, starts = 520, PACKED
     h, grads = check_channels(scan_on_device(2, 1, 17003, C, BF, starts), [0, 1, 127, 128, 258, 383, 512, C - 1],
-                              ["recur_fwd_kernel<1,2,false,8>", "recur_bwd_kernel<1,2,false>"])
+                              ["recur_fwd_kernel<1,2,8>", "recur_bwd_kernel<1,2>"])
     for t in (h, *grads[:3]):
         assert not t[:, :starts[0]].any() and not t[:, starts[-1]:].any()
 
 
-def test_scan_past_the_caches():
+def test_scan_of_tall_tiles():
     C = 2048
     check_channels(scan_on_device(3, 3, 5600, C, BF), [0, 1, 127, 128, 1000, 1025, C - 2, C - 1],
-                   ["recur_fwd_kernel<1,2,true,16>", "recur_bwd_kernel<1,2,true>"])
+                   ["recur_fwd_kernel<1,2,16>", "recur_bwd_kernel<1,2>"])
 
 
 @pytest.mark.parametrize("starts", [PACKED, [0, 128, 192, 256, 16900, 17003]])
-def test_scan_past_the_caches_packed(starts):
+def test_scan_of_tall_tiles_packed(starts):
     """Carries that tiles of 128 rows leave are those that tiles of 64 rows read, whatever row a sequence begins on."""
     C = 2048
     h, grads = check_channels(scan_on_device(4, 1, 17003, C, BF, starts), [0, 1, 127, 128, 1000, 1025, C - 2, C - 1],
-                              ["recur_fwd_kernel<1,2,true,16>", "recur_bwd_kernel<1,2,true>"])
+                              ["recur_fwd_kernel<1,2,16>", "recur_bwd_kernel<1,2>"])
     for t in (h, *grads[:3]):
         assert not t[:, :starts[0]].any() and not t[:, starts[-1]:].any()
 
 
+def test_scan_of_large_calls_of_short_sequences():
+    C = 4096
+    check_channels(scan_on_device(6, 50, 192, C, BF), [0, 1, 127, 128, 2000, C - 1], ["recur_fwd_kernel<1,2,8>", "recur_bwd_kernel<1,2>"])
+
+
+def test_scan_of_tall_tiles_at_any_pitch():
+    C = 2046
+    check_channels(scan_on_device(7, 1, 17003, C, BF), [0, 1, 127, 128, 1000, C - 1], ["recur_fwd_kernel<1,2,16>", "recur_bwd_kernel<1,2>"])
+
+
 @pytest.mark.parametrize("B,L,starts", [(4, 4200, None), (1, 17003, PACKED)])
-def test_scan_of_float32_past_the_caches(B, L, starts):
+def test_scan_of_large_float32_calls(B, L, starts):
     C = 1024
     check_channels(scan_on_device(5, B, L, C, F32, starts), [0, 1, 63, 64, 500, C - 2, C - 1],
-                   ["recur_fwd_kernel<0,1,true,8>", "recur_bwd_kernel<0,1,true>"])
+                   ["recur_fwd_kernel<0,1,8>", "recur_bwd_kernel<0,1>"])
 
 
 # ---------------------------------------------------------------------------
