@@ -707,8 +707,10 @@ int tesm_hip_gated_scan_step(const tesm_hip_recurrence_step* p, void* stream);
 
 /* Products of float matrices with what stands around them, no reference counterpart (the reference's projections are ternary).
  * up given: the gated pair of a feed-forward block, y = act(x weight^T) * (x up^T).  up NULL: y = act(x weight^T + bias) +
- * residual.  act: 0 none (not for a pair), 1 silu, 2 gelu (z (1 + erf(z / sqrt 2)) / 2).  Sums are float32, rounded to dt once;
- * float32 operands go through the matrix units in three bfloat16 parts (an infinity among them gives NaN).  z, for the
+ * residual.  act: 0 none (not for a pair), 1 silu, 2 gelu (z (1 + erf(z / sqrt 2)) / 2, erf 1.5e-7
+ * off at most).  Sums are float32, rounded to dt once;
+ * float32 operands go through the matrix units in three bfloat16 parts (an infinity among them may give NaN, values below
+ * 2^-100 in magnitude keep fewer bits).  z, for the
  * backward call (NULL: not kept): x weight^T + bias; of a pair, with z_up, x weight^T and x up^T; each (M, N) float32, or
  * with bf16 operands M * N upper 16 bits followed by M * N next 8 bits.  M < 2^31, N, K < 2^24; above
  * 2^21 values per row or pitch, calls of many rows may be refused (32-bit offsets inside a tile), and so may matrices of 2^34 values

@@ -219,7 +219,7 @@ __device__ __forceinline__ void kept_eight(const void* z, int64_t all, int64_t i
     }
   }
 }
-// dg = dh u act'(g) and du = dh act(g) beside each other in rows of 2 Np values.  Bound by HBM: 8192 x 2048 bfloat16 33 us, 6 TB/s.
+// dg = dh u act'(g) and du = dh act(g) beside each other in rows of 2 Np values.  Bound by HBM: 8192 x 2048 bfloat16 52 us for 268 MB.
 template <int DT>
 __global__ __launch_bounds__(256) void gated_grad_kernel(const void* grad, int64_t ld_g, const void* z, const void* z2, int64_t M, int64_t N,
                                                          int64_t Np, int act, uint16_t* dst) {
@@ -245,7 +245,8 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const void* grad, int64
 
 constexpr int kSumRows = 64;  // rows per sum
 // dz = dy act'(z) into its parts (dst), and the sums of kSumRows rows of it (sums); either may be left out.  A workgroup takes every
-// gridDim.y-th run of kSumRows rows.
+// gridDim.y-th run of kSumRows rows.  8192 x 768 bfloat16 7 us without an activation, 23 with one (56 MB); its time is latency, three
+// workgroups per two CUs.
 template <int DT>
 __global__ __launch_bounds__(256) void linear_grad_kernel(const void* grad, int64_t ld_g, const void* z, int64_t M, int64_t N, int64_t Np,
                                                           int act, uint16_t* dst, float* sums) {

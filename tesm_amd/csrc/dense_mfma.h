@@ -8,7 +8,7 @@ namespace tesm {
 
 constexpr int kMaxPairs = 4;
 
-// out[m, n] = sum over pairs p and k of A_p[m, k] B_p[n, k].  An operand lies with k along its rows (m or n picks the row), or, where
+// out[m, n] = sum over pairs p and k of A_p[m, k] B_p[n, k] (a gradient in two bfloat16 parts is two pairs with one B).  An operand lies with k along its rows (m or n picks the row), or, where
 // its layout is "down", with k picking the row.  All pairs share extents and pitches.  Rows start on 16 bytes; the contiguous
 // extent is a multiple of 8.  With part_a set, operands are float32 values in three bfloat16 parts, part i lying i * part_a (part_b)
 // values behind the first.
@@ -37,7 +37,6 @@ struct ProductArgs {
 };
 
 enum ProductKind : int { kProdGated = 0, kProdLinear = 1, kProdStore = 2, kProdPartial = 3 };
-enum ProductLayout : int { kAlong = 0, kDown = 1 };
 
 // dt: type of the results (kProdPartial: float32).  adown, bdown: operand layouts.
 int launch_product(ProductKind kind, int dt, bool adown, bool bdown, ProductArgs a, hipStream_t st);

@@ -236,8 +236,8 @@ def stream_copy(dst: torch.Tensor, src: torch.Tensor) -> None:
 
 
 def device_status(clear: bool = True) -> int:
-    """The device status word of the current device (bit 0: a scan look-back gave up; bit 1: a parent of
-    ``reorder_rows`` was none of the beams); synchronises."""
+    """The device status word of the current device (bit 0: a scan's poll gave up; bit 1: a parent of ``reorder_rows`` was none
+    of the beams; bit 2: a target of ``token_log_probs`` was no token); synchronises."""
     v = ctypes.c_uint32(0)
     lib = _lib.load()
     _lib.check(lib.tesm_hip_device_status(ctypes.byref(v), int(clear)))

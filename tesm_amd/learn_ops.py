@@ -367,9 +367,10 @@ class _GatedLinear(torch.autograd.Function):
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, act: str = "silu", keep: bool = False):
     """A feed-forward block's gated pair in one kernel: ``act(x w_gate^T) * (x w_up^T)``, (.., N).
 
-    x (.., K), w_gate and w_up (N, K) share a dtype; ``act`` is "silu" or "gelu" (the error function's form).  Sums and the
-    activation are float32, the result is rounded once.  float32 operands go through the matrix units in three bfloat16 parts, to the
-    error of a float32 sum; an infinity among them gives NaN.  Of few rows (up to 32, float32 64) the weights are streamed once.
+    x (.., K), w_gate and w_up (N, K) share a dtype; ``act`` is "silu" or "gelu" (the error function's form, by a polynomial that is
+    1.5e-7 off at most).  Sums and the activation are float32, the result is rounded once.  float32 operands go through the matrix
+    units in three bfloat16 parts, to the error of a float32 sum; an infinity among them may give NaN, and values below 2^-100 in
+    magnitude keep fewer bits.  Of few rows (up to 32, float32 64) the weights are streamed once.
     Rows of more than 2^21 values may be refused.  ``keep=True`` also returns what ``gated_linear_backward`` needs (both products,
     in 24 bits where x is bfloat16).
     """

@@ -68,6 +68,15 @@ def test_float32_products(M, K, N):
     assert off_in_norm(hip_ops.gated_linear(x, w, up), val * (xd @ ud.t())) <= 2.1 * f32_bound(K) + 8 * 2.0 ** -24
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -99, 2.0 ** 100])
+@pytest.mark.parametrize("M,K,N", [(40, 104, 72), (200, 500, 130)])
+def test_float32_products_of_far_scales(scale, M, K, N):
+    """Parts of operands down to 2^-100 are numbers too (few of the random ones are below 2^-100 themselves, none of weight)."""
+    c = dense_case(M, M, K, N, torch.float32)
+    x, w = _dev(c["x"]) * scale, _dev(c["w"])
+    assert off_in_norm(hip_ops.fused_linear(x, w) / scale, (x.double() / scale) @ w.double().t()) <= f32_bound(K)
+
+
 # ---------------------------------------------------------------------------
 # the recurrence's decays
 # ---------------------------------------------------------------------------
