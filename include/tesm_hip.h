@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define TESM_HIP_ABI_VERSION 9
+#define TESM_HIP_ABI_VERSION 10
 
 #define TESM_DT_F32 0
 #define TESM_DT_BF16 1
@@ -638,7 +638,8 @@ int tesm_hip_reorder_rows(const tesm_hip_rows* t, int64_t count, const int64_t* 
  * zero_rest, set to zero.  h0 / h_out: (S, C) float32,
  * the states before and after each sequence (NULL h0: zeros).  States are float32; results repeat bit for bit.  carries:
  * (tesm_hip_gated_scan_slots, C) float32, what the backward call needs (NULL: not kept).  Fewer than 2^31 rows, C and S
- * below 2^24, and fewer than 2^23 tiles of 64 rows of a sequence by 64 channels.  Outputs must not overlap operands or each other (columns of the same wider rows do not overlap). */
+ * below 2^24, and fewer than 2^23 tiles of 64 rows of a sequence by 64 channels.  Outputs must not overlap operands or each other
+ * (columns of the same wider rows do not overlap). */
 typedef struct tesm_hip_gates {
   int dt;                     /* value, write, decay, and the arrays of their shape */
   int64_t B, L, C, S;
@@ -707,12 +708,10 @@ int tesm_hip_gated_scan_step(const tesm_hip_recurrence_step* p, void* stream);
 
 /* Products of float matrices with what stands around them, no reference counterpart (the reference's projections are ternary).
  * up given: the gated pair of a feed-forward block, y = act(x weight^T) * (x up^T).  up NULL: y = act(x weight^T + bias) +
- * residual.  act: 0 none (not for a pair), 1 silu, 2 gelu (z (1 + erf(z / sqrt 2)) / 2, erf 1.5e-7
- * off at most).  Sums are float32, rounded to dt once;
- * float32 operands go through the matrix units in three bfloat16 parts (an infinity among them may give NaN, values below
- * 2^-100 in magnitude keep fewer bits).  z, for the
- * backward call (NULL: not kept): x weight^T + bias; of a pair, with z_up, x weight^T and x up^T; each (M, N) float32, or
- * with bf16 operands M * N upper 16 bits followed by M * N next 8 bits.  M < 2^31, N, K < 2^24; above
+ * residual.  act: 0 none (not for a pair), 1 silu, 2 gelu (z (1 + erf(z / sqrt 2)) / 2, erf 1.5e-7 off at most).  Sums are float32,
+ * rounded to dt once; float32 operands go through the matrix units in three bfloat16 parts (an infinity among them may give NaN, values
+ * below 2^-100 in magnitude keep fewer bits).  z, for the backward call (NULL: not kept): x weight^T + bias; of a pair, with z_up,
+ * x weight^T and x up^T; each (M, N) float32, or with bf16 operands M * N upper 16 bits followed by M * N next 8 bits.  M < 2^31, N, K < 2^24; above
  * 2^21 values per row or pitch, calls of many rows may be refused (32-bit offsets inside a tile), and so may matrices of 2^34 values
  * in rows padded to 64. */
 typedef struct tesm_hip_dense {
